@@ -68,6 +68,21 @@ EXPORTED_SYMBOLS = (
     "gdn_layer_step_tiles",
 )
 
+# include/gdn_linear_hip.h
+GDN_LINEAR_ABI_VERSION = 1
+GDN_LAYER_NORM_MAX_D = 16384
+LINEAR_SYMBOLS = (
+    "gdn_linear_abi_version",
+    "gdn_linear_attn_chunk_fwd",
+    "gdn_linear_attn_workspace_bytes",
+    "gdn_linear_attn_recurrent_fwd",
+    "gdn_linear_attn_bwd",
+    "gdn_linear_attn_bwd_workspace_bytes",
+    "gdn_layer_norm_fwd",
+    "gdn_layer_norm_bwd",
+    "gdn_layer_norm_partial_blocks",
+)
+
 GDN_CHUNK_KERNELS = 3
 CHUNK_KERNEL_NAMES = ("chunk_offsets", "chunk_prepare", "chunk_scan")
 
@@ -213,6 +228,52 @@ class GdnNormArgs(ctypes.Structure):
     )
 
 
+class GdnLinearAttnArgs(ctypes.Structure):
+    """Mirror of ``struct gdn_linear_attn_args`` (include/gdn_linear_hip.h)."""
+
+    _fields_ = (
+        [(name, ctypes.c_void_p) for name in ("q", "k", "v", "g", "h0", "ht", "o", "cu_seqlens", "workspace")]
+        + [("workspace_bytes", ctypes.c_uint64)]
+        + [(f"{t}_stride_{d}", ctypes.c_int64) for t in ("q", "k", "v", "o") for d in ("b", "t", "h")]
+        + [(name, ctypes.c_int32) for name in ("B", "T", "H", "K", "V", "N", "qk_heads", "dtype", "flags")]
+        + [("scale", ctypes.c_float)]
+    )
+
+
+class GdnLinearAttnBwdArgs(ctypes.Structure):
+    """Mirror of ``struct gdn_linear_attn_bwd_args``."""
+
+    _fields_ = (
+        [("fwd", GdnLinearAttnArgs)]
+        + [(name, ctypes.c_void_p) for name in ("dout", "dht", "dq", "dk", "dv", "dh0", "dg", "workspace")]
+        + [("workspace_bytes", ctypes.c_uint64)]
+        + [(f"{t}_stride_{d}", ctypes.c_int64) for t in ("dout", "dq", "dk", "dv") for d in ("b", "t", "h")]
+    )
+
+
+class GdnLayerNormArgs(ctypes.Structure):
+    """Mirror of ``struct gdn_layer_norm_args``."""
+
+    _fields_ = (
+        [(name, ctypes.c_void_p) for name in ("x", "weight", "bias", "y")]
+        + [(name, ctypes.c_int64) for name in ("x_stride", "y_stride", "rows")]
+        + [(name, ctypes.c_int32) for name in ("D", "dtype", "w_dtype")]
+        + [("eps", ctypes.c_float)]
+    )
+
+
+class GdnLayerNormBwdArgs(ctypes.Structure):
+    """Mirror of ``struct gdn_layer_norm_bwd_args``."""
+
+    _fields_ = (
+        [(name, ctypes.c_void_p) for name in ("x", "dy", "weight", "dx", "dweight_partial", "dbias_partial")]
+        + [(name, ctypes.c_int64) for name in ("x_stride", "dy_stride", "dx_stride", "rows")]
+        + [(name, ctypes.c_int32) for name in ("D", "dtype", "w_dtype")]
+        + [("eps", ctypes.c_float)]
+        + [(name, ctypes.c_int32) for name in ("partial_blocks", "reserved")]
+    )
+
+
 class GdnLibraryError(RuntimeError):
     pass
 
@@ -231,7 +292,7 @@ def load_library() -> ctypes.CDLL:
             "(run `python -m lm_engine_amd.build`); there is no fallback path."
         )
     lib = ctypes.CDLL(LIBRARY_PATH)
-    for symbol in EXPORTED_SYMBOLS:
+    for symbol in EXPORTED_SYMBOLS + LINEAR_SYMBOLS:
         if not hasattr(lib, symbol):
             raise GdnLibraryError(f"{LIBRARY_PATH} does not export {symbol}")
 
@@ -294,6 +355,26 @@ def load_library() -> ctypes.CDLL:
 
     lib.gdn_layer_step_tiles.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int]
     lib.gdn_layer_step_tiles.restype = ctypes.c_int
+
+    lib.gdn_linear_abi_version.argtypes = []
+    lib.gdn_linear_abi_version.restype = ctypes.c_int
+    for name in ("gdn_linear_attn_chunk_fwd", "gdn_linear_attn_recurrent_fwd"):
+        getattr(lib, name).argtypes = [ctypes.POINTER(GdnLinearAttnArgs), ctypes.c_void_p]
+        getattr(lib, name).restype = ctypes.c_int
+    lib.gdn_linear_attn_workspace_bytes.argtypes = [ctypes.POINTER(GdnLinearAttnArgs)]
+    lib.gdn_linear_attn_workspace_bytes.restype = ctypes.c_uint64
+    lib.gdn_linear_attn_bwd.argtypes = [ctypes.POINTER(GdnLinearAttnBwdArgs), ctypes.c_void_p]
+    lib.gdn_linear_attn_bwd.restype = ctypes.c_int
+    lib.gdn_linear_attn_bwd_workspace_bytes.argtypes = [ctypes.POINTER(GdnLinearAttnBwdArgs)]
+    lib.gdn_linear_attn_bwd_workspace_bytes.restype = ctypes.c_uint64
+    lib.gdn_layer_norm_fwd.argtypes = [ctypes.POINTER(GdnLayerNormArgs), ctypes.c_void_p]
+    lib.gdn_layer_norm_fwd.restype = ctypes.c_int
+    lib.gdn_layer_norm_bwd.argtypes = [ctypes.POINTER(GdnLayerNormBwdArgs), ctypes.c_void_p]
+    lib.gdn_layer_norm_bwd.restype = ctypes.c_int
+    lib.gdn_layer_norm_partial_blocks.argtypes = [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]
+    lib.gdn_layer_norm_partial_blocks.restype = ctypes.c_int
+    if lib.gdn_linear_abi_version() != GDN_LINEAR_ABI_VERSION:
+        raise GdnLibraryError(f"libgdn_hip.so: version {lib.gdn_linear_abi_version()} of its second part, this binding expects {GDN_LINEAR_ABI_VERSION}")
 
     version = lib.gdn_abi_version()
     if version != GDN_ABI_VERSION:

@@ -292,6 +292,139 @@ gated_rmsnorm_forward.register_autograd(_norm_backward, setup_context=_norm_setu
 
 
 # ---------------------------------------------------------------------------------------
+# linear attention with a decay for each head
+# ---------------------------------------------------------------------------------------
+@torch.library.custom_op(
+    "lm_engine_amd::linear_attention_forward",
+    mutates_args=(),
+    schema="(Tensor q, Tensor k, Tensor v, Tensor? g, Tensor? initial_state, Tensor? cu_seqlens, str mode, float? scale, "
+    "bool output_final_state, bool left_padded) -> (Tensor, Tensor)",
+)
+def linear_attention_forward(q, k, v, g, initial_state, cu_seqlens, mode, scale, output_final_state, left_padded):
+    from . import linear as la
+
+    o, ht = la._run(mode, q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, False, left_padded)
+    return o, _or_empty(ht, o)
+
+
+@linear_attention_forward.register_fake
+def _(q, k, v, g, initial_state, cu_seqlens, mode, scale, output_final_state, left_padded):
+    B, T, _, K = q.shape
+    H, V = v.size(2), v.size(-1)
+    N = B if cu_seqlens is None or left_padded else cu_seqlens.numel() - 1
+    return v.new_empty(B, T, H, V), (v.new_empty((N, H, K, V), dtype=torch.float32) if output_final_state else v.new_empty(0))
+
+
+@torch.library.custom_op(
+    "lm_engine_amd::linear_attention_backward",
+    mutates_args=(),
+    schema="(Tensor q, Tensor k, Tensor v, Tensor? g, Tensor? initial_state, Tensor? cu_seqlens, Tensor d_o, Tensor? d_ht, "
+    "float? scale, bool left_padded, bool needs_dg) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
+)
+def linear_attention_backward(q, k, v, g, initial_state, cu_seqlens, d_o, d_ht, scale, left_padded, needs_dg):
+    from . import linear as la
+
+    dq, dk, dv, dg, dh0 = la._backward(q, k, v, g, scale, initial_state, cu_seqlens, left_padded, d_o, d_ht, needs_dg,
+                                       initial_state is not None)  # fmt: skip
+    return dq, dk, dv, _or_empty(dg, q), _or_empty(dh0, q)
+
+
+@linear_attention_backward.register_fake
+def _(q, k, v, g, initial_state, cu_seqlens, d_o, d_ht, scale, left_padded, needs_dg):
+    empty = q.new_empty(0)
+    return (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), torch.empty_like(g) if needs_dg else empty,
+            empty if initial_state is None else initial_state.new_empty(initial_state.shape))  # fmt: skip
+
+
+def _linear_attention_setup(ctx, inputs, output):
+    q, k, v, g, initial_state, cu_seqlens, mode, scale, output_final_state, left_padded = inputs
+    ctx.save_for_backward(q, k, v, g, initial_state, cu_seqlens)
+    ctx.options = (scale, left_padded, output_final_state)
+
+
+def _linear_attention_backward(ctx, d_o, d_ht):
+    q, k, v, g, initial_state, cu_seqlens = ctx.saved_tensors
+    scale, left_padded, output_final_state = ctx.options
+    dq, dk, dv, dg, dh0 = torch.ops.lm_engine_amd.linear_attention_backward(
+        q, k, v, g, initial_state, cu_seqlens, d_o.contiguous(), d_ht if output_final_state else None, scale, left_padded,
+        ctx.needs_input_grad[3])  # fmt: skip
+    return (dq, dk, dv, dg if ctx.needs_input_grad[3] else None, None if initial_state is None else dh0, None, None, None, None, None)
+
+
+linear_attention_forward.register_autograd(_linear_attention_backward, setup_context=_linear_attention_setup)
+
+
+@torch.library.custom_op(
+    "lm_engine_amd::linear_attention_decode_",
+    mutates_args=("state",),
+    schema="(Tensor q, Tensor k, Tensor v, Tensor? g, Tensor(a!) state, Tensor? cu_seqlens, float? scale, bool left_padded) -> Tensor",
+)
+def linear_attention_decode_(q, k, v, g, state, cu_seqlens, scale, left_padded):
+    """The recurrent form with the state updated in place (inference)."""
+    from . import linear as la
+
+    return la._run("recurrent", q, k, v, g, scale, state, True, cu_seqlens, True, left_padded)[0]
+
+
+@linear_attention_decode_.register_fake
+def _(q, k, v, g, state, cu_seqlens, scale, left_padded):
+    return v.new_empty(v.shape)
+
+
+# ---------------------------------------------------------------------------------------
+# layer norm
+# ---------------------------------------------------------------------------------------
+@torch.library.custom_op(
+    "lm_engine_amd::layer_norm_forward",
+    mutates_args=(),
+    schema="(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor",
+)
+def layer_norm_forward(x, weight, bias, eps):
+    from . import norm as ln
+
+    return ln._forward(x, weight, bias, eps)
+
+
+@layer_norm_forward.register_fake
+def _(x, weight, bias, eps):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op(
+    "lm_engine_amd::layer_norm_backward",
+    mutates_args=(),
+    schema="(Tensor x, Tensor? weight, Tensor? bias, float eps, Tensor dy) -> (Tensor, Tensor, Tensor)",
+)
+def layer_norm_backward(x, weight, bias, eps, dy):
+    from . import norm as ln
+
+    dx, dw, db = ln._backward(x, weight, None if bias is None else bias.dtype, eps, dy, weight is not None, bias is not None)
+    return dx, _or_empty(dw, x), _or_empty(db, x)
+
+
+@layer_norm_backward.register_fake
+def _(x, weight, bias, eps, dy):
+    empty = x.new_empty(0)
+    like = lambda p: empty if p is None else p.new_empty(p.shape)  # noqa: E731
+    return x.new_empty(x.shape), like(weight), like(bias)
+
+
+def _layer_norm_setup(ctx, inputs, output):
+    x, weight, bias, eps = inputs
+    ctx.save_for_backward(x, weight, bias)
+    ctx.eps = eps
+
+
+def _layer_norm_backward(ctx, dy):
+    x, weight, bias = ctx.saved_tensors
+    dx, dw, db = torch.ops.lm_engine_amd.layer_norm_backward(x, weight, bias, ctx.eps, dy.contiguous())
+    return dx, None if weight is None else dw, None if bias is None else db, None
+
+
+layer_norm_forward.register_autograd(_layer_norm_backward, setup_context=_layer_norm_setup)
+
+
+# ---------------------------------------------------------------------------------------
 # what the eager entry points call while a graph is being captured
 # ---------------------------------------------------------------------------------------
 def gated_delta_rule(mode, q, k, v, g, beta, scale, initial_state, output_final_state, cu_seqlens, l2norm, inplace_state,
@@ -328,3 +461,17 @@ def delta_rule_gates(a, b, A_log, dt_bias, allow_neg_eigval):
 
 def gated_rmsnorm(o, gate, weight, eps):
     return torch.ops.lm_engine_amd.gated_rmsnorm_forward(o, gate, weight, eps)
+
+
+def linear_attention(mode, q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, inplace_state, left_padded):
+    if inplace_state:
+        if not output_final_state or initial_state is None:
+            raise ValueError("inplace_state needs an initial_state to update and output_final_state=True")
+        o = torch.ops.lm_engine_amd.linear_attention_decode_(q, k, v, g, initial_state, cu_seqlens, scale, left_padded)
+        return o, initial_state
+    o, ht = torch.ops.lm_engine_amd.linear_attention_forward(q, k, v, g, initial_state, cu_seqlens, mode, scale, output_final_state, left_padded)
+    return o, (ht if output_final_state else None)
+
+
+def layer_norm(x, weight, bias, eps):
+    return torch.ops.lm_engine_amd.layer_norm_forward(x, weight, bias, eps)

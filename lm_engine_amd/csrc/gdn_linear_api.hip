@@ -1,0 +1,275 @@
+// C ABI of linear attention with a decay for each head (include/gdn_linear_hip.h): argument checks, how long sequences are cut, and
+// the walks that make up a call.  What lives on the device (cu_seqlens) is clamped by the kernels.
+#include <algorithm>
+
+#include "gdn_launch.h"
+#include "gdn_linear_common.h"
+
+namespace gdn {
+
+namespace {
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int check_rows(const void* p, int64_t b, int64_t t, int64_t h, int dtype) {
+    const int64_t vec = dtype == GDN_BF16 ? 8 : 4;
+    if (p == nullptr) return GDN_ERR_NULL;
+    if (!aligned16(p) || b % vec != 0 || t % vec != 0 || h % vec != 0) return GDN_ERR_ALIGN;
+    return GDN_OK;
+}
+
+int check_shape(const gdn_linear_attn_args& a) {
+    if (a.B <= 0 || a.T <= 0 || a.H <= 0 || a.K <= 0 || a.V <= 0 || a.N <= 0) return GDN_ERR_SHAPE;
+    if (a.qk_heads < 0 || (a.qk_heads > 0 && a.H % a.qk_heads != 0)) return GDN_ERR_SHAPE;
+    const bool padded = (a.flags & GDN_FLAG_LEFT_PADDED) != 0;
+    if (padded && a.cu_seqlens == nullptr) return GDN_ERR_NULL;
+    if (a.cu_seqlens != nullptr && !padded) {
+        if (a.B != 1) return GDN_ERR_VARLEN;
+    } else if (a.N != a.B) {
+        return GDN_ERR_SHAPE;
+    }
+    if (a.dtype != GDN_BF16 && a.dtype != GDN_F32) return GDN_ERR_UNSUPPORTED;
+    if (a.K % 8 != 0 || a.K > 256 || a.V % 8 != 0) return GDN_ERR_UNSUPPORTED;
+    if (a.flags & ~(GDN_FLAG_LEFT_PADDED | GDN_FLAG_ZERO_PADDING)) return GDN_ERR_UNSUPPORTED;
+    // sizes that the kernels hold in 32 bits: token indexes, heads (a grid dimension), cells of a state
+    if (a.T > 1 << 30 || a.H > 65535 || a.V > 1 << 20) return GDN_ERR_UNSUPPORTED;
+    return GDN_OK;
+}
+
+int check_inputs(const gdn_linear_attn_args& a) {
+    int e;
+    if ((e = check_rows(a.q, a.q_stride_b, a.q_stride_t, a.q_stride_h, a.dtype)) != GDN_OK) return e;
+    if ((e = check_rows(a.k, a.k_stride_b, a.k_stride_t, a.k_stride_h, a.dtype)) != GDN_OK) return e;
+    if ((e = check_rows(a.v, a.v_stride_b, a.v_stride_t, a.v_stride_h, a.dtype)) != GDN_OK) return e;
+    if (!aligned16(a.h0) || !aligned16(a.ht)) return GDN_ERR_ALIGN;
+    if (reinterpret_cast<uintptr_t>(a.g) % 4 != 0 || reinterpret_cast<uintptr_t>(a.cu_seqlens) % 4 != 0) return GDN_ERR_ALIGN;
+    return GDN_OK;
+}
+
+// How the sequences are cut: `seg` tokens to a segment.
+struct Cut {
+    int seg, nseg, slots;
+    bool several;  // a sequence may have more than one segment: their states come first
+};
+
+// Workgroups that a launch should have: the walk runs two to a compute unit (one where the keys number more than 128).
+Cut cut_sequences(const gdn_linear_attn_args& a, int64_t slices, int64_t wanted, int shortest) {
+    const bool packed = a.cu_seqlens != nullptr && !(a.flags & GDN_FLAG_LEFT_PADDED);
+    const int64_t tokens = (int64_t)a.B * a.T, work = a.H * slices;
+    int64_t seg = (tokens * work + wanted - 1) / wanted;
+    seg = std::max<int64_t>((seg + 63) / 64 * 64, shortest);
+    Cut c;
+    if (seg >= a.T) {
+        c.seg = (a.T + 63) / 64 * 64, c.nseg = packed ? 0 : 1, c.slots = a.N, c.several = false;
+        return c;
+    }
+    if (packed) {
+        c.seg = (int)seg, c.nseg = 0, c.slots = a.T / c.seg + a.N;
+    } else {
+        const int64_t n = (a.T + seg - 1) / seg;
+        c.seg = (int)(((a.T + n - 1) / n + 63) / 64 * 64);
+        c.nseg = (a.T + c.seg - 1) / c.seg;
+        c.slots = a.N * c.nseg;
+    }
+    c.several = true;
+    return c;
+}
+
+int walk_columns(const gdn_linear_attn_args& a, int V) {
+    return a.dtype == GDN_BF16 ? linear_walk_columns(V) : 32;
+}
+
+Cut cut_for_walk(const gdn_linear_attn_args& a, int K, int V) {
+    const int columns = walk_columns(a, V), cus = compute_units();
+    const int64_t slices = (V + columns - 1) / columns;
+    if (a.dtype == GDN_BF16) return cut_sequences(a, slices, K <= 128 ? 2 * cus : cus, 128);
+    return cut_sequences(a, slices, 4 * cus, 64);
+}
+
+uint64_t local_bytes(const gdn_linear_attn_args& a, const Cut& c) {
+    return c.several ? ((uint64_t)c.slots * a.H * a.K * a.V * 4 + 255) / 256 * 256 : 0;
+}
+
+// what every walk over these sequences has in common
+LinearParams base_params(const gdn_linear_attn_args& a, const Cut& c) {
+    LinearParams p{};
+    p.g = a.g;
+    p.cu = a.cu_seqlens;
+    p.padded = (a.flags & GDN_FLAG_LEFT_PADDED) != 0;
+    p.B = a.B, p.T = a.T, p.H = a.H, p.N = a.N;
+    p.cells = (int64_t)a.K * a.V;
+    p.seg = c.seg, p.nseg = c.nseg, p.slots = c.slots;
+    p.zero = (a.flags & GDN_FLAG_ZERO_PADDING) != 0;
+    return p;
+}
+
+int heads_shared(const gdn_linear_attn_args& a) { return a.qk_heads == 0 ? 1 : a.H / a.qk_heads; }
+
+struct Roles {
+    LinearRole q, k, v;
+};
+Roles roles_of(const gdn_linear_attn_args& a) {
+    const int div = heads_shared(a);
+    return {{a.q, a.q_stride_b, a.q_stride_t, a.q_stride_h, div},
+            {a.k, a.k_stride_b, a.k_stride_t, a.k_stride_h, div},
+            {a.v, a.v_stride_b, a.v_stride_t, a.v_stride_h, 1}};
+}
+
+// S [K, V] as it lies: keys are the first index
+void natural(LinearParams& p, int K, int V) { p.K = K, p.V = V, p.state_k = V, p.state_v = 1; }
+
+int run(const LinearParams& p, int dtype, bool states_only, hipStream_t stream) {
+    return dtype == GDN_BF16 ? launch_linear_walk(p, states_only, stream) : launch_linear_tokens(p, dtype, 32, states_only, stream);
+}
+
+// the states that the segments start from, into p.local: their own, then the sums
+int run_states(const LinearParams& p, int dtype, hipStream_t stream) {
+    if (const int e = run(p, dtype, true, stream); e != GDN_OK) return e;
+    return launch_linear_combine(p, stream);
+}
+
+const void* offset(const void* p, int64_t elements, int dtype) { return static_cast<const char*>(p) + elements * (dtype == GDN_BF16 ? 2 : 4); }
+
+constexpr int KEYS = 256;  // of a walk at most
+
+uint64_t sums_bytes(const gdn_linear_attn_args& a) {
+    return a.V > KEYS ? ((uint64_t)a.B * a.T * a.H * a.K * 4 + 255) / 256 * 256 : 0;
+}
+
+// dq or dk: a walk whose keys are the value dim, 256 of them at a time; p.x, p.y, p.z and the states are set for all of them
+int run_transposed(LinearParams p, const gdn_linear_attn_args& a, float* sums, hipStream_t stream) {
+    const LinearParams whole = p;
+    for (int first = 0; first < a.V; first += KEYS) {
+        p.K = std::min(KEYS, a.V - first), p.V = a.K;
+        p.state_k = 1, p.state_v = a.V;
+        p.x.p = offset(whole.x.p, first, a.dtype), p.y.p = offset(whole.y.p, first, a.dtype);
+        p.init = whole.init == nullptr ? nullptr : whole.init + first;
+        p.local = whole.local == nullptr ? nullptr : whole.local + first;
+        p.sums = a.V > KEYS ? sums : nullptr;
+        p.sums_in = first > 0, p.sums_out = first + KEYS < a.V;
+        if (const int e = run(p, a.dtype, false, stream); e != GDN_OK) return e;
+    }
+    return GDN_OK;
+}
+
+}  // namespace
+}  // namespace gdn
+
+using namespace gdn;
+
+extern "C" int gdn_linear_abi_version(void) { return GDN_LINEAR_ABI_VERSION; }
+
+extern "C" uint64_t gdn_linear_attn_workspace_bytes(const gdn_linear_attn_args* a) {
+    if (a == nullptr || check_shape(*a) != GDN_OK) return 0;
+    return local_bytes(*a, cut_for_walk(*a, a->K, a->V));
+}
+
+extern "C" int gdn_linear_attn_chunk_fwd(const gdn_linear_attn_args* args, void* stream) {
+    if (args == nullptr) return GDN_ERR_NULL;
+    const gdn_linear_attn_args& a = *args;
+    if (const int e = check_shape(a); e != GDN_OK) return e;
+    if (const int e = check_inputs(a); e != GDN_OK) return e;
+    if (const int e = check_rows(a.o, a.o_stride_b, a.o_stride_t, a.o_stride_h, a.dtype); e != GDN_OK) return e;
+    if (a.h0 != nullptr && a.ht == a.h0) return GDN_ERR_UNSUPPORTED;
+    const Cut c = cut_for_walk(a, a.K, a.V);
+    if (c.several && (a.workspace == nullptr || a.workspace_bytes < local_bytes(a, c))) return GDN_ERR_WORKSPACE;
+    if (c.several && !aligned16(a.workspace)) return GDN_ERR_ALIGN;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const Roles r = roles_of(a);
+    LinearParams p = base_params(a, c);
+    natural(p, a.K, a.V);
+    p.x = r.q, p.y = r.k, p.z = r.v;
+    p.out = a.o, p.out_stride_b = a.o_stride_b, p.out_stride_t = a.o_stride_t, p.out_stride_h = a.o_stride_h;
+    p.init = a.h0, p.fin = a.ht;
+    p.reverse = 0, p.a = 1, p.os = p.ps = a.scale, p.us = 1.f;
+    if (c.several) {
+        p.local = static_cast<float*>(a.workspace);
+        if (const int e = run_states(p, a.dtype, st); e != GDN_OK) return e;
+    }
+    return run(p, a.dtype, false, st);
+}
+
+extern "C" int gdn_linear_attn_recurrent_fwd(const gdn_linear_attn_args* args, void* stream) {
+    if (args == nullptr) return GDN_ERR_NULL;
+    const gdn_linear_attn_args& a = *args;
+    if (const int e = check_shape(a); e != GDN_OK) return e;
+    if (const int e = check_inputs(a); e != GDN_OK) return e;
+    if (const int e = check_rows(a.o, a.o_stride_b, a.o_stride_t, a.o_stride_h, a.dtype); e != GDN_OK) return e;
+    const Roles r = roles_of(a);
+    Cut c;
+    c.seg = (a.T + 63) / 64 * 64, c.nseg = a.cu_seqlens != nullptr && !(a.flags & GDN_FLAG_LEFT_PADDED) ? 0 : 1, c.slots = a.N, c.several = false;
+    LinearParams p = base_params(a, c);
+    natural(p, a.K, a.V);
+    p.x = r.q, p.y = r.k, p.z = r.v;
+    p.out = a.o, p.out_stride_b = a.o_stride_b, p.out_stride_t = a.o_stride_t, p.out_stride_h = a.o_stride_h;
+    p.init = a.h0, p.fin = a.ht;
+    p.reverse = 0, p.a = 1, p.os = p.ps = a.scale, p.us = 1.f;
+    return launch_linear_tokens(p, a.dtype, linear_tokens_columns((int64_t)a.N * a.H, a.V, compute_units()), false, static_cast<hipStream_t>(stream));
+}
+
+extern "C" uint64_t gdn_linear_attn_bwd_workspace_bytes(const gdn_linear_attn_bwd_args* b) {
+    if (b == nullptr || check_shape(b->fwd) != GDN_OK) return 0;
+    const gdn_linear_attn_args& a = b->fwd;
+    return 2 * local_bytes(a, cut_for_walk(a, a.K, a.V)) + sums_bytes(a);
+}
+
+extern "C" int gdn_linear_attn_bwd(const gdn_linear_attn_bwd_args* args, void* stream) {
+    if (args == nullptr) return GDN_ERR_NULL;
+    const gdn_linear_attn_bwd_args& b = *args;
+    const gdn_linear_attn_args& a = b.fwd;
+    if (const int e = check_shape(a); e != GDN_OK) return e;
+    if (const int e = check_inputs(a); e != GDN_OK) return e;
+    if (const int e = check_rows(b.dout, b.dout_stride_b, b.dout_stride_t, b.dout_stride_h, a.dtype); e != GDN_OK) return e;
+    if (b.dq != nullptr)
+        if (const int e = check_rows(b.dq, b.dq_stride_b, b.dq_stride_t, b.dq_stride_h, a.dtype); e != GDN_OK) return e;
+    if (b.dk != nullptr)
+        if (const int e = check_rows(b.dk, b.dk_stride_b, b.dk_stride_t, b.dk_stride_h, a.dtype); e != GDN_OK) return e;
+    if (const int e = check_rows(b.dv, b.dv_stride_b, b.dv_stride_t, b.dv_stride_h, a.dtype); e != GDN_OK) return e;
+    if (!aligned16(b.dht) || !aligned16(b.dh0)) return GDN_ERR_ALIGN;
+    if (b.dg != nullptr) return GDN_ERR_UNSUPPORTED;
+    const Cut c = cut_for_walk(a, a.K, a.V);
+    const uint64_t local = local_bytes(a, c), sums = sums_bytes(a);
+    if (2 * local + sums > 0) {
+        if (b.workspace == nullptr || b.workspace_bytes < 2 * local + sums) return GDN_ERR_WORKSPACE;
+        if (!aligned16(b.workspace)) return GDN_ERR_ALIGN;
+    }
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const Roles r = roles_of(a);
+    const LinearRole d = {b.dout, b.dout_stride_b, b.dout_stride_t, b.dout_stride_h, 1};
+    char* const ws = static_cast<char*>(b.workspace);
+    float* const sums_at = reinterpret_cast<float*>(ws + 2 * local);
+
+    LinearParams s = base_params(a, c);  // of the forward's states
+    natural(s, a.K, a.V);
+    s.x = r.q, s.y = r.k, s.z = r.v;
+    s.init = a.h0;
+    s.reverse = 0, s.a = 1, s.os = s.ps = a.scale, s.us = 1.f;
+    LinearParams t = s;  // of their gradients
+    t.x = r.k, t.y = r.q, t.z = d;
+    t.init = b.dht;
+    t.reverse = 1, t.a = 0, t.os = 1.f, t.ps = t.us = a.scale;
+    if (c.several) {
+        s.local = reinterpret_cast<float*>(ws), t.local = reinterpret_cast<float*>(ws + local);
+        if (b.dq != nullptr)
+            if (const int e = run_states(s, a.dtype, st); e != GDN_OK) return e;
+        if (const int e = run_states(t, a.dtype, st); e != GDN_OK) return e;
+    }
+    t.out = b.dv, t.out_stride_b = b.dv_stride_b, t.out_stride_t = b.dv_stride_t, t.out_stride_h = b.dv_stride_h;
+    t.fin = b.dh0;
+    if (const int e = run(t, a.dtype, false, st); e != GDN_OK) return e;
+    if (b.dk != nullptr) {
+        LinearParams k = t;
+        k.x = r.v, k.y = d, k.z = r.q;
+        k.out = b.dk, k.out_stride_b = b.dk_stride_b, k.out_stride_t = b.dk_stride_t, k.out_stride_h = b.dk_stride_h;
+        k.fin = nullptr;
+        if (const int e = run_transposed(k, a, sums_at, st); e != GDN_OK) return e;
+    }
+    if (b.dq != nullptr) {
+        LinearParams q = s;
+        q.x = d, q.y = r.v, q.z = r.k;
+        q.out = b.dq, q.out_stride_b = b.dq_stride_b, q.out_stride_t = b.dq_stride_t, q.out_stride_h = b.dq_stride_h;
+        q.fin = nullptr;
+        return run_transposed(q, a, sums_at, st);
+    }
+    return GDN_OK;
+}

@@ -1,0 +1,181 @@
+// Linear attention with a decay for each head, token by token in fp32: decoding (one token, or a few, per state) and the exact path
+// of fp32 inputs.  The recurrence and its roles: gdn_linear_common.h.
+//
+// A workgroup has 4 VL columns of the value dim and all keys of one (segment, head).  A thread has 4 columns and KR keys, GROUPS
+// apart, in registers: on a single token it reads and writes 16-byte pieces, 16 VL bytes of a state row at a time, and the state
+// passes through it once.  Tokens are taken 16 at a time through LDS; per token a lane adds up its keys, the lanes of a wave their
+// groups by shuffles, and the four waves' sums meet in LDS behind the 16.
+#include <algorithm>
+
+#include "gdn_launch.h"
+#include "gdn_linear_common.h"
+
+namespace gdn {
+
+namespace {
+
+constexpr int TB = 16;  // tokens of a batch
+
+template <typename T, int KR, int VL, bool STATES_ONLY>
+__global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p) {
+    constexpr int GROUPS = 256 / VL, KP = GROUPS * KR, VC = 4 * VL;
+    __shared__ __align__(16) float sx[STATES_ONLY ? 1 : TB][KP];
+    __shared__ __align__(16) float sy[TB][KP];
+    __shared__ __align__(16) float sz[TB][VC];
+    __shared__ __align__(16) float part[STATES_ONLY ? 1 : 4][TB][VC];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const unsigned per_xcd = (gridDim.x + 7) / 8;  // as in linear_walk_kernel
+    const unsigned id = blockIdx.x % 8 * per_xcd + blockIdx.x / 8;
+    const int slices = (p.V + VC - 1) / VC;
+    if (id >= (unsigned)p.slots * p.H * slices) return;
+    const int slice = id % slices, h = id / slices % p.H, slot = id / slices / p.H;
+    const int c0 = slice * VC, columns = min(VC, p.V - c0);
+    if constexpr (!STATES_ONLY)
+        if (p.zero && p.cu != nullptr) linear_zero_gaps<T, 16 / sizeof(T)>(p, slot, h, c0, columns, tid, 256);
+    LinearSegment sg;
+    if (!linear_find(p, slot, sg, lane)) return;
+    const bool last = sg.s == linear_segments(sg.len, p.seg) - 1;
+    if (STATES_ONLY && last) return;
+    const int walked = sg.s * p.seg, total = min(p.seg, sg.len - walked);
+    const int64_t token = p.reverse ? (int64_t)sg.t0 + sg.len - 1 - walked : (int64_t)sg.t0 + walked;
+    const float w = p.g == nullptr ? 1.f : expf(p.g[h]);
+
+    const int vl = lane % VL, group = wave * (64 / VL) + lane / VL;
+    const int col = 4 * vl;
+    const bool mine = col < columns;
+    const int64_t chain = (int64_t)sg.n * p.H + h, cells = p.cells;
+    auto key = [&](int r) { return r * GROUPS + group; };
+    auto state_at = [&](int r) { return (int64_t)key(r) * p.state_k + (int64_t)(c0 + col) * p.state_v; };
+    f32x4 S[KR];
+#pragma unroll
+    for (int r = 0; r < KR; r++) S[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float* from = nullptr;
+    if (!STATES_ONLY) from = sg.s > 0 ? p.local + ((int64_t)slot * p.H + h) * cells : p.init == nullptr ? nullptr : p.init + chain * cells;
+    if (from != nullptr && mine) {
+        if (p.state_v == 1) {
+#pragma unroll
+            for (int r = 0; r < KR; r++)
+                if (key(r) < p.K) S[r] = *reinterpret_cast<const f32x4*>(from + state_at(r));
+        } else {
+            for (int r = 0; r < KR; r++)
+                for (int e = 0; e < 4; e++)
+                    if (key(r) < p.K) S[r][e] = from[state_at(r) + (int64_t)e * p.state_v];
+        }
+    }
+
+    const int64_t step = p.reverse ? -1 : 1;
+    auto role = [&](const LinearRole& x) { return static_cast<const T*>(x.p) + sg.b * x.stride_b + (h / x.div) * x.stride_h + token * x.stride_t; };
+    const T* const px = role(STATES_ONLY ? p.y : p.x);
+    const T* const py = role(p.y);
+    const T* const pz = role(p.z);
+    T* const out = static_cast<T*>(p.out) + sg.b * p.out_stride_b + h * p.out_stride_h + token * p.out_stride_t;
+    float* const sums = p.sums == nullptr ? nullptr : p.sums + ((int64_t)sg.b * p.T + token) * p.H * p.V + (int64_t)h * p.V;
+
+    for (int first = 0; first < total; first += TB) {
+        const int n = min(TB, total - first);
+        if (first > 0) __syncthreads();
+        for (int i = tid; i < n * (KP / 4); i += 256) {
+            const int t = i / (KP / 4), k = (i - t * (KP / 4)) * 4;
+            f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+            if (k < p.K) {
+                y = load4<T>(py + (first + t) * step * p.y.stride_t + k);
+                if constexpr (!STATES_ONLY) x = load4<T>(px + (first + t) * step * p.x.stride_t + k);
+            }
+            *reinterpret_cast<f32x4*>(&sy[t][k]) = y * p.us;
+            if constexpr (!STATES_ONLY) *reinterpret_cast<f32x4*>(&sx[t][k]) = x;
+        }
+        for (int i = tid; i < n * VL; i += 256) {
+            const int t = i / VL, c = (i - t * VL) * 4;
+            f32x4 z = {0.f, 0.f, 0.f, 0.f};
+            if (c < columns) z = load4<T>(pz + (first + t) * step * p.z.stride_t + c0 + c);
+            *reinterpret_cast<f32x4*>(&sz[t][c]) = z;
+        }
+        __syncthreads();
+        for (int t = 0; t < n; t++) {
+            const float factor = p.a == 1 || first + t > 0 ? w : 1.f;  // a = 0: the state decays behind a token, not in front of it
+            const f32x4 z = *reinterpret_cast<const f32x4*>(&sz[t][col]);
+            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int r = 0; r < KR; r++) {
+                S[r] = S[r] * factor + z * sy[t][key(r)];
+                if constexpr (!STATES_ONLY) o += S[r] * sx[t][key(r)];
+            }
+            if constexpr (!STATES_ONLY) {
+#pragma unroll
+                for (int off = VL; off < 64; off <<= 1)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[e] += __shfl_xor(o[e], off, WAVE);
+                if (lane < VL) *reinterpret_cast<f32x4*>(&part[wave][t][col]) = o;
+            }
+        }
+        if constexpr (!STATES_ONLY) {
+            __syncthreads();
+            for (int i = tid; i < n * VL; i += 256) {
+                const int t = i / VL, c = (i - t * VL) * 4;
+                if (c >= columns) continue;
+                f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int v = 0; v < 4; v++) o += *reinterpret_cast<const f32x4*>(&part[v][t][c]);
+                o = o * p.os;
+                if (sums != nullptr) {
+                    f32x4* const at = reinterpret_cast<f32x4*>(sums + (first + t) * step * p.H * p.V + c0 + c);
+                    if (p.sums_in) o += *at;
+                    if (p.sums_out) {
+                        *at = o;
+                        continue;
+                    }
+                }
+                store4<T>(out + (first + t) * step * p.out_stride_t + c0 + c, o);
+            }
+        }
+    }
+    if (p.a == 0 && total > 0) {
+#pragma unroll
+        for (int r = 0; r < KR; r++) S[r] = S[r] * w;
+    }
+    float* to = nullptr;
+    if constexpr (STATES_ONLY) to = p.local + ((int64_t)slot * p.H + h) * cells;
+    else if (last && p.fin != nullptr) to = p.fin + chain * cells;
+    if (to != nullptr && mine) {
+#pragma unroll
+        for (int r = 0; r < KR; r++)
+            if (key(r) < p.K) {
+                if (p.state_v == 1) *reinterpret_cast<f32x4*>(to + state_at(r)) = S[r];
+                else
+                    for (int e = 0; e < 4; e++) to[state_at(r) + (int64_t)e * p.state_v] = S[r][e];
+            }
+    }
+}
+
+template <typename T, int KR, int VL>
+int launch(const LinearParams& p, bool states_only, hipStream_t stream) {
+    const int64_t blocks = (int64_t)p.slots * p.H * ((p.V + 4 * VL - 1) / (4 * VL));
+    if (blocks > 0xfffff000ll / 256) return GDN_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)((blocks + 7) / 8 * 8)), threads(256);
+    if (states_only) hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, true>), grid, threads, 0, stream, p);
+    else hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, false>), grid, threads, 0, stream, p);
+    return (int)hipGetLastError();
+}
+
+template <typename T>
+int launch_of(const LinearParams& p, int columns, bool states_only, hipStream_t stream) {
+    if (columns == 32) {
+        if (p.K <= 64) return launch<T, 2, 8>(p, states_only, stream);
+        if (p.K <= 128) return launch<T, 4, 8>(p, states_only, stream);
+        return launch<T, 8, 8>(p, states_only, stream);
+    }
+    if (p.K <= 64) return launch<T, 8, 32>(p, states_only, stream);
+    if (p.K <= 128) return launch<T, 16, 32>(p, states_only, stream);
+    return launch<T, 32, 32>(p, states_only, stream);
+}
+
+}  // namespace
+
+int linear_tokens_columns(int64_t chains, int V, int cus) { return V >= 128 && chains * ((V + 127) / 128) >= cus ? 128 : 32; }
+
+int launch_linear_tokens(const LinearParams& p, int dtype, int columns, bool states_only, hipStream_t stream) {
+    return dtype == GDN_BF16 ? launch_of<bf16_t>(p, columns, states_only, stream) : launch_of<float>(p, columns, states_only, stream);
+}
+
+}  // namespace gdn

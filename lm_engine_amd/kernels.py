@@ -16,6 +16,9 @@ fixed-length batches whose scan fills about half of the GPU).  Results stay with
 they are not bit-identical to the two-kernel path, which every other batch takes (packed, left-padded, few or
 many sequences): switch it off - ``enable_kernels([Kernel.gated_delta_rule], reset=True)`` or
 ``ENABLE_KERNELS=gated_delta_rule`` - where runs of different batch shapes are compared bit for bit.
+
+``Kernel.linear_attention`` and ``Kernel.layer_norm`` stand for the operators of those names, on by default and without a
+second implementation as well.
 """
 
 from __future__ import annotations
@@ -28,9 +31,11 @@ from enum import Enum
 class Kernel(Enum):
     gated_delta_rule = "gated_delta_rule"
     gated_delta_rule_fused_launch = "gated_delta_rule_fused_launch"
+    linear_attention = "linear_attention"
+    layer_norm = "layer_norm"
 
 
-_ON_BY_DEFAULT = (Kernel.gated_delta_rule, Kernel.gated_delta_rule_fused_launch)
+_ON_BY_DEFAULT = tuple(Kernel)
 _KERNELS: dict[Kernel, bool] = {kernel: kernel in _ON_BY_DEFAULT for kernel in Kernel}
 
 
