@@ -136,6 +136,20 @@ uint64_t sums_bytes(const gdn_linear_attn_args& a) {
     return a.V > KEYS ? ((uint64_t)a.B * a.T * a.H * a.K * 4 + 255) / 256 * 256 : 0;
 }
 
+uint64_t dots_bytes(const gdn_linear_attn_args& a, const Cut& c) {
+    const int columns = linear_tangent_columns(a.dtype, a.V);
+    return ((uint64_t)c.slots * ((a.V + columns - 1) / columns) * a.H * 4 + 255) / 256 * 256;
+}
+
+// The backward's workspace: states that the segments start from (the forward's, their gradients, with dg the derivatives), partial
+// outputs, the parts of dg.
+struct BackwardSpace {
+    uint64_t local, slope, sums, dots;
+    BackwardSpace(const gdn_linear_attn_args& a, const Cut& c, bool dg)
+        : local(local_bytes(a, c)), slope(dg ? local : 0), sums(sums_bytes(a)), dots(dg ? dots_bytes(a, c) : 0) {}
+    uint64_t total() const { return 2 * local + slope + sums + dots; }
+};
+
 // dq or dk: a walk whose keys are the value dim, 256 of them at a time; p.x, p.y, p.z and the states are set for all of them
 int run_transposed(LinearParams p, const gdn_linear_attn_args& a, float* sums, hipStream_t stream) {
     const LinearParams whole = p;
@@ -210,7 +224,7 @@ extern "C" int gdn_linear_attn_recurrent_fwd(const gdn_linear_attn_args* args, v
 extern "C" uint64_t gdn_linear_attn_bwd_workspace_bytes(const gdn_linear_attn_bwd_args* b) {
     if (b == nullptr || check_shape(b->fwd) != GDN_OK) return 0;
     const gdn_linear_attn_args& a = b->fwd;
-    return 2 * local_bytes(a, cut_for_walk(a, a.K, a.V)) + sums_bytes(a);
+    return BackwardSpace(a, cut_for_walk(a, a.K, a.V), b->dg != nullptr).total();
 }
 
 extern "C" int gdn_linear_attn_bwd(const gdn_linear_attn_bwd_args* args, void* stream) {
@@ -220,24 +234,22 @@ extern "C" int gdn_linear_attn_bwd(const gdn_linear_attn_bwd_args* args, void* s
     if (const int e = check_shape(a); e != GDN_OK) return e;
     if (const int e = check_inputs(a); e != GDN_OK) return e;
     if (const int e = check_rows(b.dout, b.dout_stride_b, b.dout_stride_t, b.dout_stride_h, a.dtype); e != GDN_OK) return e;
-    if (b.dq != nullptr)
-        if (const int e = check_rows(b.dq, b.dq_stride_b, b.dq_stride_t, b.dq_stride_h, a.dtype); e != GDN_OK) return e;
-    if (b.dk != nullptr)
-        if (const int e = check_rows(b.dk, b.dk_stride_b, b.dk_stride_t, b.dk_stride_h, a.dtype); e != GDN_OK) return e;
+    if (const int e = check_rows(b.dq, b.dq_stride_b, b.dq_stride_t, b.dq_stride_h, a.dtype); e != GDN_OK) return e;
+    if (const int e = check_rows(b.dk, b.dk_stride_b, b.dk_stride_t, b.dk_stride_h, a.dtype); e != GDN_OK) return e;
     if (const int e = check_rows(b.dv, b.dv_stride_b, b.dv_stride_t, b.dv_stride_h, a.dtype); e != GDN_OK) return e;
     if (!aligned16(b.dht) || !aligned16(b.dh0)) return GDN_ERR_ALIGN;
-    if (b.dg != nullptr) return GDN_ERR_UNSUPPORTED;
+    if (b.dg != nullptr && a.g == nullptr) return GDN_ERR_NULL;
     const Cut c = cut_for_walk(a, a.K, a.V);
-    const uint64_t local = local_bytes(a, c), sums = sums_bytes(a);
-    if (2 * local + sums > 0) {
-        if (b.workspace == nullptr || b.workspace_bytes < 2 * local + sums) return GDN_ERR_WORKSPACE;
+    const BackwardSpace space(a, c, b.dg != nullptr);
+    if (space.total() > 0) {
+        if (b.workspace == nullptr || b.workspace_bytes < space.total()) return GDN_ERR_WORKSPACE;
         if (!aligned16(b.workspace)) return GDN_ERR_ALIGN;
     }
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const Roles r = roles_of(a);
     const LinearRole d = {b.dout, b.dout_stride_b, b.dout_stride_t, b.dout_stride_h, 1};
     char* const ws = static_cast<char*>(b.workspace);
-    float* const sums_at = reinterpret_cast<float*>(ws + 2 * local);
+    float* const sums_at = reinterpret_cast<float*>(ws + 2 * space.local + space.slope);
 
     LinearParams s = base_params(a, c);  // of the forward's states
     natural(s, a.K, a.V);
@@ -249,27 +261,29 @@ extern "C" int gdn_linear_attn_bwd(const gdn_linear_attn_bwd_args* args, void* s
     t.init = b.dht;
     t.reverse = 1, t.a = 0, t.os = 1.f, t.ps = t.us = a.scale;
     if (c.several) {
-        s.local = reinterpret_cast<float*>(ws), t.local = reinterpret_cast<float*>(ws + local);
-        if (b.dq != nullptr)
+        s.local = reinterpret_cast<float*>(ws), t.local = reinterpret_cast<float*>(ws + space.local);
+        if (b.dg == nullptr)
             if (const int e = run_states(s, a.dtype, st); e != GDN_OK) return e;
         if (const int e = run_states(t, a.dtype, st); e != GDN_OK) return e;
+    }
+    if (b.dg != nullptr) {  // (which leaves the states that the segments start from as well)
+        LinearParams u = s;
+        u.d = d, u.init_grad = b.dht;
+        u.local_slope = reinterpret_cast<float*>(ws + 2 * space.local);
+        u.dots = reinterpret_cast<float*>(ws + 2 * space.local + space.slope + space.sums);
+        if (const int e = launch_linear_tangent(u, a.dtype, c.several, b.dg, st); e != GDN_OK) return e;
     }
     t.out = b.dv, t.out_stride_b = b.dv_stride_b, t.out_stride_t = b.dv_stride_t, t.out_stride_h = b.dv_stride_h;
     t.fin = b.dh0;
     if (const int e = run(t, a.dtype, false, st); e != GDN_OK) return e;
-    if (b.dk != nullptr) {
-        LinearParams k = t;
-        k.x = r.v, k.y = d, k.z = r.q;
-        k.out = b.dk, k.out_stride_b = b.dk_stride_b, k.out_stride_t = b.dk_stride_t, k.out_stride_h = b.dk_stride_h;
-        k.fin = nullptr;
-        if (const int e = run_transposed(k, a, sums_at, st); e != GDN_OK) return e;
-    }
-    if (b.dq != nullptr) {
-        LinearParams q = s;
-        q.x = d, q.y = r.v, q.z = r.k;
-        q.out = b.dq, q.out_stride_b = b.dq_stride_b, q.out_stride_t = b.dq_stride_t, q.out_stride_h = b.dq_stride_h;
-        q.fin = nullptr;
-        return run_transposed(q, a, sums_at, st);
-    }
-    return GDN_OK;
+    LinearParams k = t;
+    k.x = r.v, k.y = d, k.z = r.q;
+    k.out = b.dk, k.out_stride_b = b.dk_stride_b, k.out_stride_t = b.dk_stride_t, k.out_stride_h = b.dk_stride_h;
+    k.fin = nullptr;
+    if (const int e = run_transposed(k, a, sums_at, st); e != GDN_OK) return e;
+    LinearParams q = s;
+    q.x = d, q.y = r.v, q.z = r.k;
+    q.out = b.dq, q.out_stride_b = b.dq_stride_b, q.out_stride_t = b.dq_stride_t, q.out_stride_h = b.dq_stride_h;
+    q.fin = nullptr;
+    return run_transposed(q, a, sums_at, st);
 }

@@ -43,6 +43,11 @@ struct LinearParams {
     int zero;             // zeros at tokens of no sequence
     float* sums;          // fp32 [B, T, H, V] contiguous or NULL: partial outputs of a key dim that is walked in pieces
     int sums_in, sums_out;  // add what is there; leave the result there instead of rounding it to out
+    // the derivative with respect to the log-decay (gdn_linear_tangent.hip)
+    LinearRole d;            // gradient of the output
+    const float* init_grad;  // of the final state, or NULL
+    float* local_slope;      // as local, of the state's derivative
+    float* dots;             // [slots * slices, H]
 };
 
 // Segment `s` (in walk order) of sequence n: row b, first token t0, sequence length.
@@ -155,5 +160,8 @@ int launch_linear_tokens(const LinearParams& p, int dtype, int columns, bool sta
 int linear_walk_columns(int V);    // columns of the value dim that a workgroup of the bf16 walk has
 int linear_tokens_columns(int64_t chains, int V, int cus);  // of the token kernel
 int launch_linear_combine(const LinearParams& p, hipStream_t stream);
+// gdn_linear_tangent.hip: p.dots, and dg [H] from them; with several segments their states first, p.local and p.local_slope
+int launch_linear_tangent(const LinearParams& p, int dtype, bool several, float* dg, hipStream_t stream);
+int linear_tangent_columns(int dtype, int V);
 
 }  // namespace gdn

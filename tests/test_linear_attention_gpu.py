@@ -122,7 +122,7 @@ def _gradients(inputs, dtype, form="chunk", learned=False, cu=None, padded=False
     ref = {n: x.double().requires_grad_(n in names) if isinstance(x, torch.Tensor) else x for n, x in inputs.items()}
     o, state = linear_attention_ref(**ref, cu_seqlens=cu, left_padded=padded, **kwargs)
     do, dht = torch.randn(o.shape, generator=gen).to(dtype), 0.1 * torch.randn(state.shape, generator=gen)
-    o = o + 0 * sum(ref[n].sum() for n in ("q", "k", "v"))  # (sequences without a token leave nothing to differentiate)
+    o = o + 0 * sum(ref[n].sum() for n in names)  # (sequences without a token leave nothing to differentiate)
     want = torch.autograd.grad((o, state), [ref[n] for n in names], (do.double(), dht.double()))
     own = _cuda(inputs)
     for n in names:
@@ -159,4 +159,19 @@ def test_backward_of_packed_and_padded_batches(lens, padded, T, dtype):
         outside[b, first : first + length] = False
     for n in ("q", "k", "v"):
         assert (got[n].cpu()[outside] == 0).all(), n
+    _check_gradients(got, want, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=_ID)
+@pytest.mark.parametrize("B, T, H, K, V, options", [s for s in SHAPES if s[5].get("decay") not in ("none", "at once")], ids=_ID)
+def test_gradient_of_the_decay(B, T, H, K, V, options, dtype):
+    got, want = _gradients(_inputs(B, T, H, K, V, dtype=dtype, **options), dtype, learned=True)
+    _check_gradients(got, want, dtype, shared="HK" in options)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=_ID)
+@pytest.mark.parametrize("lens, padded, T", LAYOUTS, ids=_ID)
+def test_gradient_of_the_decay_of_packed_and_padded_batches(lens, padded, T, dtype):
+    B = len(lens) if padded else 1
+    got, want = _gradients(_inputs(B, T, 3, 64, 96, N=len(lens), dtype=dtype), dtype, learned=True, cu=_cu(lens), padded=padded)
     _check_gradients(got, want, dtype)
