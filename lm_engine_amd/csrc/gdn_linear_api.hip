@@ -75,12 +75,12 @@ Cut cut_sequences(const gdn_linear_attn_args& a, int64_t slices, int64_t wanted,
     return c;
 }
 
-int walk_columns(const gdn_linear_attn_args& a, int V) {
-    return a.dtype == GDN_BF16 ? linear_walk_columns(V) : 32;
+int walk_columns(const gdn_linear_attn_args& a, int K, int V) {
+    return a.dtype == GDN_BF16 ? linear_walk_columns(K, V) : 32;
 }
 
 Cut cut_for_walk(const gdn_linear_attn_args& a, int K, int V) {
-    const int columns = walk_columns(a, V), cus = compute_units();
+    const int columns = walk_columns(a, K, V), cus = compute_units();
     const int64_t slices = (V + columns - 1) / columns;
     if (a.dtype == GDN_BF16) return cut_sequences(a, slices, K <= 128 ? 2 * cus : cus, 128);
     return cut_sequences(a, slices, 4 * cus, 64);
@@ -122,7 +122,7 @@ int run(const LinearParams& p, int dtype, bool states_only, hipStream_t stream) 
     return dtype == GDN_BF16 ? launch_linear_walk(p, states_only, stream) : launch_linear_tokens(p, dtype, 32, states_only, stream);
 }
 
-// the states that the segments start from, into p.local: their own, then the sums
+// the states that the segments start from, into p.local: their own, then the sums, and p.fin
 int run_states(const LinearParams& p, int dtype, hipStream_t stream) {
     if (const int e = run(p, dtype, true, stream); e != GDN_OK) return e;
     return launch_linear_combine(p, stream);
@@ -199,6 +199,7 @@ extern "C" int gdn_linear_attn_chunk_fwd(const gdn_linear_attn_args* args, void*
     if (c.several) {
         p.local = static_cast<float*>(a.workspace);
         if (const int e = run_states(p, a.dtype, st); e != GDN_OK) return e;
+        p.fin = nullptr;
     }
     return run(p, a.dtype, false, st);
 }
@@ -264,6 +265,7 @@ extern "C" int gdn_linear_attn_bwd(const gdn_linear_attn_bwd_args* args, void* s
         s.local = reinterpret_cast<float*>(ws), t.local = reinterpret_cast<float*>(ws + space.local);
         if (b.dg == nullptr)
             if (const int e = run_states(s, a.dtype, st); e != GDN_OK) return e;
+        t.fin = b.dh0;
         if (const int e = run_states(t, a.dtype, st); e != GDN_OK) return e;
     }
     if (b.dg != nullptr) {  // (which leaves the states that the segments start from as well)
@@ -274,7 +276,7 @@ extern "C" int gdn_linear_attn_bwd(const gdn_linear_attn_bwd_args* args, void* s
         if (const int e = launch_linear_tangent(u, a.dtype, c.several, b.dg, st); e != GDN_OK) return e;
     }
     t.out = b.dv, t.out_stride_b = b.dv_stride_b, t.out_stride_t = b.dv_stride_t, t.out_stride_h = b.dv_stride_h;
-    t.fin = b.dh0;
+    t.fin = c.several ? nullptr : b.dh0;
     if (const int e = run(t, a.dtype, false, st); e != GDN_OK) return e;
     LinearParams k = t;
     k.x = r.v, k.y = d, k.z = r.q;

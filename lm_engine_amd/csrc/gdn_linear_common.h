@@ -28,7 +28,7 @@ struct LinearParams {
     int64_t out_stride_b, out_stride_t, out_stride_h;
     const float* g;       // [H] or NULL
     const float* init;    // [N, H] states or NULL: what the walk starts from
-    float* fin;           // [N, H] states or NULL: what it ends with
+    float* fin;           // [N, H] states or NULL: what it ends with (several segments: for the states' launches, not for the walk)
     float* local;         // [slots, H] states: of a segment's own tokens, then (linear_combine_kernel) what the segment starts from
     int state_k, state_v;  // element (key k, value v) of a state is at k * state_k + v * state_v
     int64_t cells;         // of a state
@@ -52,7 +52,7 @@ struct LinearParams {
 
 // Segment `s` (in walk order) of sequence n: row b, first token t0, sequence length.
 struct LinearSegment {
-    int n, s, b, t0, len;
+    int n = 0, s = 0, b = 0, t0 = 0, len = 0;
 };
 
 __device__ __forceinline__ int linear_segments(int len, int seg) { return max(1, (len + seg - 1) / seg); }
@@ -104,8 +104,14 @@ __device__ __forceinline__ bool linear_find_packed(const LinearParams& p, int sl
     return false;
 }
 
+// (the same in all lanes, and said so: addresses built on it stay in scalar registers)
 __device__ __forceinline__ bool linear_find(const LinearParams& p, int slot, LinearSegment& out, int lane) {
-    if (p.nseg == 0) return linear_find_packed(p, slot, out, lane);
+    if (p.nseg == 0) {
+        const bool found = linear_find_packed(p, slot, out, lane);
+        out.n = __builtin_amdgcn_readfirstlane(out.n), out.s = __builtin_amdgcn_readfirstlane(out.s), out.b = 0;
+        out.t0 = __builtin_amdgcn_readfirstlane(out.t0), out.len = __builtin_amdgcn_readfirstlane(out.len);
+        return found;
+    }
     out.n = slot / p.nseg;
     out.s = slot - out.n * p.nseg;
     if (out.n >= p.N) return false;
@@ -157,7 +163,7 @@ __device__ __forceinline__ float linear_power(float g, int n) { return n == 0 ? 
 // launches, gdn_linear_walk.hip and gdn_linear_tokens.hip; `states_only`: the segments' own states into p.local
 int launch_linear_walk(const LinearParams& p, bool states_only, hipStream_t stream);
 int launch_linear_tokens(const LinearParams& p, int dtype, int columns, bool states_only, hipStream_t stream);
-int linear_walk_columns(int V);    // columns of the value dim that a workgroup of the bf16 walk has
+int linear_walk_columns(int K, int V);  // columns of the value dim that a workgroup of the bf16 walk has
 int linear_tokens_columns(int64_t chains, int V, int cus);  // of the token kernel
 int launch_linear_combine(const LinearParams& p, hipStream_t stream);
 // gdn_linear_tangent.hip: p.dots, and dg [H] from them; with several segments their states first, p.local and p.local_slope

@@ -107,8 +107,9 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : 1) void linear_tangen
     const int chunks = (total + LC - 1) / LC;
     for (int c = 0; c < chunks; c++) {
         const int rows = min(LC, total - c * LC);
-        ks.load(rows), vs.load(rows);
-        if constexpr (!STATES_ONLY) qs.load(rows), ds.load(rows);
+        bf16x8 rk[Stream<KD, NT>::ITERS], rv[Stream<VC, NT>::ITERS], rq[STATES_ONLY ? 1 : Stream<KD, NT>::ITERS], rd[STATES_ONLY ? 1 : Stream<VC, NT>::ITERS];
+        ks.fetch(rk, rows), vs.fetch(rv, rows);
+        if constexpr (!STATES_ONLY) qs.fetch(rq, rows), ds.fetch(rd, rows);
         __syncthreads();  // the tiles of the chunk before are read
         if (tid < LC) {
             const int left = max(rows - 1 - tid, 0);
@@ -119,8 +120,8 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : 1) void linear_tangen
                 sw[2][tid] = forward, sw[3][tid] = (float)(tid + 1) * forward;
             }
         }
-        ks.store(sk), vs.store(sv);
-        if constexpr (!STATES_ONLY) qs.store(sq), ds.store(sd);
+        ks.stage(sk, rk, rows), vs.stage(sv, rv, rows);
+        if constexpr (!STATES_ONLY) qs.stage(sq, rq, rows), ds.stage(sd, rd, rows);
         __syncthreads();
         bf16x8 hi[4], lo[4];
         if constexpr (!STATES_ONLY) {

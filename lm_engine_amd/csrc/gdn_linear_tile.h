@@ -36,39 +36,87 @@ __device__ __forceinline__ bf16x8 tile_tr8(const bf16_t* m, int row0, int col0, 
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// A thread's share of the rows of one role: granules of 8 columns, ITERS rows apart by STEP.
+// Where a lane of v_mfma_f32_32x32x16_bf16 reads a tile of LD columns.  The key of a row is that of the row 16 further on, and a step
+// of 64 columns changes no bit that the key touches; within 64 columns a step is one of bits that are exclusive-ored anyway.  So three
+// offsets do for a whole tile.
+template <int LD>
+struct TileLane {
+    int row, swapped, pair;
+
+    __device__ __forceinline__ TileLane(int lane) {
+        const int l32 = lane & 31, half = lane >> 5, q = lane & 3;
+        row = l32 * LD + ((half ^ tile_key(l32)) << 3);
+        swapped = slice_col(l32) * LD + ((half ^ tile_key(slice_col(l32))) << 3);
+        const int r = 8 * half + ((lane & 15) >> 2), c = 16 * ((lane >> 4) & 1) + 4 * (((q & 1) << 1) | (q >> 1));
+        pair = r * LD + (((c >> 3) ^ tile_key(r)) << 3) + (c & 7);
+    }
+    // x where it is used, rather than what follows from x in registers over a whole walk
+    __device__ __forceinline__ void recompute() { asm volatile("" : "+v"(row), "+v"(swapped), "+v"(pair)); }
+    // 8 columns 16 s + 8 half .. of row row0 + l32; row0 a multiple of 32
+    __device__ __forceinline__ bf16x8 fragment(const bf16_t* tile, int row0, int s) const {
+        return *reinterpret_cast<const bf16x8*>(tile + (row ^ (16 * (s & 3))) + row0 * LD + (s >> 2) * 64);
+    }
+    // ... of row row0 + swap(l32)
+    __device__ __forceinline__ bf16x8 swapped_fragment(const bf16_t* tile, int row0, int s) const {
+        return *reinterpret_cast<const bf16x8*>(tile + (swapped ^ (16 * (s & 3))) + row0 * LD + (s >> 2) * 64);
+    }
+    // rows 16 s + 8 half .. + 7 of column 32 t + swap(l32)
+    __device__ __forceinline__ bf16x8 transposed(const bf16_t* tile, int s, int t) const {
+        const bf16_t* const p = tile + 16 * s * LD + (t >> 1) * 64;
+        const int at = pair ^ (32 * (t & 1));
+        const bf16x4 lo = read(p + at), hi = read(p + (at ^ 8) + 4 * LD);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    static __device__ __forceinline__ bf16x4 read(const bf16_t* p) {
+        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+        return __builtin_bit_cast(bf16x4, v);
+    }
+};
+
+// A thread's share of the rows of one role: granules of 8 columns, ITERS rows apart by STEP.  Addresses are a base that the whole
+// workgroup shares, advanced chunk by chunk, and 32 bits of the thread's own (the host checks the strides).  There is one path: what
+// lies past the last row or column is read from the chunk's first row and column instead, and zero by the time it is in LDS.
 template <int COLS, int NT>
 struct Stream {
     static constexpr int GRANULES = COLS / 8, STEP = NT / GRANULES, ITERS = LC / STEP;
     static_assert(NT % GRANULES == 0 && LC % STEP == 0, "whole rows");
-    const bf16_t* p;    // this thread's granule of the chunk's first row
-    int64_t row;        // elements from a row to the next one of the walk
+    const char* base;
+    int64_t chunk_bytes;
+    uint32_t offset, step_bytes, first;
     int r0;
     bool in_columns;
-    bf16x8 v[ITERS];
 
+    // `token`: the first of the walk, uniform over the workgroup
     __device__ __forceinline__ Stream(const LinearRole& role, int b, int h, int64_t token, bool reverse, int c0, int columns, int tid) {
         r0 = tid / GRANULES;
         const int c = (tid % GRANULES) * 8;
         in_columns = c < columns;
-        row = reverse ? -role.stride_t : role.stride_t;
-        p = static_cast<const bf16_t*>(role.p) + b * role.stride_b + (h / role.div) * role.stride_h + token * role.stride_t + c0 + c + r0 * row;
+        const int64_t row_bytes = role.stride_t * 2;
+        const int64_t lowest = reverse ? token - (LC - 1) : token;  // of the first chunk's 64 rows in memory
+        base = static_cast<const char*>(role.p) + 2 * (b * role.stride_b + (h / role.div) * role.stride_h + c0) + lowest * row_bytes;
+        offset = (uint32_t)((reverse ? LC - 1 - r0 : r0) * row_bytes) + 2 * c;
+        first = reverse ? (uint32_t)((LC - 1) * row_bytes) : 0;
+        chunk_bytes = (reverse ? -LC : LC) * row_bytes;
+        step_bytes = (uint32_t)((reverse ? -STEP : STEP) * row_bytes);
     }
-    __device__ __forceinline__ void load(int rows) {  // of the chunk; the rest is zero
+    __device__ __forceinline__ bool there(int i, int rows) const { return in_columns && r0 + i * STEP < rows; }
+    // the next chunk, of which there are `rows` rows (more: all 64)
+    __device__ __forceinline__ void fetch(bf16x8 (&v)[ITERS], int rows) {
 #pragma unroll
         for (int i = 0; i < ITERS; i++) {
-            bf16x8 x = {};
-            if (in_columns && r0 + i * STEP < rows) x = *reinterpret_cast<const bf16x8*>(p + (int64_t)(i * STEP) * row);
-            v[i] = x;
+            const uint32_t at = there(i, rows) ? offset + i * step_bytes : first;
+            v[i] = *reinterpret_cast<const bf16x8*>(base + at);
         }
-        p += LC * row;
+        base += chunk_bytes;
     }
-    __device__ __forceinline__ void store(bf16_t* tile) const {
+    template <int LD = COLS>
+    __device__ __forceinline__ void stage(bf16_t* tile, const bf16x8 (&v)[ITERS], int rows) const {
         const int g = threadIdx.x % GRANULES;
 #pragma unroll
         for (int i = 0; i < ITERS; i++) {
             const int r = r0 + i * STEP;
-            *reinterpret_cast<bf16x8*>(tile + r * COLS + ((g ^ tile_key(r)) << 3)) = v[i];
+            const bf16x8 zero = {};
+            *reinterpret_cast<bf16x8*>(tile + r * LD + ((g ^ tile_key(r)) << 3)) = there(i, rows) ? v[i] : zero;
         }
     }
 };

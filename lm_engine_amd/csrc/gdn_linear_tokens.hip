@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p
     LinearSegment sg;
     if (!linear_find(p, slot, sg, lane)) return;
     const bool last = sg.s == linear_segments(sg.len, p.seg) - 1;
-    if (STATES_ONLY && last) return;
+    if (STATES_ONLY && last && p.fin == nullptr) return;  // nothing starts from it
     const int walked = sg.s * p.seg, total = min(p.seg, sg.len - walked);
     const int64_t token = p.reverse ? (int64_t)sg.t0 + sg.len - 1 - walked : (int64_t)sg.t0 + walked;
     const float w = p.g == nullptr ? 1.f : expf(p.g[h]);

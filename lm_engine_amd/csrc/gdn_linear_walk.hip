@@ -17,16 +17,42 @@ namespace gdn {
 
 namespace {
 
-template <int KD, int NW, bool STATES_ONLY>
-__global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : NW / 4 > 0 ? NW / 4 : 1) void linear_walk_kernel(const LinearParams p) {
+// Order of the instructions of a region that reads LDS fragments for matrix products: AHEAD reads, then PER reads to every STEP
+// products.  Left alone, the scheduler waits for every read in front of its product.
+template <int AHEAD, int STEPS, int STEP, int PER>
+__device__ __forceinline__ void reads_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, STEP, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+    }
+}
+
+// What a walk is for, and in how many bf16 parts the decayed rows of z go into the state.  Two parts, high and low, 16 bits and more
+// together, keep the state's sums to fp32 accuracy (the rows of y are exact): where the state is a result.
+enum class Walk {
+    outputs,        // one part; a segment of several, its state given
+    outputs_state,  // two parts; the only segment, its state a result
+    sums,           // as outputs, partial outputs in fp32 (LinearParams::sums)
+    states,         // the segments' own states, one part
+    exact_states,   // ... two parts
+};
+
+template <int KD, int NW, Walk MODE>
+__global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel(const LinearParams p) {
     constexpr int NT = 64 * NW, VC = 32 * NW, KT = KD / 32;
+    constexpr bool STATES_ONLY = MODE == Walk::states || MODE == Walk::exact_states, SUMS = MODE == Walk::sums;
+    constexpr int PARTS = MODE == Walk::outputs_state || MODE == Walk::exact_states ? 2 : 1;
     __shared__ __align__(16) bf16_t sx[STATES_ONLY ? 8 : LC * KD];
     __shared__ __align__(16) bf16_t sy[LC * KD];
     __shared__ __align__(16) bf16_t sz[LC * VC];
-    __shared__ __align__(16) bf16_t sp[STATES_ONLY ? 8 : 6 * 512];
-    __shared__ __align__(16) float sw[LC];  // us w^{n - a - j}
+    __shared__ __align__(16) bf16_t sp[STATES_ONLY ? 8 : 6 * 512];  // fragments of P^T
+    __shared__ __align__(16) float sw[LC];                          // us w^{n - a - j}
+    // ps w^{row - key} over a tile of P, in the order of its accumulator: on the diagonal, below it
+    __shared__ __align__(16) f32x4 sdecay[STATES_ONLY ? 1 : 2][4][64];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5;
     // blocks are dealt round the 8 XCDs: the blocks of one XCD get neighbouring places, so that those that read the same rows
     // (columns of the value dim, heads that share keys) meet in its L2
     const unsigned per_xcd = (gridDim.x + 7) / 8;
@@ -37,12 +63,12 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : NW / 4 > 0 ? NW / 4 :
     const int c0 = slice * VC, columns = min(VC, p.V - c0);
 
     if constexpr (!STATES_ONLY)
-        if (p.zero && (p.cu != nullptr)) linear_zero_gaps<bf16_t, 8>(p, slot, h, c0, columns, tid, NT);
+        if (p.zero && p.cu != nullptr) linear_zero_gaps<bf16_t, 8>(p, slot, h, c0, columns, tid, NT);
     LinearSegment sg;
     if (!linear_find(p, slot, sg, lane)) return;
     const int segments = linear_segments(sg.len, p.seg);
     const bool last = sg.s == segments - 1;
-    if (STATES_ONLY && last) return;  // nothing starts from it
+    if (MODE == Walk::states && last) return;  // nothing starts from it
     const int walked = sg.s * p.seg, total = min(p.seg, sg.len - walked);
     const int64_t token = p.reverse ? (int64_t)sg.t0 + sg.len - 1 - walked : (int64_t)sg.t0 + walked;  // the first of the walk
     const float g = p.g == nullptr ? 0.f : p.g[h];
@@ -51,94 +77,108 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : NW / 4 > 0 ? NW / 4 :
     Stream<KD, NT> ys(p.y, sg.b, h, token, p.reverse, 0, p.K, tid);
     Stream<VC, NT> zs(p.z, sg.b, h, token, p.reverse, c0, columns, tid);
     Stream<KD, NT> xs(STATES_ONLY ? p.y : p.x, sg.b, h, token, p.reverse, 0, p.K, tid);
+    bf16x8 ry[Stream<KD, NT>::ITERS], rz[Stream<VC, NT>::ITERS], rx[STATES_ONLY ? 1 : Stream<KD, NT>::ITERS];
+    auto fetch = [&](int left) __attribute__((always_inline)) {  // the next chunk's rows, on their way into registers
+        ys.fetch(ry, left), zs.fetch(rz, left);
+        if constexpr (!STATES_ONLY) xs.fetch(rx, left);
+    };
+    if (total > 0) fetch(total);  // (a segment without tokens has no row to read)
 
+    // the state: keys 32 kt + 16 (r / 8) + 8 half + r % 8 in register r of S[kt], column c0 + 32 wave + swap(l32)
     const int64_t chain = (int64_t)sg.n * p.H + h, cells = p.cells;
-    const int my_v = c0 + 32 * wave + slice_col(l32);  // the state's column of this lane
-    auto state_at = [&](int kt, int r) { return (int64_t)(32 * kt + 16 * (r >> 3) + 8 * half + (r & 7)) * p.state_k + (int64_t)my_v * p.state_v; };
-    auto state_key = [&](int kt, int r) { return 32 * kt + 16 * (r >> 3) + 8 * half + (r & 7); };
+    const int my_v = c0 + 32 * wave + slice_col(l32);
     f32x16 S[KT];
+    auto for_cells = [&](auto&& f) __attribute__((always_inline)) {
+        if (my_v >= p.V) return;
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int key = 32 * kt + 16 * (r >> 3) + 8 * half + (r & 7);
+                if (key < p.K) f(kt, r, (int64_t)key * p.state_k + (int64_t)my_v * p.state_v);
+            }
+    };
 #pragma unroll
     for (int kt = 0; kt < KT; kt++) S[kt] = f32x16{};
     const float* from = nullptr;
     if (!STATES_ONLY) from = sg.s > 0 ? p.local + ((int64_t)slot * p.H + h) * cells : p.init == nullptr ? nullptr : p.init + chain * cells;
-    if (from != nullptr && my_v < p.V) {
-#pragma unroll
-        for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-            for (int r = 0; r < 16; r++)
-                if (state_key(kt, r) < p.K) S[kt][r] = from[state_at(kt, r)];
-    }
+    if (from != nullptr) for_cells([&](int kt, int r, int64_t at) __attribute__((always_inline)) { S[kt][r] = from[at]; });
 
-    // the wave's tile of P: (key tile, row tile) (0, 0), (0, 1), (1, 1); on the diagonal rows before the key get nothing
-    constexpr int TILES = 3;
-    f32x16 decay = {};
-    if constexpr (!STATES_ONLY) {
-        const int t = wave;  // NW = 2: wave 0 has both tiles on the diagonal
-        const int ji = t == 1 ? -32 : 0;
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int distance = l32 - (16 * (r >> 3) + 8 * half + (r & 7)) - ji;
-            decay[r] = distance >= 0 ? p.ps * linear_power(g, distance) : 0.f;
-        }
-    }
+    constexpr int TILES = 3;  // of P: (key tile, row tile) (0, 0), (0, 1), (1, 1)
     float row_weight[2];
+    if constexpr (!STATES_ONLY) {
+        for (int i = wave; i < 8; i += NW) {
+            f32x4 w;
 #pragma unroll
-    for (int i = 0; i < 2; i++) row_weight[i] = p.os * linear_power(g, 32 * i + l32 + a);
+            for (int r = 0; r < 4; r++) {
+                const int distance = 32 * (i >> 2) + l32 - (16 * (i >> 1 & 1) + 8 * half + 4 * (i & 1) + r);
+                w[r] = distance >= 0 ? p.ps * linear_power(g, distance) : 0.f;
+            }
+            sdecay[i >> 2][i & 3][lane] = w;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) row_weight[i] = p.os * linear_power(g, 32 * i + l32 + a);
+    }
+    if (tid < LC) sw[tid] = p.us * linear_power(g, LC - a - tid);
+    const float whole = linear_power(g, LC);
+    TileLane<KD> tile(lane);
+    TileLane<VC> ztile(lane);
 
-    // outputs: this lane's row of the chunk's first 32, its 8 columns
-    bf16_t* out = static_cast<bf16_t*>(p.out) + sg.b * p.out_stride_b + h * p.out_stride_h + token * p.out_stride_t;
-    const int64_t out_row = p.reverse ? -p.out_stride_t : p.out_stride_t;
-    float* sums = p.sums == nullptr ? nullptr : p.sums + ((int64_t)sg.b * p.T + token) * p.H * p.V + (int64_t)h * p.V;
+    // outputs, addressed as the streams are: rows 32 i + l32 of the chunk, 8 columns
+    const int col = c0 + 32 * wave + 8 * half;
+    const int64_t out_row = p.out_stride_t * 2;
+    char* out = static_cast<char*>(p.out) + 2 * (sg.b * p.out_stride_b + h * p.out_stride_h) + (p.reverse ? token - (LC - 1) : token) * out_row;
+    const uint32_t out_at = (uint32_t)((p.reverse ? LC - 1 - l32 : l32) * out_row) + 2 * col;
+    const uint32_t out_step = (uint32_t)((p.reverse ? -32 : 32) * out_row);
+    float* const sums = SUMS ? p.sums + ((int64_t)sg.b * p.T + token) * p.H * p.V + (int64_t)h * p.V : nullptr;
     const int64_t sums_row = (p.reverse ? -1 : 1) * (int64_t)p.H * p.V;
 
     const int chunks = (total + LC - 1) / LC;
-    ys.load(total), zs.load(total);
-    if constexpr (!STATES_ONLY) xs.load(total);
     for (int c = 0; c < chunks; c++) {
         const int rows = min(LC, total - c * LC);
         __syncthreads();  // the tiles of the chunk before are read
-        if (c == 0 || rows < LC) {
-            if (tid < LC) sw[tid] = p.us * linear_power(g, max(rows - a - tid, 0));
-        }
-        ys.store(sy), zs.store(sz);
-        if constexpr (!STATES_ONLY) xs.store(sx);
+        if (rows < LC && tid < LC) sw[tid] = p.us * linear_power(g, max(rows - a - tid, 0));
+        ys.stage(sy, ry, rows), zs.stage(sz, rz, rows);
+        if constexpr (!STATES_ONLY) xs.stage(sx, rx, rows);
         __syncthreads();
-        if (c + 1 < chunks) {
-            const int left = total - (c + 1) * LC;
-            ys.load(left), zs.load(left);
-            if constexpr (!STATES_ONLY) xs.load(left);
-        }
-        bf16x8 zf[4];
-#pragma unroll
-        for (int s = 0; s < 4; s++) zf[s] = tile_tr8<VC>(sz, 16 * s, 32 * wave, lane);
+        if (c + 1 < chunks) fetch(total - (c + 1) * LC);
+        tile.recompute(), ztile.recompute();
 
         if constexpr (!STATES_ONLY) {
             for (int t = wave; t < TILES; t += NW) {
                 const int jt = t == 2, it = t >= 1;
+                const bf16_t *const yt = sy + 32 * jt * KD, *const xt = sx + 32 * it * KD;
                 f32x16 acc = {};
 #pragma unroll
-                for (int s = 0; s < KD / 16; s++)
-                    acc = mfma32_bf16(tile_row8<KD>(sy, 32 * jt + slice_col(l32), 2 * s + half), tile_row8<KD>(sx, 32 * it + l32, 2 * s + half), acc);
+                for (int s = 0; s < KD / 16; s++) acc = mfma32_bf16(tile.swapped_fragment(yt, 0, s), tile.fragment(xt, 0, s), acc);
+                reads_ahead<8, KD / 16, 1, 2>();
                 // selected, not multiplied away: a row before the key takes nothing of it, whatever its product is
 #pragma unroll
-                for (int r = 0; r < 16; r++) acc[r] = t != 1 && l32 < 16 * (r >> 3) + 8 * half + (r & 7) ? 0.f : acc[r] * decay[r];
+                for (int q = 0; q < 4; q++) {
+                    const f32x4 w = sdecay[t == 1][q][lane];
+#pragma unroll
+                    for (int r = 4 * q; r < 4 * q + 4; r++) acc[r] = t != 1 && l32 < 16 * (r >> 3) + 8 * half + (r & 7) ? 0.f : acc[r] * w[r & 3];
+                }
                 *reinterpret_cast<bf16x8*>(sp + (2 * t + 0) * 512 + lane * 8) = pack8_16(acc, 0, 1.f);
                 *reinterpret_cast<bf16x8*>(sp + (2 * t + 1) * 512 + lane * 8) = pack8_16(acc, 1, 1.f);
             }
+            __builtin_amdgcn_sched_barrier(0);
             f32x16 O[2] = {};
 #pragma unroll
-            for (int kt = 0; kt < KT; kt++)
+            for (int s = 0; s < KD / 16; s++) {
+                const bf16x8 sf = pack8_16(S[s >> 1], s & 1, 1.f);  // the state as an operand: its one rounding to bf16 for the output
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    const bf16x8 sf = pack8_16(S[kt], s, 1.f);  // the state as an operand: its one rounding to bf16 for the output
-#pragma unroll
-                    for (int i = 0; i < 2; i++) O[i] = mfma32_bf16(sf, tile_row8<KD>(sx, 32 * i + l32, 4 * kt + 2 * s + half), O[i]);
-                }
+                for (int i = 0; i < 2; i++) O[i] = mfma32_bf16(sf, tile.fragment(sx, 32 * i, s), O[i]);
+            }
+            reads_ahead<8, KD / 16, 2, 2>();
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) O[i][r] *= row_weight[i];
             __syncthreads();  // P is there
+            bf16x8 zf[4];
+#pragma unroll
+            for (int s = 0; s < 4; s++) zf[s] = ztile.transposed(sz, s, wave);
 #pragma unroll
             for (int t = 0; t < TILES; t++)
 #pragma unroll
@@ -147,65 +187,66 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : NW / 4 > 0 ? NW / 4 :
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const int row = 32 * i + l32;
-                if (row < rows) {
+                if (row >= rows) continue;
 #pragma unroll
-                    for (int s = 0; s < 2; s++) {
-                        const int col = c0 + 32 * wave + 16 * s + 8 * half;
-                        if (col >= p.V) continue;
-                        if (sums != nullptr) {
-                            float* at = sums + (c * LC + row) * sums_row + col;
+                for (int s = 0; s < 2; s++) {
+                    if (col + 16 * s >= p.V) continue;
+                    if constexpr (SUMS) {
+                        f32x4* const at = reinterpret_cast<f32x4*>(sums + (int64_t)(c * LC + row) * sums_row + col + 16 * s);
 #pragma unroll
-                            for (int e = 0; e < 8; e++) {
-                                if (p.sums_in) O[i][8 * s + e] += at[e];
-                                if (p.sums_out) at[e] = O[i][8 * s + e];
-                            }
-                            if (p.sums_out) continue;
+                        for (int e = 0; e < 8; e++)
+                            if (p.sums_in) O[i][8 * s + e] += at[e >> 2][e & 3];
+                        if (p.sums_out) {
+#pragma unroll
+                            for (int e = 0; e < 2; e++) at[e] = f32x4{O[i][8 * s + 4 * e], O[i][8 * s + 4 * e + 1], O[i][8 * s + 4 * e + 2], O[i][8 * s + 4 * e + 3]};
+                            continue;
                         }
-                        *reinterpret_cast<bf16x8*>(out + (c * LC + row) * out_row + col) = pack8_16(O[i], s, 1.f);
                     }
+                    *reinterpret_cast<bf16x8*>(out + (out_at + i * out_step + 32 * s)) = pack8_16(O[i], s, 1.f);
                 }
             }
+            out += (p.reverse ? -LC : LC) * out_row;
+            __builtin_amdgcn_sched_barrier(0);
         }
-        // The state's own sums are kept to fp32 accuracy: the decayed rows of z go in as two bf16 parts, high and low (16 bits and
-        // more together), the rows of y are exact.
-        bf16x8 hi[4], lo[4];
+        bf16x8 part[4][PARTS];
 #pragma unroll
         for (int s = 0; s < 4; s++) {
-            const float* weights = sw + 16 * s + 8 * half;
+            const bf16x8 z = ztile.transposed(sz, s, wave);
+            const float* const weights = sw + 16 * s + 8 * half;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float z = (float)zf[s][e] * weights[e];
-                hi[s][e] = (bf16_t)z;
-                lo[s][e] = (bf16_t)(z - (float)hi[s][e]);
+                const float x = (float)z[e] * weights[e];
+                part[s][0][e] = (bf16_t)x;
+                if constexpr (PARTS == 2) part[s][1][e] = (bf16_t)(x - (float)part[s][0][e]);
             }
         }
-        const float whole = linear_power(g, rows);
-#pragma unroll
-        for (int kt = 0; kt < KT; kt++) {
-#pragma unroll
-            for (int r = 0; r < 16; r++) S[kt][r] *= whole;
-#pragma unroll
-            for (int s = 0; s < 4; s++) {
-                const bf16x8 yt = tile_tr8<KD>(sy, 16 * s, 32 * kt, lane);
-                S[kt] = mfma32_bf16(yt, hi[s], S[kt]);
-                S[kt] = mfma32_bf16(yt, lo[s], S[kt]);
-            }
-        }
-    }
-    float* to = nullptr;
-    if constexpr (STATES_ONLY) to = p.local + ((int64_t)slot * p.H + h) * cells;
-    else if (last && p.fin != nullptr) to = p.fin + chain * cells;
-    if (to != nullptr && my_v < p.V) {
+        __builtin_amdgcn_sched_barrier(0);
+        const float shrink = rows < LC ? linear_power(g, rows) : whole;
 #pragma unroll
         for (int kt = 0; kt < KT; kt++)
 #pragma unroll
-            for (int r = 0; r < 16; r++)
-                if (state_key(kt, r) < p.K) to[state_at(kt, r)] = S[kt][r];
+            for (int r = 0; r < 16; r++) S[kt][r] *= shrink;
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const bf16x8 yt = tile.transposed(sy, s, kt);
+#pragma unroll
+                for (int u = 0; u < PARTS; u++) S[kt] = mfma32_bf16(yt, part[s][u], S[kt]);
+            }
+        reads_ahead<8, 4 * KT, PARTS, 2>();
+        __builtin_amdgcn_sched_barrier(0);
     }
+
+    float* to = nullptr;
+    if constexpr (STATES_ONLY) to = p.local + ((int64_t)slot * p.H + h) * cells;
+    else if (MODE == Walk::outputs_state && p.fin != nullptr) to = p.fin + chain * cells;
+    if (to != nullptr) for_cells([&](int kt, int r, int64_t at) __attribute__((always_inline)) { to[at] = S[kt][r]; });
 }
 
-// From the segments' own states (slots 0 .. of a sequence) to what every segment but the first starts from.  A thread has 4 cells
-// of a (sequence, head); the states lie contiguous, and those of a sequence H states apart.
+// From the segments' own states (slots 0 .. of a sequence) to what every segment but the first starts from, and to what the sequence ends
+// with where that is a result (then the last segment's own state is there as well).  A thread has 4 cells of a (sequence, head); the
+// states lie contiguous, and those of a sequence H states apart.
 __global__ __launch_bounds__(256) void linear_combine_kernel(const LinearParams p) {
     const int64_t cells = p.cells;
     const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
@@ -214,7 +255,7 @@ __global__ __launch_bounds__(256) void linear_combine_kernel(const LinearParams 
         int b, t0, len;
         linear_bounds(p, n, b, t0, len);
         const int segments = linear_segments(len, p.seg);
-        if (segments == 1) continue;
+        if (segments == 1 && p.fin == nullptr) continue;
         int slot0 = n * p.nseg;
         if (p.nseg == 0) {
             LinearSegment none;
@@ -229,10 +270,14 @@ __global__ __launch_bounds__(256) void linear_combine_kernel(const LinearParams 
         f32x4 own = *reinterpret_cast<const f32x4*>(local);
         for (int s = 1; s < segments; s++) {
             f32x4 following = {0.f, 0.f, 0.f, 0.f};
-            if (s + 1 < segments) following = *reinterpret_cast<const f32x4*>(local + s * next);
+            if (s + 1 < segments || p.fin != nullptr) following = *reinterpret_cast<const f32x4*>(local + s * next);
             carry = carry * whole + own;
             *reinterpret_cast<f32x4*>(local + s * next) = carry;
             own = following;
+        }
+        if (p.fin != nullptr) {  // behind the last segment, whose tokens are `rest`
+            const int rest = len - (segments - 1) * p.seg;
+            *reinterpret_cast<f32x4*>(p.fin + ((int64_t)n * p.H + h) * cells + at) = carry * linear_power(p.g == nullptr ? 0.f : p.g[h], rest) + own;
         }
     }
 }
@@ -242,20 +287,24 @@ int launch(const LinearParams& p, bool states_only, hipStream_t stream) {
     const int64_t blocks = (int64_t)p.slots * p.H * ((p.V + 32 * NW - 1) / (32 * NW));
     if (blocks > 0xfffff000ll / (64 * NW)) return GDN_ERR_UNSUPPORTED;  // (a launch holds at most 2^32 - 1 threads)
     const dim3 grid((unsigned)((blocks + 7) / 8 * 8)), threads(64 * NW);
-    if (states_only) hipLaunchKernelGGL((linear_walk_kernel<KD, NW, true>), grid, threads, 0, stream, p);
-    else hipLaunchKernelGGL((linear_walk_kernel<KD, NW, false>), grid, threads, 0, stream, p);
+    if (states_only && p.fin != nullptr) hipLaunchKernelGGL((linear_walk_kernel<KD, NW, Walk::exact_states>), grid, threads, 0, stream, p);
+    else if (states_only) hipLaunchKernelGGL((linear_walk_kernel<KD, NW, Walk::states>), grid, threads, 0, stream, p);
+    else if (p.sums != nullptr) hipLaunchKernelGGL((linear_walk_kernel<KD, NW, Walk::sums>), grid, threads, 0, stream, p);
+    else if (p.fin != nullptr) hipLaunchKernelGGL((linear_walk_kernel<KD, NW, Walk::outputs_state>), grid, threads, 0, stream, p);
+    else hipLaunchKernelGGL((linear_walk_kernel<KD, NW, Walk::outputs>), grid, threads, 0, stream, p);
     return (int)hipGetLastError();
 }
 
 }  // namespace
 
-int linear_walk_columns(int V) { return V <= 64 ? 64 : 128; }
+// (more than 128 keys: two waves would not hold the rows on their way to them in registers)
+int linear_walk_columns(int K, int V) { return V <= 64 && K <= 128 ? 64 : 128; }
 
 int launch_linear_walk(const LinearParams& p, bool states_only, hipStream_t stream) {
-    const bool narrow = linear_walk_columns(p.V) == 64;
+    const bool narrow = linear_walk_columns(p.K, p.V) == 64;
     if (p.K <= 64) return narrow ? launch<64, 2>(p, states_only, stream) : launch<64, 4>(p, states_only, stream);
     if (p.K <= 128) return narrow ? launch<128, 2>(p, states_only, stream) : launch<128, 4>(p, states_only, stream);
-    return narrow ? launch<256, 2>(p, states_only, stream) : launch<256, 4>(p, states_only, stream);
+    return launch<256, 4>(p, states_only, stream);
 }
 
 int launch_linear_combine(const LinearParams& p, hipStream_t stream) {
