@@ -86,8 +86,15 @@ Cut cut_for_walk(const gdn_linear_attn_args& a, int K, int V) {
     return cut_sequences(a, slices, 4 * cus, 64);
 }
 
-uint64_t local_bytes(const gdn_linear_attn_args& a, const Cut& c) {
-    return c.several ? ((uint64_t)c.slots * a.H * a.K * a.V * 4 + 255) / 256 * 256 : 0;
+// cells of a state between the launches: bf16 in the order of the walk's registers (whole workgroups), fp32 as it is
+int64_t local_cells(int dtype, int K, int V) {
+    if (dtype != GDN_BF16) return (int64_t)K * V;
+    const int columns = linear_walk_columns(K, V);
+    return (int64_t)linear_walk_keys(K) * ((V + columns - 1) / columns * columns);
+}
+
+uint64_t states_bytes(const gdn_linear_attn_args& a, const Cut& c, int64_t cells) {
+    return c.several ? ((uint64_t)c.slots * a.H * cells * 4 + 255) / 256 * 256 : 0;
 }
 
 // what every walk over these sequences has in common
@@ -123,7 +130,9 @@ int run(const LinearParams& p, int dtype, bool states_only, hipStream_t stream) 
 }
 
 // the states that the segments start from, into p.local: their own, then the sums, and p.fin
-int run_states(const LinearParams& p, int dtype, hipStream_t stream) {
+int run_states(LinearParams& p, int dtype, hipStream_t stream) {
+    p.local_cells = local_cells(dtype, p.K, p.V);
+    p.local_keys = dtype == GDN_BF16 ? linear_walk_keys(p.K) : 0;
     if (const int e = run(p, dtype, true, stream); e != GDN_OK) return e;
     return launch_linear_combine(p, stream);
 }
@@ -144,23 +153,38 @@ uint64_t dots_bytes(const gdn_linear_attn_args& a, const Cut& c) {
 // The backward's workspace: states that the segments start from (the forward's, their gradients, with dg the derivatives), partial
 // outputs, the parts of dg.
 struct BackwardSpace {
-    uint64_t local, slope, sums, dots;
-    BackwardSpace(const gdn_linear_attn_args& a, const Cut& c, bool dg)
-        : local(local_bytes(a, c)), slope(dg ? local : 0), sums(sums_bytes(a)), dots(dg ? dots_bytes(a, c) : 0) {}
-    uint64_t total() const { return 2 * local + slope + sums + dots; }
+    uint64_t forward, gradients, slope, sums, dots;
+    bool own_orientation;  // the forward's states are written with the value dim as keys, as dq reads them
+    BackwardSpace(const gdn_linear_attn_args& a, const Cut& c, bool dg) {
+        own_orientation = a.dtype == GDN_BF16 && !dg;
+        const int64_t natural_cells = (int64_t)a.K * a.V;
+        forward = states_bytes(a, c, own_orientation ? local_cells(a.dtype, std::min(a.V, KEYS), a.K) : natural_cells);
+        gradients = states_bytes(a, c, local_cells(a.dtype, a.K, a.V));
+        slope = dg ? states_bytes(a, c, natural_cells) : 0;
+        sums = sums_bytes(a);
+        dots = dg ? dots_bytes(a, c) : 0;
+    }
+    uint64_t total() const { return forward + gradients + slope + sums + dots; }
 };
 
-// dq or dk: a walk whose keys are the value dim, 256 of them at a time; p.x, p.y, p.z and the states are set for all of them
-int run_transposed(LinearParams p, const gdn_linear_attn_args& a, float* sums, hipStream_t stream) {
+// dq or dk: a walk whose keys are the value dim, 256 of them at a time; p.x, p.y, p.z and the states are set for all of them.
+// own_states: the states that the segments start from are formed here, in p.local, 256 keys after 256 keys as well
+int run_transposed(LinearParams p, const gdn_linear_attn_args& a, bool own_states, float* sums, hipStream_t stream) {
     const LinearParams whole = p;
     for (int first = 0; first < a.V; first += KEYS) {
         p.K = std::min(KEYS, a.V - first), p.V = a.K;
         p.state_k = 1, p.state_v = a.V;
         p.x.p = offset(whole.x.p, first, a.dtype), p.y.p = offset(whole.y.p, first, a.dtype);
         p.init = whole.init == nullptr ? nullptr : whole.init + first;
-        p.local = whole.local == nullptr ? nullptr : whole.local + first;
         p.sums = a.V > KEYS ? sums : nullptr;
         p.sums_in = first > 0, p.sums_out = first + KEYS < a.V;
+        if (own_states) {
+            if (const int e = run_states(p, a.dtype, stream); e != GDN_OK) return e;
+        } else if (p.local != nullptr && p.local_keys != 0) {
+            p.local_swapped = 1, p.local_first = first;
+        } else if (p.local != nullptr) {
+            p.local = whole.local + first;
+        }
         if (const int e = run(p, a.dtype, false, stream); e != GDN_OK) return e;
     }
     return GDN_OK;
@@ -175,7 +199,7 @@ extern "C" int gdn_linear_abi_version(void) { return GDN_LINEAR_ABI_VERSION; }
 
 extern "C" uint64_t gdn_linear_attn_workspace_bytes(const gdn_linear_attn_args* a) {
     if (a == nullptr || check_shape(*a) != GDN_OK) return 0;
-    return local_bytes(*a, cut_for_walk(*a, a->K, a->V));
+    return states_bytes(*a, cut_for_walk(*a, a->K, a->V), local_cells(a->dtype, a->K, a->V));
 }
 
 extern "C" int gdn_linear_attn_chunk_fwd(const gdn_linear_attn_args* args, void* stream) {
@@ -186,7 +210,7 @@ extern "C" int gdn_linear_attn_chunk_fwd(const gdn_linear_attn_args* args, void*
     if (const int e = check_rows(a.o, a.o_stride_b, a.o_stride_t, a.o_stride_h, a.dtype); e != GDN_OK) return e;
     if (a.h0 != nullptr && a.ht == a.h0) return GDN_ERR_UNSUPPORTED;
     const Cut c = cut_for_walk(a, a.K, a.V);
-    if (c.several && (a.workspace == nullptr || a.workspace_bytes < local_bytes(a, c))) return GDN_ERR_WORKSPACE;
+    if (c.several && (a.workspace == nullptr || a.workspace_bytes < states_bytes(a, c, local_cells(a.dtype, a.K, a.V)))) return GDN_ERR_WORKSPACE;
     if (c.several && !aligned16(a.workspace)) return GDN_ERR_ALIGN;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const Roles r = roles_of(a);
@@ -250,7 +274,8 @@ extern "C" int gdn_linear_attn_bwd(const gdn_linear_attn_bwd_args* args, void* s
     const Roles r = roles_of(a);
     const LinearRole d = {b.dout, b.dout_stride_b, b.dout_stride_t, b.dout_stride_h, 1};
     char* const ws = static_cast<char*>(b.workspace);
-    float* const sums_at = reinterpret_cast<float*>(ws + 2 * space.local + space.slope);
+    float* const gradients_at = reinterpret_cast<float*>(ws + space.forward);
+    float* const sums_at = reinterpret_cast<float*>(ws + space.forward + space.gradients + space.slope);
 
     LinearParams s = base_params(a, c);  // of the forward's states
     natural(s, a.K, a.V);
@@ -261,19 +286,20 @@ extern "C" int gdn_linear_attn_bwd(const gdn_linear_attn_bwd_args* args, void* s
     t.x = r.k, t.y = r.q, t.z = d;
     t.init = b.dht;
     t.reverse = 1, t.a = 0, t.os = 1.f, t.ps = t.us = a.scale;
-    if (c.several) {
-        s.local = reinterpret_cast<float*>(ws), t.local = reinterpret_cast<float*>(ws + space.local);
-        if (b.dg == nullptr)
-            if (const int e = run_states(s, a.dtype, st); e != GDN_OK) return e;
-        t.fin = b.dh0;
-        if (const int e = run_states(t, a.dtype, st); e != GDN_OK) return e;
-    }
     if (b.dg != nullptr) {  // (which leaves the states that the segments start from as well)
         LinearParams u = s;
         u.d = d, u.init_grad = b.dht;
-        u.local_slope = reinterpret_cast<float*>(ws + 2 * space.local);
-        u.dots = reinterpret_cast<float*>(ws + 2 * space.local + space.slope + space.sums);
+        if (c.several) u.local = reinterpret_cast<float*>(ws), u.local_slope = gradients_at + space.gradients / 4;
+        u.dots = sums_at + space.sums / 4;
         if (const int e = launch_linear_tangent(u, a.dtype, c.several, b.dg, st); e != GDN_OK) return e;
+    }
+    if (c.several) {
+        s.local = reinterpret_cast<float*>(ws), t.local = gradients_at;
+        s.local_cells = (int64_t)a.K * a.V;  // (natural, as the tangent's launch leaves them)
+        if (b.dg == nullptr && !space.own_orientation)
+            if (const int e = run_states(s, a.dtype, st); e != GDN_OK) return e;
+        t.fin = b.dh0;
+        if (const int e = run_states(t, a.dtype, st); e != GDN_OK) return e;
     }
     t.out = b.dv, t.out_stride_b = b.dv_stride_b, t.out_stride_t = b.dv_stride_t, t.out_stride_h = b.dv_stride_h;
     t.fin = c.several ? nullptr : b.dh0;
@@ -282,10 +308,10 @@ extern "C" int gdn_linear_attn_bwd(const gdn_linear_attn_bwd_args* args, void* s
     k.x = r.v, k.y = d, k.z = r.q;
     k.out = b.dk, k.out_stride_b = b.dk_stride_b, k.out_stride_t = b.dk_stride_t, k.out_stride_h = b.dk_stride_h;
     k.fin = nullptr;
-    if (const int e = run_transposed(k, a, sums_at, st); e != GDN_OK) return e;
+    if (const int e = run_transposed(k, a, false, sums_at, st); e != GDN_OK) return e;
     LinearParams q = s;
     q.x = d, q.y = r.v, q.z = r.k;
     q.out = b.dq, q.out_stride_b = b.dq_stride_b, q.out_stride_t = b.dq_stride_t, q.out_stride_h = b.dq_stride_h;
     q.fin = nullptr;
-    return run_transposed(q, a, sums_at, st);
+    return run_transposed(q, a, c.several && space.own_orientation, sums_at, st);
 }

@@ -32,6 +32,11 @@ struct LinearParams {
     float* local;         // [slots, H] states: of a segment's own tokens, then (linear_combine_kernel) what the segment starts from
     int state_k, state_v;  // element (key k, value v) of a state is at k * state_k + v * state_v
     int64_t cells;         // of a state
+    // Layout of `local`.  local_keys 0: as init and fin.  Else in the order of the bf16 walk's registers (linear_fragment), padded to
+    // local_keys keys and whole workgroups of columns; local_swapped: written by a walk whose keys are this one's columns, and whose
+    // column local_first is this one's first key.
+    int local_keys, local_swapped, local_first;
+    int64_t local_cells;
     const int32_t* cu;
     int padded;           // cu: prefix sums of the valid lengths of left-padded rows
     int B, T, H, N, K, V;  // K, V: of the roles (key dim, value dim)
@@ -157,12 +162,21 @@ __device__ __forceinline__ void linear_zero_gaps(const LinearParams& p, int slot
         }
 }
 
-// w^n; 1 for n = 0 also where g is -inf (a state that forgets at once)
-__device__ __forceinline__ float linear_power(float g, int n) { return n == 0 ? 1.f : expf(g * (float)n); }
+// log2 of a token's factor, from the natural logarithm that callers give; w^n from it, 1 for n = 0 also where the state forgets at once
+// (-inf).  One rounding in each: relative to w^n an error of some |n g| 2^-24, as exp(g n) in fp32 has.
+__device__ __forceinline__ float linear_log2(const float* g, int h) { return g == nullptr ? 0.f : g[h] * 1.4426950408889634f; }
+__device__ __forceinline__ float linear_power(float g2, int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f(g2 * (float)n); }
+
+// Where cell (key, v) lies in a state that the bf16 walk has written: [32 columns][32 keys][4 registers of 4][64 lanes][4 keys].
+__device__ __forceinline__ int64_t linear_fragment(int keys, int key, int v) {
+    const int r = 8 * (key >> 4 & 1) + (key & 7), lane = 32 * (key >> 3 & 1) + slice_col(v & 31);
+    return ((((int64_t)(v >> 5) * (keys >> 5) + (key >> 5)) * 4 + (r >> 2)) * 64 + lane) * 4 + (r & 3);
+}
 
 // launches, gdn_linear_walk.hip and gdn_linear_tokens.hip; `states_only`: the segments' own states into p.local
 int launch_linear_walk(const LinearParams& p, bool states_only, hipStream_t stream);
 int launch_linear_tokens(const LinearParams& p, int dtype, int columns, bool states_only, hipStream_t stream);
+int linear_walk_keys(int K);            // keys that the bf16 walk is built for
 int linear_walk_columns(int K, int V);  // columns of the value dim that a workgroup of the bf16 walk has
 int linear_tokens_columns(int64_t chains, int V, int cus);  // of the token kernel
 int launch_linear_combine(const LinearParams& p, hipStream_t stream);

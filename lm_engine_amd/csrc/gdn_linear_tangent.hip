@@ -56,7 +56,7 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : 1) void linear_tangen
     if (STATES_ONLY && last) return;
     const int walked = sg.s * p.seg, total = min(p.seg, sg.len - walked);
     const int64_t token = (int64_t)sg.t0 + walked;
-    const float g = p.g[h];
+    const float g = linear_log2(p.g, h);
 
     Stream<KD, NT> ks(p.y, sg.b, h, token, false, 0, p.K, tid), qs(STATES_ONLY ? p.y : p.x, sg.b, h, token, false, 0, p.K, tid);
     Stream<VC, NT> vs(p.z, sg.b, h, token, false, c0, columns, tid), ds(STATES_ONLY ? p.z : p.d, sg.b, h, token, false, c0, columns, tid);
@@ -108,8 +108,8 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : 1) void linear_tangen
     for (int c = 0; c < chunks; c++) {
         const int rows = min(LC, total - c * LC);
         bf16x8 rk[Stream<KD, NT>::ITERS], rv[Stream<VC, NT>::ITERS], rq[STATES_ONLY ? 1 : Stream<KD, NT>::ITERS], rd[STATES_ONLY ? 1 : Stream<VC, NT>::ITERS];
-        ks.fetch(rk, rows), vs.fetch(rv, rows);
-        if constexpr (!STATES_ONLY) qs.fetch(rq, rows), ds.fetch(rd, rows);
+        ks.fetch(rk, rows, false), vs.fetch(rv, rows, false);
+        if constexpr (!STATES_ONLY) qs.fetch(rq, rows, false), ds.fetch(rd, rows, false);
         __syncthreads();  // the tiles of the chunk before are read
         if (tid < LC) {
             const int left = max(rows - 1 - tid, 0);
@@ -120,8 +120,8 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : 1) void linear_tangen
                 sw[2][tid] = forward, sw[3][tid] = (float)(tid + 1) * forward;
             }
         }
-        ks.stage(sk, rk, rows), vs.stage(sv, rv, rows);
-        if constexpr (!STATES_ONLY) qs.stage(sq, rq, rows), ds.stage(sd, rd, rows);
+        ks.stage(sk, rk, rows, false), vs.stage(sv, rv, rows, false);
+        if constexpr (!STATES_ONLY) qs.stage(sq, rq, rows, false), ds.stage(sd, rd, rows, false);
         __syncthreads();
         bf16x8 hi[4], lo[4];
         if constexpr (!STATES_ONLY) {
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(256) void linear_tangent_combine_kernel(const Linea
             linear_find_packed(p, -1, none, threadIdx.x & 63, n, &slot0);
         }
         if (slot0 + segments > p.slots || at >= p.cells) continue;
-        const float whole = linear_power(p.g[h], p.seg), tokens = (float)p.seg;
+        const float whole = linear_power(linear_log2(p.g, h), p.seg), tokens = (float)p.seg;
         const int64_t first = ((int64_t)slot0 * p.H + h) * p.cells + at, next = (int64_t)p.H * p.cells;
         auto cell = [&](float* base, int s) { return reinterpret_cast<f32x4*>(base + first + s * next); };
         f32x4 S = {0.f, 0.f, 0.f, 0.f}, U = S;

@@ -74,15 +74,16 @@ struct TileLane {
 };
 
 // A thread's share of the rows of one role: granules of 8 columns, ITERS rows apart by STEP.  Addresses are a base that the whole
-// workgroup shares, advanced chunk by chunk, and 32 bits of the thread's own (the host checks the strides).  There is one path: what
-// lies past the last row or column is read from the chunk's first row and column instead, and zero by the time it is in LDS.
+// workgroup shares, advanced chunk by chunk, and 32 bits of the thread's own (the host checks the strides).  What lies past
+// the last row or column is read from the chunk's first row and column instead, and zero by the time it is in LDS: a chunk of no row
+// must not be fetched.
 template <int COLS, int NT>
 struct Stream {
     static constexpr int GRANULES = COLS / 8, STEP = NT / GRANULES, ITERS = LC / STEP;
     static_assert(NT % GRANULES == 0 && LC % STEP == 0, "whole rows");
     const char* base;
-    int64_t chunk_bytes;
-    uint32_t offset, step_bytes, first;
+    int64_t chunk_bytes, step_bytes;
+    uint32_t offset, first;
     int r0;
     bool in_columns;
 
@@ -97,26 +98,32 @@ struct Stream {
         offset = (uint32_t)((reverse ? LC - 1 - r0 : r0) * row_bytes) + 2 * c;
         first = reverse ? (uint32_t)((LC - 1) * row_bytes) : 0;
         chunk_bytes = (reverse ? -LC : LC) * row_bytes;
-        step_bytes = (uint32_t)((reverse ? -STEP : STEP) * row_bytes);
+        step_bytes = (reverse ? -STEP : STEP) * row_bytes;
     }
     __device__ __forceinline__ bool there(int i, int rows) const { return in_columns && r0 + i * STEP < rows; }
-    // the next chunk, of which there are `rows` rows (more: all 64)
-    __device__ __forceinline__ void fetch(bf16x8 (&v)[ITERS], int rows) {
+    // the next chunk, all of it, or (`whole` false) the `rows` rows and the columns that there are
+    __device__ __forceinline__ void fetch(bf16x8 (&v)[ITERS], int rows, bool whole) {
+        if (whole) {
 #pragma unroll
-        for (int i = 0; i < ITERS; i++) {
-            const uint32_t at = there(i, rows) ? offset + i * step_bytes : first;
-            v[i] = *reinterpret_cast<const bf16x8*>(base + at);
+            for (int i = 0; i < ITERS; i++) v[i] = *reinterpret_cast<const bf16x8*>(base + i * step_bytes + offset);
+        } else {
+#pragma unroll
+            for (int i = 0; i < ITERS; i++) {
+                // (an address of the chunk's, whichever: the first row's)
+                v[i] = *reinterpret_cast<const bf16x8*>(base + (there(i, rows) ? offset + (uint32_t)(i * step_bytes) : first));
+            }
         }
         base += chunk_bytes;
     }
     template <int LD = COLS>
-    __device__ __forceinline__ void stage(bf16_t* tile, const bf16x8 (&v)[ITERS], int rows) const {
-        const int g = threadIdx.x % GRANULES;
+    __device__ __forceinline__ void stage(bf16_t* tile, const bf16x8 (&v)[ITERS], int rows, bool whole) const {
+        bf16_t* const at = tile + r0 * LD + ((threadIdx.x % GRANULES ^ tile_key(r0)) << 3);  // (STEP rows on: the same key)
 #pragma unroll
         for (int i = 0; i < ITERS; i++) {
             const int r = r0 + i * STEP;
             const bf16x8 zero = {};
-            *reinterpret_cast<bf16x8*>(tile + r * LD + ((g ^ tile_key(r)) << 3)) = there(i, rows) ? v[i] : zero;
+            bf16_t* const to = STEP % 16 == 0 ? at + i * STEP * LD : tile + r * LD + ((threadIdx.x % GRANULES ^ tile_key(r)) << 3);
+            *reinterpret_cast<bf16x8*>(to) = whole || there(i, rows) ? v[i] : zero;
         }
     }
 };

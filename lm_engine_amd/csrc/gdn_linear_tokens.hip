@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p
 #pragma unroll
     for (int r = 0; r < KR; r++) S[r] = f32x4{0.f, 0.f, 0.f, 0.f};
     const float* from = nullptr;
-    if (!STATES_ONLY) from = sg.s > 0 ? p.local + ((int64_t)slot * p.H + h) * cells : p.init == nullptr ? nullptr : p.init + chain * cells;
+    if (!STATES_ONLY) from = sg.s > 0 ? p.local + ((int64_t)slot * p.H + h) * p.local_cells : p.init == nullptr ? nullptr : p.init + chain * cells;
     if (from != nullptr && mine) {
         if (p.state_v == 1) {
 #pragma unroll
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p
         for (int r = 0; r < KR; r++) S[r] = S[r] * w;
     }
     float* to = nullptr;
-    if constexpr (STATES_ONLY) to = p.local + ((int64_t)slot * p.H + h) * cells;
+    if constexpr (STATES_ONLY) to = p.local + ((int64_t)slot * p.H + h) * p.local_cells;
     else if (last && p.fin != nullptr) to = p.fin + chain * cells;
     if (to != nullptr && mine) {
 #pragma unroll

@@ -49,6 +49,7 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel
     __shared__ __align__(16) bf16_t sz[LC * VC];
     __shared__ __align__(16) bf16_t sp[STATES_ONLY ? 8 : 6 * 512];  // fragments of P^T
     __shared__ __align__(16) float sw[LC];                          // us w^{n - a - j}
+    __shared__ __align__(16) bf16_t so[STATES_ONLY || SUMS ? 8 : LC * VC];  // the chunk's output, to leave in whole rows
     // ps w^{row - key} over a tile of P, in the order of its accumulator: on the diagonal, below it
     __shared__ __align__(16) f32x4 sdecay[STATES_ONLY ? 1 : 2][4][64];
 
@@ -71,16 +72,18 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel
     if (MODE == Walk::states && last) return;  // nothing starts from it
     const int walked = sg.s * p.seg, total = min(p.seg, sg.len - walked);
     const int64_t token = p.reverse ? (int64_t)sg.t0 + sg.len - 1 - walked : (int64_t)sg.t0 + walked;  // the first of the walk
-    const float g = p.g == nullptr ? 0.f : p.g[h];
+    const float g = linear_log2(p.g, h);
     const int a = p.a;
 
     Stream<KD, NT> ys(p.y, sg.b, h, token, p.reverse, 0, p.K, tid);
     Stream<VC, NT> zs(p.z, sg.b, h, token, p.reverse, c0, columns, tid);
     Stream<KD, NT> xs(STATES_ONLY ? p.y : p.x, sg.b, h, token, p.reverse, 0, p.K, tid);
     bf16x8 ry[Stream<KD, NT>::ITERS], rz[Stream<VC, NT>::ITERS], rx[STATES_ONLY ? 1 : Stream<KD, NT>::ITERS];
+    const bool whole_rows = p.K == KD && columns == VC;
     auto fetch = [&](int left) __attribute__((always_inline)) {  // the next chunk's rows, on their way into registers
-        ys.fetch(ry, left), zs.fetch(rz, left);
-        if constexpr (!STATES_ONLY) xs.fetch(rx, left);
+        const bool all = left >= LC && whole_rows;
+        ys.fetch(ry, left, all), zs.fetch(rz, left, all);
+        if constexpr (!STATES_ONLY) xs.fetch(rx, left, all);
     };
     if (total > 0) fetch(total);  // (a segment without tokens has no row to read)
 
@@ -100,9 +103,35 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel
     };
 #pragma unroll
     for (int kt = 0; kt < KT; kt++) S[kt] = f32x16{};
-    const float* from = nullptr;
-    if (!STATES_ONLY) from = sg.s > 0 ? p.local + ((int64_t)slot * p.H + h) * cells : p.init == nullptr ? nullptr : p.init + chain * cells;
-    if (from != nullptr) for_cells([&](int kt, int r, int64_t at) __attribute__((always_inline)) { S[kt][r] = from[at]; });
+    // in the registers' own order a state is 4 keys to a lane and 1 KiB to a wave at a time
+    const int64_t own = ((int64_t)slot * p.H + h) * p.local_cells + (int64_t)(slice * NW + wave) * KT * 1024 + 4 * lane;
+    if (!STATES_ONLY && sg.s > 0) {
+        if (p.local_keys == 0) {
+            const float* const from = p.local + ((int64_t)slot * p.H + h) * p.local_cells;
+            for_cells([&](int kt, int r, int64_t at) __attribute__((always_inline)) { S[kt][r] = from[at]; });
+        } else if (p.local_swapped) {
+            const float* const from = p.local + ((int64_t)slot * p.H + h) * p.local_cells;
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int key = 32 * kt + 16 * (r >> 3) + 8 * half + (r & 7);
+                    if (key < p.K && my_v < p.V) S[kt][r] = from[linear_fragment(p.local_keys, my_v, key + p.local_first)];
+                }
+        } else {
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(p.local + own + (4 * kt + q) * 256);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) S[kt][4 * q + r] = x[r];
+                }
+        }
+    } else if (!STATES_ONLY && p.init != nullptr) {
+        const float* const from = p.init + chain * cells;
+        for_cells([&](int kt, int r, int64_t at) __attribute__((always_inline)) { S[kt][r] = from[at]; });
+    }
 
     constexpr int TILES = 3;  // of P: (key tile, row tile) (0, 0), (0, 1), (1, 1)
     float row_weight[2];
@@ -124,22 +153,38 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel
     TileLane<KD> tile(lane);
     TileLane<VC> ztile(lane);
 
-    // outputs, addressed as the streams are: rows 32 i + l32 of the chunk, 8 columns
+    // outputs, addressed as the streams are
+    using Out = Stream<VC, NT>;
+    const LinearRole out_role = {p.out, p.out_stride_b, p.out_stride_t, p.out_stride_h, 1};
+    Out os(out_role, sg.b, h, token, p.reverse, c0, columns, tid);
+    auto leave = [&](int rows) __attribute__((always_inline)) {  // the output in LDS, rows as they lie in memory
+        char* const to = const_cast<char*>(os.base);
+#pragma unroll
+        for (int i = 0; i < Out::ITERS; i++) {
+            const int r = os.r0 + i * Out::STEP;
+            if (os.there(i, rows))
+                *reinterpret_cast<bf16x8*>(to + i * os.step_bytes + os.offset) = *reinterpret_cast<const bf16x8*>(so + r * VC + ((tid % Out::GRANULES ^ tile_key(r)) << 3));
+        }
+        os.base += os.chunk_bytes;
+    };
     const int col = c0 + 32 * wave + 8 * half;
-    const int64_t out_row = p.out_stride_t * 2;
-    char* out = static_cast<char*>(p.out) + 2 * (sg.b * p.out_stride_b + h * p.out_stride_h) + (p.reverse ? token - (LC - 1) : token) * out_row;
-    const uint32_t out_at = (uint32_t)((p.reverse ? LC - 1 - l32 : l32) * out_row) + 2 * col;
-    const uint32_t out_step = (uint32_t)((p.reverse ? -32 : 32) * out_row);
     float* const sums = SUMS ? p.sums + ((int64_t)sg.b * p.T + token) * p.H * p.V + (int64_t)h * p.V : nullptr;
     const int64_t sums_row = (p.reverse ? -1 : 1) * (int64_t)p.H * p.V;
 
     const int chunks = (total + LC - 1) / LC;
     for (int c = 0; c < chunks; c++) {
         const int rows = min(LC, total - c * LC);
-        __syncthreads();  // the tiles of the chunk before are read
+        __syncthreads();  // the tiles of the chunk before are read, its output is in LDS
+        if constexpr (!STATES_ONLY && !SUMS)
+            if (c > 0) leave(LC);
         if (rows < LC && tid < LC) sw[tid] = p.us * linear_power(g, max(rows - a - tid, 0));
-        ys.stage(sy, ry, rows), zs.stage(sz, rz, rows);
-        if constexpr (!STATES_ONLY) xs.stage(sx, rx, rows);
+        if (rows == LC && whole_rows) {
+            ys.stage(sy, ry, rows, true), zs.stage(sz, rz, rows, true);
+            if constexpr (!STATES_ONLY) xs.stage(sx, rx, rows, true);
+        } else {
+            ys.stage(sy, ry, rows, false), zs.stage(sz, rz, rows, false);
+            if constexpr (!STATES_ONLY) xs.stage(sx, rx, rows, false);
+        }
         __syncthreads();
         if (c + 1 < chunks) fetch(total - (c + 1) * LC);
         tile.recompute(), ztile.recompute();
@@ -187,11 +232,10 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const int row = 32 * i + l32;
-                if (row >= rows) continue;
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
-                    if (col + 16 * s >= p.V) continue;
                     if constexpr (SUMS) {
+                        if (row >= rows || col + 16 * s >= p.V) continue;
                         f32x4* const at = reinterpret_cast<f32x4*>(sums + (int64_t)(c * LC + row) * sums_row + col + 16 * s);
 #pragma unroll
                         for (int e = 0; e < 8; e++)
@@ -201,11 +245,14 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel
                             for (int e = 0; e < 2; e++) at[e] = f32x4{O[i][8 * s + 4 * e], O[i][8 * s + 4 * e + 1], O[i][8 * s + 4 * e + 2], O[i][8 * s + 4 * e + 3]};
                             continue;
                         }
+                        const int64_t token_row = token + (p.reverse ? -1 : 1) * (int64_t)(c * LC + row);
+                        bf16_t* const out = static_cast<bf16_t*>(p.out) + sg.b * p.out_stride_b + h * p.out_stride_h + token_row * p.out_stride_t;
+                        *reinterpret_cast<bf16x8*>(out + col + 16 * s) = pack8_16(O[i], s, 1.f);
+                    } else {
+                        *reinterpret_cast<bf16x8*>(so + row * VC + ((4 * wave + 2 * s + half ^ tile_key(row)) << 3)) = pack8_16(O[i], s, 1.f);
                     }
-                    *reinterpret_cast<bf16x8*>(out + (out_at + i * out_step + 32 * s)) = pack8_16(O[i], s, 1.f);
                 }
             }
-            out += (p.reverse ? -LC : LC) * out_row;
             __builtin_amdgcn_sched_barrier(0);
         }
         bf16x8 part[4][PARTS];
@@ -238,19 +285,38 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    float* to = nullptr;
-    if constexpr (STATES_ONLY) to = p.local + ((int64_t)slot * p.H + h) * cells;
-    else if (MODE == Walk::outputs_state && p.fin != nullptr) to = p.fin + chain * cells;
-    if (to != nullptr) for_cells([&](int kt, int r, int64_t at) __attribute__((always_inline)) { to[at] = S[kt][r]; });
+    if constexpr (!STATES_ONLY && !SUMS) {
+        if (chunks > 0) {
+            __syncthreads();
+            leave(total - (chunks - 1) * LC);
+        }
+    }
+    if constexpr (STATES_ONLY) {
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) *reinterpret_cast<f32x4*>(p.local + own + (4 * kt + q) * 256) = f32x4{S[kt][4 * q], S[kt][4 * q + 1], S[kt][4 * q + 2], S[kt][4 * q + 3]};
+    } else if (MODE == Walk::outputs_state && p.fin != nullptr) {
+        float* const to = p.fin + chain * cells;
+        for_cells([&](int kt, int r, int64_t at) __attribute__((always_inline)) { to[at] = S[kt][r]; });
+    }
 }
 
 // From the segments' own states (slots 0 .. of a sequence) to what every segment but the first starts from, and to what the sequence ends
 // with where that is a result (then the last segment's own state is there as well).  A thread has 4 cells of a (sequence, head); the
 // states lie contiguous, and those of a sequence H states apart.
 __global__ __launch_bounds__(256) void linear_combine_kernel(const LinearParams p) {
-    const int64_t cells = p.cells;
     const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     const int h = blockIdx.y;
+    // the 4 cells in init and fin: a step of `apart`, `there` of them (in the registers' order the last keys and columns are padding)
+    int64_t cell = at, apart = 1;
+    bool there = at < p.cells;
+    if (p.local_keys != 0) {
+        const int lane = at / 4 % 64, q = at / 256 % 4, kt = at / 1024 % (p.local_keys / 32), v = (int)(at / 1024 / (p.local_keys / 32)) * 32 + slice_col(lane & 31);
+        const int key = 32 * kt + 16 * (q >> 1) + 8 * (lane >> 5) + 4 * (q & 1);  // (a multiple of 4, as K is of 8)
+        there = key < p.K && v < p.V;
+        cell = (int64_t)key * p.state_k + (int64_t)v * p.state_v, apart = p.state_k;
+    }
     for (int n = blockIdx.z; n < p.N; n += gridDim.z) {
         int b, t0, len;
         linear_bounds(p, n, b, t0, len);
@@ -261,12 +327,15 @@ __global__ __launch_bounds__(256) void linear_combine_kernel(const LinearParams 
             LinearSegment none;
             linear_find_packed(p, -1, none, threadIdx.x & 63, n, &slot0);
         }
-        if (slot0 + segments > p.slots || at >= cells) continue;
-        const float whole = linear_power(p.g == nullptr ? 0.f : p.g[h], p.seg);
-        float* local = p.local + ((int64_t)slot0 * p.H + h) * cells + at;
-        const int64_t next = (int64_t)p.H * cells;
+        if (slot0 + segments > p.slots || at >= p.local_cells) continue;
+        const float g = linear_log2(p.g, h), whole = linear_power(g, p.seg);
+        float* local = p.local + ((int64_t)slot0 * p.H + h) * p.local_cells + at;
+        const int64_t next = (int64_t)p.H * p.local_cells, chain = ((int64_t)n * p.H + h) * p.cells + cell;
         f32x4 carry = {0.f, 0.f, 0.f, 0.f};
-        if (p.init != nullptr) carry = *reinterpret_cast<const f32x4*>(p.init + ((int64_t)n * p.H + h) * cells + at);
+        if (p.init != nullptr && there) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) carry[e] = p.init[chain + e * apart];
+        }
         f32x4 own = *reinterpret_cast<const f32x4*>(local);
         for (int s = 1; s < segments; s++) {
             f32x4 following = {0.f, 0.f, 0.f, 0.f};
@@ -275,9 +344,10 @@ __global__ __launch_bounds__(256) void linear_combine_kernel(const LinearParams 
             *reinterpret_cast<f32x4*>(local + s * next) = carry;
             own = following;
         }
-        if (p.fin != nullptr) {  // behind the last segment, whose tokens are `rest`
-            const int rest = len - (segments - 1) * p.seg;
-            *reinterpret_cast<f32x4*>(p.fin + ((int64_t)n * p.H + h) * cells + at) = carry * linear_power(p.g == nullptr ? 0.f : p.g[h], rest) + own;
+        if (p.fin != nullptr && there) {  // behind the last segment, whose tokens are `rest`
+            const float last = linear_power(g, len - (segments - 1) * p.seg);
+#pragma unroll
+            for (int e = 0; e < 4; e++) p.fin[chain + e * apart] = carry[e] * last + own[e];
         }
     }
 }
@@ -298,6 +368,7 @@ int launch(const LinearParams& p, bool states_only, hipStream_t stream) {
 }  // namespace
 
 // (more than 128 keys: two waves would not hold the rows on their way to them in registers)
+int linear_walk_keys(int K) { return K <= 64 ? 64 : K <= 128 ? 128 : 256; }
 int linear_walk_columns(int K, int V) { return V <= 64 && K <= 128 ? 64 : 128; }
 
 int launch_linear_walk(const LinearParams& p, bool states_only, hipStream_t stream) {
@@ -308,7 +379,7 @@ int launch_linear_walk(const LinearParams& p, bool states_only, hipStream_t stre
 }
 
 int launch_linear_combine(const LinearParams& p, hipStream_t stream) {
-    hipLaunchKernelGGL(linear_combine_kernel, dim3((unsigned)((p.cells + 1023) / 1024), (unsigned)p.H, (unsigned)std::min(p.N, 32768)), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL(linear_combine_kernel, dim3((unsigned)((p.local_cells + 1023) / 1024), (unsigned)p.H, (unsigned)std::min(p.N, 32768)), dim3(256), 0, stream, p);
     return (int)hipGetLastError();
 }
 
