@@ -15,6 +15,7 @@ int check_rows(const void* p, int64_t b, int64_t t, int64_t h, int dtype) {
     const int64_t vec = dtype == GDN_BF16 ? 8 : 4;
     if (p == nullptr) return GDN_ERR_NULL;
     if (!aligned16(p) || b % vec != 0 || t % vec != 0 || h % vec != 0) return GDN_ERR_ALIGN;
+    if (t > 1 << 24 || t < -(1 << 24)) return GDN_ERR_UNSUPPORTED;  // the bytes of a chunk of 64 tokens are counted in 32 bits
     return GDN_OK;
 }
 
@@ -49,6 +50,7 @@ int check_inputs(const gdn_linear_attn_args& a) {
 // How the sequences are cut: `seg` tokens to a segment.
 struct Cut {
     int seg, nseg, slots;
+    bool chain;    // bf16: whole sequences, split over the columns of the value dim (gdn_linear_chain.hip)
     bool several;  // a sequence may have more than one segment: their states come first
 };
 
@@ -59,6 +61,7 @@ Cut cut_sequences(const gdn_linear_attn_args& a, int64_t slices, int64_t wanted,
     int64_t seg = (tokens * work + wanted - 1) / wanted;
     seg = std::max<int64_t>((seg + 63) / 64 * 64, shortest);
     Cut c;
+    c.chain = false;
     if (seg >= a.T) {
         c.seg = (a.T + 63) / 64 * 64, c.nseg = packed ? 0 : 1, c.slots = a.N, c.several = false;
         return c;
@@ -79,11 +82,31 @@ int walk_columns(const gdn_linear_attn_args& a, int K, int V) {
     return a.dtype == GDN_BF16 ? linear_walk_columns(K, V) : 32;
 }
 
-Cut cut_for_walk(const gdn_linear_attn_args& a, int K, int V) {
-    const int columns = walk_columns(a, K, V), cus = compute_units();
-    const int64_t slices = (V + columns - 1) / columns;
-    if (a.dtype == GDN_BF16) return cut_sequences(a, slices, K <= 128 ? 2 * cus : cus, 128);
+Cut cut_segments(const gdn_linear_attn_args& a) {
+    const int width = walk_columns(a, a.K, a.V), cus = compute_units();
+    const int64_t slices = (a.V + width - 1) / width;
+    if (a.dtype == GDN_BF16) return cut_sequences(a, slices, a.K <= 128 ? 2 * cus : cus, 128);
     return cut_sequences(a, slices, 4 * cus, 64);
+}
+
+// The forward in bf16: where segments would take three launches, a walk over whole sequences, 32 columns to a workgroup and one
+// workgroup to a compute unit, may be faster.  It takes 6 us and 1.2 us a chunk (0.8 up to 64 keys) of the longest sequence, for each
+// round of workgroups; the segments 30 us and 17 ns (7) for every chunk of 64 rows and 128 columns.  Measured, whole sequences against
+// segments, us, with 16 heads of 128: 4 x 4096 tokens 88 | 102, 4 x 1024 27 | 49, 8 x 4096 182 | 203, 1 x 2048 39 | 37, 2 x 4096 73 | 65,
+// 1 x 65536 with 32 heads and V = 256 1230 | 1067, 32 x 512 (one launch either way) 129 | 80; 16 heads of 64: 16 x 1024 38 | 58, 4 x 4096 56 | 58.  In the backward, where the states
+// serve two walks, the two are level (370 us at 4 x 4096 tokens), and it has segments alone.  How long the longest of packed sequences is
+// lives on the device: it may have nearly all tokens (11 of them in 32768 tokens: 404 | 257).
+Cut cut_forward(const gdn_linear_attn_args& a) {
+    const Cut segments = cut_segments(a);
+    if (a.dtype != GDN_BF16 || a.K > 128 || !segments.several) return segments;
+    const int64_t chunks = (a.T + 63) / 64, cus = compute_units();
+    const int64_t rounds = ((int64_t)a.N * a.H * ((a.V + 31) / 32) + cus - 1) / cus;
+    const int64_t blocks = (int64_t)a.B * a.H * chunks * ((a.V + 127) / 128);
+    if (rounds * (6000 + (a.K <= 64 ? 800 : 1200) * chunks) >= 30000 + (a.K <= 64 ? 7 : 17) * blocks) return segments;  // ns
+    Cut c;
+    c.seg = (a.T + 63) / 64 * 64, c.nseg = a.cu_seqlens != nullptr && !(a.flags & GDN_FLAG_LEFT_PADDED) ? 0 : 1;
+    c.slots = a.N, c.chain = true, c.several = false;
+    return c;
 }
 
 // cells of a state between the launches: bf16 in the order of the walk's registers (whole workgroups), fp32 as it is
@@ -105,7 +128,7 @@ LinearParams base_params(const gdn_linear_attn_args& a, const Cut& c) {
     p.padded = (a.flags & GDN_FLAG_LEFT_PADDED) != 0;
     p.B = a.B, p.T = a.T, p.H = a.H, p.N = a.N;
     p.cells = (int64_t)a.K * a.V;
-    p.seg = c.seg, p.nseg = c.nseg, p.slots = c.slots;
+    p.seg = c.seg, p.nseg = c.nseg, p.slots = c.slots, p.chain = c.chain;
     p.zero = (a.flags & GDN_FLAG_ZERO_PADDING) != 0;
     return p;
 }
@@ -126,6 +149,7 @@ Roles roles_of(const gdn_linear_attn_args& a) {
 void natural(LinearParams& p, int K, int V) { p.K = K, p.V = V, p.state_k = V, p.state_v = 1; }
 
 int run(const LinearParams& p, int dtype, bool states_only, hipStream_t stream) {
+    if (p.chain) return launch_linear_chain(p, stream);
     return dtype == GDN_BF16 ? launch_linear_walk(p, states_only, stream) : launch_linear_tokens(p, dtype, 32, states_only, stream);
 }
 
@@ -199,7 +223,7 @@ extern "C" int gdn_linear_abi_version(void) { return GDN_LINEAR_ABI_VERSION; }
 
 extern "C" uint64_t gdn_linear_attn_workspace_bytes(const gdn_linear_attn_args* a) {
     if (a == nullptr || check_shape(*a) != GDN_OK) return 0;
-    return states_bytes(*a, cut_for_walk(*a, a->K, a->V), local_cells(a->dtype, a->K, a->V));
+    return states_bytes(*a, cut_forward(*a), local_cells(a->dtype, a->K, a->V));
 }
 
 extern "C" int gdn_linear_attn_chunk_fwd(const gdn_linear_attn_args* args, void* stream) {
@@ -209,7 +233,7 @@ extern "C" int gdn_linear_attn_chunk_fwd(const gdn_linear_attn_args* args, void*
     if (const int e = check_inputs(a); e != GDN_OK) return e;
     if (const int e = check_rows(a.o, a.o_stride_b, a.o_stride_t, a.o_stride_h, a.dtype); e != GDN_OK) return e;
     if (a.h0 != nullptr && a.ht == a.h0) return GDN_ERR_UNSUPPORTED;
-    const Cut c = cut_for_walk(a, a.K, a.V);
+    const Cut c = cut_forward(a);
     if (c.several && (a.workspace == nullptr || a.workspace_bytes < states_bytes(a, c, local_cells(a.dtype, a.K, a.V)))) return GDN_ERR_WORKSPACE;
     if (c.several && !aligned16(a.workspace)) return GDN_ERR_ALIGN;
     const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -236,7 +260,7 @@ extern "C" int gdn_linear_attn_recurrent_fwd(const gdn_linear_attn_args* args, v
     if (const int e = check_rows(a.o, a.o_stride_b, a.o_stride_t, a.o_stride_h, a.dtype); e != GDN_OK) return e;
     const Roles r = roles_of(a);
     Cut c;
-    c.seg = (a.T + 63) / 64 * 64, c.nseg = a.cu_seqlens != nullptr && !(a.flags & GDN_FLAG_LEFT_PADDED) ? 0 : 1, c.slots = a.N, c.several = false;
+    c.seg = (a.T + 63) / 64 * 64, c.nseg = a.cu_seqlens != nullptr && !(a.flags & GDN_FLAG_LEFT_PADDED) ? 0 : 1, c.slots = a.N, c.chain = false, c.several = false;
     LinearParams p = base_params(a, c);
     natural(p, a.K, a.V);
     p.x = r.q, p.y = r.k, p.z = r.v;
@@ -249,7 +273,7 @@ extern "C" int gdn_linear_attn_recurrent_fwd(const gdn_linear_attn_args* args, v
 extern "C" uint64_t gdn_linear_attn_bwd_workspace_bytes(const gdn_linear_attn_bwd_args* b) {
     if (b == nullptr || check_shape(b->fwd) != GDN_OK) return 0;
     const gdn_linear_attn_args& a = b->fwd;
-    return BackwardSpace(a, cut_for_walk(a, a.K, a.V), b->dg != nullptr).total();
+    return BackwardSpace(a, cut_segments(a), b->dg != nullptr).total();
 }
 
 extern "C" int gdn_linear_attn_bwd(const gdn_linear_attn_bwd_args* args, void* stream) {
@@ -264,7 +288,7 @@ extern "C" int gdn_linear_attn_bwd(const gdn_linear_attn_bwd_args* args, void* s
     if (const int e = check_rows(b.dv, b.dv_stride_b, b.dv_stride_t, b.dv_stride_h, a.dtype); e != GDN_OK) return e;
     if (!aligned16(b.dht) || !aligned16(b.dh0)) return GDN_ERR_ALIGN;
     if (b.dg != nullptr && a.g == nullptr) return GDN_ERR_NULL;
-    const Cut c = cut_for_walk(a, a.K, a.V);
+    const Cut c = cut_segments(a);
     const BackwardSpace space(a, c, b.dg != nullptr);
     if (space.total() > 0) {
         if (b.workspace == nullptr || b.workspace_bytes < space.total()) return GDN_ERR_WORKSPACE;

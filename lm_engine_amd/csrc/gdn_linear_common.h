@@ -43,6 +43,7 @@ struct LinearParams {
     int seg;              // tokens of a segment
     int nseg;             // segments per row (batches, left-padded rows); 0: packed
     int slots;            // segments there is room for
+    int chain;            // the walk is the one over whole sequences (host only)
     int reverse, a;
     float os, ps, us;
     int zero;             // zeros at tokens of no sequence
@@ -175,6 +176,7 @@ __device__ __forceinline__ int64_t linear_fragment(int keys, int key, int v) {
 
 // launches, gdn_linear_walk.hip and gdn_linear_tokens.hip; `states_only`: the segments' own states into p.local
 int launch_linear_walk(const LinearParams& p, bool states_only, hipStream_t stream);
+int launch_linear_chain(const LinearParams& p, hipStream_t stream);  // gdn_linear_chain.hip: forward, bf16, up to 128 keys, whole sequences
 int launch_linear_tokens(const LinearParams& p, int dtype, int columns, bool states_only, hipStream_t stream);
 int linear_walk_keys(int K);            // keys that the bf16 walk is built for
 int linear_walk_columns(int K, int V);  // columns of the value dim that a workgroup of the bf16 walk has

@@ -80,11 +80,13 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : 1) void linear_tangen
         else if (p.init != nullptr) for_cells([&](int kt, int r, int64_t at) { S[kt][r] = p.init[chain * cells + at]; });
     }
 
+    const TileLane<KD> tile(lane);
+    const TileLane<VC> ztile(lane);
     // B fragments (reduction over rows, column = this lane's) of a tile's columns of this wave, weighted, in two parts
-    auto weighted = [&](const bf16_t* tile, const float* weights, bf16x8 (&hi)[4], bf16x8 (&lo)[4]) {
+    auto weighted = [&](const bf16_t* rows_of, const float* weights, bf16x8 (&hi)[4], bf16x8 (&lo)[4]) {
 #pragma unroll
         for (int s = 0; s < 4; s++) {
-            const bf16x8 rows = tile_tr8<VC>(tile, 16 * s, 32 * wave, lane);
+            const bf16x8 rows = ztile.transposed(rows_of, s, wave);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float x = (float)rows[e] * weights[16 * s + 8 * half + e];
@@ -93,10 +95,10 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : 1) void linear_tangen
             }
         }
     };
-    auto product = [&](const bf16_t* tile, int kt, const bf16x8 (&hi)[4], const bf16x8 (&lo)[4], f32x16 acc) {
+    auto product = [&](const bf16_t* rows_of, int kt, const bf16x8 (&hi)[4], const bf16x8 (&lo)[4], f32x16 acc) {
 #pragma unroll
         for (int s = 0; s < 4; s++) {
-            const bf16x8 a = tile_tr8<KD>(tile, 16 * s, 32 * kt, lane);
+            const bf16x8 a = tile.transposed(rows_of, s, kt);
             acc = mfma32_bf16(a, hi[s], acc);
             acc = mfma32_bf16(a, lo[s], acc);
         }
@@ -146,10 +148,10 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : 1) void linear_tangen
                 f32x16 A = {}, B = {};
 #pragma unroll
                 for (int s = 0; s < KD / 16; s++)
-                    A = mfma32_bf16(tile_row8<KD>(sk, 32 * jt + l32, 2 * s + half), tile_row8<KD>(sq, 32 * it + l32, 2 * s + half), A);
+                    A = mfma32_bf16(tile.fragment(sk, 32 * jt, s), tile.fragment(sq, 32 * it, s), A);
 #pragma unroll
                 for (int s = 0; s < 2; s++)
-                    B = mfma32_bf16(tile_row8<VC>(sv, 32 * jt + l32, 4 * wave + 2 * s + half), tile_row8<VC>(sd, 32 * it + l32, 4 * wave + 2 * s + half), B);
+                    B = mfma32_bf16(ztile.fragment(sv, 32 * jt, 2 * wave + s), ztile.fragment(sd, 32 * it, 2 * wave + s), B);
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const int distance = 32 * it + l32 - (32 * jt + 8 * (r >> 2) + 4 * half + (r & 3));

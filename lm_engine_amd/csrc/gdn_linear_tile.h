@@ -8,65 +8,49 @@ namespace gdn {
 
 constexpr int LC = 64;  // tokens of a chunk
 
-// 16-byte granule g of row r of an LDS tile lies at granule g ^ key(r): 8 lanes that read one granule of 8 consecutive rows, or of
-// rows {0 - 3, 8 - 11} (the swapped order), and 16 lanes that read two neighbouring granules of 4 rows (the transposing read), then
-// touch every bank once.
-__device__ __forceinline__ int tile_key(int r) { return ((r & 3) << 1) | (((r >> 2) ^ (r >> 3)) & 1); }
-
+// 16-byte granule g of row r of an LDS tile of LD columns lies at granule g ^ key(r).  LDS has 64 banks of 4 bytes; a read of 16 bytes
+// per lane takes 16 lanes at a time, the transposing read of 8 bytes 32.  With this key one granule of 16 consecutive rows, and 4
+// neighbouring granules of 4 consecutive rows, touch every bank once.  (Rows of LD = 64 or 192 columns are odd multiples of half the
+// banks: the row's lowest bit is in the address already.)
 template <int LD>
-__device__ __forceinline__ bf16x8 tile_row8(const bf16_t* m, int row, int granule) {
-    return *reinterpret_cast<const bf16x8*>(m + row * LD + ((granule ^ tile_key(row)) << 3));
+__device__ __forceinline__ constexpr int tile_key(int r) {
+    return LD % 128 == 0 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r & 2) << 1) | ((r >> 2) & 3);
 }
 
-// lane i of a 16-lane group: rows row0 .. row0 + 3 of column col0 + sigma(i), sigma the swap of bits 2 and 3
-template <int LD>
-__device__ __forceinline__ bf16x4 tile_tr4(const bf16_t* m, int row0, int col0, int l16) {
-    const int q = l16 & 3, row = row0 + (l16 >> 2);
-    const int col = col0 + 4 * (((q & 1) << 1) | (q >> 1));
-    const bf16_t* p = m + row * LD + (((col >> 3) ^ tile_key(row)) << 3) + (col & 7);
-    const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
-    return __builtin_bit_cast(bf16x4, v);
-}
-
-// A operand: row m = column col0 + swap(m) of the tile, reduction index = rows row0 + 0 .. 15
-template <int LD>
-__device__ __forceinline__ bf16x8 tile_tr8(const bf16_t* m, int row0, int col0, int lane) {
-    const int r = row0 + 8 * (lane >> 5), c = col0 + 16 * ((lane >> 4) & 1), l16 = lane & 15;
-    const bf16x4 lo = tile_tr4<LD>(m, r, c, l16), hi = tile_tr4<LD>(m, r + 4, c, l16);
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-
-// Where a lane of v_mfma_f32_32x32x16_bf16 reads a tile of LD columns.  The key of a row is that of the row 16 further on, and a step
-// of 64 columns changes no bit that the key touches; within 64 columns a step is one of bits that are exclusive-ored anyway.  So three
+// Where a lane of v_mfma_f32_32x32x16_bf16 reads a tile of LD columns.  The key of a row is that of the row 16 further on, a step of
+// PERIOD columns changes no bit that the key touches, and smaller steps are ones of bits that are exclusive-ored anyway.  So three
 // offsets do for a whole tile.
 template <int LD>
 struct TileLane {
+    static constexpr int PERIOD = LD % 128 == 0 ? 128 : 64;
     int row, swapped, pair;
 
     __device__ __forceinline__ TileLane(int lane) {
         const int l32 = lane & 31, half = lane >> 5, q = lane & 3;
-        row = l32 * LD + ((half ^ tile_key(l32)) << 3);
-        swapped = slice_col(l32) * LD + ((half ^ tile_key(slice_col(l32))) << 3);
+        row = l32 * LD + ((half ^ tile_key<LD>(l32)) << 3);
+        swapped = slice_col(l32) * LD + ((half ^ tile_key<LD>(slice_col(l32))) << 3);
         const int r = 8 * half + ((lane & 15) >> 2), c = 16 * ((lane >> 4) & 1) + 4 * (((q & 1) << 1) | (q >> 1));
-        pair = r * LD + (((c >> 3) ^ tile_key(r)) << 3) + (c & 7);
+        pair = r * LD + (((c >> 3) ^ tile_key<LD>(r)) << 3) + (c & 7);
     }
     // x where it is used, rather than what follows from x in registers over a whole walk
     __device__ __forceinline__ void recompute() { asm volatile("" : "+v"(row), "+v"(swapped), "+v"(pair)); }
     // 8 columns 16 s + 8 half .. of row row0 + l32; row0 a multiple of 32
     __device__ __forceinline__ bf16x8 fragment(const bf16_t* tile, int row0, int s) const {
-        return *reinterpret_cast<const bf16x8*>(tile + (row ^ (16 * (s & 3))) + row0 * LD + (s >> 2) * 64);
+        return *reinterpret_cast<const bf16x8*>(tile + (row ^ (16 * s % PERIOD)) + row0 * LD + 16 * s / PERIOD * PERIOD);
     }
     // ... of row row0 + swap(l32)
     __device__ __forceinline__ bf16x8 swapped_fragment(const bf16_t* tile, int row0, int s) const {
-        return *reinterpret_cast<const bf16x8*>(tile + (swapped ^ (16 * (s & 3))) + row0 * LD + (s >> 2) * 64);
+        return *reinterpret_cast<const bf16x8*>(tile + (swapped ^ (16 * s % PERIOD)) + row0 * LD + 16 * s / PERIOD * PERIOD);
     }
     // rows 16 s + 8 half .. + 7 of column 32 t + swap(l32)
     __device__ __forceinline__ bf16x8 transposed(const bf16_t* tile, int s, int t) const {
-        const bf16_t* const p = tile + 16 * s * LD + (t >> 1) * 64;
-        const int at = pair ^ (32 * (t & 1));
+        const bf16_t* const p = tile + 16 * s * LD + 32 * t / PERIOD * PERIOD;
+        const int at = pair ^ (32 * t % PERIOD);
+        // 4 rows on, the key's lowest bit is the other
         const bf16x4 lo = read(p + at), hi = read(p + (at ^ 8) + 4 * LD);
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
+    // 4 rows of 16 columns: lane i of a 16-lane group gets column i of them; lanes 4 r .. 4 r + 3 address row r, 4 columns each
     static __device__ __forceinline__ bf16x4 read(const bf16_t* p) {
         const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
         return __builtin_bit_cast(bf16x4, v);
@@ -101,28 +85,34 @@ struct Stream {
         step_bytes = (reverse ? -STEP : STEP) * row_bytes;
     }
     __device__ __forceinline__ bool there(int i, int rows) const { return in_columns && r0 + i * STEP < rows; }
-    // the next chunk, all of it, or (`whole` false) the `rows` rows and the columns that there are
-    __device__ __forceinline__ void fetch(bf16x8 (&v)[ITERS], int rows, bool whole) {
+    // chunk c, all of it, or (`whole` false) the `rows` rows and the columns that there are
+    __device__ __forceinline__ void fetch_chunk(int c, bf16x8 (&v)[ITERS], int rows, bool whole) const {
+        const char* const from = base + c * chunk_bytes;
         if (whole) {
 #pragma unroll
-            for (int i = 0; i < ITERS; i++) v[i] = *reinterpret_cast<const bf16x8*>(base + i * step_bytes + offset);
+            for (int i = 0; i < ITERS; i++) v[i] = *reinterpret_cast<const bf16x8*>(from + i * step_bytes + offset);
         } else {
 #pragma unroll
             for (int i = 0; i < ITERS; i++) {
-                // (an address of the chunk's, whichever: the first row's)
-                v[i] = *reinterpret_cast<const bf16x8*>(base + (there(i, rows) ? offset + (uint32_t)(i * step_bytes) : first));
+                // (else an address of the chunk's, whichever: the first row's; by bits, a choice between the two members goes through memory)
+                const uint32_t here = there(i, rows) ? ~0u : 0u;
+                v[i] = *reinterpret_cast<const bf16x8*>(from + (((offset + (uint32_t)(i * step_bytes)) & here) | (first & ~here)));
             }
         }
+    }
+    // the next chunk
+    __device__ __forceinline__ void fetch(bf16x8 (&v)[ITERS], int rows, bool whole) {
+        fetch_chunk(0, v, rows, whole);
         base += chunk_bytes;
     }
     template <int LD = COLS>
     __device__ __forceinline__ void stage(bf16_t* tile, const bf16x8 (&v)[ITERS], int rows, bool whole) const {
-        bf16_t* const at = tile + r0 * LD + ((threadIdx.x % GRANULES ^ tile_key(r0)) << 3);  // (STEP rows on: the same key)
+        bf16_t* const at = tile + r0 * LD + ((threadIdx.x % GRANULES ^ tile_key<LD>(r0)) << 3);  // (STEP rows on: the same key)
 #pragma unroll
         for (int i = 0; i < ITERS; i++) {
             const int r = r0 + i * STEP;
             const bf16x8 zero = {};
-            bf16_t* const to = STEP % 16 == 0 ? at + i * STEP * LD : tile + r * LD + ((threadIdx.x % GRANULES ^ tile_key(r)) << 3);
+            bf16_t* const to = STEP % 16 == 0 ? at + i * STEP * LD : tile + r * LD + ((threadIdx.x % GRANULES ^ tile_key<LD>(r)) << 3);
             *reinterpret_cast<bf16x8*>(to) = whole || there(i, rows) ? v[i] : zero;
         }
     }

@@ -163,7 +163,7 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel
         for (int i = 0; i < Out::ITERS; i++) {
             const int r = os.r0 + i * Out::STEP;
             if (os.there(i, rows))
-                *reinterpret_cast<bf16x8*>(to + i * os.step_bytes + os.offset) = *reinterpret_cast<const bf16x8*>(so + r * VC + ((tid % Out::GRANULES ^ tile_key(r)) << 3));
+                *reinterpret_cast<bf16x8*>(to + i * os.step_bytes + os.offset) = *reinterpret_cast<const bf16x8*>(so + r * VC + ((tid % Out::GRANULES ^ tile_key<VC>(r)) << 3));
         }
         os.base += os.chunk_bytes;
     };
@@ -175,8 +175,6 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel
     for (int c = 0; c < chunks; c++) {
         const int rows = min(LC, total - c * LC);
         __syncthreads();  // the tiles of the chunk before are read, its output is in LDS
-        if constexpr (!STATES_ONLY && !SUMS)
-            if (c > 0) leave(LC);
         if (rows < LC && tid < LC) sw[tid] = p.us * linear_power(g, max(rows - a - tid, 0));
         if (rows == LC && whole_rows) {
             ys.stage(sy, ry, rows, true), zs.stage(sz, rz, rows, true);
@@ -185,6 +183,9 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel
             ys.stage(sy, ry, rows, false), zs.stage(sz, rz, rows, false);
             if constexpr (!STATES_ONLY) xs.stage(sx, rx, rows, false);
         }
+        // (behind the wait for the rows, which stores in front of it would be part of)
+        if constexpr (!STATES_ONLY && !SUMS)
+            if (c > 0) leave(LC);
         __syncthreads();
         if (c + 1 < chunks) fetch(total - (c + 1) * LC);
         tile.recompute(), ztile.recompute();
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel
                         bf16_t* const out = static_cast<bf16_t*>(p.out) + sg.b * p.out_stride_b + h * p.out_stride_h + token_row * p.out_stride_t;
                         *reinterpret_cast<bf16x8*>(out + col + 16 * s) = pack8_16(O[i], s, 1.f);
                     } else {
-                        *reinterpret_cast<bf16x8*>(so + row * VC + ((4 * wave + 2 * s + half ^ tile_key(row)) << 3)) = pack8_16(O[i], s, 1.f);
+                        *reinterpret_cast<bf16x8*>(so + row * VC + (((4 * wave + 2 * s + half) ^ tile_key<VC>(row)) << 3)) = pack8_16(O[i], s, 1.f);
                     }
                 }
             }

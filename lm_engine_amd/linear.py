@@ -93,8 +93,8 @@ def _aligned(x: torch.Tensor) -> torch.Tensor:
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
-    """``x``, or a copy where its rows cannot be read in 16-byte pieces."""
-    return kernel_rows(x, 16 // x.element_size())
+    """``x``, or a copy where its rows cannot be read in 16-byte pieces or lie too far apart for the kernels' 32-bit offsets in a chunk."""
+    return x.clone(memory_format=torch.contiguous_format) if x.stride(1) > 1 << 24 else kernel_rows(x, 16 // x.element_size())
 
 
 def _set_rows(args, name, x) -> None:
