@@ -1,4 +1,5 @@
-// The host path of the entry points and of their backward passes: from torch tensors to the calls of the C ABI (include/gdn_hip.h).
+// The host path of the entry points and of their backward passes: from torch tensors to the calls of the C ABI (include/gdn_hip.h,
+// include/gdn_linear_hip.h).
 //
 // On a decode step, a short prompt or a short training sequence the GPU needs a few microseconds per kernel, and reading shapes,
 // strides and pointers out of tensors, allocating the results and filling the argument structs takes 10 to 60 in Python per call.
@@ -19,6 +20,7 @@
 #include <initializer_list>
 
 #include "gdn_hip.h"
+#include "gdn_linear_hip.h"
 
 namespace {
 
@@ -40,6 +42,15 @@ decltype(&gdn_gated_rmsnorm_bwd) norm_bwd_fn = nullptr;
 decltype(&gdn_column_sums) column_sums_fn = nullptr;
 decltype(&gdn_fold_heads) fold_heads_fn = nullptr;
 decltype(&gdn_layer_front) layer_front_fn = nullptr;
+decltype(&gdn_linear_attn_chunk_fwd) linear_chunk_fn = nullptr;
+decltype(&gdn_linear_attn_workspace_bytes) linear_workspace_fn = nullptr;
+decltype(&gdn_linear_attn_recurrent_fwd) linear_recurrent_fn = nullptr;
+decltype(&gdn_linear_attn_bwd) linear_bwd_fn = nullptr;
+decltype(&gdn_linear_attn_bwd_workspace_bytes) linear_bwd_workspace_fn = nullptr;
+decltype(&gdn_linear_fold_heads) linear_fold_fn = nullptr;
+decltype(&gdn_layer_norm_fwd) layer_norm_fn = nullptr;
+decltype(&gdn_layer_norm_bwd) layer_norm_bwd_fn = nullptr;
+decltype(&gdn_layer_norm_partial_blocks) layer_norm_blocks_fn = nullptr;
 PyObject* check_status = nullptr;  // _lib.check_status: raises what a status stands for
 
 // bind(check_status, addresses...)
@@ -47,7 +58,10 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     void** slots[] = {(void**)&layer_step_fn, (void**)&layer_step_tiles_fn, (void**)&conv_fn, (void**)&gates_fn, (void**)&norm_fn,
                       (void**)&recurrent_fn, (void**)&chunk_fn, (void**)&workspace_bytes_fn, (void**)&one_launch_fn,
                       (void**)&sweeps_fn, (void**)&sweeps_workspace_fn, (void**)&local_fn, (void**)&conv_bwd_fn, (void**)&gates_bwd_fn,
-                      (void**)&norm_bwd_fn, (void**)&column_sums_fn, (void**)&fold_heads_fn, (void**)&layer_front_fn};
+                      (void**)&norm_bwd_fn, (void**)&column_sums_fn, (void**)&fold_heads_fn, (void**)&layer_front_fn,
+                      (void**)&linear_chunk_fn, (void**)&linear_workspace_fn, (void**)&linear_recurrent_fn, (void**)&linear_bwd_fn,
+                      (void**)&linear_bwd_workspace_fn, (void**)&linear_fold_fn, (void**)&layer_norm_fn, (void**)&layer_norm_bwd_fn,
+                      (void**)&layer_norm_blocks_fn};
     constexpr Py_ssize_t count = sizeof(slots) / sizeof(slots[0]);
     if (n != count + 1) return PyErr_Format(PyExc_TypeError, "bind takes a function and %zd addresses, got %zd arguments", count, n);
     for (Py_ssize_t i = 0; i < count; i++) {
@@ -718,6 +732,182 @@ PyObject* norm_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// ---- linear attention with a decay for each head, layer norm
+
+struct LinearOperands {
+    gdn_linear_attn_args s{};
+    const at::Tensor *g, *h0, *cu;
+    int64_t B, T, HK, K, H, V, N;
+
+    // q, k, v, g, scale or None, initial_state, cu_seqlens, left_padded
+    LinearOperands(Operands& operand, PyObject* const* args) : g(operand.optional(args[3])), h0(operand.optional(args[5])), cu(operand.optional(args[6])) {
+        const at::Tensor &q = operand(args[0]), &k = operand(args[1]), &v = operand(args[2]);
+        const bool padded = truth(args[7]);
+        s.dtype = code_of(q);
+        need(q.dim() == 4 && k.sizes() == q.sizes() && v.dim() == 4 && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type());
+        B = q.size(0), T = q.size(1), HK = q.size(2), K = q.size(3), H = v.size(2), V = v.size(3);
+        need(v.size(0) == B && v.size(1) == T && B > 0 && T > 0 && HK > 0 && H > 0 && H % HK == 0 && q.stride(3) == 1 && k.stride(3) == 1 && v.stride(3) == 1);
+        N = B;
+        if (padded) need(cu != nullptr && cu->dim() == 1 && cu->numel() == B + 1);
+        else if (cu != nullptr) {
+            need(B == 1 && cu->dim() == 1 && cu->numel() >= 2);
+            N = cu->numel() - 1;
+        }
+        if (cu != nullptr) need(cu->scalar_type() == at::kInt && cu->is_contiguous());
+        if (g != nullptr) need(g->scalar_type() == at::kFloat && g->dim() == 1 && g->size(0) == H && g->is_contiguous());
+        if (h0 != nullptr) need(h0->scalar_type() == at::kFloat && h0->sizes() == at::IntArrayRef({N, H, K, V}) && h0->is_contiguous());
+        s.B = size32(B), s.T = size32(T), s.H = size32(H), s.K = size32(K), s.V = size32(V), s.N = size32(N);
+        s.qk_heads = HK == H ? 0 : (int32_t)HK;
+        s.flags = GDN_FLAG_ZERO_PADDING | (padded ? GDN_FLAG_LEFT_PADDED : 0);
+        s.scale = args[4] == Py_None ? (float)std::pow((double)K, -0.5) : (float)number(args[4]);
+        s.q = ptr(q), s.k = ptr(k), s.v = ptr(v);
+        s.g = static_cast<const float*>(ptr(g)), s.h0 = static_cast<const float*>(ptr(h0)), s.cu_seqlens = static_cast<const int32_t*>(ptr(cu));
+        s.q_stride_b = q.stride(0), s.q_stride_t = q.stride(1), s.q_stride_h = q.stride(2);
+        s.k_stride_b = k.stride(0), s.k_stride_t = k.stride(1), s.k_stride_h = k.stride(2);
+        s.v_stride_b = v.stride(0), s.v_stride_t = v.stride(1), s.v_stride_h = v.stride(2);
+    }
+};
+
+at::Tensor workspace_of(uint64_t bytes, const at::Tensor& like) {
+    return bytes == 0 ? at::Tensor() : at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+}
+
+// linear_attention(stream, chunked, q, k, v, g, scale or None, initial_state, cu_seqlens, left_padded, output_final_state, inplace)
+//   -> (o, final_state or None)
+PyObject* linear_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return fast_path(n, 12, [&]() -> PyObject* {
+        Operands operand;
+        void* const stream = stream_of(args[0]);
+        const bool chunked = truth(args[1]), output_final = truth(args[10]), inplace = truth(args[11]);
+        const at::Tensor& v = operand(args[4]);
+        LinearOperands x(operand, args + 2);
+        gdn_linear_attn_args& s = x.s;
+        at::Tensor workspace, o, ht;
+        if (inplace) need(!chunked && output_final && x.h0 != nullptr), ht = *x.h0;
+        without_interpreter_lock([&] {
+            if (chunked && (s.workspace_bytes = linear_workspace_fn(&s)) > 0) workspace = workspace_of(s.workspace_bytes, v), s.workspace = ptr(workspace);
+            o = fresh(v, {x.B, x.T, x.H, x.V});
+            if (output_final && !inplace) ht = fresh_f32(v, {x.N, x.H, x.K, x.V});
+        });
+        if (output_final) s.ht = static_cast<float*>(ptr(ht));
+        s.o = ptr(o), s.o_stride_b = o.stride(0), s.o_stride_t = o.stride(1), s.o_stride_h = o.stride(2);
+        THPObjectPtr results(pack_results({o, ht}));
+        if (results && inplace) PyTuple_SetItem(results.get(), 1, Py_NewRef(args[7]));  // the caller's own tensor object
+        return launch(chunked ? "gdn_linear_attn_chunk_fwd" : "gdn_linear_attn_recurrent_fwd", results.release(),
+                      [&] { return (chunked ? linear_chunk_fn : linear_recurrent_fn)(&s, stream); });
+    });
+}
+
+// linear_attention_bwd(stream, q, k, v, g, scale or None, initial_state, cu_seqlens, left_padded, do, dht, needs_dg, needs_dh0)
+//   -> (dq, dk, dv, dg, dh0)
+PyObject* linear_attention_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return fast_path(n, 13, [&]() -> PyObject* {
+        Operands operand;
+        void* const stream = stream_of(args[0]);
+        const at::Tensor &v = operand(args[3]), &d = operand(args[9]);
+        const at::Tensor* const dht = operand.optional(args[10]);
+        const bool needs_dg = truth(args[11]), needs_dh0 = truth(args[12]);
+        const LinearOperands x(operand, args + 1);
+        gdn_linear_attn_bwd_args b{};
+        b.fwd = x.s;
+        need(d.scalar_type() == v.scalar_type() && d.sizes() == v.sizes() && d.stride(3) == 1 && (!needs_dg || x.g != nullptr));
+        if (dht != nullptr) need(dht->scalar_type() == at::kFloat && dht->sizes() == at::IntArrayRef({x.N, x.H, x.K, x.V}) && dht->is_contiguous());
+        const bool shared = x.HK < x.H;
+        const int group = (int)(x.H / x.HK);
+        at::Tensor dq, dk, dv, dg, dh0, workspace, dq_shared, dk_shared;
+        static float wanted;  // (that dg is not NULL is what its workspace goes by)
+        b.dg = needs_dg ? &wanted : nullptr;
+        without_interpreter_lock([&] {
+            b.workspace_bytes = linear_bwd_workspace_fn(&b);
+            workspace = workspace_of(b.workspace_bytes, v);
+            dq = fresh(v, {x.B, x.T, x.H, x.K}), dk = fresh(v, {x.B, x.T, x.H, x.K}), dv = fresh(v, {x.B, x.T, x.H, x.V});
+            if (shared) dq_shared = fresh(v, {x.B, x.T, x.HK, x.K}), dk_shared = fresh(v, {x.B, x.T, x.HK, x.K});
+            if (needs_dg) dg = fresh_f32(v, {x.H});
+            if (needs_dh0) dh0 = fresh_f32(v, {x.N, x.H, x.K, x.V});
+        });
+        b.workspace = workspace.defined() ? ptr(workspace) : nullptr;
+        b.dout = ptr(d), b.dht = static_cast<const float*>(ptr(dht));
+        b.dq = ptr(dq), b.dk = ptr(dk), b.dv = ptr(dv);
+        b.dg = needs_dg ? static_cast<float*>(ptr(dg)) : nullptr, b.dh0 = needs_dh0 ? static_cast<float*>(ptr(dh0)) : nullptr;
+        b.dout_stride_b = d.stride(0), b.dout_stride_t = d.stride(1), b.dout_stride_h = d.stride(2);
+        b.dq_stride_b = b.dk_stride_b = x.T * x.H * x.K, b.dq_stride_t = b.dk_stride_t = x.H * x.K, b.dq_stride_h = b.dk_stride_h = x.K;
+        b.dv_stride_b = x.T * x.H * x.V, b.dv_stride_t = x.H * x.V, b.dv_stride_h = x.V;
+        return launch("gdn_linear_attn_bwd", pack_results({shared ? dq_shared : dq, shared ? dk_shared : dk, dv, dg, dh0}), [&] {
+            const int status = linear_bwd_fn(&b, stream);
+            if (status != GDN_OK || !shared) return status;
+            const int64_t tokens = x.B * x.T, row = x.HK * x.K;
+            if (x.s.dtype == GDN_BF16) return fold_heads_fn(b.dq, b.dk, ptr(dq_shared), ptr(dk_shared), tokens, (int)x.HK, group, (int)x.K, row, stream);
+            return linear_fold_fn(static_cast<const float*>(b.dq), static_cast<const float*>(b.dk), static_cast<float*>(ptr(dq_shared)),
+                                  static_cast<float*>(ptr(dk_shared)), tokens, (int)x.HK, group, (int)x.K, stream);
+        });
+    });
+}
+
+// x [.., D] as rows, weight and bias [D]
+struct LayerNormOperands {
+    int64_t D, rows, stride;
+    int32_t dtype, w_dtype = GDN_F32;
+    LayerNormOperands(const at::Tensor& x, const at::Tensor* weight, const at::Tensor* bias) {
+        need(x.dim() >= 2 && x.numel() > 0);
+        dtype = code_of(x), D = x.size(-1), rows = x.numel() / D, stride = row_stride(x, D);
+        need(D <= GDN_LAYER_NORM_MAX_D);
+        for (const at::Tensor* const p : {weight, bias})
+            if (p != nullptr) {
+                need(p->dim() == 1 && p->size(0) == D && p->is_contiguous());
+                w_dtype = code_of(*p);
+            }
+        if (weight != nullptr && bias != nullptr) need(weight->scalar_type() == bias->scalar_type());
+    }
+};
+
+// layer_norm(stream, x, weight, bias, eps) -> y
+PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return fast_path(n, 5, [&]() -> PyObject* {
+        Operands operand;
+        void* const stream = stream_of(args[0]);
+        const at::Tensor& x = operand(args[1]);
+        const at::Tensor *weight = operand.optional(args[2]), *bias = operand.optional(args[3]);
+        const LayerNormOperands l(x, weight, bias);
+        gdn_layer_norm_args s{};
+        const at::Tensor y = without_interpreter_lock([&] { return at::empty(x.sizes(), x.options()); });
+        s.x = ptr(x), s.weight = ptr(weight), s.bias = ptr(bias), s.y = ptr(y);
+        s.x_stride = l.stride, s.y_stride = l.D, s.rows = l.rows, s.D = (int32_t)l.D, s.dtype = l.dtype, s.w_dtype = l.w_dtype, s.eps = (float)number(args[4]);
+        return launch("gdn_layer_norm_fwd", THPVariable_Wrap(y), [&] { return layer_norm_fn(&s, stream); });
+    });
+}
+
+// layer_norm_bwd(stream, x, weight, eps, dy, needs_dweight, needs_dbias, dbias_is_bf16) -> (dx, dweight, dbias)
+PyObject* layer_norm_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return fast_path(n, 8, [&]() -> PyObject* {
+        Operands operand;
+        void* const stream = stream_of(args[0]);
+        const at::Tensor &x = operand(args[1]), &dy = operand(args[4]);
+        const at::Tensor* weight = operand.optional(args[2]);
+        const bool needs_dw = truth(args[5]), needs_db = truth(args[6]);
+        const auto db_type = truth(args[7]) ? at::kBFloat16 : at::kFloat;
+        const LayerNormOperands l(x, weight, nullptr);
+        need(dy.scalar_type() == x.scalar_type() && dy.sizes() == x.sizes() && (!needs_dw || weight != nullptr));
+        gdn_layer_norm_bwd_args s{};
+        s.x_stride = l.stride, s.dy_stride = row_stride(dy, l.D), s.dx_stride = l.D, s.rows = l.rows, s.D = (int32_t)l.D;
+        s.dtype = l.dtype, s.w_dtype = l.w_dtype, s.eps = (float)number(args[3]);
+        at::Tensor dx, dw_part, db_part, dw, db;
+        without_interpreter_lock([&] {
+            s.partial_blocks = layer_norm_blocks_fn(l.rows, s.D, l.dtype);
+            dx = at::empty(x.sizes(), x.options());
+            if (needs_dw) dw_part = fresh_f32(x, {s.partial_blocks, l.D}), dw = at::empty({l.D}, weight->options());
+            if (needs_db) db_part = fresh_f32(x, {s.partial_blocks, l.D}), db = at::empty({l.D}, x.options().dtype(db_type));
+        });
+        s.x = ptr(x), s.dy = ptr(dy), s.weight = ptr(weight), s.dx = ptr(dx);
+        ColumnSums sums;
+        if (needs_dw) s.dweight_partial = static_cast<float*>(ptr(dw_part)), sums.add(dw_part, dw);
+        if (needs_db) s.dbias_partial = static_cast<float*>(ptr(db_part)), sums.add(db_part, db);
+        return launch("gdn_layer_norm_bwd, gdn_column_sums", pack_results({dx, dw, db}), [&] {
+            const int status = layer_norm_bwd_fn(&s, stream);
+            return status == GDN_OK && sums.s.arrays > 0 ? column_sums_fn(&sums.s, stream) : status;
+        });
+    });
+}
+
 PyMethodDef methods[] = {
     {"bind", (PyCFunction)(void (*)())bind, METH_FASTCALL, "takes the addresses of the library's entry points"},
     {"layer_step", (PyCFunction)(void (*)())layer_step, METH_FASTCALL, "gdn_layer_step"},
@@ -730,6 +920,10 @@ PyMethodDef methods[] = {
     {"conv_bwd", (PyCFunction)(void (*)())conv_bwd, METH_FASTCALL, "gdn_causal_conv1d_bwd, gdn_column_sums"},
     {"gates_bwd", (PyCFunction)(void (*)())gates_bwd, METH_FASTCALL, "gdn_gates_bwd, gdn_column_sums"},
     {"norm_bwd", (PyCFunction)(void (*)())norm_bwd, METH_FASTCALL, "gdn_gated_rmsnorm_bwd, gdn_column_sums"},
+    {"linear_attention", (PyCFunction)(void (*)())linear_attention, METH_FASTCALL, "gdn_linear_attn_chunk_fwd or gdn_linear_attn_recurrent_fwd"},
+    {"linear_attention_bwd", (PyCFunction)(void (*)())linear_attention_bwd, METH_FASTCALL, "gdn_linear_attn_bwd"},
+    {"layer_norm", (PyCFunction)(void (*)())layer_norm, METH_FASTCALL, "gdn_layer_norm_fwd"},
+    {"layer_norm_bwd", (PyCFunction)(void (*)())layer_norm_bwd, METH_FASTCALL, "gdn_layer_norm_bwd, gdn_column_sums"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "gdn_host", "host path of the entry points and their backward passes", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -170,6 +170,31 @@ int launch_of(const LinearParams& p, int columns, bool states_only, hipStream_t 
     return launch<T, 32, 32>(p, states_only, stream);
 }
 
+// Gradients of shared heads of q and k, added up: a thread has 4 columns of one head (blockIdx.y: of which of the two).  Bound by
+// memory: group + 1 rows for each one written.
+struct FoldParams {
+    const float* in[2];
+    float* out[2];
+    int64_t pieces;  // of 4 columns, over all tokens
+    int group, D;
+};
+
+__global__ __launch_bounds__(256) void linear_fold_kernel(const FoldParams p) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= p.pieces) return;
+    const int per_head = p.D / 4;
+    const int64_t row = i / per_head;
+    const int c = (int)(i - row * per_head) * 4;
+    const float* const in = p.in[blockIdx.y] + row * p.group * p.D + c;
+    f32x4 sum = *reinterpret_cast<const f32x4*>(in);
+    for (int j = 1; j < p.group; j++) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(in + (int64_t)j * p.D);
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum[e] += x[e];
+    }
+    *reinterpret_cast<f32x4*>(p.out[blockIdx.y] + row * p.D + c) = sum;
+}
+
 }  // namespace
 
 int linear_tokens_columns(int64_t chains, int V, int cus) { return V >= 128 && chains * ((V + 127) / 128) >= cus ? 128 : 32; }
@@ -179,3 +204,20 @@ int launch_linear_tokens(const LinearParams& p, int dtype, int columns, bool sta
 }
 
 }  // namespace gdn
+
+extern "C" int gdn_linear_fold_heads(const float* a, const float* b, float* out_a, float* out_b, int64_t tokens, int heads, int group, int D,
+                                     void* stream) {
+    const void* ptrs[] = {a, b, out_a, out_b};
+    for (const void* x : ptrs)
+        if (x == nullptr) return GDN_ERR_NULL;
+        else if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return GDN_ERR_ALIGN;
+    if (tokens <= 0 || heads <= 0 || group <= 0 || D <= 0) return GDN_ERR_SHAPE;
+    if (D % 4 != 0) return GDN_ERR_ALIGN;
+    gdn::FoldParams p;
+    p.in[0] = a, p.in[1] = b, p.out[0] = out_a, p.out[1] = out_b;
+    p.pieces = tokens * heads * (D / 4), p.group = group, p.D = D;
+    const int64_t blocks = (p.pieces + 255) / 256;
+    if (blocks > (int64_t)0xffffffff / 256) return GDN_ERR_UNSUPPORTED;  // (a launch holds at most 2^32 - 1 threads)
+    hipLaunchKernelGGL(gdn::linear_fold_kernel, dim3((unsigned)blocks, 2), dim3(256), 0, static_cast<hipStream_t>(stream), p);
+    return (int)hipGetLastError();
+}

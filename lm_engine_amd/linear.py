@@ -28,6 +28,7 @@ import torch
 
 from . import _lib
 from ._autograd import kernel_rows
+from ._host import host, raw_stream
 from .kernels import Kernel, is_kernel_allowed
 from .ops import RECURRENT_MAX_TOKENS, _dtype_code
 
@@ -160,6 +161,14 @@ def _run(mode, q, k, v, g, scale, initial_state, output_final_state, cu_seqlens,
     return o, (initial_state if inplace_state else ht)
 
 
+def _on_host_path(mode, q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, inplace_state, left_padded):
+    """``(o, final_state)``, or None where the operands need a conversion, a gradient or a report."""
+    if not q.is_cuda or not is_kernel_allowed(Kernel.linear_attention):
+        return None
+    return host().linear_attention(raw_stream(q.get_device()), mode == "chunk", q, k, v, g, scale, initial_state, cu_seqlens, left_padded,
+                                   output_final_state, inplace_state)  # fmt: skip
+
+
 def _backward(q, k, v, g, scale, initial_state, cu_seqlens, left_padded, do, dht, needs_dg, needs_dh0):
     """``gdn_linear_attn_bwd``: (dq, dk, dv, dg or None, dh0 or None)."""
     _require_hip_path()
@@ -197,13 +206,14 @@ def _backward(q, k, v, g, scale, initial_state, cu_seqlens, left_padded, do, dht
         b.workspace, b.workspace_bytes = (None if workspace is None else workspace.data_ptr()), nbytes
         _lib.check_status(lib.gdn_linear_attn_bwd(ctypes.byref(b), stream), "gdn_linear_attn_bwd")
         if HK < H:  # heads of q and k that value heads share
+            shared = new(B, T, HK, K), new(B, T, HK, K)
             if dtype == torch.bfloat16:
-                shared = new(B, T, HK, K), new(B, T, HK, K)
                 _lib.check_status(lib.gdn_fold_heads(dq.data_ptr(), dk.data_ptr(), shared[0].data_ptr(), shared[1].data_ptr(), B * T, HK,
                                                      H // HK, K, HK * K, stream), "gdn_fold_heads")  # fmt: skip
-                dq, dk = shared
             else:
-                dq, dk = (x.view(B, T, HK, H // HK, K).sum(dim=3) for x in (dq, dk))
+                _lib.check_status(lib.gdn_linear_fold_heads(dq.data_ptr(), dk.data_ptr(), shared[0].data_ptr(), shared[1].data_ptr(), B * T, HK,
+                                                            H // HK, K, stream), "gdn_linear_fold_heads")  # fmt: skip
+            dq, dk = shared
     return dq, dk, dv, (None if dg is None else dg.to(g_dtype)), dh0
 
 
@@ -212,7 +222,9 @@ class _LinearAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, mode, scale, output_final_state, left_padded, q, k, v, g, initial_state, cu_seqlens):
-        o, ht = _run(mode, q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, False, left_padded)
+        operands = (q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, False, left_padded)
+        result = _on_host_path(mode, *operands)
+        o, ht = _run(mode, *operands) if result is None else result
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(q, k, v, g, initial_state, cu_seqlens)
         ctx.options = (scale, left_padded)
@@ -225,9 +237,14 @@ class _LinearAttention(torch.autograd.Function):
         scale, left_padded = ctx.options
         if do is None and dht is None:
             return (None,) * 10
-        dq, dk, dv, dg, dh0 = _backward(q, k, v, g, scale, initial_state, cu_seqlens, left_padded, do, dht, ctx.needs_input_grad[7],
-                                        ctx.needs_input_grad[8])  # fmt: skip
-        return None, None, None, None, dq, dk, dv, dg, dh0, None
+        needs_dg, needs_dh0 = ctx.needs_input_grad[7:9]
+        grads = None
+        if do is not None and is_kernel_allowed(Kernel.linear_attention):
+            grads = host().linear_attention_bwd(raw_stream(q.get_device()), q, k, v, g, scale, initial_state, cu_seqlens, left_padded, do, dht,
+                                                needs_dg, needs_dh0)  # fmt: skip
+        if grads is None:
+            grads = _backward(q, k, v, g, scale, initial_state, cu_seqlens, left_padded, do, dht, needs_dg, needs_dh0)
+        return None, None, None, None, *grads, None
 
 
 def _dispatch(mode, q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, inplace_state, left_padded):
@@ -235,11 +252,14 @@ def _dispatch(mode, q, k, v, g, scale, initial_state, output_final_state, cu_seq
         from . import _opaque
 
         return _opaque.linear_attention(mode, q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, inplace_state, left_padded)
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, initial_state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (g is not None and g.requires_grad)
+                                    or (initial_state is not None and initial_state.requires_grad)):  # fmt: skip
         if inplace_state:
             raise ValueError("inplace_state overwrites the initial state the backward needs; it is for inference")
         return _LinearAttention.apply(mode, scale, output_final_state, left_padded, q, k, v, g, initial_state, cu_seqlens)
-    return _run(mode, q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, inplace_state, left_padded)
+    operands = (q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, inplace_state, left_padded)
+    result = _on_host_path(mode, *operands)
+    return _run(mode, *operands) if result is None else result
 
 
 def chunk_linear_attention(

@@ -11,6 +11,7 @@ import ctypes
 import torch
 
 from . import _lib
+from ._host import host, raw_stream
 from .kernels import Kernel, is_kernel_allowed
 from .layer_ops import _dtype_code, column_sums
 
@@ -102,12 +103,21 @@ def _backward(x, weight, bias_dtype, eps, dy, needs_dw, needs_db):
     return dx, (sums[0] if needs_dw else None), (sums[-1] if needs_db else None)
 
 
+def _on_host_path(x, weight, bias, eps):
+    """y, or None where the operands need a conversion, a gradient or a report."""
+    if not x.is_cuda or not is_kernel_allowed(Kernel.layer_norm):
+        return None
+    return host().layer_norm(raw_stream(x.get_device()), x, weight, bias, eps)
+
+
 class _LayerNorm(torch.autograd.Function):
     """Forward and backward on the HIP kernels; the forward keeps nothing but its inputs."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y = _forward(x, weight, bias, eps)
+        y = _on_host_path(x, weight, bias, eps)
+        if y is None:
+            y = _forward(x, weight, bias, eps)
         ctx.save_for_backward(x, weight)
         ctx.options = (None if bias is None else bias.dtype, eps)
         return y
@@ -117,7 +127,13 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight = ctx.saved_tensors
         bias_dtype, eps = ctx.options
-        return (*_backward(x, weight, bias_dtype, eps, dy, ctx.needs_input_grad[1], ctx.needs_input_grad[2]), None)
+        needs_dw, needs_db = ctx.needs_input_grad[1:3]
+        grads = None
+        if is_kernel_allowed(Kernel.layer_norm):
+            grads = host().layer_norm_bwd(raw_stream(x.get_device()), x, weight, eps, dy, needs_dw, needs_db, bias_dtype == torch.bfloat16)
+        if grads is None:
+            grads = _backward(x, weight, bias_dtype, eps, dy, needs_dw, needs_db)
+        return (*grads, None)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
@@ -131,4 +147,5 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         return _opaque.layer_norm(x, weight, bias, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNorm.apply(x, weight, bias, eps)
-    return _forward(x, weight, bias, eps)
+    y = _on_host_path(x, weight, bias, eps)
+    return _forward(x, weight, bias, eps) if y is None else y
