@@ -3,9 +3,10 @@
 //     u = dy w;  dx = r (u - mean(u) - xh mean(u xh));   dw = sum_rows dy xh;   db = sum_rows dy
 // A row is held in registers by TPR threads, PER elements each: x (and dy) are read once, the mean first, then the squares of what is
 // left of it, in fp32.  The backward forms mean and r again from the row that it reads anyway, so the forward keeps nothing.
-// Workgroups walk the rows; weight, bias and the backward's sums of dw and db stay in registers on the way, and every workgroup leaves
+// Workgroups walk the rows (the next one on its way where there are registers for it); weight, bias and the backward's sums of dw and db stay in registers on the way, and every workgroup leaves
 // one partial row of each, added up in a fixed order.
 #include <algorithm>
+#include <type_traits>
 
 #include "gdn_common.h"
 #include "gdn_launch.h"
@@ -31,22 +32,24 @@ struct Layout {
     static constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
     static __device__ __forceinline__ int index(int i, int t) { return (i / E * TPR + t) * E + i % E; }
 
-    static __device__ __forceinline__ void load(const T* row, int D, int t, float (&v)[PER]) {
+    using Piece = std::conditional_t<!VEC, T, std::conditional_t<sizeof(T) == 2, bf16x8, f32x4>>;
+    struct Row {
+        Piece piece[PER / E];
+    };
+    // Every thread reads, past the row's end its last piece again: nothing but the loads themselves stands between them.
+    static __device__ __forceinline__ void fetch(const T* row, int D, int t, Row& x) {
+#pragma unroll
+        for (int i = 0; i < PER; i += E) x.piece[i / E] = *reinterpret_cast<const Piece*>(row + min(index(i, t), D - E));
+    }
+    // as fp32, zeros past D
+    static __device__ __forceinline__ void widen(const Row& x, int D, int t, float (&v)[PER]) {
 #pragma unroll
         for (int i = 0; i < PER; i += E) {
-            const int at = index(i, t);
-            if constexpr (VEC && sizeof(T) == 2) {
-                bf16x8 x = {};
-                if (at < D) x = *reinterpret_cast<const bf16x8*>(row + at);
+            const bool there = index(i, t) < D;
 #pragma unroll
-                for (int e = 0; e < E; e++) v[i + e] = (float)x[e];
-            } else if constexpr (VEC) {
-                f32x4 x = {0.f, 0.f, 0.f, 0.f};
-                if (at < D) x = *reinterpret_cast<const f32x4*>(row + at);
-#pragma unroll
-                for (int e = 0; e < E; e++) v[i + e] = x[e];
-            } else {
-                v[i] = at < D ? (float)row[at] : 0.f;
+            for (int e = 0; e < E; e++) {
+                if constexpr (VEC) v[i + e] = there ? (float)x.piece[i / E][e] : 0.f;
+                else v[i] = there ? (float)x.piece[i] : 0.f;
             }
         }
     }
@@ -67,14 +70,29 @@ struct Layout {
             }
         }
     }
-    // weight or bias; `otherwise` where there is none
+    // weight or bias, in pieces of four where they lie so that they can be read like this; `otherwise` where there is none
     static __device__ __forceinline__ void parameter(const void* p, int bf16, int D, int t, float otherwise, float (&v)[PER]) {
+        if (p == nullptr) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) v[i] = otherwise;
+            return;
+        }
+        if (VEC && reinterpret_cast<uintptr_t>(p) % (bf16 ? 8 : 16) == 0) {
+            constexpr int Q = VEC ? 4 : 1;
+#pragma unroll
+            for (int i = 0; i < PER; i += Q) {
+                const int at = min(index(i, t), D - Q);
+#pragma unroll
+                for (int e = 0; e < Q; e++)
+                    v[i + e] = bf16 ? (float)(*reinterpret_cast<const bf16x4*>(static_cast<const bf16_t*>(p) + at))[e]
+                                    : (*reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + at))[e];
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-            const int at = index(i, t);
-            v[i] = p == nullptr || at >= D ? otherwise
-                   : bf16                  ? (float)static_cast<const bf16_t*>(p)[at]
-                                           : static_cast<const float*>(p)[at];
+            const int at = min(index(i, t), D - 1);
+            v[i] = bf16 ? (float)static_cast<const bf16_t*>(p)[at] : static_cast<const float*>(p)[at];
         }
     }
 };
@@ -119,15 +137,22 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_fwd_kernel(c
     float w[PER], b[PER];
     L::parameter(p.weight, p.w_bf16, p.D, t, 1.f, w);
     L::parameter(p.bias, p.w_bf16, p.D, t, 0.f, b);
-    for (int64_t first = (int64_t)blockIdx.x * RPB; first < p.rows; first += (int64_t)gridDim.x * RPB) {
-        const int64_t row = first + threadIdx.x / TPR;
-        const bool live = row < p.rows;  // (a group of threads without a row walks along: the sums cross lanes)
+    const int64_t step = (int64_t)gridDim.x * RPB, last = p.rows - 1;
+    int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    auto fetch = [&](int64_t r, typename L::Row& x) { L::fetch(static_cast<const T*>(p.x) + min(r, last) * p.x_stride, p.D, t, x); };
+    constexpr bool AHEAD = VEC && TPR <= 256;  // the next row is on its way, where there are registers for it
+    typename L::Row next;
+    if (AHEAD) fetch(row, next);
+    // (a group of threads without a row walks along on the last one: the sums cross lanes)
+    for (int64_t first = (int64_t)blockIdx.x * RPB; first < p.rows; first += step, row += step) {
         float v[PER], mean, r;
-        L::load(static_cast<const T*>(p.x) + (live ? row : 0) * p.x_stride, live ? p.D : 0, t, v);
+        if (!AHEAD) fetch(row, next);
+        L::widen(next, p.D, t, v);
+        if (AHEAD) fetch(row + step, next);
         row_statistics<L, TPR>(v, p.D, p.eps, t, shared, mean, r);
 #pragma unroll
         for (int i = 0; i < PER; i++) v[i] = (v[i] - mean) * r * w[i] + b[i];
-        if (live) L::store(static_cast<T*>(p.y) + row * p.y_stride, p.D, t, v);
+        if (row < p.rows) L::store(static_cast<T*>(p.y) + row * p.y_stride, p.D, t, v);
     }
 }
 
@@ -139,12 +164,22 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_bwd_kernel(c
     const int t = threadIdx.x % TPR;
     float w[PER], dw[PER] = {}, db[PER] = {};
     L::parameter(p.weight, p.w_bf16, p.D, t, 1.f, w);
-    for (int64_t first = (int64_t)blockIdx.x * RPB; first < p.rows; first += (int64_t)gridDim.x * RPB) {
-        const int64_t row = first + threadIdx.x / TPR;
+    const int64_t step = (int64_t)gridDim.x * RPB, last = p.rows - 1;
+    int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    auto fetch = [&](int64_t r, typename L::Row& x, typename L::Row& d) {
+        L::fetch(static_cast<const T*>(p.x) + min(r, last) * p.x_stride, p.D, t, x);
+        L::fetch(static_cast<const T*>(p.dy) + min(r, last) * p.dy_stride, p.D, t, d);
+    };
+    constexpr bool AHEAD = VEC && TPR <= 256 && PER <= 16;
+    typename L::Row next, next_dy;
+    if (AHEAD) fetch(row, next, next_dy);
+    for (int64_t first = (int64_t)blockIdx.x * RPB; first < p.rows; first += step, row += step) {
         const bool live = row < p.rows;
         float v[PER], u[PER], mean, r;
-        L::load(static_cast<const T*>(p.x) + (live ? row : 0) * p.x_stride, live ? p.D : 0, t, v);
-        L::load(static_cast<const T*>(p.dy) + (live ? row : 0) * p.dy_stride, live ? p.D : 0, t, u);
+        if (!AHEAD) fetch(row, next, next_dy);
+        L::widen(next, p.D, t, v);
+        L::widen(next_dy, live ? p.D : 0, t, u);
+        if (AHEAD) fetch(row + step, next, next_dy);
         row_statistics<L, TPR>(v, p.D, p.eps, t, shared, mean, r);
         float sum = 0.f, product = 0.f;
 #pragma unroll
@@ -214,7 +249,7 @@ template <bool BACKWARD, typename T, bool VEC, int TPR, int PER>
 int launch_one(const NormRows& p, hipStream_t stream) {
     const dim3 threads(TPR > 256 ? TPR : 256);
     if constexpr (BACKWARD) hipLaunchKernelGGL((layer_norm_bwd_kernel<T, VEC, TPR, PER>), dim3((unsigned)backward_blocks(p.rows, p.D)), threads, 0, stream, p);
-    else hipLaunchKernelGGL((layer_norm_fwd_kernel<T, VEC, TPR, PER>), dim3((unsigned)blocks_for(p.rows, p.D, 8)), threads, 0, stream, p);
+    else hipLaunchKernelGGL((layer_norm_fwd_kernel<T, VEC, TPR, PER>), dim3((unsigned)blocks_for(p.rows, p.D, 2)), threads, 0, stream, p);
     return (int)hipGetLastError();
 }
 
