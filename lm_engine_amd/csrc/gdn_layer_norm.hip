@@ -3,8 +3,11 @@
 //     u = dy w;  dx = r (u - mean(u) - xh mean(u xh));   dw = sum_rows dy xh;   db = sum_rows dy
 // A row is held in registers by TPR threads, PER elements each: x (and dy) are read once, the mean first, then the squares of what is
 // left of it, in fp32.  The backward forms mean and r again from the row that it reads anyway, so the forward keeps nothing.
-// Workgroups walk the rows (the next one on its way where there are registers for it); weight, bias and the backward's sums of dw and db stay in registers on the way, and every workgroup leaves
-// one partial row of each, added up in a fixed order.
+// Workgroups walk the rows, the next one on its way where there are registers for it; weight, bias and the backward's sums of dw and db
+// stay in registers, and every workgroup leaves one partial row of each, added up in a fixed order.
+// Bound by memory: 16384 rows of 2048, bf16: forward 29 us (25 the shortest), 134 MB at 4.7 TB/s; backward 42 us, 201 MB at 4.8.  Two
+// workgroups to a compute unit: with eight, and every thread reading its parameters for two rows, the forward took 51 us; a prefetch
+// takes the backward past 256 registers, and to 72 us.
 #include <algorithm>
 #include <type_traits>
 

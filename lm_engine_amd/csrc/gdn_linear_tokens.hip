@@ -1,10 +1,13 @@
 // Linear attention with a decay for each head, token by token in fp32: decoding (one token, or a few, per state) and the exact path
 // of fp32 inputs.  The recurrence and its roles: gdn_linear_common.h.
 //
-// A workgroup has 4 VL columns of the value dim and all keys of one (segment, head).  A thread has 4 columns and KR keys, GROUPS
-// apart, in registers: on a single token it reads and writes 16-byte pieces, 16 VL bytes of a state row at a time, and the state
-// passes through it once.  Tokens are taken 16 at a time through LDS; per token a lane adds up its keys, the lanes of a wave their
-// groups by shuffles, and the four waves' sums meet in LDS behind the 16.
+// A workgroup has 4 VL columns of the value dim and all keys of one (segment, head).  A thread has 4 columns of KR keys in a row, in
+// registers: on a single token it reads and writes 16-byte pieces, 16 VL bytes of a state row at a time, and the state passes through it
+// once, past the caches.  Tokens are taken TB at a time through LDS; per token a lane adds up its keys, the lanes of a wave their
+// groups by shuffles, and the four waves' sums meet in LDS behind the TB.
+// Bound by memory on one token: 256 states of 32 heads, K = V = 128, 1.07 GB to and fro: 178 us, 6.0 TB/s (203 through the caches; at 128
+// states, which they hold from call to call, 93 against 78: a model's other layers would not leave them there).  On many tokens by the
+// chain from one token to the next: 0.36 us a token in the smallest calls, 4 x 1024 tokens of 16 heads of 128 in fp32 280 us.
 #include <algorithm>
 
 #include "gdn_launch.h"
@@ -14,9 +17,8 @@ namespace gdn {
 
 namespace {
 
-constexpr int TB = 16;  // tokens of a batch
-
-template <typename T, int KR, int VL, bool STATES_ONLY>
+// TB: tokens of a batch
+template <typename T, int KR, int VL, int TB, bool STATES_ONLY>
 __global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p) {
     constexpr int GROUPS = 256 / VL, KP = GROUPS * KR, VC = 4 * VL;
     __shared__ __align__(16) float sx[STATES_ONLY ? 1 : TB][KP];
@@ -45,7 +47,7 @@ __global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p
     const int col = 4 * vl;
     const bool mine = col < columns;
     const int64_t chain = (int64_t)sg.n * p.H + h, cells = p.cells;
-    auto key = [&](int r) { return r * GROUPS + group; };
+    auto key = [&](int r) { return group * KR + r; };
     auto state_at = [&](int r) { return (int64_t)key(r) * p.state_k + (int64_t)(c0 + col) * p.state_v; };
     f32x4 S[KR];
 #pragma unroll
@@ -56,7 +58,7 @@ __global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p
         if (p.state_v == 1) {
 #pragma unroll
             for (int r = 0; r < KR; r++)
-                if (key(r) < p.K) S[r] = *reinterpret_cast<const f32x4*>(from + state_at(r));
+                if (key(r) < p.K) S[r] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(from + state_at(r)));
         } else {
             for (int r = 0; r < KR; r++)
                 for (int e = 0; e < 4; e++)
@@ -141,7 +143,7 @@ __global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p
 #pragma unroll
         for (int r = 0; r < KR; r++)
             if (key(r) < p.K) {
-                if (p.state_v == 1) *reinterpret_cast<f32x4*>(to + state_at(r)) = S[r];
+                if (p.state_v == 1) __builtin_nontemporal_store(S[r], reinterpret_cast<f32x4*>(to + state_at(r)));
                 else
                     for (int e = 0; e < 4; e++) to[state_at(r) + (int64_t)e * p.state_v] = S[r][e];
             }
@@ -153,8 +155,9 @@ int launch(const LinearParams& p, bool states_only, hipStream_t stream) {
     const int64_t blocks = (int64_t)p.slots * p.H * ((p.V + 4 * VL - 1) / (4 * VL));
     if (blocks > 0xfffff000ll / 256) return GDN_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)((blocks + 7) / 8 * 8)), threads(256);
-    if (states_only) hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, true>), grid, threads, 0, stream, p);
-    else hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, false>), grid, threads, 0, stream, p);
+    if (states_only) hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 16, true>), grid, threads, 0, stream, p);
+    else if (p.T == 1) hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 1, false>), grid, threads, 0, stream, p);
+    else hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 16, false>), grid, threads, 0, stream, p);
     return (int)hipGetLastError();
 }
 
