@@ -85,12 +85,13 @@ struct Stream {
         step_bytes = (reverse ? -STEP : STEP) * row_bytes;
     }
     __device__ __forceinline__ bool there(int i, int rows) const { return in_columns && r0 + i * STEP < rows; }
-    // chunk c, all of it, or (`whole` false) the `rows` rows and the columns that there are
+    // chunk c, all of it, or (`whole` false) the `rows` rows and the columns that there are; past the caches, which rows that are read once
+    // gain nothing from (with the outputs' stores: 255 -> 245 us at 32768 packed tokens, 369 -> 352 training on 4 x 4096)
     __device__ __forceinline__ void fetch_chunk(int c, bf16x8 (&v)[ITERS], int rows, bool whole) const {
         const char* const from = base + c * chunk_bytes;
         if (whole) {
 #pragma unroll
-            for (int i = 0; i < ITERS; i++) v[i] = *reinterpret_cast<const bf16x8*>(from + i * step_bytes + offset);
+            for (int i = 0; i < ITERS; i++) v[i] = __builtin_nontemporal_load(reinterpret_cast<const bf16x8*>(from + i * step_bytes + offset));
         } else {
 #pragma unroll
             for (int i = 0; i < ITERS; i++) {

@@ -163,7 +163,7 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel
         for (int i = 0; i < Out::ITERS; i++) {
             const int r = os.r0 + i * Out::STEP;
             if (os.there(i, rows))
-                *reinterpret_cast<bf16x8*>(to + i * os.step_bytes + os.offset) = *reinterpret_cast<const bf16x8*>(so + r * VC + ((tid % Out::GRANULES ^ tile_key<VC>(r)) << 3));
+                __builtin_nontemporal_store(*reinterpret_cast<const bf16x8*>(so + r * VC + ((tid % Out::GRANULES ^ tile_key<VC>(r)) << 3)), reinterpret_cast<bf16x8*>(to + i * os.step_bytes + os.offset));
         }
         os.base += os.chunk_bytes;
     };
