@@ -76,8 +76,7 @@ int gdn_linear_attn_recurrent_fwd(const gdn_linear_attn_args *args, void *stream
 /*
  * Gradients of gdn_linear_attn_chunk_fwd (and of the recurrent form, which is the same function): from the forward's inputs, dout
  * and dht (NULL: zero) it writes
- *   dq, dk [B, T, H, K]  one row per VALUE head: where heads of q and k are shared the caller adds them up (gdn_fold_heads,
- *                        gdn_linear_fold_heads)
+ *   dq, dk [B, T, qk_heads, K]  (the gradients of value heads that share one of q and k are added up in fp32)
  *   dv     [B, T, H, V]
  *   dh0    [N, H, K, V] fp32 or NULL
  *   dg     [H] fp32 or NULL: the derivative with respect to g[h], over all sequences
@@ -106,9 +105,6 @@ int gdn_linear_attn_bwd(const gdn_linear_attn_bwd_args *args, void *stream);
 
 /* Bytes of args->workspace; reads of args what gdn_linear_attn_workspace_bytes reads, and whether dg is NULL. */
 uint64_t gdn_linear_attn_bwd_workspace_bytes(const gdn_linear_attn_bwd_args *args);
-
-/* gdn_fold_heads for fp32: a, b [tokens][heads group][D] and out_a, out_b [tokens][heads][D] contiguous, D a multiple of 4. */
-int gdn_linear_fold_heads(const float *a, const float *b, float *out_a, float *out_b, int64_t tokens, int heads, int group, int D, void *stream);
 
 /*
  * Layer norm over rows of D elements:  y = (x - mean) / sqrt(var + eps) * weight + bias, var over D (not D - 1).

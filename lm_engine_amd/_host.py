@@ -23,7 +23,7 @@ _BOUND = ("gdn_layer_step", "gdn_layer_step_tiles", "gdn_causal_conv1d_fwd", "gd
           "gdn_chunk_bwd_sweeps_workspace_bytes", "gdn_chunk_bwd_local", "gdn_causal_conv1d_bwd", "gdn_gates_bwd",
           "gdn_gated_rmsnorm_bwd", "gdn_column_sums", "gdn_fold_heads", "gdn_layer_front", "gdn_linear_attn_chunk_fwd",
           "gdn_linear_attn_workspace_bytes", "gdn_linear_attn_recurrent_fwd", "gdn_linear_attn_bwd", "gdn_linear_attn_bwd_workspace_bytes",
-          "gdn_linear_fold_heads", "gdn_layer_norm_fwd", "gdn_layer_norm_bwd", "gdn_layer_norm_partial_blocks")  # fmt: skip
+          "gdn_layer_norm_fwd", "gdn_layer_norm_bwd", "gdn_layer_norm_partial_blocks")  # fmt: skip
 
 # device index -> hipStream_t of the calling thread's current stream (a torch build without GPU support has no such function,
 # nor a device tensor that would lead here)

@@ -78,7 +78,6 @@ LINEAR_SYMBOLS = (
     "gdn_linear_attn_recurrent_fwd",
     "gdn_linear_attn_bwd",
     "gdn_linear_attn_bwd_workspace_bytes",
-    "gdn_linear_fold_heads",
     "gdn_layer_norm_fwd",
     "gdn_layer_norm_bwd",
     "gdn_layer_norm_partial_blocks",
@@ -372,8 +371,6 @@ def load_library() -> ctypes.CDLL:
     lib.gdn_layer_norm_fwd.restype = ctypes.c_int
     lib.gdn_layer_norm_bwd.argtypes = [ctypes.POINTER(GdnLayerNormBwdArgs), ctypes.c_void_p]
     lib.gdn_layer_norm_bwd.restype = ctypes.c_int
-    lib.gdn_linear_fold_heads.argtypes = [ctypes.c_void_p] * 4 + [ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
-    lib.gdn_linear_fold_heads.restype = ctypes.c_int
     lib.gdn_layer_norm_partial_blocks.argtypes = [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]
     lib.gdn_layer_norm_partial_blocks.restype = ctypes.c_int
     if lib.gdn_linear_abi_version() != GDN_LINEAR_ABI_VERSION:

@@ -47,7 +47,6 @@ decltype(&gdn_linear_attn_workspace_bytes) linear_workspace_fn = nullptr;
 decltype(&gdn_linear_attn_recurrent_fwd) linear_recurrent_fn = nullptr;
 decltype(&gdn_linear_attn_bwd) linear_bwd_fn = nullptr;
 decltype(&gdn_linear_attn_bwd_workspace_bytes) linear_bwd_workspace_fn = nullptr;
-decltype(&gdn_linear_fold_heads) linear_fold_fn = nullptr;
 decltype(&gdn_layer_norm_fwd) layer_norm_fn = nullptr;
 decltype(&gdn_layer_norm_bwd) layer_norm_bwd_fn = nullptr;
 decltype(&gdn_layer_norm_partial_blocks) layer_norm_blocks_fn = nullptr;
@@ -60,7 +59,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
                       (void**)&sweeps_fn, (void**)&sweeps_workspace_fn, (void**)&local_fn, (void**)&conv_bwd_fn, (void**)&gates_bwd_fn,
                       (void**)&norm_bwd_fn, (void**)&column_sums_fn, (void**)&fold_heads_fn, (void**)&layer_front_fn,
                       (void**)&linear_chunk_fn, (void**)&linear_workspace_fn, (void**)&linear_recurrent_fn, (void**)&linear_bwd_fn,
-                      (void**)&linear_bwd_workspace_fn, (void**)&linear_fold_fn, (void**)&layer_norm_fn, (void**)&layer_norm_bwd_fn,
+                      (void**)&linear_bwd_workspace_fn, (void**)&layer_norm_fn, (void**)&layer_norm_bwd_fn,
                       (void**)&layer_norm_blocks_fn};
     constexpr Py_ssize_t count = sizeof(slots) / sizeof(slots[0]);
     if (n != count + 1) return PyErr_Format(PyExc_TypeError, "bind takes a function and %zd addresses, got %zd arguments", count, n);
@@ -812,16 +811,13 @@ PyObject* linear_attention_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
         b.fwd = x.s;
         need(d.scalar_type() == v.scalar_type() && d.sizes() == v.sizes() && d.stride(3) == 1 && (!needs_dg || x.g != nullptr));
         if (dht != nullptr) need(dht->scalar_type() == at::kFloat && dht->sizes() == at::IntArrayRef({x.N, x.H, x.K, x.V}) && dht->is_contiguous());
-        const bool shared = x.HK < x.H;
-        const int group = (int)(x.H / x.HK);
-        at::Tensor dq, dk, dv, dg, dh0, workspace, dq_shared, dk_shared;
+        at::Tensor dq, dk, dv, dg, dh0, workspace;
         static float wanted;  // (that dg is not NULL is what its workspace goes by)
         b.dg = needs_dg ? &wanted : nullptr;
         without_interpreter_lock([&] {
             b.workspace_bytes = linear_bwd_workspace_fn(&b);
             workspace = workspace_of(b.workspace_bytes, v);
-            dq = fresh(v, {x.B, x.T, x.H, x.K}), dk = fresh(v, {x.B, x.T, x.H, x.K}), dv = fresh(v, {x.B, x.T, x.H, x.V});
-            if (shared) dq_shared = fresh(v, {x.B, x.T, x.HK, x.K}), dk_shared = fresh(v, {x.B, x.T, x.HK, x.K});
+            dq = fresh(v, {x.B, x.T, x.HK, x.K}), dk = fresh(v, {x.B, x.T, x.HK, x.K}), dv = fresh(v, {x.B, x.T, x.H, x.V});
             if (needs_dg) dg = fresh_f32(v, {x.H});
             if (needs_dh0) dh0 = fresh_f32(v, {x.N, x.H, x.K, x.V});
         });
@@ -830,16 +826,9 @@ PyObject* linear_attention_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
         b.dq = ptr(dq), b.dk = ptr(dk), b.dv = ptr(dv);
         b.dg = needs_dg ? static_cast<float*>(ptr(dg)) : nullptr, b.dh0 = needs_dh0 ? static_cast<float*>(ptr(dh0)) : nullptr;
         b.dout_stride_b = d.stride(0), b.dout_stride_t = d.stride(1), b.dout_stride_h = d.stride(2);
-        b.dq_stride_b = b.dk_stride_b = x.T * x.H * x.K, b.dq_stride_t = b.dk_stride_t = x.H * x.K, b.dq_stride_h = b.dk_stride_h = x.K;
+        b.dq_stride_b = b.dk_stride_b = x.T * x.HK * x.K, b.dq_stride_t = b.dk_stride_t = x.HK * x.K, b.dq_stride_h = b.dk_stride_h = x.K;
         b.dv_stride_b = x.T * x.H * x.V, b.dv_stride_t = x.H * x.V, b.dv_stride_h = x.V;
-        return launch("gdn_linear_attn_bwd", pack_results({shared ? dq_shared : dq, shared ? dk_shared : dk, dv, dg, dh0}), [&] {
-            const int status = linear_bwd_fn(&b, stream);
-            if (status != GDN_OK || !shared) return status;
-            const int64_t tokens = x.B * x.T, row = x.HK * x.K;
-            if (x.s.dtype == GDN_BF16) return fold_heads_fn(b.dq, b.dk, ptr(dq_shared), ptr(dk_shared), tokens, (int)x.HK, group, (int)x.K, row, stream);
-            return linear_fold_fn(static_cast<const float*>(b.dq), static_cast<const float*>(b.dk), static_cast<float*>(ptr(dq_shared)),
-                                  static_cast<float*>(ptr(dk_shared)), tokens, (int)x.HK, group, (int)x.K, stream);
-        });
+        return launch("gdn_linear_attn_bwd", pack_results({dq, dk, dv, dg, dh0}), [&] { return linear_bwd_fn(&b, stream); });
     });
 }
 

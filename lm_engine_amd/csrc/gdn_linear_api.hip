@@ -165,8 +165,9 @@ const void* offset(const void* p, int64_t elements, int dtype) { return static_c
 
 constexpr int KEYS = 256;  // of a walk at most
 
+// outputs of dq and dk in fp32: where their keys, the value dim, are walked in pieces, and where value heads share a head of q and k
 uint64_t sums_bytes(const gdn_linear_attn_args& a) {
-    return a.V > KEYS ? ((uint64_t)a.B * a.T * a.H * a.K * 4 + 255) / 256 * 256 : 0;
+    return a.V > KEYS || heads_shared(a) > 1 ? ((uint64_t)a.B * a.T * a.H * a.K * 4 + 255) / 256 * 256 : 0;
 }
 
 uint64_t dots_bytes(const gdn_linear_attn_args& a, const Cut& c) {
@@ -200,8 +201,8 @@ int run_transposed(LinearParams p, const gdn_linear_attn_args& a, bool own_state
         p.state_k = 1, p.state_v = a.V;
         p.x.p = offset(whole.x.p, first, a.dtype), p.y.p = offset(whole.y.p, first, a.dtype);
         p.init = whole.init == nullptr ? nullptr : whole.init + first;
-        p.sums = a.V > KEYS ? sums : nullptr;
-        p.sums_in = first > 0, p.sums_out = first + KEYS < a.V;
+        p.sums = sums;
+        p.sums_in = first > 0, p.sums_only = heads_shared(a) > 1, p.sums_out = p.sums_only || first + KEYS < a.V;
         if (own_states) {
             if (const int e = run_states(p, a.dtype, stream); e != GDN_OK) return e;
         } else if (p.local != nullptr && p.local_keys != 0) {
@@ -211,7 +212,12 @@ int run_transposed(LinearParams p, const gdn_linear_attn_args& a, bool own_state
         }
         if (const int e = run(p, a.dtype, false, stream); e != GDN_OK) return e;
     }
-    return GDN_OK;
+    if (!p.sums_only) return GDN_OK;
+    LinearFold f;
+    f.in = sums, f.out = p.out, f.stride_b = p.out_stride_b, f.stride_t = p.out_stride_t, f.stride_h = p.out_stride_h;
+    f.T = a.T, f.heads = a.qk_heads, f.group = heads_shared(a), f.D = a.K;
+    f.pieces = (int64_t)a.B * a.T * a.qk_heads * (a.K / 4);
+    return launch_linear_fold(f, a.dtype, stream);
 }
 
 }  // namespace
@@ -299,7 +305,7 @@ extern "C" int gdn_linear_attn_bwd(const gdn_linear_attn_bwd_args* args, void* s
     const LinearRole d = {b.dout, b.dout_stride_b, b.dout_stride_t, b.dout_stride_h, 1};
     char* const ws = static_cast<char*>(b.workspace);
     float* const gradients_at = reinterpret_cast<float*>(ws + space.forward);
-    float* const sums_at = reinterpret_cast<float*>(ws + space.forward + space.gradients + space.slope);
+    float* const sums_at = space.sums == 0 ? nullptr : reinterpret_cast<float*>(ws + space.forward + space.gradients + space.slope);
 
     LinearParams s = base_params(a, c);  // of the forward's states
     natural(s, a.K, a.V);
@@ -314,7 +320,7 @@ extern "C" int gdn_linear_attn_bwd(const gdn_linear_attn_bwd_args* args, void* s
         LinearParams u = s;
         u.d = d, u.init_grad = b.dht;
         if (c.several) u.local = reinterpret_cast<float*>(ws), u.local_slope = gradients_at + space.gradients / 4;
-        u.dots = sums_at + space.sums / 4;
+        u.dots = reinterpret_cast<float*>(ws + space.forward + space.gradients + space.slope + space.sums);
         if (const int e = launch_linear_tangent(u, a.dtype, c.several, b.dg, st); e != GDN_OK) return e;
     }
     if (c.several) {

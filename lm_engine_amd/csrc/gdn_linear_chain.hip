@@ -9,7 +9,7 @@
 //     S waves    S_{c+1} = w^n S_c + y^T (w^{n - a - j} z): tiles of 32 keys x 32 columns          (v_mfma_f32_32x32x16_bf16)
 //     O waves    out_{c-1}^T = ... + z^T P_{c-1}^T, stored; then out_c^T = (S_c^T x^T) w^{i + a}: 16 rows each
 // P, and the state as bf16 fragments, go round through LDS.  Rows are on their way in registers two chunks ahead, in LDS one chunk
-// ahead; the P waves bring in x and z (and its decayed rows, in one or two bf16 parts), the S waves y.  The O waves load nothing: the
+// ahead; the P waves bring in x and z (and its decayed rows, in two or three bf16 parts), the S waves y.  The O waves load nothing: the
 // compiler's wait for rows would be one for their stores.
 //
 // Measured at 4 sequences of 4096 tokens, 16 heads, K = V = 128, which is one workgroup to a compute unit: 79 to 85 us, 1.2 us a chunk, of
@@ -75,6 +75,7 @@ template <int KD, bool EXACT>
 __global__ __launch_bounds__(768) void linear_chain_kernel(const LinearParams p) {
     using Shape = ChainShape<KD>;
     constexpr int GROUP = Shape::GROUP, VC = Shape::VC, ZLD = Shape::ZLD, KT = Shape::KT;
+    constexpr int PARTS = EXACT ? 3 : 2;  // of a decayed row of z, as in linear_walk_kernel
     extern __shared__ __align__(16) bf16_t lds[];  // everything twice
     bf16_t* const tx = lds;
     bf16_t* const ty = tx + 2 * Shape::XY;
@@ -90,7 +91,7 @@ __global__ __launch_bounds__(768) void linear_chain_kernel(const LinearParams p)
     if (id >= (unsigned)p.slots * p.H * slices) return;
     const int slice = id % slices, h = id / slices % p.H, slot = id / slices / p.H;
     const int c0 = slice * VC, columns = min(VC, p.V - c0);
-    if (p.zero && p.cu != nullptr) linear_zero_gaps<bf16_t, 8>(p, slot, h, c0, columns, threadIdx.x, Shape::THREADS);
+    if (p.zero && p.cu != nullptr) linear_zero_gaps<bf16_t>(p, slot, h, c0, columns, threadIdx.x, Shape::THREADS);
     LinearSegment sg;
     if (!linear_find(p, slot, sg, lane)) return;  // (one segment to a sequence)
     const int total = sg.len;
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(768) void linear_chain_kernel(const LinearParams p)
 #pragma unroll
                 for (int i = 0; i < ZI; i++) {
                     const int r = zs.r0 + i * Stream<VC, GROUP>::STEP;
-                    bf16x8 x = rz[R][i], hi, lo;
+                    bf16x8 x = rz[R][i], part[PARTS];
                     float w = z_weight[i];
                     if (rows < LC || !all_columns) {
                         const bf16x8 zero = {};
@@ -174,15 +175,15 @@ __global__ __launch_bounds__(768) void linear_chain_kernel(const LinearParams p)
                     }
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float z = (float)x[e] * w;
-                        hi[e] = (bf16_t)z;
-                        if constexpr (EXACT) lo[e] = (bf16_t)(z - (float)hi[e]);
+                        float z = (float)x[e] * w;
+#pragma unroll
+                        for (int u = 0; u < PARTS; u++) part[u][e] = (bf16_t)z, z -= (float)part[u][e];
                     }
                     bf16_t* const to = tz + buf * Shape::Z + r * ZLD;
                     const int g = tid % Stream<VC, GROUP>::GRANULES, key = tile_key<ZLD>(r);
                     *reinterpret_cast<bf16x8*>(to + ((g ^ key) << 3)) = x;
-                    *reinterpret_cast<bf16x8*>(to + (((4 + g) ^ key) << 3)) = hi;
-                    if constexpr (EXACT) *reinterpret_cast<bf16x8*>(to + (((8 + g) ^ key) << 3)) = lo;
+#pragma unroll
+                    for (int u = 0; u < PARTS; u++) *reinterpret_cast<bf16x8*>(to + (((4 + 4 * u + g) ^ key) << 3)) = part[u];
                 }
             },
             [] {},
@@ -268,27 +269,30 @@ __global__ __launch_bounds__(768) void linear_chain_kernel(const LinearParams p)
                 const bf16_t *const y = ty + B * Shape::XY, *const z = tz + B * Shape::Z;
                 const float shrink = rows < LC ? linear_power(g, rows) : whole;
                 if (mine) {
-                    bf16x8 yt[4], zh[4], zl[4];
+                    bf16x8 yt[4], zt[4];
 #pragma unroll
-                    for (int s = 0; s < 4; s++) {
-                        yt[s] = tile.transposed(y, s, w4), zh[s] = ztile.transposed(z, 16 * s, 1);
-                        if constexpr (EXACT) zl[s] = ztile.transposed(z, 16 * s, 2);
-                    }
+                    for (int s = 0; s < 4; s++) yt[s] = tile.transposed(y, s, w4), zt[s] = ztile.transposed(z, 16 * s, 1);
                     f32x16 low = {};
 #pragma unroll
                     for (int r = 0; r < 16; r++) S[r] *= shrink;
 #pragma unroll
-                    for (int s = 0; s < 4; s++) {
-                        S = mfma32_bf16(yt[s], zh[s], S);
-                        if constexpr (EXACT) low = mfma32_bf16(yt[s], zl[s], low);
-                    }
-                    // all reads first, then the products: left alone, the scheduler waits for every read in front of its product
-                    __builtin_amdgcn_sched_group_barrier(0x100, EXACT ? 24 : 16, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x008, EXACT ? 8 : 4, 0);
-                    if constexpr (EXACT) {
+                    for (int u = 0; u < PARTS; u++)
 #pragma unroll
-                        for (int r = 0; r < 16; r++) S[r] += low[r];
+                        for (int s = 0; s < 4; s++) {
+                            f32x16& to = u == 0 ? S : low;
+                            to = mfma32_bf16(yt[s], zt[s], to);
+                            if (u + 1 < PARTS) zt[s] = ztile.transposed(z, 16 * s, u + 2);
+                        }
+                    // all reads of the first products first, then theirs and the next part's reads: left alone, the scheduler waits for
+                    // every read in front of its product
+                    __builtin_amdgcn_sched_group_barrier(0x100, 16, 0);
+#pragma unroll
+                    for (int i = 0; i < 4 * PARTS; i++) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        if (i < 4 * PARTS - 4) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
                     }
+#pragma unroll
+                    for (int r = 0; r < 16; r++) S[r] += low[r];
                 }
                 publish(1 - B);
             });

@@ -47,8 +47,9 @@ struct LinearParams {
     int reverse, a;
     float os, ps, us;
     int zero;             // zeros at tokens of no sequence
-    float* sums;          // fp32 [B, T, H, V] contiguous or NULL: partial outputs of a key dim that is walked in pieces
+    float* sums;          // fp32 [B, T, H, V] contiguous or NULL: outputs of a key dim that is walked in pieces, of heads that are added up
     int sums_in, sums_out;  // add what is there; leave the result there instead of rounding it to out
+    int sums_only;          // out is not written: tokens of no sequence have their zeros in sums
     // the derivative with respect to the log-decay (gdn_linear_tangent.hip)
     LinearRole d;            // gradient of the output
     const float* init_grad;  // of the final state, or NULL
@@ -151,16 +152,22 @@ __device__ __forceinline__ LinearGaps linear_gaps(const LinearParams& p, int slo
 
 // zeros at those tokens, columns [c0, c0 + width) of head h; T_out has 16-byte pieces of VEC elements, width a multiple of VEC
 template <typename T_out, int VEC>
-__device__ __forceinline__ void linear_zero_gaps(const LinearParams& p, int slot, int h, int c0, int width, int tid, int threads) {
+__device__ __forceinline__ void linear_zero_rows(const LinearParams& p, void* to, int64_t stride_b, int64_t stride_t, int64_t stride_h, int slot, int h, int c0,
+                                                 int width, int tid, int threads) {
     const LinearGaps gap = linear_gaps(p, slot);
-    T_out* const out = static_cast<T_out*>(p.out) + gap.b * p.out_stride_b + h * p.out_stride_h + c0;
+    T_out* const out = static_cast<T_out*>(to) + gap.b * stride_b + h * stride_h + c0;
     const int pieces = width / VEC;
     for (int side = 0; side < 2; side++)
         for (int64_t i = tid; i < (int64_t)gap.count[side] * pieces; i += threads) {
             const int row = (int)(i / pieces), c = (int)(i - (int64_t)row * pieces) * VEC;
             f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-            *reinterpret_cast<f32x4*>(out + (int64_t)(gap.first[side] + row) * p.out_stride_t + c) = zero;
+            *reinterpret_cast<f32x4*>(out + (int64_t)(gap.first[side] + row) * stride_t + c) = zero;
         }
+}
+template <typename T_out>
+__device__ __forceinline__ void linear_zero_gaps(const LinearParams& p, int slot, int h, int c0, int width, int tid, int threads) {
+    if (p.sums_only) linear_zero_rows<float, 4>(p, p.sums, (int64_t)p.T * p.H * p.V, (int64_t)p.H * p.V, p.V, slot, h, c0, width, tid, threads);
+    else linear_zero_rows<T_out, 16 / sizeof(T_out)>(p, p.out, p.out_stride_b, p.out_stride_t, p.out_stride_h, slot, h, c0, width, tid, threads);
 }
 
 // log2 of a token's factor, from the natural logarithm that callers give; w^n from it, 1 for n = 0 also where the state forgets at once
@@ -176,6 +183,15 @@ __device__ __forceinline__ int64_t linear_fragment(int keys, int key, int v) {
 
 // launches, gdn_linear_walk.hip and gdn_linear_tokens.hip; `states_only`: the segments' own states into p.local
 int launch_linear_walk(const LinearParams& p, bool states_only, hipStream_t stream);
+// gdn_linear_tokens.hip: fp32 [B, T, heads group, D], each group's rows added up, to rows of dtype
+struct LinearFold {
+    const float* in;
+    void* out;
+    int64_t stride_b, stride_t, stride_h;  // of out
+    int64_t pieces;                        // of 4 columns, over all of out
+    int T, heads, group, D;
+};
+int launch_linear_fold(const LinearFold& p, int dtype, hipStream_t stream);
 int launch_linear_chain(const LinearParams& p, hipStream_t stream);  // gdn_linear_chain.hip: forward, bf16, up to 128 keys, whole sequences
 int launch_linear_tokens(const LinearParams& p, int dtype, int columns, bool states_only, hipStream_t stream);
 int linear_walk_keys(int K);            // keys that the bf16 walk is built for

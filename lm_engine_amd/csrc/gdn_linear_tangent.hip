@@ -6,7 +6,7 @@
 // the length).  Per chunk of n tokens, i and j from 0:
 //     dg += scale ( <G', S> + <G, U> + sum_{j <= i} (i - j) w^{i - j} (q_i . k_j) (do_i . v_j) ),   G = sum_i w^{i+1} q_i do_i^T,
 //     G' = sum_i (i + 1) w^{i+1} q_i do_i^T;   U = w^n (U + n S) + sum_j (n - 1 - j) w^{n-1-j} k_j v_j^T,   S as ever
-// bf16: on the matrix units, decayed rows in two bf16 parts (as the walk's states), S and U only ever as fp32: dg is good to fp32 sums
+// bf16: on the matrix units, decayed rows in three bf16 parts (as the walk's states), S and U only ever as fp32: dg is good to fp32 sums
 // of such terms, 1e-5.  A workgroup leaves one number per segment, head and columns; the sums over them are one more launch, in order.
 // No prefetch here: two workgroups to a compute unit cover each other's loads (one where the keys number more than 128).
 #include <algorithm>
@@ -32,7 +32,7 @@ __device__ __forceinline__ float block_sum(float x, float* shared) {
 }
 
 template <int KD, int NW, bool STATES_ONLY>
-__global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : 1) void linear_tangent_kernel(const LinearParams p) {
+__global__ __launch_bounds__(64 * NW, KD <= 64 ? NW / 2 : 1) void linear_tangent_kernel(const LinearParams p) {
     constexpr int NT = 64 * NW, VC = 32 * NW, KT = KD / 32;
     __shared__ __align__(16) bf16_t sq[STATES_ONLY ? 8 : LC * KD];
     __shared__ __align__(16) bf16_t sk[LC * KD];
@@ -82,25 +82,25 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : 1) void linear_tangen
 
     const TileLane<KD> tile(lane);
     const TileLane<VC> ztile(lane);
-    // B fragments (reduction over rows, column = this lane's) of a tile's columns of this wave, weighted, in two parts
-    auto weighted = [&](const bf16_t* rows_of, const float* weights, bf16x8 (&hi)[4], bf16x8 (&lo)[4]) {
+    // B fragments (reduction over rows, column = this lane's) of a tile's columns of this wave, weighted, in three parts
+    auto weighted = [&](const bf16_t* rows_of, const float* weights, bf16x8 (&part)[3][4]) {
 #pragma unroll
         for (int s = 0; s < 4; s++) {
             const bf16x8 rows = ztile.transposed(rows_of, s, wave);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float x = (float)rows[e] * weights[16 * s + 8 * half + e];
-                hi[s][e] = (bf16_t)x;
-                lo[s][e] = (bf16_t)(x - (float)hi[s][e]);
+                float x = (float)rows[e] * weights[16 * s + 8 * half + e];
+#pragma unroll
+                for (int u = 0; u < 3; u++) part[u][s][e] = (bf16_t)x, x -= (float)part[u][s][e];
             }
         }
     };
-    auto product = [&](const bf16_t* rows_of, int kt, const bf16x8 (&hi)[4], const bf16x8 (&lo)[4], f32x16 acc) {
+    auto product = [&](const bf16_t* rows_of, int kt, const bf16x8 (&part)[3][4], f32x16 acc) {
 #pragma unroll
         for (int s = 0; s < 4; s++) {
             const bf16x8 a = tile.transposed(rows_of, s, kt);
-            acc = mfma32_bf16(a, hi[s], acc);
-            acc = mfma32_bf16(a, lo[s], acc);
+#pragma unroll
+            for (int u = 0; u < 3; u++) acc = mfma32_bf16(a, part[u][s], acc);
         }
         return acc;
     };
@@ -125,19 +125,19 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : 1) void linear_tangen
         ks.stage(sk, rk, rows, false), vs.stage(sv, rv, rows, false);
         if constexpr (!STATES_ONLY) qs.stage(sq, rq, rows, false), ds.stage(sd, rd, rows, false);
         __syncthreads();
-        bf16x8 hi[4], lo[4];
+        bf16x8 part[3][4];
         if constexpr (!STATES_ONLY) {
-            weighted(sd, sw[3], hi, lo);
+            weighted(sd, sw[3], part);
 #pragma unroll
             for (int kt = 0; kt < KT; kt++) {
-                const f32x16 G = product(sq, kt, hi, lo, f32x16{});
+                const f32x16 G = product(sq, kt, part, f32x16{});
 #pragma unroll
                 for (int r = 0; r < 16; r++) sum += G[r] * S[kt][r];
             }
-            weighted(sd, sw[2], hi, lo);
+            weighted(sd, sw[2], part);
 #pragma unroll
             for (int kt = 0; kt < KT; kt++) {
-                const f32x16 G = product(sq, kt, hi, lo, f32x16{});
+                const f32x16 G = product(sq, kt, part, f32x16{});
 #pragma unroll
                 for (int r = 0; r < 16; r++) sum += G[r] * U[kt][r];
             }
@@ -167,12 +167,12 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? NW / 2 : 1) void linear_tangen
                 U[kt][r] = whole * (U[kt][r] + (float)rows * S[kt][r]);
                 S[kt][r] *= whole;
             }
-        weighted(sv, sw[1], hi, lo);
+        weighted(sv, sw[1], part);
 #pragma unroll
-        for (int kt = 0; kt < KT; kt++) U[kt] = product(sk, kt, hi, lo, U[kt]);
-        weighted(sv, sw[0], hi, lo);
+        for (int kt = 0; kt < KT; kt++) U[kt] = product(sk, kt, part, U[kt]);
+        weighted(sv, sw[0], part);
 #pragma unroll
-        for (int kt = 0; kt < KT; kt++) S[kt] = product(sk, kt, hi, lo, S[kt]);
+        for (int kt = 0; kt < KT; kt++) S[kt] = product(sk, kt, part, S[kt]);
     }
     if constexpr (STATES_ONLY) {
         for_cells([&](int kt, int r, int64_t at) { p.local[own + at] = S[kt][r], p.local_slope[own + at] = U[kt][r]; });

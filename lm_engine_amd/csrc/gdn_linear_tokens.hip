@@ -34,7 +34,7 @@ __global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p
     const int slice = id % slices, h = id / slices % p.H, slot = id / slices / p.H;
     const int c0 = slice * VC, columns = min(VC, p.V - c0);
     if constexpr (!STATES_ONLY)
-        if (p.zero && p.cu != nullptr) linear_zero_gaps<T, 16 / sizeof(T)>(p, slot, h, c0, columns, tid, 256);
+        if (p.zero && p.cu != nullptr) linear_zero_gaps<T>(p, slot, h, c0, columns, tid, 256);
     LinearSegment sg;
     if (!linear_find(p, slot, sg, lane)) return;
     const bool last = sg.s == linear_segments(sg.len, p.seg) - 1;
@@ -173,29 +173,24 @@ int launch_of(const LinearParams& p, int columns, bool states_only, hipStream_t 
     return launch<T, 32, 32>(p, states_only, stream);
 }
 
-// Gradients of shared heads of q and k, added up: a thread has 4 columns of one head (blockIdx.y: of which of the two).  Bound by
-// memory: group + 1 rows for each one written.
-struct FoldParams {
-    const float* in[2];
-    float* out[2];
-    int64_t pieces;  // of 4 columns, over all tokens
-    int group, D;
-};
-
-__global__ __launch_bounds__(256) void linear_fold_kernel(const FoldParams p) {
+// Gradients of shared heads of q and k, added up and rounded once: a thread has 4 columns of one head.  Bound by memory: group fp32 rows
+// for each one written.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_fold_kernel(const LinearFold p) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= p.pieces) return;
     const int per_head = p.D / 4;
-    const int64_t row = i / per_head;
+    const int64_t row = i / per_head, token = row / p.heads;  // token and head; b and t
     const int c = (int)(i - row * per_head) * 4;
-    const float* const in = p.in[blockIdx.y] + row * p.group * p.D + c;
+    const float* const in = p.in + row * p.group * p.D + c;
     f32x4 sum = *reinterpret_cast<const f32x4*>(in);
     for (int j = 1; j < p.group; j++) {
         const f32x4 x = *reinterpret_cast<const f32x4*>(in + (int64_t)j * p.D);
 #pragma unroll
         for (int e = 0; e < 4; e++) sum[e] += x[e];
     }
-    *reinterpret_cast<f32x4*>(p.out[blockIdx.y] + row * p.D + c) = sum;
+    const int64_t b = token / p.T;
+    store4<T>(static_cast<T*>(p.out) + b * p.stride_b + (token - b * p.T) * p.stride_t + (row - token * p.heads) * p.stride_h + c, sum);
 }
 
 }  // namespace
@@ -206,21 +201,12 @@ int launch_linear_tokens(const LinearParams& p, int dtype, int columns, bool sta
     return dtype == GDN_BF16 ? launch_of<bf16_t>(p, columns, states_only, stream) : launch_of<float>(p, columns, states_only, stream);
 }
 
-}  // namespace gdn
-
-extern "C" int gdn_linear_fold_heads(const float* a, const float* b, float* out_a, float* out_b, int64_t tokens, int heads, int group, int D,
-                                     void* stream) {
-    const void* ptrs[] = {a, b, out_a, out_b};
-    for (const void* x : ptrs)
-        if (x == nullptr) return GDN_ERR_NULL;
-        else if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return GDN_ERR_ALIGN;
-    if (tokens <= 0 || heads <= 0 || group <= 0 || D <= 0) return GDN_ERR_SHAPE;
-    if (D % 4 != 0) return GDN_ERR_ALIGN;
-    gdn::FoldParams p;
-    p.in[0] = a, p.in[1] = b, p.out[0] = out_a, p.out[1] = out_b;
-    p.pieces = tokens * heads * (D / 4), p.group = group, p.D = D;
+int launch_linear_fold(const LinearFold& p, int dtype, hipStream_t stream) {
     const int64_t blocks = (p.pieces + 255) / 256;
-    if (blocks > (int64_t)0xffffffff / 256) return GDN_ERR_UNSUPPORTED;  // (a launch holds at most 2^32 - 1 threads)
-    hipLaunchKernelGGL(gdn::linear_fold_kernel, dim3((unsigned)blocks, 2), dim3(256), 0, static_cast<hipStream_t>(stream), p);
+    if (blocks > 0xfffff000ll / 256) return GDN_ERR_UNSUPPORTED;  // (a launch holds at most 2^32 - 1 threads)
+    if (dtype == GDN_BF16) hipLaunchKernelGGL(linear_fold_kernel<bf16_t>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL(linear_fold_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
     return (int)hipGetLastError();
 }
+
+}  // namespace gdn

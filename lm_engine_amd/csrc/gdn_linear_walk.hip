@@ -29,21 +29,22 @@ __device__ __forceinline__ void reads_ahead() {
     }
 }
 
-// What a walk is for, and in how many bf16 parts the decayed rows of z go into the state.  Two parts, high and low, 16 bits and more
-// together, keep the state's sums to fp32 accuracy (the rows of y are exact): where the state is a result.
+// What a walk is for, and in how many bf16 parts the decayed rows of z go into the state (the rows of y are exact).  Three hold all 24
+// bits of an fp32 product: where the state is a result.  Two, 16 bits and more, where it only goes on into outputs, which round it to
+// 8 as an operand: with one the state would carry as much error as that rounding adds.
 enum class Walk {
-    outputs,        // one part; a segment of several, its state given
-    outputs_state,  // two parts; the only segment, its state a result
+    outputs,        // two parts; a segment of several, its state given
+    outputs_state,  // three parts; the only segment, its state a result
     sums,           // as outputs, partial outputs in fp32 (LinearParams::sums)
-    states,         // the segments' own states, one part
-    exact_states,   // ... two parts
+    states,         // the segments' own states, two parts
+    exact_states,   // ... three parts
 };
 
 template <int KD, int NW, Walk MODE>
 __global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel(const LinearParams p) {
     constexpr int NT = 64 * NW, VC = 32 * NW, KT = KD / 32;
     constexpr bool STATES_ONLY = MODE == Walk::states || MODE == Walk::exact_states, SUMS = MODE == Walk::sums;
-    constexpr int PARTS = MODE == Walk::outputs_state || MODE == Walk::exact_states ? 2 : 1;
+    constexpr int PARTS = MODE == Walk::outputs_state || MODE == Walk::exact_states ? 3 : 2;
     __shared__ __align__(16) bf16_t sx[STATES_ONLY ? 8 : LC * KD];
     __shared__ __align__(16) bf16_t sy[LC * KD];
     __shared__ __align__(16) bf16_t sz[LC * VC];
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel
     const int c0 = slice * VC, columns = min(VC, p.V - c0);
 
     if constexpr (!STATES_ONLY)
-        if (p.zero && p.cu != nullptr) linear_zero_gaps<bf16_t, 8>(p, slot, h, c0, columns, tid, NT);
+        if (p.zero && p.cu != nullptr) linear_zero_gaps<bf16_t>(p, slot, h, c0, columns, tid, NT);
     LinearSegment sg;
     if (!linear_find(p, slot, sg, lane)) return;
     const int segments = linear_segments(sg.len, p.seg);
@@ -263,9 +264,9 @@ __global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel
             const float* const weights = sw + 16 * s + 8 * half;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float x = (float)z[e] * weights[e];
-                part[s][0][e] = (bf16_t)x;
-                if constexpr (PARTS == 2) part[s][1][e] = (bf16_t)(x - (float)part[s][0][e]);
+                float x = (float)z[e] * weights[e];
+#pragma unroll
+                for (int u = 0; u < PARTS; u++) part[s][u][e] = (bf16_t)x, x -= (float)part[s][u][e];
             }
         }
         __builtin_amdgcn_sched_barrier(0);

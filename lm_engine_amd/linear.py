@@ -176,7 +176,7 @@ def _backward(q, k, v, g, scale, initial_state, cu_seqlens, left_padded, do, dht
     B, T, H, K, V, N = dims
     HK, dev, dtype = q.size(2), q.device, v.dtype
     new = lambda *shape: torch.empty(*shape, dtype=dtype, device=dev)  # noqa: E731
-    dq, dk, dv = new(B, T, H, K), new(B, T, H, K), new(B, T, H, V)
+    dq, dk, dv = new(B, T, HK, K), new(B, T, HK, K), new(B, T, H, V)
     dg = torch.empty(H, dtype=torch.float32, device=dev) if needs_dg else None
     dh0 = torch.empty(N, H, K, V, dtype=torch.float32, device=dev) if needs_dh0 else None
     if v.numel() == 0:
@@ -205,15 +205,6 @@ def _backward(q, k, v, g, scale, initial_state, cu_seqlens, left_padded, do, dht
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         b.workspace, b.workspace_bytes = (None if workspace is None else workspace.data_ptr()), nbytes
         _lib.check_status(lib.gdn_linear_attn_bwd(ctypes.byref(b), stream), "gdn_linear_attn_bwd")
-        if HK < H:  # heads of q and k that value heads share
-            shared = new(B, T, HK, K), new(B, T, HK, K)
-            if dtype == torch.bfloat16:
-                _lib.check_status(lib.gdn_fold_heads(dq.data_ptr(), dk.data_ptr(), shared[0].data_ptr(), shared[1].data_ptr(), B * T, HK,
-                                                     H // HK, K, HK * K, stream), "gdn_fold_heads")  # fmt: skip
-            else:
-                _lib.check_status(lib.gdn_linear_fold_heads(dq.data_ptr(), dk.data_ptr(), shared[0].data_ptr(), shared[1].data_ptr(), B * T, HK,
-                                                            H // HK, K, stream), "gdn_linear_fold_heads")  # fmt: skip
-            dq, dk = shared
     return dq, dk, dv, (None if dg is None else dg.to(g_dtype)), dh0
 
 

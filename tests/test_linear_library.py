@@ -119,15 +119,6 @@ def test_outputs_and_workspaces_are_checked_before_any_launch():
         assert backward(**over) == status, over
 
 
-def test_fold_of_shared_heads_rejects_bad_arguments():
-    fold = _lib.load_library().gdn_linear_fold_heads
-    assert fold(None, FAKE, FAKE, FAKE, 4, 2, 2, 64, None) == -1
-    assert fold(FAKE, FAKE, FAKE, FAKE + 4, 4, 2, 2, 64, None) == -4
-    assert fold(FAKE, FAKE, FAKE, FAKE, 0, 2, 2, 64, None) == -2
-    assert fold(FAKE, FAKE, FAKE, FAKE, 4, 2, 0, 64, None) == -2
-    assert fold(FAKE, FAKE, FAKE, FAKE, 4, 2, 2, 6, None) == -4
-
-
 def test_layer_norm_rejects_bad_arguments_before_any_launch():
     lib = _lib.load_library()
 
