@@ -90,19 +90,20 @@ Cut cut_segments(const gdn_linear_attn_args& a) {
 }
 
 // The forward in bf16: where segments would take three launches, a walk over whole sequences, 32 columns to a workgroup and one
-// workgroup to a compute unit, may be faster.  It takes 6 us and 1.2 us a chunk (0.8 up to 64 keys) of the longest sequence, for each
-// round of workgroups; the segments 30 us and 17 ns (7) for every chunk of 64 rows and 128 columns.  Measured, whole sequences against
-// segments, us, with 16 heads of 128: 4 x 4096 tokens 88 | 102, 4 x 1024 27 | 49, 8 x 4096 182 | 203, 1 x 2048 39 | 37, 2 x 4096 73 | 65,
-// 1 x 65536 with 32 heads and V = 256 1230 | 1067, 32 x 512 (one launch either way) 129 | 80; 16 heads of 64: 16 x 1024 38 | 58, 4 x 4096 56 | 58.  In the backward, where the states
-// serve two walks, the two are level (370 us at 4 x 4096 tokens), and it has segments alone.  How long the longest of packed sequences is
-// lives on the device: it may have nearly all tokens (11 of them in 32768 tokens: 404 | 257).
+// workgroup to a compute unit, may be faster.  It takes 6 us and 1.25 us a chunk (0.8 up to 64 keys) of the longest sequence, for each
+// round of workgroups; the segments 30 us and 18 ns (7) for every chunk of 64 rows and 128 columns.  Measured, whole sequences against
+// segments, us, with 16 heads of 128: 4 x 1024 tokens 28 | 50, 4 x 2048 46 | 67, 8 x 4096 190 | 202, 2 x 4096 75 | 69,
+// 1 x 2048 40 | 37, 1 x 4096 72 | 52; 1 x 65536 with 32 heads and V = 256 1320 | 1297; 16 heads of 64: 16 x 1024 39 | 63, 4 x 4096 60 | 64.
+// It errs where a second round of workgroups is half empty (6 x 2048 tokens of 16 heads of 128, 88 | 107).
+// In the backward, where the states serve two walks, the two were level (370 us at 4 x 4096 tokens), and it has segments alone.  How
+// long the longest of packed sequences is lives on the device: it may have nearly all tokens (11 of them in 32768 tokens: 404 | 257).
 Cut cut_forward(const gdn_linear_attn_args& a) {
     const Cut segments = cut_segments(a);
     if (a.dtype != GDN_BF16 || a.K > 128 || !segments.several) return segments;
     const int64_t chunks = (a.T + 63) / 64, cus = compute_units();
     const int64_t rounds = ((int64_t)a.N * a.H * ((a.V + 31) / 32) + cus - 1) / cus;
     const int64_t blocks = (int64_t)a.B * a.H * chunks * ((a.V + 127) / 128);
-    if (rounds * (6000 + (a.K <= 64 ? 800 : 1200) * chunks) >= 30000 + (a.K <= 64 ? 7 : 17) * blocks) return segments;  // ns
+    if (rounds * (6000 + (a.K <= 64 ? 800 : 1250) * chunks) >= 30000 + (a.K <= 64 ? 7 : 18) * blocks) return segments;  // ns
     Cut c;
     c.seg = (a.T + 63) / 64 * 64, c.nseg = a.cu_seqlens != nullptr && !(a.flags & GDN_FLAG_LEFT_PADDED) ? 0 : 1;
     c.slots = a.N, c.chain = true, c.several = false;

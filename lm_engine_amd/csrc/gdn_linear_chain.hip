@@ -12,9 +12,10 @@
 // ahead; the P waves bring in x and z (and its decayed rows, in two or three bf16 parts), the S waves y.  The O waves load nothing: the
 // compiler's wait for rows would be one for their stores.
 //
-// Measured at 4 sequences of 4096 tokens, 16 heads, K = V = 128, which is one workgroup to a compute unit: 79 to 85 us, 1.2 us a chunk, of
-// which some 0.9 us are the S waves' own work (an operand read, 4 products of 64 cycles one behind the other, a write) and the rest the
-// barrier and the other groups; 268 MB in and out are 51 us at a large copy's rate.
+// Measured at 4 sequences of 4096 tokens, 16 heads, K = V = 128, which is one workgroup to a compute unit: 80 us, with a final state
+// 88, 1.25 us a chunk, of which some 0.9 us are the S waves' own work (an operand read, products one behind the other, a write) and
+// the rest the barrier and the other groups; 268 MB in and out are 51 us at a large copy's rate.  With the tiles of P on the diagonal
+// formed by the O waves, 83; with 64 columns to a workgroup registers spill.
 #include <algorithm>
 
 #include "gdn_launch.h"
