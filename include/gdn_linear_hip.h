@@ -33,7 +33,8 @@ int gdn_linear_abi_version(void);
  *   flags  GDN_FLAG_LEFT_PADDED, GDN_FLAG_ZERO_PADDING: zeros are written at tokens that belong to no sequence (the
  *          padding, tokens behind the last packed sequence); without it nothing is written there
  *
- * K a multiple of 8 up to 256, V a multiple of 8.  dtype: of q, k, v, o.  Rows, and with them strides, 16-byte aligned.
+ * K a multiple of 8 up to 256, V a multiple of 8.  dtype: of q, k, v, o.  Rows, and with them strides, 16-byte aligned;
+ * tokens 0 to 2^24 elements apart.
  */
 typedef struct gdn_linear_attn_args {
     const void *q;
@@ -76,7 +77,8 @@ int gdn_linear_attn_recurrent_fwd(const gdn_linear_attn_args *args, void *stream
 /*
  * Gradients of gdn_linear_attn_chunk_fwd (and of the recurrent form, which is the same function): from the forward's inputs, dout
  * and dht (NULL: zero) it writes
- *   dq, dk [B, T, qk_heads, K]  (the gradients of value heads that share one of q and k are added up in fp32)
+ *   dq, dk [B, T, qk_heads, K]  (the gradients of value heads that share one of q and k are added up in fp32; where heads
+ *                              are shared, tokens of no sequence get zeros with or without GDN_FLAG_ZERO_PADDING)
  *   dv     [B, T, H, V]
  *   dh0    [N, H, K, V] fp32 or NULL
  *   dg     [H] fp32 or NULL: the derivative with respect to g[h], over all sequences

@@ -15,7 +15,7 @@ int check_rows(const void* p, int64_t b, int64_t t, int64_t h, int dtype) {
     const int64_t vec = dtype == GDN_BF16 ? 8 : 4;
     if (p == nullptr) return GDN_ERR_NULL;
     if (!aligned16(p) || b % vec != 0 || t % vec != 0 || h % vec != 0) return GDN_ERR_ALIGN;
-    if (t > 1 << 24 || t < -(1 << 24)) return GDN_ERR_UNSUPPORTED;  // the bytes of a chunk of 64 tokens are counted in 32 bits
+    if (t < 0 || t > 1 << 24) return GDN_ERR_UNSUPPORTED;  // the bytes of a chunk of 64 tokens are counted in 32 bits, without a sign
     return GDN_OK;
 }
 
@@ -204,6 +204,7 @@ int run_transposed(LinearParams p, const gdn_linear_attn_args& a, bool own_state
         p.init = whole.init == nullptr ? nullptr : whole.init + first;
         p.sums = sums;
         p.sums_in = first > 0, p.sums_only = heads_shared(a) > 1, p.sums_out = p.sums_only || first + KEYS < a.V;
+        if (p.sums_only) p.zero = 1;  // (all rows of sums are added up)
         if (own_states) {
             if (const int e = run_states(p, a.dtype, stream); e != GDN_OK) return e;
         } else if (p.local != nullptr && p.local_keys != 0) {

@@ -68,7 +68,7 @@ def _attention(**over):
 BAD = [
     (dict(q=None), -1), (dict(v=None), -1), (dict(T=0), -2), (dict(B=-1), -2), (dict(N=3), -2), (dict(qk_heads=3), -2), (dict(qk_heads=-1), -2),
     (dict(K=60), -3), (dict(K=264), -3), (dict(V=20), -3), (dict(dtype=7), -3), (dict(flags=1 << 20), -3), (dict(H=65536, qk_heads=0), -3),
-    (dict(T=(1 << 30) + 1), -3), (dict(q_stride_t=(1 << 24) + 8), -3), (dict(v_stride_t=-(1 << 24) - 8), -3),
+    (dict(T=(1 << 30) + 1), -3), (dict(q_stride_t=(1 << 24) + 8), -3), (dict(v_stride_t=-(1 << 24) - 8), -3), (dict(k_stride_t=-8), -3),
     (dict(k=FAKE + 8), -4), (dict(q_stride_h=68), -4), (dict(v_stride_b=4), -4), (dict(h0=FAKE + 4), -4), (dict(g=FAKE + 2), -4),
     (dict(cu_seqlens=FAKE), -6), (dict(flags=_lib.GDN_FLAG_LEFT_PADDED), -1), (dict(flags=_lib.GDN_FLAG_LEFT_PADDED, cu_seqlens=FAKE, N=3), -2),
 ]  # fmt: skip

@@ -412,3 +412,31 @@ def test_a_switched_off_kernel_is_refused_in_the_backward_too():
         for out in (o, y):
             with pytest.raises(RuntimeError, match="disabled"):
                 torch.autograd.grad(out, q, torch.ones_like(out), retain_graph=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_shared_heads_of_a_packed_batch_leave_zeros_outside(dtype):
+    """The fold of shared heads reads every token: those in front of and behind the sequences are zeros, whatever the workspace held."""
+    lens, T = [40, 0, 333], 400
+    inputs = _inputs(1, T, 4, 64, 72, HK=2, N=3, dtype=dtype)
+    torch.full((1 << 24,), float("nan"), device="cuda")
+    got, want = _gradients(inputs, dtype, cu=_cu(lens))
+    for n in ("q", "k", "v"):
+        assert (got[n][:, 373:] == 0).all(), n
+    _check_gradients(got, want, dtype, shared=True)
+    shifted = torch.tensor([20, 60, 60, 393], dtype=torch.int32).cuda()
+    leaves = {n: x.cuda().requires_grad_() for n, x in inputs.items()}
+    o, _ = chunk_linear_attention(**leaves, cu_seqlens=shifted)
+    for n, x in zip(("q", "k", "v"), torch.autograd.grad(o, [leaves[n] for n in ("q", "k", "v")], torch.ones_like(o))):
+        assert x.isfinite().all() and (x[:, :20] == 0).all() and (x[:, 393:] == 0).all() and (x[:, 20:393] != 0).any(), n
+
+
+def test_a_decay_at_either_end():
+    """No memory at all (-inf: 0 to the power 0 is 1), none of it lost (0), and in between the products of 64 tokens below fp32's range."""
+    inputs = _inputs(1, 200, 4, 64, 64)
+    inputs["g"] = torch.tensor([-float("inf"), 0.0, -87.0, -1e-30])
+    want, want_state = linear_attention_ref(**inputs)
+    for fn in (chunk_linear_attention, fused_recurrent_linear_attention):
+        o, state = fn(**_cuda(inputs), output_final_state=True)
+        _check("o", o, want, OUT[BF16])
+        _check("state", state, want_state, STATE[BF16])
