@@ -7,7 +7,8 @@
 // groups by shuffles, and the four waves' sums meet in LDS behind the TB.
 // Bound by memory on one token: 256 states of 32 heads, K = V = 128, 1.07 GB to and fro: 178 us, 6.0 TB/s (203 through the caches; at 128
 // states, which they hold from call to call, 93 against 78: a model's other layers would not leave them there).  On many tokens by the
-// chain from one token to the next: 0.36 us a token in the smallest calls, 4 x 1024 tokens of 16 heads of 128 in fp32 280 us.
+// chain from one token to the next: 0.36 us a token in the smallest calls, 4 x 1024 tokens of 16 heads of 128 in fp32 299 us (280 with a
+// token's factor as one number).
 #include <algorithm>
 
 #include "gdn_launch.h"
@@ -41,7 +42,11 @@ __global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p
     if (STATES_ONLY && last && p.fin == nullptr) return;  // nothing starts from it
     const int walked = sg.s * p.seg, total = min(p.seg, sg.len - walked);
     const int64_t token = p.reverse ? (int64_t)sg.t0 + sg.len - 1 - walked : (int64_t)sg.t0 + walked;
-    const float w = p.g == nullptr ? 1.f : expf(p.g[h]);
+    // A token's factor e^g as kept + rest, 1 and e^g - 1 where the state lasts: exact to 2^-24 of what it takes away then; as one number its
+    // rounding would come back once for every token that the state remembers.
+    const float log_decay = p.g == nullptr ? 0.f : p.g[h];
+    const bool lasts = log_decay > -0.5f;
+    const float kept_by_all = lasts ? 1.f : 0.f, rest_of_all = lasts ? expm1f(log_decay) : expf(log_decay);
 
     const int vl = lane % VL, group = wave * (64 / VL) + lane / VL;
     const int col = 4 * vl;
@@ -95,12 +100,13 @@ __global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p
         }
         __syncthreads();
         for (int t = 0; t < n; t++) {
-            const float factor = p.a == 1 || first + t > 0 ? w : 1.f;  // a = 0: the state decays behind a token, not in front of it
+            const bool decays = p.a == 1 || first + t > 0;  // a = 0: the state decays behind a token, not in front of it
+            const float kept = decays ? kept_by_all : 1.f, rest = decays ? rest_of_all : 0.f;
             const f32x4 z = *reinterpret_cast<const f32x4*>(&sz[t][col]);
             f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int r = 0; r < KR; r++) {
-                S[r] = S[r] * factor + z * sy[t][key(r)];
+                S[r] = (S[r] * rest + S[r] * kept) + z * sy[t][key(r)];
                 if constexpr (!STATES_ONLY) o += S[r] * sx[t][key(r)];
             }
             if constexpr (!STATES_ONLY) {
@@ -134,7 +140,7 @@ __global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p
     }
     if (p.a == 0 && total > 0) {
 #pragma unroll
-        for (int r = 0; r < KR; r++) S[r] = S[r] * w;
+        for (int r = 0; r < KR; r++) S[r] = S[r] * rest_of_all + S[r] * kept_by_all;
     }
     float* to = nullptr;
     if constexpr (STATES_ONLY) to = p.local + ((int64_t)slot * p.H + h) * p.local_cells;
