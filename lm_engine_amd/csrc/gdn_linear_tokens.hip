@@ -162,6 +162,8 @@ int launch(const LinearParams& p, bool states_only, hipStream_t stream) {
     if (blocks > 0xfffff000ll / 256) return GDN_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)((blocks + 7) / 8 * 8)), threads(256);
     if (states_only) hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 16, true>), grid, threads, 0, stream, p);
+    // room for one token where there is no second, so that more workgroups fit a unit: 64 states of 32 heads 49.5 us against 51.4, 32 24.5
+    // against 25.5, 256 179 either way
     else if (p.T == 1) hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 1, false>), grid, threads, 0, stream, p);
     else hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 16, false>), grid, threads, 0, stream, p);
     return (int)hipGetLastError();
@@ -201,6 +203,7 @@ __global__ __launch_bounds__(256) void linear_fold_kernel(const LinearFold p) {
 
 }  // namespace
 
+// 128 columns to a workgroup where they make one to every unit (16 states of 32 heads 11.0 us, with 32 columns 14.1), else 32: more of them
 int linear_tokens_columns(int64_t chains, int V, int cus) { return V >= 128 && chains * ((V + 127) / 128) >= cus ? 128 : 32; }
 
 int launch_linear_tokens(const LinearParams& p, int dtype, int columns, bool states_only, hipStream_t stream) {
