@@ -18,6 +18,13 @@ def kernel_rows(grad: torch.Tensor, stride_elements: int = 8, address_bytes: int
     return grad.clone(memory_format=torch.contiguous_format)  # (contiguous() returns a dense tensor at an odd offset as it is)
 
 
+def mark_written(x: torch.Tensor) -> None:
+    """What a torch operation in place tells autograd: a backward that saved ``x``, or a tensor that shares its memory, raises from here on.
+    (Tensors made in inference mode are never saved, and have no version.)"""
+    if not x.is_inference():
+        torch.autograd.graph.increment_version(x)
+
+
 class _KernelWithFormulaBackward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, kernel, formula, *inputs):

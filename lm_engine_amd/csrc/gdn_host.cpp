@@ -196,6 +196,11 @@ PyObject* launch(const char* what, PyObject* made, F&& entry) {
     return PyObject_CallFunction(check_status, "is", status, what);
 }
 
+// mark_written of _autograd.py, behind a launch that was not refused
+void mark_written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 at::Tensor fresh(const at::Tensor& like, at::IntArrayRef sizes) { return at::empty(sizes, like.options()); }
 at::Tensor fresh_f32(const at::Tensor& like, at::IntArrayRef sizes) { return at::empty(sizes, like.options().dtype(at::kFloat)); }
 
@@ -792,8 +797,11 @@ PyObject* linear_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         s.o = ptr(o), s.o_stride_b = o.stride(0), s.o_stride_t = o.stride(1), s.o_stride_h = o.stride(2);
         THPObjectPtr results(pack_results({o, ht}));
         if (results && inplace) PyTuple_SetItem(results.get(), 1, Py_NewRef(args[7]));  // the caller's own tensor object
-        return launch(chunked ? "gdn_linear_attn_chunk_fwd" : "gdn_linear_attn_recurrent_fwd", results.release(),
-                      [&] { return (chunked ? linear_chunk_fn : linear_recurrent_fn)(&s, stream); });
+        return launch(chunked ? "gdn_linear_attn_chunk_fwd" : "gdn_linear_attn_recurrent_fwd", results.release(), [&] {
+            const int status = (chunked ? linear_chunk_fn : linear_recurrent_fn)(&s, stream);
+            if (inplace && status >= 0) mark_written(ht);
+            return status;
+        });
     });
 }
 

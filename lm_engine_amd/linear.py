@@ -27,7 +27,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._autograd import kernel_rows
+from ._autograd import kernel_rows, mark_written
 from ._host import host, raw_stream
 from .kernels import Kernel, is_kernel_allowed
 from .ops import RECURRENT_MAX_TOKENS, _dtype_code
@@ -158,6 +158,8 @@ def _run(mode, q, k, v, g, scale, initial_state, output_final_state, cu_seqlens,
             _lib.check_status(lib.gdn_linear_attn_chunk_fwd(ctypes.byref(args), stream), "gdn_linear_attn_chunk_fwd")
         else:
             _lib.check_status(lib.gdn_linear_attn_recurrent_fwd(ctypes.byref(args), stream), "gdn_linear_attn_recurrent_fwd")
+    if inplace_state:
+        mark_written(initial_state)
     return o, (initial_state if inplace_state else ht)
 
 
@@ -292,7 +294,7 @@ def fused_recurrent_linear_attention(
     """One token per sequence, or a few: every state passes through registers once, fp32 throughout.
 
     With ``inplace_state=True`` (and ``output_final_state=True``) the final state overwrites ``initial_state`` and that same tensor is
-    returned, as in ``fused_recurrent_gated_delta_rule``."""
+    returned, as in ``fused_recurrent_gated_delta_rule``; autograd counts it as written (not where a captured graph is replayed)."""
     return _dispatch("recurrent", q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, inplace_state, left_padded)
 
 
