@@ -479,8 +479,11 @@ PyObject* delta_rule(PyObject*, PyObject* const* args, Py_ssize_t n) {
         s.scale = args[7] == Py_None ? (float)std::pow((double)K, -0.5) : (float)number(args[7]);
         THPObjectPtr results(pack_results({o, ht}));
         if (results && output_final && inplace) PyTuple_SetItem(results.get(), 1, Py_NewRef(args[8]));  // the caller's own tensor object
-        return launch(chunked ? "gdn_chunk_fwd" : "gdn_recurrent_fwd", results.release(),
-                      [&] { return (chunked ? chunk_fn : recurrent_fn)(&s, stream); });
+        return launch(chunked ? "gdn_chunk_fwd" : "gdn_recurrent_fwd", results.release(), [&] {
+            const int status = (chunked ? chunk_fn : recurrent_fn)(&s, stream);
+            if (output_final && inplace && status >= 0) mark_written(ht);
+            return status;
+        });
     });
 }
 

@@ -31,7 +31,7 @@ from collections import OrderedDict
 import torch
 
 from . import _lib
-from ._autograd import kernel_rows
+from ._autograd import kernel_rows, mark_written
 from ._host import host, raw_stream
 from .backward import gated_delta_rule_backward
 from .kernels import Kernel, is_kernel_allowed
@@ -295,6 +295,8 @@ def _run(mode, q, k, v, g, beta, scale, initial_state, output_final_state, cu_se
                 raise
         else:
             _lib.check_status(lib.gdn_recurrent_fwd(ctypes.byref(args), stream), "gdn_recurrent_fwd")
+    if inplace_state and ht is not None:
+        mark_written(initial_state)
     return o, ht
 
 

@@ -4,7 +4,7 @@ instead of computing with what it has become."""
 import pytest
 import torch
 
-from lm_engine_amd import chunk_linear_attention, fused_recurrent_linear_attention
+from lm_engine_amd import chunk_gated_delta_rule, chunk_linear_attention, fused_recurrent_gated_delta_rule, fused_recurrent_linear_attention
 
 
 pytestmark = pytest.mark.gpu
@@ -24,7 +24,17 @@ class LinearAttention:
     whole, step = chunk_linear_attention, fused_recurrent_linear_attention
 
 
-OPERATORS = [LinearAttention]
+class DeltaRule:
+    @staticmethod
+    def inputs(tokens, wide):
+        q, k, v = (torch.randn(2, tokens, 2, 64, device="cuda").to(BF16) for _ in range(3))
+        g = -0.1 * torch.rand(2, tokens, 2, device="cuda", dtype=torch.float64 if wide else torch.float32)
+        return dict(q=q, k=torch.nn.functional.normalize(k, dim=-1), v=v, g=g, beta=torch.rand(2, tokens, 2, device="cuda"))
+
+    whole, step = chunk_gated_delta_rule, fused_recurrent_gated_delta_rule
+
+
+OPERATORS = [LinearAttention, DeltaRule]
 
 
 def _state():
