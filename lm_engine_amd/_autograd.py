@@ -7,6 +7,7 @@ elementwise or row-wise and memory-bound: the backward costs a few passes over t
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 
 def kernel_rows(grad: torch.Tensor, stride_elements: int = 8, address_bytes: int = 16) -> torch.Tensor:
@@ -23,6 +24,13 @@ def mark_written(x: torch.Tensor) -> None:
     (Tensors made in inference mode are never saved, and have no version.)"""
     if not x.is_inference():
         torch.autograd.graph.increment_version(x)
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """Raises where one of ``tensors`` (or None) is a dual tensor: the kernels know of no tangents, and a result without one would stand for
+    a derivative of zero."""
+    if any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 class _KernelWithFormulaBackward(torch.autograd.Function):

@@ -78,7 +78,7 @@ void need(bool ok) {
     if (!ok) throw NotHere{};
 }
 
-// The operands of one call: all on one device, which is the current one, plain tensors, no gradient wanted.
+// The operands of one call: all on one device, which is the current one, plain tensors, no gradient wanted, no tangent carried (forward mode).
 struct Operands {
     c10::Device device{c10::DeviceType::CPU};
     bool grad = c10::GradMode::is_enabled();
@@ -88,6 +88,7 @@ struct Operands {
         const at::Tensor& t = THPVariable_Unpack(x);
         need(t.defined() && t.device().type() == c10::DeviceType::CUDA && !(grad && t.requires_grad()) && t.layout() == at::kStrided);
         need(!t.unsafeGetTensorImpl()->key_set().has(c10::DispatchKey::Python) && t.unsafeGetTensorImpl()->has_storage() && !t.is_conj() && !t.is_neg());
+        need(!t._fw_grad(0).defined());
         if (device.type() == c10::DeviceType::CPU) {
             device = t.device();
             need(c10::impl::VirtualGuardImpl(c10::DeviceType::CUDA).getDevice().index() == device.index());

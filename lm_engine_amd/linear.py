@@ -16,7 +16,8 @@ K and V are multiples of 8, K at most 256.  Tokens that belong to no sequence (p
 read as zeros in ``o`` and in the gradients.  A token whose values are not finite spoils the outputs of the 64 tokens around it that
 are computed together with it, earlier ones among them.
 
-Both forms are differentiable; the backward works from the saved inputs (``gdn_linear_attn_bwd``).  The kernels
+Both forms are differentiable; the backward works from the saved inputs (``gdn_linear_attn_bwd``).  Second derivatives and dual tensors
+(forward mode) are refused.  The kernels
 are those of ``csrc/gdn_linear_*.hip``; there is no fallback.
 """
 
@@ -27,7 +28,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._autograd import kernel_rows, mark_written
+from ._autograd import kernel_rows, mark_written, refuse_tangents
 from ._host import host, raw_stream
 from .kernels import Kernel, is_kernel_allowed
 from .ops import RECURRENT_MAX_TOKENS, _dtype_code
@@ -131,6 +132,7 @@ def _run(mode, q, k, v, g, scale, initial_state, output_final_state, cu_seqlens,
     _require_hip_path()
     dims = _check_inputs(q, k, v, g, initial_state, cu_seqlens, left_padded)
     B, T, H, K, V, N = dims
+    refuse_tangents("linear attention", q, k, v, g, initial_state)
     if inplace_state and (mode != "recurrent" or not output_final_state or initial_state is None or not initial_state.is_contiguous()
                           or initial_state.data_ptr() % 16 != 0):  # fmt: skip
         raise ValueError("inplace_state needs a contiguous initial_state to update and output_final_state=True")
@@ -176,6 +178,7 @@ def _backward(q, k, v, g, scale, initial_state, cu_seqlens, left_padded, do, dht
     _require_hip_path()
     dims = _check_inputs(q, k, v, g, initial_state, cu_seqlens, left_padded)
     B, T, H, K, V, N = dims
+    refuse_tangents("the backward of linear attention", q, k, v, g, initial_state, do, dht)
     HK, dev, dtype = q.size(2), q.device, v.dtype
     new = lambda *shape: torch.empty(*shape, dtype=dtype, device=dev)  # noqa: E731
     dq, dk, dv = new(B, T, HK, K), new(B, T, HK, K), new(B, T, H, V)

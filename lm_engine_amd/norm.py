@@ -11,6 +11,7 @@ import ctypes
 import torch
 
 from . import _lib
+from ._autograd import refuse_tangents
 from ._host import host, raw_stream
 from .kernels import Kernel, is_kernel_allowed
 from .layer_ops import _dtype_code, column_sums
@@ -51,6 +52,7 @@ def _as_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int]:
 
 def _forward(x, weight, bias, eps):
     D = _check(x, weight, bias)
+    refuse_tangents("layer norm", x, weight, bias)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if x.numel() == 0:
         return y
@@ -75,6 +77,7 @@ def _forward(x, weight, bias, eps):
 def _backward(x, weight, bias_dtype, eps, dy, needs_dw, needs_db):
     """``gdn_layer_norm_bwd``: (dx, dweight or None, dbias or None)."""
     D = _check(x, weight, None)
+    refuse_tangents("the backward of layer norm", x, weight, dy)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if x.numel() == 0:
         return dx, (torch.zeros_like(weight) if needs_dw else None), (torch.zeros(D, dtype=bias_dtype, device=x.device) if needs_db else None)
@@ -139,7 +142,7 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
     """x ``[..., D]`` (bf16 or fp32, D up to 16384; leading dims that collapse to rows of one stride are read where they lie); weight and
     bias ``[D]`` (bf16 or fp32) or None.  Returns ``(x - mean) / sqrt(var + eps) * weight + bias`` over D, shape and dtype of x, contiguous;
-    mean, variance and everything up to the result in fp32."""
+    mean, variance and everything up to the result in fp32.  Differentiable, but neither twice nor in forward mode."""
     eps = float(eps)
     if torch.compiler.is_compiling():  # a graph is being captured: the kernel goes in as an opaque operator
         from . import _opaque
