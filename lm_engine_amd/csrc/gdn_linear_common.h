@@ -175,6 +175,17 @@ __device__ __forceinline__ void linear_zero_gaps(const LinearParams& p, int slot
 __device__ __forceinline__ float linear_log2(const float* g, int h) { return g == nullptr ? 0.f : g[h] * 1.4426950408889634f; }
 __device__ __forceinline__ float linear_power(float g2, int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f(g2 * (float)n); }
 
+// A factor w = e^x that is applied again and again, as kept + rest: 1 and w - 1 where the state lasts, exact to 2^-24 of what it takes away
+// then.  As one number its rounding, up to 2^-25, would come back with every application that the state remembers.
+struct LinearFactor {
+    float kept, rest;
+    __device__ __forceinline__ explicit LinearFactor(float x) : kept(x > -0.5f ? 1.f : 0.f), rest(x > -0.5f ? expm1f(x) : expf(x)) {}
+    template <typename T>
+    __device__ __forceinline__ T operator()(T s) const {
+        return s * rest + s * kept;
+    }
+};
+
 // Where cell (key, v) lies in a state that the bf16 walk has written: [32 columns][32 keys][4 registers of 4][64 lanes][4 keys].
 __device__ __forceinline__ int64_t linear_fragment(int keys, int key, int v) {
     const int r = 8 * (key >> 4 & 1) + (key & 7), lane = 32 * (key >> 3 & 1) + slice_col(v & 31);

@@ -210,7 +210,7 @@ __global__ __launch_bounds__(256) void linear_tangent_tokens_kernel(const Linear
     if (STATES_ONLY && last) return;
     const int walked = sg.s * p.seg, total = min(p.seg, sg.len - walked);
     const int64_t token = (int64_t)sg.t0 + walked;
-    const float w = expf(p.g[h]);
+    const LinearFactor w(p.g[h]);
 
     const int group = wave * (64 / VL) + lane / VL, col = 4 * (lane % VL);
     const bool mine = col < columns;
@@ -246,20 +246,25 @@ __global__ __launch_bounds__(256) void linear_tangent_tokens_kernel(const Linear
             if constexpr (!STATES_ONLY) *reinterpret_cast<f32x4*>(&sd[t][c]) = c < columns ? load4<float>(pd + row * p.d.stride_t + c0 + c) : none;
         }
         __syncthreads();
-        for (int t = 0; t < n; t++) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(&sv[t][col]);
-            f32x4 o = none;
+        auto walk = [&](auto shrunk) __attribute__((always_inline)) {
+            for (int t = 0; t < n; t++) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(&sv[t][col]);
+                f32x4 o = none;
 #pragma unroll
-            for (int r = 0; r < KR; r++) {
-                U[r] = (U[r] + S[r]) * w;
-                S[r] = S[r] * w + v * sk[t][key(r)];
-                if constexpr (!STATES_ONLY) o += U[r] * sq[t][key(r)];
+                for (int r = 0; r < KR; r++) {
+                    U[r] = shrunk(U[r] + S[r]);
+                    S[r] = shrunk(S[r]) + v * sk[t][key(r)];
+                    if constexpr (!STATES_ONLY) o += U[r] * sq[t][key(r)];
+                }
+                if constexpr (!STATES_ONLY) {
+                    const f32x4 d = *reinterpret_cast<const f32x4*>(&sd[t][col]);
+                    sum += o[0] * d[0] + o[1] * d[1] + o[2] * d[2] + o[3] * d[3];
+                }
             }
-            if constexpr (!STATES_ONLY) {
-                const f32x4 d = *reinterpret_cast<const f32x4*>(&sd[t][col]);
-                sum += o[0] * d[0] + o[1] * d[1] + o[2] * d[2] + o[3] * d[3];
-            }
-        }
+        };
+        // (one operation each: with both parts multiplied 4 x 1024 tokens of 16 heads of 128 take 5 % longer, forward and backward)
+        if (w.kept == 1.f) walk([&](f32x4 s) { return s * w.rest + s; });
+        else walk([&](f32x4 s) { return s * w.rest; });
     }
     if constexpr (STATES_ONLY) {
 #pragma unroll

@@ -42,11 +42,7 @@ __global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p
     if (STATES_ONLY && last && p.fin == nullptr) return;  // nothing starts from it
     const int walked = sg.s * p.seg, total = min(p.seg, sg.len - walked);
     const int64_t token = p.reverse ? (int64_t)sg.t0 + sg.len - 1 - walked : (int64_t)sg.t0 + walked;
-    // A token's factor e^g as kept + rest, 1 and e^g - 1 where the state lasts: exact to 2^-24 of what it takes away then; as one number its
-    // rounding would come back once for every token that the state remembers.
-    const float log_decay = p.g == nullptr ? 0.f : p.g[h];
-    const bool lasts = log_decay > -0.5f;
-    const float kept_by_all = lasts ? 1.f : 0.f, rest_of_all = lasts ? expm1f(log_decay) : expf(log_decay);
+    const LinearFactor factor(p.g == nullptr ? 0.f : p.g[h]), none(0.f);  // of a token
 
     const int vl = lane % VL, group = wave * (64 / VL) + lane / VL;
     const int col = 4 * vl;
@@ -100,13 +96,12 @@ __global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p
         }
         __syncthreads();
         for (int t = 0; t < n; t++) {
-            const bool decays = p.a == 1 || first + t > 0;  // a = 0: the state decays behind a token, not in front of it
-            const float kept = decays ? kept_by_all : 1.f, rest = decays ? rest_of_all : 0.f;
+            const LinearFactor w = p.a == 1 || first + t > 0 ? factor : none;  // a = 0: the state decays behind a token, not in front of it
             const f32x4 z = *reinterpret_cast<const f32x4*>(&sz[t][col]);
             f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int r = 0; r < KR; r++) {
-                S[r] = (S[r] * rest + S[r] * kept) + z * sy[t][key(r)];
+                S[r] = w(S[r]) + z * sy[t][key(r)];
                 if constexpr (!STATES_ONLY) o += S[r] * sx[t][key(r)];
             }
             if constexpr (!STATES_ONLY) {
@@ -140,7 +135,7 @@ __global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p
     }
     if (p.a == 0 && total > 0) {
 #pragma unroll
-        for (int r = 0; r < KR; r++) S[r] = S[r] * rest_of_all + S[r] * kept_by_all;
+        for (int r = 0; r < KR; r++) S[r] = factor(S[r]);
     }
     float* to = nullptr;
     if constexpr (STATES_ONLY) to = p.local + ((int64_t)slot * p.H + h) * p.local_cells;
