@@ -185,6 +185,8 @@ struct LinearFactor {
         return s * rest + s * kept;
     }
 };
+// ... of n tokens; 1 for none also where the state forgets at once (-inf)
+__device__ __forceinline__ LinearFactor linear_factor(float g, int n) { return LinearFactor(n == 0 ? 0.f : g * (float)n); }
 
 // Where cell (key, v) lies in a state that the bf16 walk has written: [32 columns][32 keys][4 registers of 4][64 lanes][4 keys].
 __device__ __forceinline__ int64_t linear_fragment(int keys, int key, int v) {

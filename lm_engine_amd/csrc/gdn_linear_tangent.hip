@@ -300,7 +300,8 @@ __global__ __launch_bounds__(256) void linear_tangent_combine_kernel(const Linea
             linear_find_packed(p, -1, none, threadIdx.x & 63, n, &slot0);
         }
         if (slot0 + segments > p.slots || at >= p.cells) continue;
-        const float whole = linear_power(linear_log2(p.g, h), p.seg), tokens = (float)p.seg;
+        const LinearFactor whole = linear_factor(p.g[h], p.seg);
+        const float tokens = (float)p.seg;
         const int64_t first = ((int64_t)slot0 * p.H + h) * p.cells + at, next = (int64_t)p.H * p.cells;
         auto cell = [&](float* base, int s) { return reinterpret_cast<f32x4*>(base + first + s * next); };
         f32x4 S = {0.f, 0.f, 0.f, 0.f}, U = S;
@@ -309,8 +310,8 @@ __global__ __launch_bounds__(256) void linear_tangent_combine_kernel(const Linea
         for (int s = 1; s < segments; s++) {
             f32x4 next_S = {0.f, 0.f, 0.f, 0.f}, next_U = next_S;
             if (s + 1 < segments) next_S = *cell(p.local, s), next_U = *cell(p.local_slope, s);
-            U = (U + S * tokens) * whole + own_U;
-            S = S * whole + own_S;
+            U = whole(U + S * tokens) + own_U;
+            S = whole(S) + own_S;
             *cell(p.local, s) = S, *cell(p.local_slope, s) = U;
             own_S = next_S, own_U = next_U;
         }

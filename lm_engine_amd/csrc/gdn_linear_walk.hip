@@ -335,7 +335,8 @@ __global__ __launch_bounds__(256) void linear_combine_kernel(const LinearParams 
             linear_find_packed(p, -1, none, threadIdx.x & 63, n, &slot0);
         }
         if (slot0 + segments > p.slots || at >= p.local_cells) continue;
-        const float g = linear_log2(p.g, h), whole = linear_power(g, p.seg);
+        const float g = p.g == nullptr ? 0.f : p.g[h];
+        const LinearFactor whole = linear_factor(g, p.seg);
         float* local = p.local + ((int64_t)slot0 * p.H + h) * p.local_cells + at;
         const int64_t next = (int64_t)p.H * p.local_cells, chain = ((int64_t)n * p.H + h) * p.cells + cell;
         f32x4 carry = {0.f, 0.f, 0.f, 0.f};
@@ -347,14 +348,14 @@ __global__ __launch_bounds__(256) void linear_combine_kernel(const LinearParams 
         for (int s = 1; s < segments; s++) {
             f32x4 following = {0.f, 0.f, 0.f, 0.f};
             if (s + 1 < segments || p.fin != nullptr) following = *reinterpret_cast<const f32x4*>(local + s * next);
-            carry = carry * whole + own;
+            carry = whole(carry) + own;
             *reinterpret_cast<f32x4*>(local + s * next) = carry;
             own = following;
         }
         if (p.fin != nullptr && there) {  // behind the last segment, whose tokens are `rest`
-            const float last = linear_power(g, len - (segments - 1) * p.seg);
+            carry = linear_factor(g, len - (segments - 1) * p.seg)(carry) + own;
 #pragma unroll
-            for (int e = 0; e < 4; e++) p.fin[chain + e * apart] = carry[e] * last + own[e];
+            for (int e = 0; e < 4; e++) p.fin[chain + e * apart] = carry[e];
         }
     }
 }

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from lm_engine_amd import chunk_linear_attention
+from tests.helpers import rel_l2
 
 
 pytestmark = pytest.mark.gpu
@@ -43,3 +44,52 @@ def test_gradient_of_a_slow_decay_in_fp32():
     error = ((got.to(F64) - want) / want).abs()
     print(error.tolist(), flush=True)
     assert (error <= 2e-6).all(), error.tolist()
+
+
+@pytest.mark.parametrize("g", [-1.5360825273091905e-05, -1.6082474758150056e-05, -1.226804124598857e-05, -1.041237101162551e-05,
+                               -1.4845360965409782e-05, -1.1752576938306447e-05])  # fmt: skip
+def test_states_of_many_segments_in_fp32(g):
+    """1024 segments of 64 tokens of one head, joined by factors e^{64 g} that fp32 numbers are 2.7e-8 off from or more: some 1e-5 in all.
+    Two roundings a join and two a token of a segment: sqrt(2 (1024 + 64) / 3) 2^-24 = 1.6e-6 at most, 3e-6 is asked."""
+    T, D = 65536, 8
+    q, k, v, do = (_normal(1, T, 1, D, seed=s) for s in range(4))
+    decay = torch.tensor([g], device="cuda")
+    state = torch.zeros(1, 1, D, D, device="cuda", requires_grad=True)
+    o, final = chunk_linear_attention(q, k, v, decay, initial_state=state, output_final_state=True)
+    dh0, = torch.autograd.grad(o, state, do)
+    n = torch.arange(T, device="cuda", dtype=F64)
+    flat = lambda x: x[0, :, 0].to(F64)  # noqa: E731
+    w = decay.to(F64)
+    want = (flat(k) * torch.exp(w * (T - 1 - n))[:, None]).t().contiguous() @ flat(v)
+    want_dh0 = D**-0.5 * (flat(q) * torch.exp(w * (n + 1))[:, None]).t().contiguous() @ flat(do)
+    errors = rel_l2(final[0, 0], want), rel_l2(dh0[0, 0], want_dh0)
+    print(errors, flush=True)
+    assert max(errors) <= 3e-6, errors
+
+
+@pytest.mark.parametrize("g", [-1.5360825273091905e-05, -1.226804124598857e-05, -1.1752576938306447e-05])
+def test_gradient_of_a_slow_decay_over_many_segments_in_fp32(g):
+    """As above, of the state's derivative, which remembers twice as long: twice the limit."""
+    T, D = 65536, 8
+    q, k, v, do = (_normal(1, T, 1, D, seed=s) for s in range(4))
+    decay = torch.tensor([g], device="cuda", requires_grad=True)
+    o, _ = chunk_linear_attention(q, k, v, decay)
+    got, = torch.autograd.grad(o, decay, do)
+    # sum_t do_t . sum_{j < t} (t - j) w^{t - j} (q_t . k_j) v_j, 1024 tokens of each at a time
+    flat = lambda x: x[0, :, 0].to(F64)  # noqa: E731
+    qf, kf, vf, df, w, C = flat(q), flat(k), flat(v), flat(do), decay.detach().to(F64), 1024
+    S = torch.zeros(D, D, device="cuda", dtype=F64)
+    U, want, n = S.clone(), 0.0, torch.arange(C, device="cuda", dtype=F64)
+    first, last = torch.exp(w * (n + 1))[:, None], torch.exp(w * (C - 1 - n))[:, None]
+    gap = (n[:, None] - n[None, :]).clamp(min=0)
+    inside = gap * torch.exp(w * gap) * (gap > 0)
+    for a in range(0, T, C):
+        qb, kb, vb, db = (x[a : a + C] for x in (qf, kf, vf, df))
+        by_g = first * ((n + 1)[:, None] * (qb @ S) + qb @ U) + ((qb @ kb.t().contiguous()) * inside) @ vb
+        want += (by_g * db).sum()
+        U = torch.exp(w * C) * (U + C * S) + (kb * last * (C - 1 - n)[:, None]).t().contiguous() @ vb
+        S = torch.exp(w * C) * S + (kb * last).t().contiguous() @ vb
+    want = D**-0.5 * want
+    error = abs((got.item() - want) / want).item()
+    print(error, flush=True)
+    assert error <= 6e-6
