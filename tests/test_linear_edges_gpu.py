@@ -1,11 +1,12 @@
-"""Linear attention and layer norm where a call could be answered without an error and wrongly."""
+"""Linear attention and layer norm where a call could be answered without an error and wrongly: dual tensors, decays that grow the state."""
 
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 from lm_engine_amd import chunk_linear_attention, fused_recurrent_linear_attention, layer_norm
-from tests.test_linear_attention_gpu import _cuda, _inputs
+from oracle.linear_attention_oracle import linear_attention_ref
+from tests.test_linear_attention_gpu import BF16, F32, OUT, STATE, _check, _check_gradients, _cu, _cuda, _gradients, _inputs
 
 
 pytestmark = pytest.mark.gpu
@@ -54,3 +55,22 @@ def test_tangents_are_refused_by_layer_norm(grad):
     with forward_ad.dual_level(), pytest.raises(NotImplementedError):
         torch.autograd.grad(y, x, _dual(torch.ones_like(y)), retain_graph=True)
     assert torch.autograd.grad(y, x, torch.ones_like(y))[0].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lens", [[5], [1], [33], [50], [5, 17, 0, 33, 3]], ids=str)
+def test_a_state_that_grows(lens, dtype):
+    """g = 1.5: 50 tokens grow a state by e^75, and fp32 holds it; e^89 (59 tokens) it would not.  Whatever a short chunk has in the place of
+    its missing tokens must not overflow into the results.  A power w^n is off by n g 2^-24 < 5e-6 relative, inside the state's limit."""
+    T, H = sum(lens) + (3 if len(lens) > 1 else 0), 2
+    inputs = _inputs(1, T, H, 64, 72, N=len(lens), dtype=dtype)
+    inputs["g"] = torch.tensor([1.5, 1.4])
+    cu = _cu(lens) if len(lens) > 1 else None
+    cu_gpu = None if cu is None else torch.tensor(cu, dtype=torch.int32).cuda()
+    want, want_state = linear_attention_ref(**inputs, cu_seqlens=cu)
+    for fn in (chunk_linear_attention, fused_recurrent_linear_attention):
+        o, state = fn(**_cuda(inputs), output_final_state=True, cu_seqlens=cu_gpu)
+        _check("o", o, want, OUT[dtype])
+        _check("state", state, want_state, STATE[dtype])
+    got, expected = _gradients(inputs, dtype, learned=True, cu=cu)
+    _check_gradients(got, expected, dtype)
