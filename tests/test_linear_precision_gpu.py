@@ -3,13 +3,23 @@
 fp32, decays near one.  A factor w = e^{n g} held as one fp32 number is off by up to 2^-25 relative, the same way every time it is applied: a
 state that remembers m applications is off by m 2^-25, and m is in the thousands here.  Held as 1 and w - 1 it is exact; what is left
 are the roundings of the sums, independent of each other: with r of them remembered, each of at most 2^-24 relative (rms 2^-24 / sqrt 3),
-sqrt(r / 3) 2^-24."""
+sqrt(r / 3) 2^-24.
+
+bf16.  A state that is a result takes the decayed rows in three bf16 parts, all 24 bits of an fp32 product, in 12 additions a chunk of
+64 tokens, and is multiplied once a chunk: 13 roundings, 33 chunks at most here, sqrt(13 * 33 / 3) 2^-24 = 7.1e-7 if nothing were forgotten;
+1e-6 is asked.  (Two parts leave 2^-17 of a term, 2.4e-6 rms.)  Outputs and gradients: rounding normally distributed values to bf16 changes
+them by 1.66e-3 relative-L2; the state as an operand is rounded like that and makes one part of a sum, the weights of the tokens inside the
+chunk make the other part, so the sum is off by 1.66e-3 of its own before its own rounding: sqrt(2) 1.66e-3 = 2.35e-3, and 2.6e-3 is asked.
+Gradients of heads that share one of q and k are added up in fp32 and rounded once: no more than that.  (A second rounding would make
+sqrt(3) 1.66e-3 = 2.9e-3.)"""
 
 import pytest
 import torch
 
-from lm_engine_amd import chunk_linear_attention
+from lm_engine_amd import chunk_linear_attention, fused_recurrent_linear_attention
+from oracle.linear_attention_oracle import linear_attention_ref
 from tests.helpers import rel_l2
+from tests.test_linear_attention_gpu import BF16, _check, _cu, _cuda, _gradients, _inputs
 
 
 pytestmark = pytest.mark.gpu
@@ -93,3 +103,46 @@ def test_gradient_of_a_slow_decay_over_many_segments_in_fp32(g):
     error = abs((got.item() - want) / want).item()
     print(error, flush=True)
     assert error <= 6e-6
+
+
+STATE, OUT = 1e-6, 2.6e-3
+
+# (B, T, H, K, V, lengths of packed sequences, options): one segment on the walk (K above 128) and on whole sequences, several, shared heads,
+# more columns than a backward walk has keys
+SHAPES = [
+    (1, 64, 3, 128, 128, None, {}),
+    (2, 65, 2, 128, 128, None, {}),
+    (1, 129, 1, 256, 512, None, {}),
+    (2, 130, 2, 96, 80, None, {}),
+    (1, 1100, 2, 128, 128, None, {}),
+    (1, 2101, 2, 128, 128, None, {}),
+    (1, 1790, 1, 256, 64, None, {}),
+    (1, 400, 2, 64, 64, None, dict(decay="slow")),
+    (1, 700, 4, 64, 64, None, dict(HK=2)),
+    (2, 140, 6, 128, 128, None, dict(HK=2)),
+    (1, 900, 4, 72, 264, None, dict(HK=1)),
+    (1, 2000, 4, 64, 128, [1200, 3, 0, 400, 397], dict(HK=2)),
+]
+
+
+@pytest.mark.parametrize("B, T, H, K, V, lens, options", SHAPES, ids=str)
+def test_forward_in_bf16(B, T, H, K, V, lens, options):
+    inputs = _inputs(B, T, H, K, V, N=None if lens is None else len(lens), **options)
+    cu = None if lens is None else _cu(lens)
+    cu_gpu = None if cu is None else torch.tensor(cu, dtype=torch.int32).cuda()
+    want, want_state = linear_attention_ref(**inputs, cu_seqlens=cu)
+    for fn in (chunk_linear_attention, fused_recurrent_linear_attention):
+        o, state = fn(**_cuda(inputs), output_final_state=True, cu_seqlens=cu_gpu)
+        _check("o", o, want, OUT)
+        _check("state", state, want_state, STATE)
+
+
+@pytest.mark.parametrize("learned", [False, True], ids=["", "decay"])
+@pytest.mark.parametrize("B, T, H, K, V, lens, options", SHAPES, ids=str)
+def test_gradients_in_bf16(B, T, H, K, V, lens, options, learned):
+    """The decay's: sums of fp32 terms and products of bf16 numbers in three parts, 1e-5 (of its own size, which a sum over tokens and
+    columns may leave smaller than its terms)."""
+    inputs = _inputs(B, T, H, K, V, N=None if lens is None else len(lens), **options)
+    got, want = _gradients(inputs, BF16, learned=learned, cu=None if lens is None else _cu(lens))
+    for name, x in got.items():
+        _check("d" + name, x, want[name], {"initial_state": STATE, "g": 1e-5}.get(name, OUT))
