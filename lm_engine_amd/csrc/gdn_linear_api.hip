@@ -78,12 +78,8 @@ Cut cut_sequences(const gdn_linear_attn_args& a, int64_t slices, int64_t wanted,
     return c;
 }
 
-int walk_columns(const gdn_linear_attn_args& a, int K, int V) {
-    return a.dtype == GDN_BF16 ? linear_walk_columns(K, V) : 32;
-}
-
 Cut cut_segments(const gdn_linear_attn_args& a) {
-    const int width = walk_columns(a, a.K, a.V), cus = compute_units();
+    const int width = a.dtype == GDN_BF16 ? WALK_COLUMNS : 32, cus = compute_units();
     const int64_t slices = (a.V + width - 1) / width;
     if (a.dtype == GDN_BF16) return cut_sequences(a, slices, a.K <= 128 ? 2 * cus : cus, 128);
     return cut_sequences(a, slices, 4 * cus, 64);
@@ -113,8 +109,7 @@ Cut cut_forward(const gdn_linear_attn_args& a) {
 // cells of a state between the launches: bf16 in the order of the walk's registers (whole workgroups), fp32 as it is
 int64_t local_cells(int dtype, int K, int V) {
     if (dtype != GDN_BF16) return (int64_t)K * V;
-    const int columns = linear_walk_columns(K, V);
-    return (int64_t)linear_walk_keys(K) * ((V + columns - 1) / columns * columns);
+    return (int64_t)linear_walk_keys(K) * ((V + WALK_COLUMNS - 1) / WALK_COLUMNS * WALK_COLUMNS);
 }
 
 uint64_t states_bytes(const gdn_linear_attn_args& a, const Cut& c, int64_t cells) {

@@ -10,6 +10,7 @@
 // chain from one token to the next: 0.36 us a token in the smallest calls, 4 x 1024 tokens of 16 heads of 128 in fp32 299 us (280 with a
 // token's factor as one number).
 #include <algorithm>
+#include <type_traits>
 
 #include "gdn_launch.h"
 #include "gdn_linear_common.h"
@@ -156,10 +157,17 @@ int launch(const LinearParams& p, bool states_only, hipStream_t stream) {
     const int64_t blocks = (int64_t)p.slots * p.H * ((p.V + 4 * VL - 1) / (4 * VL));
     if (blocks > 0xfffff000ll / 256) return GDN_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)((blocks + 7) / 8 * 8)), threads(256);
-    if (states_only) hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 16, true>), grid, threads, 0, stream, p);
+    if constexpr (std::is_same_v<T, float> && VL == 8) {
+        if (states_only) {
+            hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 16, true>), grid, threads, 0, stream, p);
+            return (int)hipGetLastError();
+        }
+    } else if (states_only) {
+        return GDN_ERR_UNSUPPORTED;  // (bf16 segments are walked, fp32 ones in 32 columns)
+    }
     // room for one token where there is no second, so that more workgroups fit a unit: 64 states of 32 heads 49.5 us against 51.4, 32 24.5
     // against 25.5, 256 179 either way
-    else if (p.T == 1) hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 1, false>), grid, threads, 0, stream, p);
+    if (p.T == 1) hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 1, false>), grid, threads, 0, stream, p);
     else hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 16, false>), grid, threads, 0, stream, p);
     return (int)hipGetLastError();
 }

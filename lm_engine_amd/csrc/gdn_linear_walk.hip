@@ -34,6 +34,10 @@ __device__ __forceinline__ void reads_ahead() {
     }
 }
 
+// Where the value dim has 64 columns or fewer two of the four waves have none, and two waves to a workgroup take as long: 4 x 4096 tokens
+// of 16 heads of 64, the backward 157 us against 156.
+constexpr int WALK_WAVES = WALK_COLUMNS / 32;
+
 // What a walk is for, and in how many bf16 parts the decayed rows of z go into the state (the rows of y are exact).  Three hold all 24
 // bits of an fp32 product: where the state is a result.  Two, 16 bits and more, where it only goes on into outputs, which round it to
 // 8 as an operand: with one the state would carry as much error as that rounding adds.
@@ -45,9 +49,9 @@ enum class Walk {
     exact_states,   // ... three parts
 };
 
-template <int KD, int NW, Walk MODE>
-__global__ __launch_bounds__(64 * NW, KD <= 128 ? 2 : 1) void linear_walk_kernel(const LinearParams p) {
-    constexpr int NT = 64 * NW, VC = 32 * NW, KT = KD / 32;
+template <int KD, Walk MODE>
+__global__ __launch_bounds__(64 * WALK_WAVES, KD <= 128 ? 2 : 1) void linear_walk_kernel(const LinearParams p) {
+    constexpr int NW = WALK_WAVES, NT = 64 * NW, VC = WALK_COLUMNS, KT = KD / 32;
     constexpr bool STATES_ONLY = MODE == Walk::states || MODE == Walk::exact_states, SUMS = MODE == Walk::sums;
     constexpr int PARTS = MODE == Walk::outputs_state || MODE == Walk::exact_states ? 3 : 2;
     __shared__ __align__(16) bf16_t sx[STATES_ONLY ? 8 : LC * KD];
@@ -360,30 +364,27 @@ __global__ __launch_bounds__(256) void linear_combine_kernel(const LinearParams 
     }
 }
 
-template <int KD, int NW>
+template <int KD>
 int launch(const LinearParams& p, bool states_only, hipStream_t stream) {
-    const int64_t blocks = (int64_t)p.slots * p.H * ((p.V + 32 * NW - 1) / (32 * NW));
-    if (blocks > 0xfffff000ll / (64 * NW)) return GDN_ERR_UNSUPPORTED;  // (a launch holds at most 2^32 - 1 threads)
-    const dim3 grid((unsigned)((blocks + 7) / 8 * 8)), threads(64 * NW);
-    if (states_only && p.fin != nullptr) hipLaunchKernelGGL((linear_walk_kernel<KD, NW, Walk::exact_states>), grid, threads, 0, stream, p);
-    else if (states_only) hipLaunchKernelGGL((linear_walk_kernel<KD, NW, Walk::states>), grid, threads, 0, stream, p);
-    else if (p.sums != nullptr) hipLaunchKernelGGL((linear_walk_kernel<KD, NW, Walk::sums>), grid, threads, 0, stream, p);
-    else if (p.fin != nullptr) hipLaunchKernelGGL((linear_walk_kernel<KD, NW, Walk::outputs_state>), grid, threads, 0, stream, p);
-    else hipLaunchKernelGGL((linear_walk_kernel<KD, NW, Walk::outputs>), grid, threads, 0, stream, p);
+    const int64_t blocks = (int64_t)p.slots * p.H * ((p.V + WALK_COLUMNS - 1) / WALK_COLUMNS);
+    if (blocks > 0xfffff000ll / (64 * WALK_WAVES)) return GDN_ERR_UNSUPPORTED;  // (a launch holds at most 2^32 - 1 threads)
+    const dim3 grid((unsigned)((blocks + 7) / 8 * 8)), threads(64 * WALK_WAVES);
+    if (states_only && p.fin != nullptr) hipLaunchKernelGGL((linear_walk_kernel<KD, Walk::exact_states>), grid, threads, 0, stream, p);
+    else if (states_only) hipLaunchKernelGGL((linear_walk_kernel<KD, Walk::states>), grid, threads, 0, stream, p);
+    else if (p.sums != nullptr) hipLaunchKernelGGL((linear_walk_kernel<KD, Walk::sums>), grid, threads, 0, stream, p);
+    else if (p.fin != nullptr) hipLaunchKernelGGL((linear_walk_kernel<KD, Walk::outputs_state>), grid, threads, 0, stream, p);
+    else hipLaunchKernelGGL((linear_walk_kernel<KD, Walk::outputs>), grid, threads, 0, stream, p);
     return (int)hipGetLastError();
 }
 
 }  // namespace
 
-// (where the value dim has 64 columns or fewer two of the four waves have none, and two waves to a workgroup take as long: 4 x 4096 tokens
-// of 16 heads of 64, the backward 157 us against 156)
 int linear_walk_keys(int K) { return K <= 64 ? 64 : K <= 128 ? 128 : 256; }
-int linear_walk_columns(int, int) { return 128; }
 
 int launch_linear_walk(const LinearParams& p, bool states_only, hipStream_t stream) {
-    if (p.K <= 64) return launch<64, 4>(p, states_only, stream);
-    if (p.K <= 128) return launch<128, 4>(p, states_only, stream);
-    return launch<256, 4>(p, states_only, stream);
+    if (p.K <= 64) return launch<64>(p, states_only, stream);
+    if (p.K <= 128) return launch<128>(p, states_only, stream);
+    return launch<256>(p, states_only, stream);
 }
 
 int launch_linear_combine(const LinearParams& p, hipStream_t stream) {
