@@ -5,7 +5,10 @@
 // left of it, in fp32.  The backward forms mean and r again from the row that it reads anyway, so the forward keeps nothing.
 // Workgroups walk the rows, the next one on its way where there are registers for it; weight, bias and the backward's sums of dw and db
 // stay in registers, and every workgroup leaves one partial row of each, added up in a fixed order.
-// Bound by memory: 16384 rows of 2048, bf16: forward 29 us (25 the shortest), 134 MB at 4.7 TB/s; backward 42 us, 201 MB at 4.8.  Two
+// Bound by memory: 16384 rows of 2048, bf16: forward 25 to 29 us, 134 MB at 4.7 to 5.3 TB/s; backward 42 us, 201 MB at 4.8, and 4 for the
+// sums over the partial rows.  Rows that 16-byte pieces do not fit are read in single elements: 16384 of 2049 57 us, forward and backward 154 (71
+// at 2048), of 777 17 and 46 (776: 15 and 43), of 2048 at an odd address 27 and 271.  Above 8192 the backward of 1024 threads, 128 registers
+// each, spills 39 to 51 of them: 2048 rows of 16384 189 us, forward and backward, where 4096 of 8192 take 93.  Two
 // workgroups to a compute unit: with eight, and every thread reading its parameters for two rows, the forward took 51 us; a prefetch
 // takes the backward past 256 registers, and to 72 us.
 #include <algorithm>

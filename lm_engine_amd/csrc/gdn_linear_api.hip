@@ -54,7 +54,7 @@ struct Cut {
     bool several;  // a sequence may have more than one segment: their states come first
 };
 
-// Workgroups that a launch should have: the walk runs two to a compute unit (one where the keys number more than 128).
+// Workgroups that a launch should have (`wanted`), and the shortest segment that is worth another one.
 Cut cut_sequences(const gdn_linear_attn_args& a, int64_t slices, int64_t wanted, int shortest) {
     const bool packed = a.cu_seqlens != nullptr && !(a.flags & GDN_FLAG_LEFT_PADDED);
     const int64_t tokens = (int64_t)a.B * a.T, work = a.H * slices;
@@ -78,6 +78,12 @@ Cut cut_sequences(const gdn_linear_attn_args& a, int64_t slices, int64_t wanted,
     return c;
 }
 
+// The walk runs two workgroups to a compute unit (one where the keys number more than 128), and as many are wanted: half as many or twice as
+// many, forward and backward, 4 x 4096 tokens of 16 heads of 128 371 | 349 | 414 us, 6 x 1500 of 16 / 8 heads of 64 186 | 156 | 173; forward, 32768
+// of 16 heads of 128 235 | 201 | 230, 65536 of 32 heads of 128 x 256 1548 | 1309 | 1317; 4 x 4096 of 2 heads of 256 x 512 1005 | 585 | 512 (which
+// twice as many would suit).  No segment under 128 tokens: 777 tokens of 2 heads of 256 x 512 38 us, with 64 41, with 256 51.
+// fp32 walks of 256 threads, four to a unit, no segment under 64 tokens: forward and backward, half | as it is | twice as many, 4 x 1024 tokens of
+// 16 heads of 128 1308 | 1093 | 1079 us, 1 x 2048 681 | 592 | 605; 256 tokens of 2 heads of 64 135 us, with segments of 128 231.
 Cut cut_segments(const gdn_linear_attn_args& a) {
     const int width = a.dtype == GDN_BF16 ? WALK_COLUMNS : 32, cus = compute_units();
     const int64_t slices = (a.V + width - 1) / width;

@@ -12,10 +12,12 @@
 // ahead; the P waves bring in x and z (and its decayed rows, in two or three bf16 parts), the S waves y.  The O waves load nothing: the
 // compiler's wait for rows would be one for their stores.
 //
-// Measured at 4 sequences of 4096 tokens, 16 heads, K = V = 128, which is one workgroup to a compute unit: 80 us, with a final state
-// 88, 1.25 us a chunk, of which some 0.9 us are the S waves' own work (an operand read, products one behind the other, a write) and
-// the rest the barrier and the other groups; 268 MB in and out are 51 us at a large copy's rate.  With the tiles of P on the diagonal
-// formed by the O waves, 83; with 64 columns to a workgroup registers spill.
+// Measured at 4 sequences of 4096 tokens, 16 heads, K = V = 128, which is one workgroup to a compute unit: 77 us, with a final state
+// 80 to 91 (two registers spilled), 1.25 us a chunk, of which some 0.9 us are the S waves' own work and the rest the barrier and the other
+// groups.  Their eight or twelve products are no more than 0.11 to 0.16 us of that (32 cycles of the matrix unit each); what takes the time is
+// that one thing waits for the other: operand reads that begin behind the barrier, the products, the state's rounding and its way to LDS.
+// 268 MB in and out are 51 us at a large copy's rate.  With the tiles of P on the diagonal formed by the O waves, 83; with 64 columns to a
+// workgroup registers spill.
 #include <algorithm>
 
 #include "gdn_launch.h"

@@ -9,8 +9,11 @@
 // bf16: on the matrix units, decayed rows in three bf16 parts (as the walk's states), S and U only ever as fp32: dg is good to fp32 sums
 // of such terms, 1e-5.  A workgroup leaves one number per segment, head and columns; the sums over them are one more launch, in order.
 // No prefetch here: where the keys number 64 at most two workgroups to a compute unit cover each other's loads.  Bound by latency and
-// LDS: 6 left-padded rows of 1500 tokens, 16 heads of 64: the states and their derivatives 27 us, their sums 6, the dots 42, dg 5.
-// With 128 keys S, U and the fragments fill all registers of a wave (4 x 4096 tokens, 16 heads of 128: 250 us of the backward's 500).
+// LDS: 6 left-padded rows of 1500 tokens, 16 heads of 64: the states and their derivatives 27 us, their sums 7, the dots 40, dg 5.
+// S and U of all keys are one wave's: with 128 keys they and the fragments fill all its registers (4 x 4096 tokens, 16 heads of 128: 242 us of
+// 596, forward and backward).  With 256 keys they do not fit, and the kernels live in scratch: the dots spill some 850 registers, the states
+// some 100 (2 heads of 256 x 512: 557 us of 1141).  With 64 keys and four waves, which two workgroups to a unit hold to 256 registers, the
+// dots spill some 95.
 #include <algorithm>
 #include <cfloat>
 
@@ -349,6 +352,8 @@ void run_one(const LinearParams& p, int dtype, bool states_only, unsigned blocks
         if (p.K <= 128) return launch_tokens<4>(p, states_only, blocks, stream);
         return launch_tokens<8>(p, states_only, blocks, stream);
     }
+    // Two waves have all columns of a value dim up to 64, and twice the workgroups fit: 4 x 4096 tokens, heads of 64 x 64 (16) 281 us, forward and
+    // backward, with four waves 339, of 128 x 64 402 | 490, of 256 x 64 (8) 859 | 907, of 64 x 32 269 | 332.
     const bool narrow = p.V <= 64;
     if (p.K <= 64) return narrow ? launch<64, 2>(p, states_only, blocks, stream) : launch<64, 4>(p, states_only, blocks, stream);
     if (p.K <= 128) return narrow ? launch<128, 2>(p, states_only, blocks, stream) : launch<128, 4>(p, states_only, blocks, stream);

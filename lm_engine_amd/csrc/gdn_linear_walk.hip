@@ -11,8 +11,9 @@
 //
 // 32 columns to a wave, so that a fragment of x or y feeds as many columns as a product takes, and the four waves of 128 columns share the
 // rows of x and y: 16 columns to a wave read LDS twice as often and were slower.  Bound by memory and LDS together: 32768 packed tokens,
-// 16 heads of 128: the states' pass 98 us (268 MB of rows, 2.7 TB/s, its three-part products beside them; 83 with two parts), their
-// sums 18, the walk 176 (536 MB of rows, 3.0 TB/s); without states to form, 4 x 4096 tokens backward: 35, 12, 67 us.
+// 16 heads of 128, 11 sequences: the states' pass 94 us (268 MB of rows, 2.9 TB/s, its three-part products beside them; with two parts the
+// forward of one sequence takes 190 us instead of 202), their sums 18, the walk 168 (536 MB of rows, 3.2 TB/s); in the backward of 4 x 4096
+// tokens 31 (two parts), 11 and 62 us.
 #include <algorithm>
 
 #include "gdn_launch.h"
@@ -159,6 +160,8 @@ __global__ __launch_bounds__(64 * WALK_WAVES, KD <= 128 ? 2 : 1) void linear_wal
         for (int i = 0; i < 2; i++) row_weight[i] = p.os * linear_power(g, 32 * i + l32 + a);
     }
     if (tid < LC) sw[tid] = p.us * linear_power(g, LC - a - tid);
+    // A chunk's factor is one number: its rounding, up to 2^-25, comes back with every chunk of the segment, 1e-6 of the state after 32.  (In two
+    // parts, as a segment's: 1 x 65536 tokens 1347 us instead of 1285, the decay's gradient a third longer.)
     const float whole = linear_power(g, LC);
     TileLane<KD> tile(lane);
     TileLane<VC> ztile(lane);
