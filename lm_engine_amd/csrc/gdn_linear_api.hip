@@ -152,7 +152,8 @@ void natural(LinearParams& p, int K, int V) { p.K = K, p.V = V, p.state_k = V, p
 
 int run(const LinearParams& p, int dtype, bool states_only, hipStream_t stream) {
     if (p.chain) return launch_linear_chain(p, stream);
-    return dtype == GDN_BF16 ? launch_linear_walk(p, states_only, stream) : launch_linear_tokens(p, dtype, 32, states_only, stream);
+    if (dtype == GDN_BF16) return launch_linear_walk(p, states_only, stream);
+    return states_only ? launch_linear_token_states(p, stream) : launch_linear_tokens(p, dtype, 32, stream);
 }
 
 // the states that the segments start from, into p.local: their own, then the sums, and p.fin
@@ -276,7 +277,7 @@ extern "C" int gdn_linear_attn_recurrent_fwd(const gdn_linear_attn_args* args, v
     p.out = a.o, p.out_stride_b = a.o_stride_b, p.out_stride_t = a.o_stride_t, p.out_stride_h = a.o_stride_h;
     p.init = a.h0, p.fin = a.ht;
     p.reverse = 0, p.a = 1, p.os = p.ps = a.scale, p.us = 1.f;
-    return launch_linear_tokens(p, a.dtype, linear_tokens_columns((int64_t)a.N * a.H, a.V, compute_units()), false, static_cast<hipStream_t>(stream));
+    return launch_linear_tokens(p, a.dtype, linear_tokens_columns((int64_t)a.N * a.H, a.V, compute_units()), static_cast<hipStream_t>(stream));
 }
 
 extern "C" uint64_t gdn_linear_attn_bwd_workspace_bytes(const gdn_linear_attn_bwd_args* b) {

@@ -194,7 +194,7 @@ __device__ __forceinline__ int64_t linear_fragment(int keys, int key, int v) {
     return ((((int64_t)(v >> 5) * (keys >> 5) + (key >> 5)) * 4 + (r >> 2)) * 64 + lane) * 4 + (r & 3);
 }
 
-// launches, gdn_linear_walk.hip and gdn_linear_tokens.hip; `states_only` (the latter: fp32 in 32 columns): the segments' own states into p.local
+// launches, gdn_linear_walk.hip and gdn_linear_tokens.hip; `states_only`, token_states (fp32): the segments' own states into p.local
 int launch_linear_walk(const LinearParams& p, bool states_only, hipStream_t stream);
 // gdn_linear_tokens.hip: fp32 [B, T, heads group, D], each group's rows added up, to rows of dtype
 struct LinearFold {
@@ -206,7 +206,8 @@ struct LinearFold {
 };
 int launch_linear_fold(const LinearFold& p, int dtype, hipStream_t stream);
 int launch_linear_chain(const LinearParams& p, hipStream_t stream);  // gdn_linear_chain.hip: forward, bf16, up to 128 keys, whole sequences
-int launch_linear_tokens(const LinearParams& p, int dtype, int columns, bool states_only, hipStream_t stream);
+int launch_linear_tokens(const LinearParams& p, int dtype, int columns, hipStream_t stream);
+int launch_linear_token_states(const LinearParams& p, hipStream_t stream);
 int linear_walk_keys(int K);            // keys that the bf16 walk is built for
 constexpr int WALK_COLUMNS = 128;       // of the value dim that a workgroup of the bf16 walk has
 int linear_tokens_columns(int64_t chains, int V, int cus);  // of the token kernel

@@ -10,7 +10,6 @@
 // chain from one token to the next: 0.36 us a token in the smallest calls, 4 x 1024 tokens of 16 heads of 128 in fp32 299 us (280 with a
 // token's factor as one number).
 #include <algorithm>
-#include <type_traits>
 
 #include "gdn_launch.h"
 #include "gdn_linear_common.h"
@@ -152,36 +151,43 @@ __global__ __launch_bounds__(256) void linear_tokens_kernel(const LinearParams p
     }
 }
 
-template <typename T, int KR, int VL>
-int launch(const LinearParams& p, bool states_only, hipStream_t stream) {
+// blocks of 4 VL columns
+template <int VL>
+bool grid_of(const LinearParams& p, dim3& grid) {
     const int64_t blocks = (int64_t)p.slots * p.H * ((p.V + 4 * VL - 1) / (4 * VL));
-    if (blocks > 0xfffff000ll / 256) return GDN_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)((blocks + 7) / 8 * 8)), threads(256);
-    if constexpr (std::is_same_v<T, float> && VL == 8) {
-        if (states_only) {
-            hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 16, true>), grid, threads, 0, stream, p);
-            return (int)hipGetLastError();
-        }
-    } else if (states_only) {
-        return GDN_ERR_UNSUPPORTED;  // (bf16 segments are walked, fp32 ones in 32 columns)
-    }
+    grid = dim3((unsigned)((blocks + 7) / 8 * 8));
+    return blocks <= 0xfffff000ll / 256;  // (a launch holds at most 2^32 - 1 threads)
+}
+
+template <typename T, int KR, int VL>
+int launch(const LinearParams& p, hipStream_t stream) {
+    dim3 grid;
+    if (!grid_of<VL>(p, grid)) return GDN_ERR_UNSUPPORTED;
     // room for one token where there is no second, so that more workgroups fit a unit: 64 states of 32 heads 49.5 us against 51.4, 32 24.5
     // against 25.5, 256 179 either way
-    if (p.T == 1) hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 1, false>), grid, threads, 0, stream, p);
-    else hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 16, false>), grid, threads, 0, stream, p);
+    if (p.T == 1) hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 1, false>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((linear_tokens_kernel<T, KR, VL, 16, false>), grid, dim3(256), 0, stream, p);
     return (int)hipGetLastError();
 }
 
 template <typename T>
-int launch_of(const LinearParams& p, int columns, bool states_only, hipStream_t stream) {
+int launch_of(const LinearParams& p, int columns, hipStream_t stream) {
     if (columns == 32) {
-        if (p.K <= 64) return launch<T, 2, 8>(p, states_only, stream);
-        if (p.K <= 128) return launch<T, 4, 8>(p, states_only, stream);
-        return launch<T, 8, 8>(p, states_only, stream);
+        if (p.K <= 64) return launch<T, 2, 8>(p, stream);
+        if (p.K <= 128) return launch<T, 4, 8>(p, stream);
+        return launch<T, 8, 8>(p, stream);
     }
-    if (p.K <= 64) return launch<T, 8, 32>(p, states_only, stream);
-    if (p.K <= 128) return launch<T, 16, 32>(p, states_only, stream);
-    return launch<T, 32, 32>(p, states_only, stream);
+    if (p.K <= 64) return launch<T, 8, 32>(p, stream);
+    if (p.K <= 128) return launch<T, 16, 32>(p, stream);
+    return launch<T, 32, 32>(p, stream);
+}
+
+template <int KR>
+int launch_states(const LinearParams& p, hipStream_t stream) {
+    dim3 grid;
+    if (!grid_of<8>(p, grid)) return GDN_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((linear_tokens_kernel<float, KR, 8, 16, true>), grid, dim3(256), 0, stream, p);
+    return (int)hipGetLastError();
 }
 
 // Gradients of shared heads of q and k, added up and rounded once: a thread has 4 columns of one head.  Bound by memory: group fp32 rows
@@ -209,8 +215,13 @@ __global__ __launch_bounds__(256) void linear_fold_kernel(const LinearFold p) {
 // 128 columns to a workgroup where they make one to every unit (16 states of 32 heads 11.0 us, with 32 columns 14.1), else 32: more of them
 int linear_tokens_columns(int64_t chains, int V, int cus) { return V >= 128 && chains * ((V + 127) / 128) >= cus ? 128 : 32; }
 
-int launch_linear_tokens(const LinearParams& p, int dtype, int columns, bool states_only, hipStream_t stream) {
-    return dtype == GDN_BF16 ? launch_of<bf16_t>(p, columns, states_only, stream) : launch_of<float>(p, columns, states_only, stream);
+int launch_linear_tokens(const LinearParams& p, int dtype, int columns, hipStream_t stream) {
+    return dtype == GDN_BF16 ? launch_of<bf16_t>(p, columns, stream) : launch_of<float>(p, columns, stream);
+}
+
+int launch_linear_token_states(const LinearParams& p, hipStream_t stream) {
+    if (p.K <= 64) return launch_states<2>(p, stream);
+    return p.K <= 128 ? launch_states<4>(p, stream) : launch_states<8>(p, stream);
 }
 
 int launch_linear_fold(const LinearFold& p, int dtype, hipStream_t stream) {
