@@ -23,7 +23,9 @@ _BOUND = ("gdn_layer_step", "gdn_layer_step_tiles", "gdn_causal_conv1d_fwd", "gd
           "gdn_chunk_bwd_sweeps_workspace_bytes", "gdn_chunk_bwd_local", "gdn_causal_conv1d_bwd", "gdn_gates_bwd",
           "gdn_gated_rmsnorm_bwd", "gdn_column_sums", "gdn_fold_heads", "gdn_layer_front", "gdn_linear_attn_chunk_fwd",
           "gdn_linear_attn_workspace_bytes", "gdn_linear_attn_recurrent_fwd", "gdn_linear_attn_bwd", "gdn_linear_attn_bwd_workspace_bytes",
-          "gdn_layer_norm_fwd", "gdn_layer_norm_bwd", "gdn_layer_norm_partial_blocks")  # fmt: skip
+          "gdn_layer_norm_fwd", "gdn_layer_norm_bwd", "gdn_layer_norm_partial_blocks", "gdn_qk_norm_rotary_fwd", "gdn_qk_norm_rotary_bwd",
+          "gdn_qk_rotary_partial_blocks", "gdn_window_attn_fwd", "gdn_window_attn_workspace_bytes", "gdn_window_attn_bwd",
+          "gdn_window_attn_bwd_workspace_bytes", "gdn_cache_write", "gdn_cache_read", "gdn_cache_attn", "gdn_cache_attn_workspace_bytes")  # fmt: skip
 
 # device index -> hipStream_t of the calling thread's current stream (a torch build without GPU support has no such function,
 # nor a device tensor that would lead here)

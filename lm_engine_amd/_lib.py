@@ -83,6 +83,24 @@ LINEAR_SYMBOLS = (
     "gdn_layer_norm_partial_blocks",
 )
 
+# include/gdn_attention_hip.h
+GDN_ATTENTION_ABI_VERSION = 1
+GDN_QK_ROTARY_MAX_D = 512
+ATTENTION_SYMBOLS = (
+    "gdn_attention_abi_version",
+    "gdn_qk_norm_rotary_fwd",
+    "gdn_qk_norm_rotary_bwd",
+    "gdn_qk_rotary_partial_blocks",
+    "gdn_window_attn_fwd",
+    "gdn_window_attn_workspace_bytes",
+    "gdn_window_attn_bwd",
+    "gdn_window_attn_bwd_workspace_bytes",
+    "gdn_cache_write",
+    "gdn_cache_read",
+    "gdn_cache_attn",
+    "gdn_cache_attn_workspace_bytes",
+)
+
 GDN_CHUNK_KERNELS = 3
 CHUNK_KERNEL_NAMES = ("chunk_offsets", "chunk_prepare", "chunk_scan")
 
@@ -274,6 +292,98 @@ class GdnLayerNormBwdArgs(ctypes.Structure):
     )
 
 
+class GdnQkRotaryArgs(ctypes.Structure):
+    """Mirror of ``struct gdn_qk_rotary_args`` (include/gdn_attention_hip.h)."""
+
+    _fields_ = (
+        [(name, ctypes.c_void_p * 2) for name in ("x", "weight", "y")]
+        + [(name, ctypes.c_void_p) for name in ("cos", "sin", "pos")]
+        + [("pos_stride_b", ctypes.c_int64)]
+        + [(f"x_stride_{d}", ctypes.c_int64 * 2) for d in ("b", "t", "h")]
+        + [("heads", ctypes.c_int32 * 2)]
+        + [(name, ctypes.c_int32) for name in ("B", "T", "D", "R", "table_rows", "dtype", "w_dtype")]
+        + [("eps", ctypes.c_float)]
+    )
+
+
+class GdnQkRotaryBwdArgs(ctypes.Structure):
+    """Mirror of ``struct gdn_qk_rotary_bwd_args``."""
+
+    _fields_ = (
+        [("fwd", GdnQkRotaryArgs)]
+        + [(name, ctypes.c_void_p * 2) for name in ("dy", "dx", "dweight_partial")]
+        + [(f"dy_stride_{d}", ctypes.c_int64 * 2) for d in ("b", "t", "h")]
+        + [(name, ctypes.c_int32) for name in ("partial_blocks", "reserved")]
+    )
+
+
+class GdnWindowAttnArgs(ctypes.Structure):
+    """Mirror of ``struct gdn_window_attn_args``."""
+
+    _fields_ = (
+        [(name, ctypes.c_void_p) for name in ("q", "k", "v", "o", "lse", "cu_seqlens", "workspace")]
+        + [("workspace_bytes", ctypes.c_uint64)]
+        + [(f"{t}_stride_{d}", ctypes.c_int64) for t in ("q", "k", "v", "o") for d in ("b", "t", "h")]
+        + [(name, ctypes.c_int32) for name in ("B", "T", "S", "H", "HK", "D", "N", "window", "sinks", "dtype", "flags")]
+        + [("scale", ctypes.c_float)]
+    )
+
+
+class GdnWindowAttnBwdArgs(ctypes.Structure):
+    """Mirror of ``struct gdn_window_attn_bwd_args``."""
+
+    _fields_ = (
+        [("fwd", GdnWindowAttnArgs)]
+        + [(name, ctypes.c_void_p) for name in ("dout", "dq", "dk", "dv", "workspace")]
+        + [("workspace_bytes", ctypes.c_uint64)]
+        + [(f"{t}_stride_{d}", ctypes.c_int64) for t in ("dout", "dq", "dk", "dv") for d in ("b", "t", "h")]
+    )
+
+
+class GdnPagedCache(ctypes.Structure):
+    """Mirror of ``struct gdn_paged_cache``."""
+
+    _fields_ = (
+        [(name, ctypes.c_void_p) for name in ("k_codes", "v_codes", "k_scales", "v_scales", "table")]
+        + [("table_stride", ctypes.c_int64)]
+        + [(name, ctypes.c_int32) for name in ("pages", "P", "HK", "D", "N", "table_pages")]
+    )
+
+
+class GdnCacheWriteArgs(ctypes.Structure):
+    """Mirror of ``struct gdn_cache_write_args``."""
+
+    _fields_ = (
+        [("cache", GdnPagedCache)]
+        + [(name, ctypes.c_void_p) for name in ("k", "v", "start", "cu_seqlens")]
+        + [(f"{t}_stride_{d}", ctypes.c_int64) for t in ("k", "v") for d in ("b", "t", "h")]
+        + [(name, ctypes.c_int32) for name in ("B", "T", "dtype", "flags")]
+    )
+
+
+class GdnCacheReadArgs(ctypes.Structure):
+    """Mirror of ``struct gdn_cache_read_args``."""
+
+    _fields_ = (
+        [("cache", GdnPagedCache)]
+        + [(name, ctypes.c_void_p) for name in ("k", "v", "lengths")]
+        + [(name, ctypes.c_int32) for name in ("T", "dtype")]
+    )
+
+
+class GdnCacheAttnArgs(ctypes.Structure):
+    """Mirror of ``struct gdn_cache_attn_args``."""
+
+    _fields_ = (
+        [("cache", GdnPagedCache)]
+        + [(name, ctypes.c_void_p) for name in ("q", "o", "lengths", "workspace")]
+        + [("workspace_bytes", ctypes.c_uint64)]
+        + [(f"{t}_stride_{d}", ctypes.c_int64) for t in ("q", "o") for d in ("b", "t", "h")]
+        + [(name, ctypes.c_int32) for name in ("T", "H", "window", "sinks")]
+        + [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
+    )
+
+
 class GdnLibraryError(RuntimeError):
     pass
 
@@ -292,7 +402,7 @@ def load_library() -> ctypes.CDLL:
             "(run `python -m lm_engine_amd.build`); there is no fallback path."
         )
     lib = ctypes.CDLL(LIBRARY_PATH)
-    for symbol in EXPORTED_SYMBOLS + LINEAR_SYMBOLS:
+    for symbol in EXPORTED_SYMBOLS + LINEAR_SYMBOLS + ATTENTION_SYMBOLS:
         if not hasattr(lib, symbol):
             raise GdnLibraryError(f"{LIBRARY_PATH} does not export {symbol}")
 
@@ -375,6 +485,22 @@ def load_library() -> ctypes.CDLL:
     lib.gdn_layer_norm_partial_blocks.restype = ctypes.c_int
     if lib.gdn_linear_abi_version() != GDN_LINEAR_ABI_VERSION:
         raise GdnLibraryError(f"libgdn_hip.so: version {lib.gdn_linear_abi_version()} of its second part, this binding expects {GDN_LINEAR_ABI_VERSION}")
+
+    lib.gdn_attention_abi_version.argtypes = []
+    lib.gdn_attention_abi_version.restype = ctypes.c_int
+    for name, args in (("gdn_qk_norm_rotary_fwd", GdnQkRotaryArgs), ("gdn_qk_norm_rotary_bwd", GdnQkRotaryBwdArgs), ("gdn_window_attn_fwd", GdnWindowAttnArgs),
+                       ("gdn_window_attn_bwd", GdnWindowAttnBwdArgs), ("gdn_cache_write", GdnCacheWriteArgs), ("gdn_cache_read", GdnCacheReadArgs),
+                       ("gdn_cache_attn", GdnCacheAttnArgs)):  # fmt: skip
+        getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+        getattr(lib, name).restype = ctypes.c_int
+    for name, args in (("gdn_window_attn_workspace_bytes", GdnWindowAttnArgs), ("gdn_window_attn_bwd_workspace_bytes", GdnWindowAttnBwdArgs),
+                       ("gdn_cache_attn_workspace_bytes", GdnCacheAttnArgs)):  # fmt: skip
+        getattr(lib, name).argtypes = [ctypes.POINTER(args)]
+        getattr(lib, name).restype = ctypes.c_uint64
+    lib.gdn_qk_rotary_partial_blocks.argtypes = [ctypes.POINTER(GdnQkRotaryArgs)]
+    lib.gdn_qk_rotary_partial_blocks.restype = ctypes.c_int
+    if lib.gdn_attention_abi_version() != GDN_ATTENTION_ABI_VERSION:
+        raise GdnLibraryError(f"libgdn_hip.so: version {lib.gdn_attention_abi_version()} of its third part, this binding expects {GDN_ATTENTION_ABI_VERSION}")
 
     version = lib.gdn_abi_version()
     if version != GDN_ABI_VERSION:

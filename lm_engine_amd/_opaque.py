@@ -425,6 +425,167 @@ layer_norm_forward.register_autograd(_layer_norm_backward, setup_context=_layer_
 
 
 # ---------------------------------------------------------------------------------------
+# norm and rotation of queries and keys
+# ---------------------------------------------------------------------------------------
+@torch.library.custom_op(
+    "lm_engine_amd::qk_norm_rotary_forward",
+    mutates_args=(),
+    schema="(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor cos, Tensor sin, Tensor? positions, float eps) -> (Tensor, Tensor)",
+)
+def qk_norm_rotary_forward(q, k, q_weight, k_weight, cos, sin, positions, eps):
+    from . import rotary
+
+    return tuple(rotary._forward(q, k, q_weight, k_weight, cos, sin, positions, eps))
+
+
+@qk_norm_rotary_forward.register_fake
+def _(q, k, q_weight, k_weight, cos, sin, positions, eps):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op(
+    "lm_engine_amd::qk_norm_rotary_backward",
+    mutates_args=(),
+    schema="(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor cos, Tensor sin, Tensor? positions, float eps, Tensor dq, Tensor dk) "
+    "-> (Tensor, Tensor, Tensor, Tensor)",
+)
+def qk_norm_rotary_backward(q, k, q_weight, k_weight, cos, sin, positions, eps, dq, dk):
+    from . import rotary
+
+    gq, gk, gwq, gwk = rotary._backward(q, k, q_weight, k_weight, cos, sin, positions, eps, dq, dk, q_weight is not None, k_weight is not None)
+    return gq, gk, _or_empty(gwq, q), _or_empty(gwk, k)
+
+
+@qk_norm_rotary_backward.register_fake
+def _(q, k, q_weight, k_weight, cos, sin, positions, eps, dq, dk):
+    like = lambda w: q.new_empty(0) if w is None else w.new_empty(w.shape)  # noqa: E731
+    return q.new_empty(q.shape), k.new_empty(k.shape), like(q_weight), like(k_weight)
+
+
+def _qk_norm_rotary_setup(ctx, inputs, output):
+    *tensors, eps = inputs
+    ctx.save_for_backward(*tensors)
+    ctx.eps = eps
+
+
+def _qk_norm_rotary_backward(ctx, dq, dk):
+    q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
+    gq, gk, gwq, gwk = torch.ops.lm_engine_amd.qk_norm_rotary_backward(
+        q, k, q_weight, k_weight, cos, sin, positions, ctx.eps, dq.contiguous(), dk.contiguous())  # fmt: skip
+    return gq, gk, None if q_weight is None else gwq, None if k_weight is None else gwk, None, None, None, None
+
+
+qk_norm_rotary_forward.register_autograd(_qk_norm_rotary_backward, setup_context=_qk_norm_rotary_setup)
+
+
+# ---------------------------------------------------------------------------------------
+# attention over a window
+# ---------------------------------------------------------------------------------------
+@torch.library.custom_op(
+    "lm_engine_amd::window_attention_forward",
+    mutates_args=(),
+    schema="(Tensor q, Tensor k, Tensor v, Tensor? cu_seqlens, int window, int sinks, float scale, bool left_padded) -> (Tensor, Tensor)",
+)
+def window_attention_forward(q, k, v, cu_seqlens, window, sinks, scale, left_padded):
+    from . import attention
+
+    return tuple(attention._forward(q, k, v, window, sinks, scale, cu_seqlens, left_padded, True))
+
+
+@window_attention_forward.register_fake
+def _(q, k, v, cu_seqlens, window, sinks, scale, left_padded):
+    return q.new_empty(q.shape), q.new_empty((*q.shape[:3], *(() if q.dtype == torch.bfloat16 else (2,))), dtype=torch.float32)
+
+
+@torch.library.custom_op(
+    "lm_engine_amd::window_attention_backward",
+    mutates_args=(),
+    schema="(Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor? cu_seqlens, Tensor d_o, int window, int sinks, float scale, bool left_padded) "
+    "-> (Tensor, Tensor, Tensor)",
+)
+def window_attention_backward(q, k, v, o, lse, cu_seqlens, d_o, window, sinks, scale, left_padded):
+    from . import attention
+
+    return tuple(attention._backward(q, k, v, o, lse, window, sinks, scale, cu_seqlens, left_padded, d_o))
+
+
+@window_attention_backward.register_fake
+def _(q, k, v, o, lse, cu_seqlens, d_o, window, sinks, scale, left_padded):
+    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+
+
+def _window_attention_setup(ctx, inputs, output):
+    q, k, v, cu_seqlens, *options = inputs
+    ctx.save_for_backward(q, k, v, *output, cu_seqlens)
+    ctx.options = options
+    ctx.mark_non_differentiable(output[1])
+
+
+def _window_attention_backward(ctx, d_o, d_lse):
+    q, k, v, o, lse, cu_seqlens = ctx.saved_tensors
+    grads = torch.ops.lm_engine_amd.window_attention_backward(q, k, v, o, lse, cu_seqlens, d_o.contiguous(), *ctx.options)
+    return (*grads, None, None, None, None, None)
+
+
+window_attention_forward.register_autograd(_window_attention_backward, setup_context=_window_attention_setup)
+
+
+# ---------------------------------------------------------------------------------------
+# the paged cache
+# ---------------------------------------------------------------------------------------
+@torch.library.custom_op(
+    "lm_engine_amd::paged_cache_write_",
+    mutates_args=("k_codes", "v_codes", "k_scales", "v_scales"),
+    schema="(Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) k_scales, Tensor(d!) v_scales, Tensor k, Tensor v, Tensor block_table, "
+    "Tensor start, Tensor? cu_seqlens, bool left_padded) -> ()",
+)
+def paged_cache_write_(k_codes, v_codes, k_scales, v_scales, k, v, block_table, start, cu_seqlens, left_padded):
+    from . import cache
+
+    cache._write(cache.PagedCache(k_codes, v_codes, k_scales, v_scales), k, v, block_table, start, cu_seqlens, left_padded)
+
+
+@paged_cache_write_.register_fake
+def _(k_codes, v_codes, k_scales, v_scales, k, v, block_table, start, cu_seqlens, left_padded):
+    return None
+
+
+@torch.library.custom_op(
+    "lm_engine_amd::paged_cache_read",
+    mutates_args=(),
+    schema="(Tensor k_codes, Tensor v_codes, Tensor k_scales, Tensor v_scales, Tensor block_table, Tensor lengths, int max_tokens, ScalarType dtype) "
+    "-> (Tensor, Tensor)",
+)
+def paged_cache_read(k_codes, v_codes, k_scales, v_scales, block_table, lengths, max_tokens, dtype):
+    from . import cache
+
+    return tuple(cache._read(cache.PagedCache(k_codes, v_codes, k_scales, v_scales), block_table, lengths, max_tokens, dtype))
+
+
+@paged_cache_read.register_fake
+def _(k_codes, v_codes, k_scales, v_scales, block_table, lengths, max_tokens, dtype):
+    shape = (block_table.size(0), max_tokens, k_codes.size(1), k_codes.size(3))
+    return k_codes.new_empty(shape, dtype=dtype), k_codes.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op(
+    "lm_engine_amd::paged_cache_attend",
+    mutates_args=(),
+    schema="(Tensor q, Tensor k_codes, Tensor v_codes, Tensor k_scales, Tensor v_scales, Tensor block_table, Tensor lengths, int window, int sinks, "
+    "float scale) -> Tensor",
+)
+def paged_cache_attend(q, k_codes, v_codes, k_scales, v_scales, block_table, lengths, window, sinks, scale):
+    from . import cache
+
+    return cache._attend(q, cache.PagedCache(k_codes, v_codes, k_scales, v_scales), block_table, lengths, window, sinks, scale)
+
+
+@paged_cache_attend.register_fake
+def _(q, k_codes, v_codes, k_scales, v_scales, block_table, lengths, window, sinks, scale):
+    return q.new_empty(q.shape)
+
+
+# ---------------------------------------------------------------------------------------
 # what the eager entry points call while a graph is being captured
 # ---------------------------------------------------------------------------------------
 def gated_delta_rule(mode, q, k, v, g, beta, scale, initial_state, output_final_state, cu_seqlens, l2norm, inplace_state,
@@ -475,3 +636,24 @@ def linear_attention(mode, q, k, v, g, scale, initial_state, output_final_state,
 
 def layer_norm(x, weight, bias, eps):
     return torch.ops.lm_engine_amd.layer_norm_forward(x, weight, bias, eps)
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, eps):
+    return torch.ops.lm_engine_amd.qk_norm_rotary_forward(q, k, q_weight, k_weight, cos, sin, positions, eps)
+
+
+def sliding_window_attention(q, k, v, window, sinks, scale, cu_seqlens, left_padded):
+    return torch.ops.lm_engine_amd.window_attention_forward(q, k, v, cu_seqlens, window, sinks, scale, left_padded)[0]
+
+
+def write_paged_cache(cache, k, v, block_table, start, cu_seqlens, left_padded):
+    torch.ops.lm_engine_amd.paged_cache_write_(*cache, k, v, block_table, start, cu_seqlens, left_padded)
+    return cache
+
+
+def read_paged_cache(cache, block_table, lengths, max_tokens, dtype):
+    return torch.ops.lm_engine_amd.paged_cache_read(*cache, block_table, lengths, max_tokens, dtype)
+
+
+def paged_cache_attention(q, cache, block_table, lengths, window, sinks, scale):
+    return torch.ops.lm_engine_amd.paged_cache_attend(q, *cache, block_table, lengths, window, sinks, scale)

@@ -1,5 +1,5 @@
 // The host path of the entry points and of their backward passes: from torch tensors to the calls of the C ABI (include/gdn_hip.h,
-// include/gdn_linear_hip.h).
+// include/gdn_linear_hip.h, include/gdn_attention_hip.h).
 //
 // On a decode step, a short prompt or a short training sequence the GPU needs a few microseconds per kernel, and reading shapes,
 // strides and pointers out of tensors, allocating the results and filling the argument structs takes 10 to 60 in Python per call.
@@ -18,9 +18,11 @@
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
+#include <vector>
 
 #include "gdn_hip.h"
 #include "gdn_linear_hip.h"
+#include "gdn_attention_hip.h"
 
 namespace {
 
@@ -50,6 +52,17 @@ decltype(&gdn_linear_attn_bwd_workspace_bytes) linear_bwd_workspace_fn = nullptr
 decltype(&gdn_layer_norm_fwd) layer_norm_fn = nullptr;
 decltype(&gdn_layer_norm_bwd) layer_norm_bwd_fn = nullptr;
 decltype(&gdn_layer_norm_partial_blocks) layer_norm_blocks_fn = nullptr;
+decltype(&gdn_qk_norm_rotary_fwd) rotary_fn = nullptr;
+decltype(&gdn_qk_norm_rotary_bwd) rotary_bwd_fn = nullptr;
+decltype(&gdn_qk_rotary_partial_blocks) rotary_blocks_fn = nullptr;
+decltype(&gdn_window_attn_fwd) window_fn = nullptr;
+decltype(&gdn_window_attn_workspace_bytes) window_workspace_fn = nullptr;
+decltype(&gdn_window_attn_bwd) window_bwd_fn = nullptr;
+decltype(&gdn_window_attn_bwd_workspace_bytes) window_bwd_workspace_fn = nullptr;
+decltype(&gdn_cache_write) cache_write_fn = nullptr;
+decltype(&gdn_cache_read) cache_read_fn = nullptr;
+decltype(&gdn_cache_attn) cache_attn_fn = nullptr;
+decltype(&gdn_cache_attn_workspace_bytes) cache_attn_workspace_fn = nullptr;
 PyObject* check_status = nullptr;  // _lib.check_status: raises what a status stands for
 
 // bind(check_status, addresses...)
@@ -60,7 +73,9 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
                       (void**)&norm_bwd_fn, (void**)&column_sums_fn, (void**)&fold_heads_fn, (void**)&layer_front_fn,
                       (void**)&linear_chunk_fn, (void**)&linear_workspace_fn, (void**)&linear_recurrent_fn, (void**)&linear_bwd_fn,
                       (void**)&linear_bwd_workspace_fn, (void**)&layer_norm_fn, (void**)&layer_norm_bwd_fn,
-                      (void**)&layer_norm_blocks_fn};
+                      (void**)&layer_norm_blocks_fn, (void**)&rotary_fn, (void**)&rotary_bwd_fn, (void**)&rotary_blocks_fn, (void**)&window_fn,
+                      (void**)&window_workspace_fn, (void**)&window_bwd_fn, (void**)&window_bwd_workspace_fn, (void**)&cache_write_fn,
+                      (void**)&cache_read_fn, (void**)&cache_attn_fn, (void**)&cache_attn_workspace_fn};
     constexpr Py_ssize_t count = sizeof(slots) / sizeof(slots[0]);
     if (n != count + 1) return PyErr_Format(PyExc_TypeError, "bind takes a function and %zd addresses, got %zd arguments", count, n);
     for (Py_ssize_t i = 0; i < count; i++) {
@@ -909,6 +924,278 @@ PyObject* layer_norm_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// ---- norm and rotation of queries and keys, attention over a window, its paged cache
+
+// q, k, q_weight, k_weight, cos, sin, positions, eps
+struct RotaryOperands {
+    gdn_qk_rotary_args s{};
+    const at::Tensor* weight[2];
+
+    RotaryOperands(Operands& operand, PyObject* const* args) : weight{operand.optional(args[2]), operand.optional(args[3])} {
+        const at::Tensor* const x[2] = {&operand(args[0]), &operand(args[1])};
+        const at::Tensor &cos = operand(args[4]), &sin = operand(args[5]);
+        const at::Tensor* const positions = operand.optional(args[6]);
+        const int64_t B = x[0]->dim() == 4 ? x[0]->size(0) : 0, T = B > 0 ? x[0]->size(1) : 0, D = B > 0 ? x[0]->size(3) : 0;
+        need(B > 0 && T > 0 && D > 0);
+        s.dtype = code_of(*x[0]), s.w_dtype = GDN_F32;
+        for (int i = 0; i < 2; i++) {
+            need(x[i]->dim() == 4 && x[i]->size(0) == B && x[i]->size(1) == T && x[i]->size(3) == D && x[i]->stride(3) == 1 && x[i]->scalar_type() == x[0]->scalar_type());
+            s.x[i] = ptr(x[i]), s.heads[i] = size32(x[i]->size(2));
+            s.x_stride_b[i] = x[i]->stride(0), s.x_stride_t[i] = x[i]->stride(1), s.x_stride_h[i] = x[i]->stride(2);
+            if (weight[i] == nullptr) continue;
+            need(weight[i]->dim() == 1 && weight[i]->size(0) == D && weight[i]->is_contiguous());
+            s.weight[i] = ptr(weight[i]), s.w_dtype = code_of(*weight[i]);
+        }
+        if (weight[0] != nullptr && weight[1] != nullptr) need(weight[0]->scalar_type() == weight[1]->scalar_type());
+        need(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat && cos.dim() == 2 && sin.sizes() == cos.sizes() && cos.is_contiguous() && sin.is_contiguous());
+        s.cos = static_cast<const float*>(ptr(cos)), s.sin = static_cast<const float*>(ptr(sin));
+        s.B = size32(B), s.T = size32(T), s.D = size32(D), s.R = size32(2 * cos.size(1)), s.table_rows = size32(cos.size(0)), s.eps = (float)number(args[7]);
+        if (positions == nullptr) {
+            need(T <= cos.size(0));
+            return;
+        }
+        const int64_t d = positions->dim();
+        need(positions->scalar_type() == at::kInt && (d == 1 || (d == 2 && positions->size(0) == B)) && positions->size(d - 1) == T && (T == 1 || positions->stride(d - 1) == 1));
+        s.pos = static_cast<const int32_t*>(ptr(positions)), s.pos_stride_b = d == 2 ? positions->stride(0) : 0;
+    }
+};
+
+// qk_rotary(stream, q, k, q_weight, k_weight, cos, sin, positions, eps) -> (q', k')
+PyObject* qk_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return fast_path(n, 9, [&]() -> PyObject* {
+        Operands operand;
+        void* const stream = stream_of(args[0]);
+        RotaryOperands x(operand, args + 1);
+        const at::Tensor &q = operand(args[1]), &k = operand(args[2]);
+        at::Tensor y[2];
+        without_interpreter_lock([&] { y[0] = fresh(q, q.sizes()), y[1] = fresh(k, k.sizes()); });
+        for (int i = 0; i < 2; i++) x.s.y[i] = ptr(y[i]);
+        return launch("gdn_qk_norm_rotary_fwd", pack_results({y[0], y[1]}), [&] { return rotary_fn(&x.s, stream); });
+    });
+}
+
+// qk_rotary_bwd(stream, q, k, q_weight, k_weight, cos, sin, positions, eps, dq', dk', needs_q_weight, needs_k_weight) -> (dq, dk, dq_weight, dk_weight)
+PyObject* qk_rotary_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return fast_path(n, 13, [&]() -> PyObject* {
+        Operands operand;
+        void* const stream = stream_of(args[0]);
+        const RotaryOperands x(operand, args + 1);
+        const at::Tensor* const in[2] = {&operand(args[1]), &operand(args[2])};
+        gdn_qk_rotary_bwd_args b{};
+        b.fwd = x.s;
+        at::Tensor dx[2], part[2], dw[2];
+        bool needs[2];
+        for (int i = 0; i < 2; i++) {
+            const at::Tensor& dy = operand(args[9 + i]);
+            need(dy.scalar_type() == in[i]->scalar_type() && dy.sizes() == in[i]->sizes() && dy.stride(3) == 1);
+            needs[i] = truth(args[11 + i]);
+            need(!needs[i] || x.weight[i] != nullptr);
+            b.dy[i] = ptr(dy), b.dy_stride_b[i] = dy.stride(0), b.dy_stride_t[i] = dy.stride(1), b.dy_stride_h[i] = dy.stride(2);
+        }
+        without_interpreter_lock([&] {
+            b.partial_blocks = rotary_blocks_fn(&b.fwd);
+            for (int i = 0; i < 2; i++) {
+                dx[i] = fresh(*in[i], in[i]->sizes());
+                if (needs[i]) part[i] = fresh_f32(*in[i], {b.partial_blocks, in[i]->size(3)}), dw[i] = at::empty(x.weight[i]->sizes(), x.weight[i]->options());
+            }
+        });
+        ColumnSums sums;
+        for (int i = 0; i < 2; i++) {
+            b.dx[i] = ptr(dx[i]);
+            if (needs[i]) b.dweight_partial[i] = static_cast<float*>(ptr(part[i])), sums.add(part[i], dw[i]);
+        }
+        return launch("gdn_qk_norm_rotary_bwd, gdn_column_sums", pack_results({dx[0], dx[1], dw[0], dw[1]}), [&] {
+            const int status = rotary_bwd_fn(&b, stream);
+            return status == GDN_OK && sums.s.arrays > 0 ? column_sums_fn(&sums.s, stream) : status;
+        });
+    });
+}
+
+// q, k, v of a call, its options
+struct WindowOperands {
+    gdn_window_attn_args s{};
+
+    WindowOperands(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, PyObject* window, PyObject* sinks, PyObject* scale, const at::Tensor* cu, bool padded) {
+        s.dtype = code_of(q);
+        need(q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes() && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type());
+        need(k.size(0) == q.size(0) && k.size(3) == q.size(3) && q.numel() > 0 && k.numel() > 0 && q.size(2) % k.size(2) == 0);
+        need(q.stride(3) == 1 && k.stride(3) == 1 && v.stride(3) == 1);
+        int64_t N = q.size(0);
+        if (cu != nullptr) {
+            need(cu->scalar_type() == at::kInt && cu->dim() == 1 && cu->is_contiguous() && cu->numel() >= 2 && k.size(1) == q.size(1));
+            if (padded) need(cu->numel() == N + 1);
+            else need(N == 1), N = cu->numel() - 1;
+        } else {
+            need(!padded);
+        }
+        s.B = size32(q.size(0)), s.T = size32(q.size(1)), s.S = size32(k.size(1)), s.H = size32(q.size(2)), s.HK = size32(k.size(2)), s.D = size32(q.size(3));
+        s.N = size32(N), s.window = size32(integer(window)), s.sinks = size32(integer(sinks)), s.flags = padded ? GDN_FLAG_LEFT_PADDED : 0, s.scale = (float)number(scale);
+        s.q = ptr(q), s.k = ptr(k), s.v = ptr(v), s.cu_seqlens = static_cast<const int32_t*>(ptr(cu));
+        s.q_stride_b = q.stride(0), s.q_stride_t = q.stride(1), s.q_stride_h = q.stride(2);
+        s.k_stride_b = k.stride(0), s.k_stride_t = k.stride(1), s.k_stride_h = k.stride(2);
+        s.v_stride_b = v.stride(0), s.v_stride_t = v.stride(1), s.v_stride_h = v.stride(2);
+    }
+    // fp32 keeps two numbers of a row
+    std::vector<int64_t> lse_sizes() const {
+        std::vector<int64_t> sizes{s.B, s.T, s.H};
+        if (s.dtype == GDN_F32) sizes.push_back(2);
+        return sizes;
+    }
+    void output(const at::Tensor& o) {
+        s.o = ptr(o), s.o_stride_b = o.stride(0), s.o_stride_t = o.stride(1), s.o_stride_h = o.stride(2);
+    }
+};
+
+// window_attention(stream, q, k, v, window, sinks, scale, cu_seqlens, left_padded, wants_lse) -> (o, lse or None)
+PyObject* window_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return fast_path(n, 10, [&]() -> PyObject* {
+        Operands operand;
+        void* const stream = stream_of(args[0]);
+        const at::Tensor &q = operand(args[1]), &k = operand(args[2]), &v = operand(args[3]);
+        WindowOperands x(q, k, v, args[4], args[5], args[6], operand.optional(args[7]), truth(args[8]));
+        const bool wants_lse = truth(args[9]);
+        at::Tensor o, lse, workspace;
+        without_interpreter_lock([&] {
+            x.s.workspace_bytes = window_workspace_fn(&x.s);
+            workspace = workspace_of(x.s.workspace_bytes, q);
+            o = fresh(q, q.sizes());
+            if (wants_lse) lse = fresh_f32(q, x.lse_sizes());
+        });
+        if (workspace.defined()) x.s.workspace = ptr(workspace);
+        if (wants_lse) x.s.lse = static_cast<float*>(ptr(lse));
+        x.output(o);
+        return launch("gdn_window_attn_fwd", pack_results({o, lse}), [&] { return window_fn(&x.s, stream); });
+    });
+}
+
+// window_attention_bwd(stream, q, k, v, o, lse, window, sinks, scale, cu_seqlens, left_padded, do) -> (dq, dk, dv)
+PyObject* window_attention_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return fast_path(n, 12, [&]() -> PyObject* {
+        Operands operand;
+        void* const stream = stream_of(args[0]);
+        const at::Tensor &q = operand(args[1]), &k = operand(args[2]), &v = operand(args[3]), &o = operand(args[4]), &lse = operand(args[5]), &d = operand(args[11]);
+        WindowOperands x(q, k, v, args[6], args[7], args[8], operand.optional(args[9]), truth(args[10]));
+        need(o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() && o.stride(3) == 1);
+        need(lse.scalar_type() == at::kFloat && lse.sizes() == at::IntArrayRef(x.lse_sizes()) && lse.is_contiguous());
+        need(d.sizes() == q.sizes() && d.scalar_type() == q.scalar_type() && d.stride(3) == 1);
+        x.s.lse = static_cast<float*>(ptr(lse));
+        x.output(o);
+        gdn_window_attn_bwd_args b{};
+        b.fwd = x.s;
+        at::Tensor dq, dk, dv, workspace;
+        without_interpreter_lock([&] {
+            b.workspace_bytes = window_bwd_workspace_fn(&b);
+            workspace = workspace_of(b.workspace_bytes, q);
+            dq = fresh(q, q.sizes()), dk = fresh(k, k.sizes()), dv = fresh(v, v.sizes());
+        });
+        b.workspace = workspace.defined() ? ptr(workspace) : nullptr;
+        b.dout = ptr(d), b.dq = ptr(dq), b.dk = ptr(dk), b.dv = ptr(dv);
+        b.dout_stride_b = d.stride(0), b.dout_stride_t = d.stride(1), b.dout_stride_h = d.stride(2);
+        b.dq_stride_b = dq.stride(0), b.dq_stride_t = dq.stride(1), b.dq_stride_h = dq.stride(2);
+        b.dk_stride_b = b.dv_stride_b = dk.stride(0), b.dk_stride_t = b.dv_stride_t = dk.stride(1), b.dk_stride_h = b.dv_stride_h = dk.stride(2);
+        return launch("gdn_window_attn_bwd", pack_results({dq, dk, dv}), [&] { return window_bwd_fn(&b, stream); });
+    });
+}
+
+// cache.k, cache.v, cache.k_scale, cache.v_scale, block_table
+struct CacheOperands {
+    gdn_paged_cache s{};
+    const at::Tensor* tensors[4];
+
+    CacheOperands(Operands& operand, PyObject* const* args) {
+        for (int i = 0; i < 4; i++) {
+            tensors[i] = &operand(args[i]);
+            need(tensors[i]->is_contiguous() && tensors[i]->scalar_type() == (i < 2 ? at::kFloat8_e4m3fn : at::kByte));
+        }
+        const at::Tensor &k = *tensors[0], &v = *tensors[1], &table = operand(args[4]);
+        need(k.dim() == 4 && v.dim() == 5 && k.numel() > 0 && k.size(2) % 16 == 0);
+        need(v.sizes() == at::IntArrayRef({k.size(0), k.size(1), k.size(2) / 16, k.size(3), 16}));
+        for (int i = 2; i < 4; i++) need(tensors[i]->sizes() == at::IntArrayRef({k.size(0), k.size(1)}));
+        need(table.scalar_type() == at::kInt && table.dim() == 2 && table.numel() > 0 && (table.stride(1) == 1 || table.size(1) == 1));
+        s.k_codes = ptr(k), s.v_codes = ptr(v), s.k_scales = static_cast<uint8_t*>(ptr(tensors[2])), s.v_scales = static_cast<uint8_t*>(ptr(tensors[3]));
+        s.table = static_cast<const int32_t*>(ptr(table)), s.table_stride = table.stride(0);
+        s.pages = size32(k.size(0)), s.HK = size32(k.size(1)), s.P = size32(k.size(2)), s.D = size32(k.size(3));
+        s.N = size32(table.size(0)), s.table_pages = size32(table.size(1));
+    }
+    // int32 [N]
+    const int32_t* counts(const at::Tensor& t) const {
+        need(t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == s.N && t.is_contiguous());
+        return static_cast<const int32_t*>(ptr(t));
+    }
+};
+
+// cache_write(stream, cache (4), block_table, k, v, start, cu_seqlens, left_padded) -> True
+PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return fast_path(n, 11, [&]() -> PyObject* {
+        Operands operand;
+        void* const stream = stream_of(args[0]);
+        const CacheOperands c(operand, args + 1);
+        const at::Tensor &k = operand(args[6]), &v = operand(args[7]);
+        const at::Tensor* const cu = operand.optional(args[9]);
+        gdn_cache_write_args s{};
+        s.cache = c.s;
+        const bool padded = truth(args[10]);
+        s.dtype = code_of(k);
+        need(k.dim() == 4 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && k.size(2) == c.s.HK && k.size(3) == c.s.D && k.numel() > 0);
+        need(k.stride(3) == 1 && v.stride(3) == 1);
+        if (cu != nullptr) need(cu->scalar_type() == at::kInt && cu->dim() == 1 && cu->numel() == c.s.N + 1 && cu->is_contiguous());
+        s.k = ptr(k), s.v = ptr(v), s.start = c.counts(operand(args[8])), s.cu_seqlens = static_cast<const int32_t*>(ptr(cu));
+        s.k_stride_b = k.stride(0), s.k_stride_t = k.stride(1), s.k_stride_h = k.stride(2);
+        s.v_stride_b = v.stride(0), s.v_stride_t = v.stride(1), s.v_stride_h = v.stride(2);
+        s.B = size32(k.size(0)), s.T = size32(k.size(1)), s.flags = padded ? GDN_FLAG_LEFT_PADDED : 0;
+        return launch("gdn_cache_write", Py_NewRef(Py_True), [&] {
+            const int status = cache_write_fn(&s, stream);
+            if (status >= 0)
+                for (const at::Tensor* const t : c.tensors) mark_written(*t);
+            return status;
+        });
+    });
+}
+
+// cache_read(stream, cache (4), block_table, lengths, tokens, bf16) -> (k, v)
+PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return fast_path(n, 9, [&]() -> PyObject* {
+        Operands operand;
+        void* const stream = stream_of(args[0]);
+        const CacheOperands c(operand, args + 1);
+        gdn_cache_read_args s{};
+        s.cache = c.s, s.lengths = c.counts(operand(args[6])), s.T = size32(integer(args[7]));
+        const bool bf16 = truth(args[8]);
+        s.dtype = bf16 ? GDN_BF16 : GDN_F32;
+        need(s.T > 0);
+        at::Tensor out[2];
+        without_interpreter_lock([&] {
+            for (at::Tensor& t : out) t = at::empty({c.s.N, s.T, c.s.HK, c.s.D}, c.tensors[0]->options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
+        });
+        s.k = ptr(out[0]), s.v = ptr(out[1]);
+        return launch("gdn_cache_read", pack_results({out[0], out[1]}), [&] { return cache_read_fn(&s, stream); });
+    });
+}
+
+// cache_attention(stream, q, cache (4), block_table, lengths, window, sinks, scale) -> o
+PyObject* cache_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return fast_path(n, 11, [&]() -> PyObject* {
+        Operands operand;
+        void* const stream = stream_of(args[0]);
+        const at::Tensor& q = operand(args[1]);
+        const CacheOperands c(operand, args + 2);
+        gdn_cache_attn_args s{};
+        s.cache = c.s, s.lengths = c.counts(operand(args[7]));
+        need(q.scalar_type() == at::kBFloat16 && q.dim() == 4 && q.size(0) == c.s.N && q.size(3) == c.s.D && q.stride(3) == 1 && q.numel() > 0 && q.size(2) % c.s.HK == 0);
+        s.T = size32(q.size(1)), s.H = size32(q.size(2)), s.window = size32(integer(args[8])), s.sinks = size32(integer(args[9])), s.scale = (float)number(args[10]);
+        at::Tensor o, workspace;
+        without_interpreter_lock([&] {
+            s.workspace_bytes = cache_attn_workspace_fn(&s);
+            workspace = workspace_of(s.workspace_bytes, q);
+            o = fresh(q, q.sizes());
+        });
+        s.workspace = workspace.defined() ? ptr(workspace) : nullptr;
+        s.q = ptr(q), s.q_stride_b = q.stride(0), s.q_stride_t = q.stride(1), s.q_stride_h = q.stride(2);
+        s.o = ptr(o), s.o_stride_b = o.stride(0), s.o_stride_t = o.stride(1), s.o_stride_h = o.stride(2);
+        return launch("gdn_cache_attn", THPVariable_Wrap(o), [&] { return cache_attn_fn(&s, stream); });
+    });
+}
+
 PyMethodDef methods[] = {
     {"bind", (PyCFunction)(void (*)())bind, METH_FASTCALL, "takes the addresses of the library's entry points"},
     {"layer_step", (PyCFunction)(void (*)())layer_step, METH_FASTCALL, "gdn_layer_step"},
@@ -925,6 +1212,13 @@ PyMethodDef methods[] = {
     {"linear_attention_bwd", (PyCFunction)(void (*)())linear_attention_bwd, METH_FASTCALL, "gdn_linear_attn_bwd"},
     {"layer_norm", (PyCFunction)(void (*)())layer_norm, METH_FASTCALL, "gdn_layer_norm_fwd"},
     {"layer_norm_bwd", (PyCFunction)(void (*)())layer_norm_bwd, METH_FASTCALL, "gdn_layer_norm_bwd, gdn_column_sums"},
+    {"qk_rotary", (PyCFunction)(void (*)())qk_rotary, METH_FASTCALL, "gdn_qk_norm_rotary_fwd"},
+    {"qk_rotary_bwd", (PyCFunction)(void (*)())qk_rotary_bwd, METH_FASTCALL, "gdn_qk_norm_rotary_bwd, gdn_column_sums"},
+    {"window_attention", (PyCFunction)(void (*)())window_attention, METH_FASTCALL, "gdn_window_attn_fwd"},
+    {"window_attention_bwd", (PyCFunction)(void (*)())window_attention_bwd, METH_FASTCALL, "gdn_window_attn_bwd"},
+    {"cache_write", (PyCFunction)(void (*)())cache_write, METH_FASTCALL, "gdn_cache_write"},
+    {"cache_read", (PyCFunction)(void (*)())cache_read, METH_FASTCALL, "gdn_cache_read"},
+    {"cache_attention", (PyCFunction)(void (*)())cache_attention, METH_FASTCALL, "gdn_cache_attn"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "gdn_host", "host path of the entry points and their backward passes", -1, methods, nullptr, nullptr, nullptr, nullptr};

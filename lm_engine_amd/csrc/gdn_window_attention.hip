@@ -1,0 +1,234 @@
+// Softmax attention over a window, forward, bf16 (include/gdn_attention_hip.h, gdn_window_attention.h).
+//
+// A workgroup has 128 rows, 32 to a wave, and walks over the keys that they see in tiles of 64.  Scores are formed as S^T = K Q^T, so that a
+// lane holds one row: its maximum and sum need one exchange between lanes, and P^T is the next product's operand O^T += V^T P^T as it
+// lies in registers.  Keys and values go from memory into LDS without registers, the next tile while this one is worked on.
+// Softmax in one pass: weights are 2^(c s - m), m the largest c s that was met when it last passed the reference by 8 (2^8 is no harm
+// to fp32 sums, and bf16 rounds relative to the weight), so that the outputs are seldom rescaled.
+#include <algorithm>
+
+#include "gdn_launch.h"
+#include "gdn_window_attention.h"
+
+namespace gdn {
+
+namespace {
+
+// zeros in the place of what is not finite; whether there was any
+__device__ __forceinline__ bool make_finite(bf16x8& x) {
+    i32x4 w = __builtin_bit_cast(i32x4, x);
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 4; e++) bad |= (w[e] & 0x7f80) == 0x7f80 || (w[e] & 0x7f800000) == 0x7f800000;
+    if (!bad) return false;
+#pragma unroll
+    for (int e = 0; e < 4; e++) w[e] = ((w[e] & 0x7f80) == 0x7f80 ? 0 : w[e] & 0xffff) | ((w[e] & 0x7f800000) == 0x7f800000 ? 0 : w[e] & 0xffff0000);
+    x = __builtin_bit_cast(bf16x8, w);
+    return true;
+}
+
+template <int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_fwd_kernel(const WindowParams p) {
+    constexpr int KS = DP / 16, DT = DP / 32;
+    using Loads = TileLoads<DP>;
+    __shared__ __attribute__((aligned(1024))) bf16_t tiles[2][2][64 * DP];
+    int pair, block;
+    if (!work_item(p, blockIdx.x, pair, block)) return;
+    block = p.blocks - 1 - block;  // the rows that see most keys first
+    const int b = pair / p.HK, hk = pair - b * p.HK;
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), half = lane >> 5;
+    const int r0 = block * WINDOW_ROWS;
+    const int row = r0 + 32 * wave + (lane & 31), r = min(row, p.rows - 1);  // (past the end: the last row once more, and not stored)
+    const int t = p.G == 1 ? r : r / p.G, g = r - t * p.G;
+
+    bf16x8 q[KS];
+    load_row_fragments<DP>(static_cast<const bf16_t*>(p.q.p) + b * p.q.b + t * p.q.t + (hk * p.G + g) * p.q.h, p.D, half, true, q);
+    if (p.negative)
+#pragma unroll
+        for (int s = 0; s < KS; s++) q[s] = -q[s];
+
+    const RowView view = row_view(p, b, r);
+    // keys that the workgroup needs: [lo, end) and the first ones of its first row's sequence, [sink, sink_end)
+    const WaveView w = wave_view(view);
+    __shared__ int bounds[4][6];
+    const WaveView all = join_waves<4>(w, bounds, wave, lane);
+    const int lo = all.lo, end = all.end, sink = all.sink, sink_end = min(all.sink_end, lo);
+
+    const int sink_tiles = sink_end > sink ? (sink_end - sink + 63) / 64 : 0, near_tiles = end > lo ? (end - lo + 63) / 64 : 0;
+    int first_tile = 0, last_tile = sink_tiles + near_tiles;
+    if (p.splits > 1) {
+        const int each = (last_tile + p.splits - 1) / p.splits;
+        first_tile = min((int)blockIdx.y * each, last_tile), last_tile = min(first_tile + each, last_tile);
+    }
+
+    const char* const kb = reinterpret_cast<const char*>(static_cast<const bf16_t*>(p.k.p) + b * p.k.b + hk * p.k.h);
+    const char* const vb = reinterpret_cast<const char*>(static_cast<const bf16_t*>(p.v.p) + b * p.v.b + hk * p.v.h);
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&tiles[0][0][0];
+    auto tile_at = [&](int i, int& j0, int& count) {
+        const bool s = i < sink_tiles;
+        j0 = s ? sink + 64 * i : lo + 64 * (i - sink_tiles);
+        count = min((s ? sink_end : end) - j0, 64);
+    };
+    auto load_tile = [&](int i) {
+        int j0, count;
+        tile_at(i, j0, count);
+        const char *const k0 = kb + (int64_t)j0 * p.k.t * 2, *const v0 = vb + (int64_t)j0 * p.v.t * 2;
+        const uint32_t to = lds + (i & 1) * 2 * 64 * DP * 2;
+#pragma unroll
+        for (int x = 0; x < Loads::ITERS; x++) {
+            const int kr = Loads::row(wave, lane, x), c = Loads::column(wave, lane, x);
+            const bool there = kr < count && c < p.D;
+            Loads::load(k0, there ? (uint32_t)(kr * (int)p.k.t + c) * 2 : PAST, to, wave, x);
+            Loads::load(v0, there ? (uint32_t)(kr * (int)p.v.t + c) * 2 : PAST, to + 64 * DP * 2, wave, x);
+        }
+    };
+
+    const TileReader<DP> reader(lane);
+    f32x16 o[DT] = {};
+    float m = LOWEST, l = 0.f;
+    bool taken_out = false;
+    if (first_tile < last_tile) load_tile(first_tile);
+    for (int i = first_tile; i < last_tile; i++) {
+        loads_done();
+        __syncthreads();
+        if (i + 1 < last_tile) load_tile(i + 1);
+        int j0, count;
+        tile_at(i, j0, count);
+        const bf16_t *const kt = tiles[i & 1][0], *const vt = tiles[i & 1][1];
+        const bool near = i >= sink_tiles, full = near && j0 >= w.full_lo && j0 + 64 <= w.full_end;
+        // A tile that some row does not see all of: 0 times a value that is not finite must not reach that row.  Such values are taken
+        // out here, and go to the rows that see them in the end.
+        if (!near || j0 < all.full_lo || j0 + 64 > all.full_end) {
+            bf16x8* const v8 = reinterpret_cast<bf16x8*>(tiles[i & 1][1]);
+            bool found = false;
+#pragma unroll
+            for (int x = 0; x < 64 * DP / 8 / 256; x++) {
+                bf16x8 v = v8[threadIdx.x + 256 * x];
+                if (make_finite(v)) v8[threadIdx.x + 256 * x] = v, found = true;
+            }
+            taken_out |= __syncthreads_or(found) != 0;
+        }
+        f32x16 s[2];
+        if (w.meets(j0, count)) {
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                f32x16 acc = {};
+#pragma unroll
+                for (int y = 0; y < KS; y++) acc = mma(reader.across(kt, 32 * x, y), q[y], acc);
+                s[x] = acc;
+            }
+            float c = p.c;
+            if (!full) {
+                const TileView own(view, near, sink_end);
+                c = 1.f;
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int j = j0 + 32 * x + acc_row(e, half);
+                        s[x][e] = own.sees(j) ? s[x][e] * p.c : -__builtin_inff();
+                    }
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) top = fmaxf(top, s[x][e]);
+            top = fmaxf(top, other_half(top)) * c;
+            if (__builtin_amdgcn_ballot_w64(top > m + 8.f) != 0) {
+                const float next = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - next);
+                m = next;
+                l *= alpha;
+#pragma unroll
+                for (int x = 0; x < DT; x++) o[x] *= alpha;
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    s[x][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], c, -m));
+                    sum += s[x][e];
+                }
+            l += sum;
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                const bf16x8 weights = pack8(s[y >> 1], y & 1);
+#pragma unroll
+                for (int x = 0; x < DT; x++) o[x] = mma(reader.down(vt, y, x), weights, o[x]);
+            }
+        }
+    }
+
+    l += other_half(l);
+    const int64_t part = (((int64_t)blockIdx.y * p.B + b) * p.HK + hk) * p.rows + r0;
+    bf16_t* const out = static_cast<bf16_t*>(const_cast<void*>(p.o.p)) + b * p.o.b + hk * p.G * p.o.h;
+    if (row < p.rows) {
+        if (p.splits > 1) {
+            const int64_t at = part + row - r0;
+            if (half == 0) p.part_m[2 * at] = m, p.part_m[2 * at + 1] = l;
+            float* const to = p.part_o + at * p.D;
+#pragma unroll
+            for (int x = 0; x < DT; x++)
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    const int c = 32 * x + 8 * y + 4 * half;
+                    if (c < p.D) *reinterpret_cast<f32x4*>(to + c) = f32x4{o[x][4 * y], o[x][4 * y + 1], o[x][4 * y + 2], o[x][4 * y + 3]};
+                }
+        } else {
+            if (p.lse != nullptr && half == 0) p.lse[((int64_t)b * p.T + t) * p.H + hk * p.G + g] = l == 0.f ? __builtin_inff() : m + log2f(l);
+            store_transposed<DP>(out + t * p.o.t + g * p.o.h, p.D, half, o, l == 0.f ? 0.f : 1.f / l);
+        }
+    }
+    if (!taken_out) return;
+    add_taken_out<bf16_t>(p, b, hk, r0, WINDOW_ROWS, all, first_tile, last_tile, sink_tiles, tile_at, part);
+}
+
+// The parts of a row joined: a wave a row.
+template <typename T>
+__global__ __launch_bounds__(256) void window_combine_kernel(const WindowParams p) {
+    const int64_t all = (int64_t)p.B * p.HK * p.rows, at = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;
+    const int lane = threadIdx.x % WAVE;
+    if (at >= all) return;
+    float m = LOWEST;
+    for (int s = 0; s < p.splits; s++) m = fmaxf(m, p.part_m[2 * (s * all + at)]);
+    float l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < p.splits; s++) {
+        const int64_t part = s * all + at;
+        const float weight = __builtin_amdgcn_exp2f(p.part_m[2 * part] - m);
+        l += weight * p.part_m[2 * part + 1];
+        if (4 * lane < p.D) o += *reinterpret_cast<const f32x4*>(p.part_o + part * p.D + 4 * lane) * weight;
+    }
+    const int64_t pair = at / p.rows;
+    const int r = (int)(at - pair * p.rows), b = (int)(pair / p.HK), hk = (int)(pair - (int64_t)b * p.HK), t = r / p.G, g = r - t * p.G;
+    if (p.lse != nullptr && lane == 0) {
+        const int64_t head = ((int64_t)b * p.T + t) * p.H + hk * p.G + g;
+        if constexpr (sizeof(T) == 2) p.lse[head] = l == 0.f ? __builtin_inff() : m + log2f(l);
+        else p.lse[2 * head] = l == 0.f ? 0.f : m, p.lse[2 * head + 1] = l == 0.f ? 0.f : 1.f / l;
+    }
+    if (4 * lane >= p.D) return;
+    T* const to = static_cast<T*>(const_cast<void*>(p.o.p)) + b * p.o.b + t * p.o.t + (hk * p.G + g) * p.o.h;
+    store4<T>(to + 4 * lane, o * (l == 0.f ? 0.f : 1.f / l));
+}
+
+}  // namespace
+
+int launch_window_fwd(const WindowParams& p, hipStream_t stream) {
+    const int64_t items = (int64_t)p.B * p.HK * p.blocks;
+    const dim3 grid((unsigned)((items + 7) / 8 * 8), p.splits);
+    if (p.D <= 64) hipLaunchKernelGGL((window_fwd_kernel<64>), grid, dim3(256), 0, stream, p);
+    else if (p.D <= 128) hipLaunchKernelGGL((window_fwd_kernel<128>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((window_fwd_kernel<256>), grid, dim3(256), 0, stream, p);
+    if (const int e = (int)hipGetLastError(); e != 0) return e;
+    return p.splits > 1 ? launch_window_combine(p, GDN_BF16, stream) : GDN_OK;
+}
+
+int launch_window_combine(const WindowParams& p, int dtype, hipStream_t stream) {
+    const dim3 grid((unsigned)(((int64_t)p.B * p.HK * p.rows + 3) / 4));
+    if (dtype == GDN_BF16) hipLaunchKernelGGL((window_combine_kernel<bf16_t>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((window_combine_kernel<float>), grid, dim3(256), 0, stream, p);
+    return (int)hipGetLastError();
+}
+
+}  // namespace gdn

@@ -17,7 +17,8 @@ they are not bit-identical to the two-kernel path, which every other batch takes
 many sequences): switch it off - ``enable_kernels([Kernel.gated_delta_rule], reset=True)`` or
 ``ENABLE_KERNELS=gated_delta_rule`` - where runs of different batch shapes are compared bit for bit.
 
-``Kernel.linear_attention`` and ``Kernel.layer_norm`` stand for the operators of those names, on by default and without a
+``Kernel.linear_attention``, ``Kernel.layer_norm``, ``Kernel.window_attention`` (``sliding_window_attention``), ``Kernel.qk_norm_rotary`` and
+``Kernel.paged_cache`` (writing, reading and attention over it) stand for the operators of those names, on by default and without a
 second implementation as well.
 """
 
@@ -33,6 +34,9 @@ class Kernel(Enum):
     gated_delta_rule_fused_launch = "gated_delta_rule_fused_launch"
     linear_attention = "linear_attention"
     layer_norm = "layer_norm"
+    window_attention = "window_attention"
+    qk_norm_rotary = "qk_norm_rotary"
+    paged_cache = "paged_cache"
 
 
 _ON_BY_DEFAULT = tuple(Kernel)

@@ -1,0 +1,119 @@
+"""Softmax attention over a window on the GPU, through its public entry point, against the formula in 64 bits.
+
+Tolerances, relative-L2 per tensor.  bf16 inputs are exact as they are.  The output's own rounding is off by at most 2^-8 (half a step of bf16)
+relative to the value, and each weight, as an operand, by at most 2^-8 of itself: with uniformly spread roundings (rms 1 / sqrt(3) of the
+maximum) independent of each other sqrt(2) 2^-8 / sqrt(3) = 3.2e-3; a weighted sum of values of both signs is smaller than the root of the sum of
+its terms' squares at worst by what the sum cancels, and 5e-3 is asked.  dv: the same two.  dq, dk: ds = w (dw - delta) is rounded once more as an
+operand, and delta comes from the rounded output, 2^-8 / sqrt(3) of each term of delta: three roundings, sqrt(3) 2^-8 / sqrt(3) = 3.9e-3 of terms of
+which a row's add up to zero (sum of ds is none), so that what is left is smaller than the terms: 1e-2.  fp32 inputs: sums of up to 1e3
+terms and exponents up to 2^5 with an error of 2^-24 relative: 1e-5."""
+
+import pytest
+import torch
+
+import lm_engine_amd
+from lm_engine_amd import sliding_window_attention
+from oracle.attention_oracle import window_attention_ref
+from tests.helpers import rel_l2
+
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+OUT = {BF16: 5e-3, F32: 1e-5}
+GRAD = {BF16: 1e-2, F32: 1e-5}
+
+
+def inputs(B, T, H, HK, D, S=None, dtype=BF16, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    randn = lambda *shape: torch.randn(*shape, generator=gen)  # noqa: E731
+    S = T if S is None else S
+    return (1.5 * randn(B, T, H, D)).to(dtype), randn(B, S, HK, D).to(dtype), randn(B, S, HK, D).to(dtype)
+
+
+def check(name, got, want, tolerance):
+    assert got.shape == want.shape, f"{name}: {tuple(got.shape)} {tuple(want.shape)}"
+    error = rel_l2(got, want)
+    print(f"{name} {error:.2e}", flush=True)
+    assert torch.isfinite(got.float()).all() and error <= tolerance, f"{name}: relative-L2 {error:.3e} above {tolerance:.1e}"
+
+
+def cu_of(lens):
+    return [0] + torch.tensor(lens).cumsum(0).tolist()
+
+
+def check_call(q, k, v, dtype, cu=None, backward=True, **options):
+    leaves = [x.cuda().requires_grad_(backward) for x in (q, k, v)]
+    cu_gpu = None if cu is None else torch.tensor(cu, dtype=torch.int32).cuda()
+    o = sliding_window_attention(*leaves, cu_seqlens=cu_gpu, **options)
+    ref = [x.double().requires_grad_(backward) for x in (q, k, v)]
+    want = window_attention_ref(*ref, cu_seqlens=cu, **options)
+    check("o", o, want.detach(), OUT[dtype])
+    assert o.dtype == dtype and o.is_contiguous()
+    if not backward:
+        return
+    do = torch.randn(o.shape, generator=torch.Generator().manual_seed(99)).to(dtype)
+    got, expected = torch.autograd.grad(o, leaves, do.cuda()), torch.autograd.grad(want, ref, do.double())
+    for name, x, y in zip(("dq", "dk", "dv"), got, expected):
+        if y.norm() < 1e-9:  # (one visible key each: a weight of one whatever the scores are)
+            assert x.float().norm() <= GRAD[dtype] * do.double().norm()
+        else:
+            check(name, x, y, GRAD[dtype])
+
+
+# (B, T, H, HK, D, window, sinks)
+WHOLE = [
+    (1, 1, 1, 1, 64, None, 0),
+    (2, 63, 2, 1, 64, None, 0),
+    (1, 64, 4, 4, 128, 16, 0),
+    (2, 65, 2, 2, 128, 64, 1),
+    (1, 130, 8, 1, 128, 33, 5),
+    (1, 300, 6, 2, 128, 100, 70),
+    (2, 257, 2, 1, 256, 128, 4),
+    (1, 200, 3, 3, 96, 50, 2),
+    (1, 150, 4, 2, 80, None, 0),
+    (1, 140, 2, 1, 24, 7, 3),
+    (1, 140, 2, 2, 200, 64, 64),
+    (1, 500, 5, 1, 64, 1, 0),
+    (1, 500, 2, 1, 64, 1, 1),
+    (1, 333, 16, 2, 64, 300, 130),
+    (3, 700, 4, 2, 64, 200, 4),
+    (1, 90, 2, 1, 64, 5000, 10),
+    (1, 700, 2, 1, 8, 90, 300),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B, T, H, HK, D, window, sinks", WHOLE, ids=str)
+def test_whole_sequences(B, T, H, HK, D, window, sinks, dtype):
+    check_call(*inputs(B, T, H, HK, D, dtype=dtype), dtype, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lens, H, HK, D, window, sinks", [
+    ([70, 1, 0, 129, 300], 4, 2, 64, 50, 3), ([200], 2, 1, 128, None, 0), ([5, 3, 2, 1, 1, 4, 7, 60, 64, 65], 2, 2, 64, 20, 2),
+    ([150, 400], 8, 1, 128, 100, 40), ([1] * 100, 2, 1, 64, 8, 1),
+], ids=str)  # fmt: skip
+def test_packed_sequences(lens, H, HK, D, window, sinks, dtype):
+    check_call(*inputs(1, sum(lens), H, HK, D, dtype=dtype), dtype, cu=cu_of(lens), window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("T, lens, window, sinks", [(200, [200, 0, 77, 1], 64, 4), (130, [3, 130], None, 0), (400, [399, 100], 30, 150)], ids=str)
+def test_left_padded_rows(T, lens, window, sinks, dtype):
+    check_call(*inputs(len(lens), T, 4, 2, 64, dtype=dtype), dtype, cu=cu_of(lens), left_padded=True, window=window, sinks=sinks)
+
+
+# (T queries, S keys): continuations, single tokens over many keys (cut into parts), queries in front of the first key
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("T, S, window, sinks", [(1, 700, None, 0), (1, 3000, None, 0), (1, 5000, 2000, 100), (7, 2049, None, 0), (100, 230, 60, 4),
+                                                 (50, 20, None, 0), (130, 1, 4, 1), (64, 1500, 700, 64)], ids=str)  # fmt: skip
+def test_other_keys_than_queries(T, S, window, sinks, dtype):
+    for H, HK, D in ((4, 1, 64), (2, 2, 128)):
+        check_call(*inputs(2, T, H, HK, D, S=S, dtype=dtype), dtype, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1.5])
+def test_scales(scale):
+    for dtype in (BF16, F32):
+        check_call(*inputs(1, 150, 2, 1, 64, dtype=dtype), dtype, window=100, sinks=3, scale=scale)
