@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "gdn_join.h"
 #include "gdn_launch.h"
 #include "gdn_paged_cache.h"
 
@@ -265,29 +266,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attn_kernel(cons
     }
 }
 
-// The parts of a row joined: a wave a row.
+// The parts of a row joined: a workgroup a row.
 __global__ __launch_bounds__(256) void cache_join_kernel(const AttendParams p) {
-    const int64_t all = (int64_t)p.c.N * p.c.HK * p.rows, at = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;
-    const int lane = threadIdx.x % WAVE;
-    if (at >= all) return;
-    // (a part of no key: m is the lowest number, and its sum and results are zeros)
-    float m = LOWEST;
-    for (int s = lane; s < p.splits; s += WAVE) m = fmaxf(m, p.part_m[2 * (s * all + at)]);
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, WAVE));
-    float l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = 0; s < p.splits; s++) {
-        const int64_t part = s * all + at;
-        const float weight = __builtin_amdgcn_exp2f(p.part_m[2 * part] - m);
-        l += weight * p.part_m[2 * part + 1];
-        if (4 * lane < p.c.D) o += *reinterpret_cast<const f32x4*>(p.part_o + part * p.c.D + 4 * lane) * weight;
-    }
-    if (4 * lane >= p.c.D) return;
+    const int64_t at = blockIdx.x;
+    float m, l;
+    f32x4 o;
+    int col;
+    if (!join_row(p.part_o, p.part_m, (int64_t)p.c.N * p.c.HK * p.rows, at, p.splits, p.c.D, m, l, o, col)) return;
     const int64_t pair = at / p.rows;
     const int r = (int)(at - pair * p.rows), n = (int)(pair / p.c.HK), hk = (int)(pair - (int64_t)n * p.c.HK), t = r / p.G;
-    store4<bf16_t>(p.o + n * p.o_b + t * p.o_t + (hk * p.G + r - t * p.G) * p.o_h + 4 * lane, o * (l == 0.f ? 0.f : 1.f / l));
+    store4<bf16_t>(p.o + n * p.o_b + t * p.o_t + (hk * p.G + r - t * p.G) * p.o_h + col, o * (l == 0.f ? 0.f : 1.f / l));
 }
 
 int check_attend(const gdn_cache_attn_args& a) {
@@ -302,7 +290,7 @@ int check_attend(const gdn_cache_attn_args& a) {
 int splits_of(const gdn_cache_attn_args& a) {
     const int64_t groups = (int64_t)a.cache.N * a.cache.HK * (((int64_t)a.T * (a.H / a.cache.HK) + ROWS - 1) / ROWS);
     const int64_t room = (int64_t)a.cache.table_pages * a.cache.P, keys = a.window == 0 ? room : std::min<int64_t>(room, (int64_t)a.window + a.T + a.sinks + CHUNK);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({2 * compute_units() / groups, keys / (4 * CHUNK), 128}));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({2 * compute_units() / groups, keys / (4 * CHUNK), JOIN_MOST}));
 }
 uint64_t part_o_bytes(const gdn_cache_attn_args& a, int splits) { return ((uint64_t)splits * a.cache.N * a.T * a.H * a.cache.D * 4 + 255) / 256 * 256; }
 uint64_t attend_bytes(const gdn_cache_attn_args& a) {
@@ -351,6 +339,6 @@ extern "C" int gdn_cache_attn(const gdn_cache_attn_args* args, void* stream) {
     else if (a.cache.D <= 128) hipLaunchKernelGGL((cache_attn_kernel<128>), grid, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((cache_attn_kernel<256>), grid, dim3(256), 0, st, p);
     if (const int e = (int)hipGetLastError(); e != 0 || p.splits == 1) return e;
-    hipLaunchKernelGGL(cache_join_kernel, dim3((unsigned)(((int64_t)a.cache.N * a.cache.HK * p.rows + 3) / 4)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(cache_join_kernel, dim3((unsigned)((int64_t)a.cache.N * a.cache.HK * p.rows)), dim3(256), 0, st, p);
     return (int)hipGetLastError();
 }

@@ -204,6 +204,94 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const WriteParams p) {
     }
 }
 
+// A few new tokens per sequence: a group of L lanes, eight columns each, has one head of one touched page, keys or values, and goes over its new
+// rows; nothing of the page is read but the scale, unless that grows.  Values leave code by code (16 bytes apart).
+template <typename T, int L>
+__global__ __launch_bounds__(256) void cache_append_kernel(const WriteParams p) {
+    const int P = p.c.P, D = p.c.D, lane = threadIdx.x % L;
+    const int64_t unit = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L, slot = unit / (2 * p.c.HK);
+    const int rest = (int)(unit - slot * 2 * p.c.HK), value = rest & 1, h = rest >> 1;
+    const int n = (int)(slot / p.each), nth = (int)(slot - (int64_t)n * p.each), col = 8 * lane;
+    if (n >= p.c.N) return;
+    const NewTokens s = new_tokens(p, n);
+    const int index = s.start / P + nth;
+    if (nth >= pages_of(s.start, s.len, P)) return;
+    const int page = cache_page(p.c, n, index);
+    const int o0 = max(s.start - index * P, 0), o1 = min(s.start + s.len - index * P, P);
+    const T* const rows = static_cast<const T*>(value ? p.x[1] : p.x[0]) + s.b * (value ? p.b[1] : p.b[0]) + h * (value ? p.h[1] : p.h[0]) + col;
+    const int64_t stride = value ? p.t[1] : p.t[0], row0 = (int64_t)s.first + (index * P - s.start);
+    const bool there = col < D;
+    float first[8], top = 0.f;
+    for (int o = o1 - 1; o >= o0; o--) {
+        float x[8] = {};
+        if (there) load_row<T>(rows + (row0 + o) * stride, x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float a = fabsf(x[e]);
+            top = fmaxf(top, a < __builtin_inff() ? a : 0.f), first[e] = x[e];
+        }
+    }
+#pragma unroll
+    for (int off = L / 2; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, WAVE));
+    if (page < 0) return;
+    const int64_t head = (int64_t)page * p.c.HK + h;
+    uint8_t* const codes = static_cast<uint8_t*>(value ? p.c.v_codes : p.c.k_codes) + head * P * D;
+    uint8_t* const scales = value ? p.c.v_scales : p.c.k_scales;
+    int e = cache_exponent(top);
+    if (o0 > 0) {
+        const int before = cache_scale(scales, head);
+        if (e > before) {
+            const float shift = power_of_two(max(before - e, -126));
+            auto rescale = [&](unsigned w) {
+                const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+                return cache_codes(lo.x * shift, lo.y * shift, hi.x * shift, hi.y * shift);
+            };
+            if (there && value) {
+                for (int g = 0; 16 * g < o0; g++) {
+                    uint8_t* const from = codes + ((int64_t)g * D + col) * 16;
+                    for (int x = 0; x < 32; x++) {  // four tokens of a column; those from o0 on are written anew, or hold nothing
+                        unsigned* const to = reinterpret_cast<unsigned*>(from) + x;
+                        const int held = min(o0 - 16 * g - 4 * (x & 3), 4);
+                        const unsigned keep = held >= 4 ? ~0u : held <= 0 ? 0 : (1u << (8 * held)) - 1, w = *to;
+                        *to = (rescale(w) & keep) | (w & ~keep);
+                    }
+                }
+            } else if (there) {
+                for (int o = 0; o < o0; o++) {
+                    u32x2* const to = reinterpret_cast<u32x2*>(codes + (int64_t)o * D + col);
+                    u32x2 w = *to;
+                    w.x = rescale(w.x), w.y = rescale(w.y);
+                    *to = w;
+                }
+            }
+        }
+        e = max(e, before);
+    }
+    if (lane == 0) scales[head] = (uint8_t)(e + 127);
+    if (!there) return;
+    const float by = power_of_two(-e);
+    auto one = [&](float v) { return fabsf(v) < __builtin_inff() ? v * by : __builtin_nanf(""); };
+    for (int o = o0; o < o1; o++) {
+        float x[8];
+        if (o == o0) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = first[i];
+        } else {
+            load_row<T>(rows + (row0 + o) * stride, x);
+        }
+        const unsigned lo = cache_codes(one(x[0]), one(x[1]), one(x[2]), one(x[3])), hi = cache_codes(one(x[4]), one(x[5]), one(x[6]), one(x[7]));
+        if (value) {
+            uint8_t* const to = codes + ((int64_t)(o / 16) * D + col) * 16 + o % 16;
+#pragma unroll
+            for (int i = 0; i < 4; i++) to[16 * i] = (uint8_t)(lo >> (8 * i)), to[16 * (i + 4)] = (uint8_t)(hi >> (8 * i));
+        } else {
+            u32x2 out;
+            out.x = lo, out.y = hi;
+            *reinterpret_cast<u32x2*>(codes + (int64_t)o * D + col) = out;
+        }
+    }
+}
+
 struct ReadParams {
     gdn_paged_cache c;
     void* out[2];
@@ -273,6 +361,8 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const ReadParams p) {
     }
 }
 
+constexpr int APPEND_TOKENS = 8;  // up to here rows of tokens go by cache_append_kernel
+
 int threads_for(int P, int D) { return std::min(256, (P / 16 * (D / 8) + WAVE - 1) / WAVE * WAVE); }
 
 int check_rows16(const void* p, int64_t b, int64_t t, int64_t h, int dtype) {
@@ -314,6 +404,16 @@ extern "C" int gdn_cache_write(const gdn_cache_write_args* a, void* stream) {
     // packed: sequences of a token or more touch at most (tokens - 1) / P + 2 pages each
     const int64_t slots = packed ? (int64_t)a->T / P + 2 * (int64_t)std::min(a->cache.N, a->T) : (int64_t)a->cache.N * p.each;
     if (slots > INT32_MAX) return GDN_ERR_UNSUPPORTED;
+    if (!packed && a->T <= APPEND_TOKENS) {
+        const int lanes = a->cache.D <= 64 ? 8 : a->cache.D <= 128 ? 16 : 32;
+        const int64_t groups = slots * a->cache.HK * 2, blocks = (groups + 256 / lanes - 1) / (256 / lanes);
+        if (blocks > INT32_MAX) return GDN_ERR_UNSUPPORTED;
+        const hipStream_t st = static_cast<hipStream_t>(stream);
+        const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, p); };
+        if (a->dtype == GDN_BF16) lanes == 8 ? go(cache_append_kernel<bf16_t, 8>) : lanes == 16 ? go(cache_append_kernel<bf16_t, 16>) : go(cache_append_kernel<bf16_t, 32>);
+        else lanes == 8 ? go(cache_append_kernel<float, 8>) : lanes == 16 ? go(cache_append_kernel<float, 16>) : go(cache_append_kernel<float, 32>);
+        return (int)hipGetLastError();
+    }
     const dim3 grid((unsigned)slots, a->cache.HK, 2), block(threads_for(P, a->cache.D));
     if (a->dtype == GDN_BF16) hipLaunchKernelGGL((cache_write_kernel<bf16_t>), grid, block, 0, static_cast<hipStream_t>(stream), p);
     else hipLaunchKernelGGL((cache_write_kernel<float>), grid, block, 0, static_cast<hipStream_t>(stream), p);

@@ -24,6 +24,8 @@ struct RotaryParams {
     int heads[2];
     int T, D, R, table_rows, slices, w_bf16;
     uint32_t units;  // (token, slice of the heads)
+    int bwd_slices[2];
+    uint32_t bwd_units[2];
     float eps;
 };
 
@@ -162,92 +164,88 @@ __global__ __launch_bounds__(256) void rotary_fwd_kernel(const RotaryParams p) {
     }
 }
 
+// q first, then k, so that one set of weights and of their gradients is in registers.
 template <typename T, int VEC, int L>
 __global__ __launch_bounds__(256) void rotary_bwd_kernel(const RotaryParams p) {
     constexpr int GROUPS = 256 / L;
+    __shared__ float total[L * 2 * VEC];
     const int lane = threadIdx.x % L;
     const Chunk<VEC> c(p, lane);
-    const int all = p.heads[0] + p.heads[1];
-    const Vec<VEC> wq_lo = weight_at<VEC>(p.w[0], p.w_bf16, c.lo), wq_hi = weight_at<VEC>(p.w[0], p.w_bf16, c.hi);
-    const Vec<VEC> wk_lo = weight_at<VEC>(p.w[1], p.w_bf16, c.lo), wk_hi = weight_at<VEC>(p.w[1], p.w_bf16, c.hi);
-    float dw[2][2 * VEC] = {};
     const float over = 1.f / (float)p.D;
-    // (the lanes of a group walk together, groups of a wave need not: nothing crosses groups before the end)
-    for (uint32_t unit = blockIdx.x * (uint32_t)GROUPS + threadIdx.x / L; unit < p.units; unit += gridDim.x * (uint32_t)GROUPS) {
-        int b, t, slice;
-        unit_of(p, unit, b, t, slice);
-        auto fetch = [&](int h, Row<T, VEC>& x, Row<T, VEC>& d) {
-            const int which = h >= p.heads[0], head = which ? h - p.heads[0] : h;
-            x.fetch(static_cast<const T*>(which ? p.x[1] : p.x[0]) + row_at(p.x_b, p.x_t, p.x_h, b, t, which, head), c);
-            d.fetch(static_cast<const T*>(which ? p.dy[1] : p.dy[0]) + row_at(p.dy_b, p.dy_t, p.dy_h, b, t, which, head), c);
-        };
-        Row<T, VEC> next, next_dy;
-        fetch(slice, next, next_dy);
-        Vec<VEC> cs, sn;
-        c.angle(p, b, t, cs, sn);
-        for (int h = slice; h < all; h += p.slices) {
-            Vec<VEC> lo = widen<T, VEC>(next.lo), hi = widen<T, VEC>(next.hi);
-            const Vec<VEC> dy_lo = widen<T, VEC>(next_dy.lo), dy_hi = widen<T, VEC>(next_dy.hi);
-            if (h + p.slices < all) fetch(h + p.slices, next, next_dy);
-            float squares = 0.f;
+    for (int which = 0; which < 2; which++) {
+        const int heads = p.heads[which], slices = p.bwd_slices[which];
+        const int64_t x_b = p.x_b[which], x_t = p.x_t[which], x_h = p.x_h[which], dy_b = p.dy_b[which], dy_t = p.dy_t[which], dy_h = p.dy_h[which];
+        const T *const xs = static_cast<const T*>(p.x[which]), *const dys = static_cast<const T*>(p.dy[which]);
+        const Vec<VEC> w_lo = weight_at<VEC>(p.w[which], p.w_bf16, c.lo), w_hi = weight_at<VEC>(p.w[which], p.w_bf16, c.hi);
+        float dw[2 * VEC] = {};
+        const uint32_t units = p.bwd_units[which];
+        // (the lanes of a group walk together, groups of a wave need not: nothing crosses groups before the end)
+        for (uint32_t unit = blockIdx.x * (uint32_t)GROUPS + threadIdx.x / L; unit < units; unit += gridDim.x * (uint32_t)GROUPS) {
+            const uint32_t token = unit / (uint32_t)slices;
+            const int slice = (int)(unit - token * (uint32_t)slices), b = (int)(token / (uint32_t)p.T), t = (int)(token - (uint32_t)b * (uint32_t)p.T);
+            const T *x_row = xs + b * x_b + t * x_t + slice * x_h, *dy_row = dys + b * dy_b + t * dy_t + slice * dy_h;
+            T* to = static_cast<T*>(p.dx[which]) + ((int64_t)token * heads + slice) * p.D;
+            Row<T, VEC> next, next_dy;
+            next.fetch(x_row, c), next_dy.fetch(dy_row, c);
+            Vec<VEC> cs, sn;
+            c.angle(p, b, t, cs, sn);
+            for (int h = slice; h < heads; h += slices) {
+                Vec<VEC> lo = widen<T, VEC>(next.lo), hi = widen<T, VEC>(next.hi);
+                const Vec<VEC> dy_lo = widen<T, VEC>(next_dy.lo), dy_hi = widen<T, VEC>(next_dy.hi);
+                if (h + slices < heads) {
+                    x_row += slices * x_h, dy_row += slices * dy_h;
+                    next.fetch(x_row, c), next_dy.fetch(dy_row, c);
+                }
+                float squares = 0.f;
 #pragma unroll
-            for (int e = 0; e < VEC; e++) squares += lo.v[e] * lo.v[e] + hi.v[e] * hi.v[e];
-            const float r = 1.f / sqrtf(group_sum<L>(c.there ? squares : 0.f) * over + p.eps);
-            const bool key = h >= p.heads[0];
-            float product = 0.f;
-            Vec<VEC> du_lo, du_hi;
+                for (int e = 0; e < VEC; e++) squares += lo.v[e] * lo.v[e] + hi.v[e] * hi.v[e];
+                const float r = 1.f / sqrtf(group_sum<L>(c.there ? squares : 0.f) * over + p.eps);
+                float product = 0.f;
+                Vec<VEC> du_lo, du_hi;
 #pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                const float dn_lo = dy_lo.v[e] * cs.v[e] + dy_hi.v[e] * sn.v[e], dn_hi = dy_hi.v[e] * cs.v[e] - dy_lo.v[e] * sn.v[e];
-                lo.v[e] *= r, hi.v[e] *= r;
-                const float at_lo = dn_lo * lo.v[e], at_hi = dn_hi * hi.v[e];
-                if (key) dw[1][e] += at_lo, dw[1][VEC + e] += at_hi;
-                else dw[0][e] += at_lo, dw[0][VEC + e] += at_hi;
-                du_lo.v[e] = dn_lo * (key ? wk_lo.v[e] : wq_lo.v[e]), du_hi.v[e] = dn_hi * (key ? wk_hi.v[e] : wq_hi.v[e]);
-                product += du_lo.v[e] * lo.v[e] + du_hi.v[e] * hi.v[e];
-            }
-            product = group_sum<L>(c.there ? product : 0.f) * over;
+                for (int e = 0; e < VEC; e++) {
+                    const float dn_lo = dy_lo.v[e] * cs.v[e] + dy_hi.v[e] * sn.v[e], dn_hi = dy_hi.v[e] * cs.v[e] - dy_lo.v[e] * sn.v[e];
+                    lo.v[e] *= r, hi.v[e] *= r;
+                    dw[e] += dn_lo * lo.v[e], dw[VEC + e] += dn_hi * hi.v[e];
+                    du_lo.v[e] = dn_lo * w_lo.v[e], du_hi.v[e] = dn_hi * w_hi.v[e];
+                    product += du_lo.v[e] * lo.v[e] + du_hi.v[e] * hi.v[e];
+                }
+                product = group_sum<L>(c.there ? product : 0.f) * over;
 #pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                du_lo.v[e] = r * (du_lo.v[e] - lo.v[e] * product);
-                du_hi.v[e] = r * (du_hi.v[e] - hi.v[e] * product);
-            }
-            if (c.there) {
-                const int64_t token = (int64_t)b * p.T + t;
-                T* const to = static_cast<T*>(key ? p.dx[1] : p.dx[0]) + (token * (key ? p.heads[1] : p.heads[0]) + (key ? h - p.heads[0] : h)) * p.D;
-                store<T, VEC>(to + c.lo, du_lo);
-                store<T, VEC>(to + c.hi, du_hi);
+                for (int e = 0; e < VEC; e++) {
+                    du_lo.v[e] = r * (du_lo.v[e] - lo.v[e] * product);
+                    du_hi.v[e] = r * (du_hi.v[e] - hi.v[e] * product);
+                }
+                if (c.there) {
+                    store<T, VEC>(to + c.lo, du_lo);
+                    store<T, VEC>(to + c.hi, du_hi);
+                }
+                to += (int64_t)slices * p.D;
             }
         }
-    }
-    if (p.dw[0] == nullptr && p.dw[1] == nullptr) return;
-    // the workgroup's rows: a wave's groups by shuffles, then the waves one after the other through LDS
-    __shared__ float total[2][L * 2 * VEC];
+        if (p.dw[which] == nullptr) continue;
+        // the workgroup's rows: a wave's groups by shuffles, then the waves one after the other through LDS
 #pragma unroll
-    for (int wave = 0; wave < 256 / WAVE; wave++) {
-        if ((int)threadIdx.x / WAVE == wave) {
-#pragma unroll
-            for (int i = 0; i < 2; i++)
+        for (int wave = 0; wave < 256 / WAVE; wave++) {
+            if ((int)threadIdx.x / WAVE == wave) {
 #pragma unroll
                 for (int e = 0; e < 2 * VEC; e++) {
-                    float x = dw[i][e];
+                    float x = dw[e];
 #pragma unroll
                     for (int off = L; off < WAVE; off <<= 1) x += __shfl_xor(x, off, WAVE);
-                    if ((int)threadIdx.x % WAVE < L) total[i][lane * 2 * VEC + e] = wave == 0 ? x : total[i][lane * 2 * VEC + e] + x;
+                    if ((int)threadIdx.x % WAVE < L) total[lane * 2 * VEC + e] = wave == 0 ? x : total[lane * 2 * VEC + e] + x;
                 }
+            }
+            __syncthreads();
         }
-        __syncthreads();
-    }
-    if (threadIdx.x < L && c.there) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            if (p.dw[i] == nullptr) continue;
+        if (threadIdx.x < L && c.there) {
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
-                p.dw[i][(int64_t)blockIdx.x * p.D + c.lo + e] = total[i][lane * 2 * VEC + e];
-                p.dw[i][(int64_t)blockIdx.x * p.D + c.hi + e] = total[i][lane * 2 * VEC + VEC + e];
+                p.dw[which][(int64_t)blockIdx.x * p.D + c.lo + e] = total[lane * 2 * VEC + e];
+                p.dw[which][(int64_t)blockIdx.x * p.D + c.hi + e] = total[lane * 2 * VEC + VEC + e];
             }
         }
+        __syncthreads();
     }
 }
 
@@ -267,6 +265,14 @@ int slices_of(const gdn_qk_rotary_args& a) {
 }
 
 int64_t units_of(const gdn_qk_rotary_args& a) { return (int64_t)a.B * a.T * slices_of(a); }
+
+// The same in the backward, which goes over q and k one after the other.
+int bwd_slices_of(const gdn_qk_rotary_args& a, int which) {
+    const int64_t rows = (int64_t)a.B * a.T * a.heads[which], groups = (int64_t)compute_units() * 16 * (WAVE / lanes_of(a));
+    const int64_t each = std::min<int64_t>(std::max<int64_t>(rows / groups, 1), 4);
+    return (int)((a.heads[which] + each - 1) / each);
+}
+int64_t bwd_units_of(const gdn_qk_rotary_args& a, int which) { return (int64_t)a.B * a.T * bwd_slices_of(a, which); }
 
 int check_rotary(const gdn_qk_rotary_args& a) {
     if (a.B <= 0 || a.T <= 0 || a.heads[0] <= 0 || a.heads[1] <= 0 || a.D <= 0 || a.R <= 0 || a.table_rows <= 0) return GDN_ERR_SHAPE;
@@ -308,7 +314,7 @@ RotaryParams params_of(const gdn_qk_rotary_args& a) {
 
 int blocks_of_bwd(const gdn_qk_rotary_args& a) {
     const int64_t groups = 256 / lanes_of(a);
-    return (int)std::min<int64_t>((units_of(a) + groups - 1) / groups, 4 * compute_units());
+    return (int)std::min<int64_t>((std::max(bwd_units_of(a, 0), bwd_units_of(a, 1)) + groups - 1) / groups, 4 * compute_units());
 }
 
 template <bool BACKWARD, typename T, int VEC, int L>
@@ -362,6 +368,7 @@ extern "C" int gdn_qk_norm_rotary_bwd(const gdn_qk_rotary_bwd_args* b, void* str
         if (b->dx[i] == nullptr) return GDN_ERR_NULL;
         if (!on(b->dx[i], 16) || !on(b->dweight_partial[i], 4)) return GDN_ERR_ALIGN;
         p.dy[i] = b->dy[i], p.dx[i] = b->dx[i], p.dw[i] = b->dweight_partial[i];
+        p.bwd_slices[i] = bwd_slices_of(a, i), p.bwd_units[i] = (uint32_t)bwd_units_of(a, i);
         p.dy_b[i] = b->dy_stride_b[i], p.dy_t[i] = b->dy_stride_t[i], p.dy_h[i] = b->dy_stride_h[i];
     }
     if ((p.dw[0] != nullptr || p.dw[1] != nullptr) && b->partial_blocks != blocks_of_bwd(a)) return GDN_ERR_WORKSPACE;

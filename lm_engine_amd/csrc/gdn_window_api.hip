@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "gdn_join.h"
 #include "gdn_launch.h"
 #include "gdn_window_attention.h"
 
@@ -75,7 +76,7 @@ int splits_of(const gdn_window_attn_args& a) {
     const int64_t groups = (int64_t)a.B * a.HK * ((rows + edge - 1) / edge);
     const int64_t tokens = (edge + a.H / a.HK - 1) / (a.H / a.HK);
     const int64_t keys = a.window == 0 ? a.S : std::min<int64_t>(a.S, (int64_t)a.window + tokens + a.sinks);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({2 * compute_units() / groups, keys / 256, 128}));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({2 * compute_units() / groups, keys / 256, JOIN_MOST}));
 }
 
 uint64_t part_o_bytes(const gdn_window_attn_args& a, int splits) {
@@ -86,17 +87,20 @@ uint64_t workspace_of(const gdn_window_attn_args& a) {
     return splits <= 1 ? 0 : part_o_bytes(a, splits) + (uint64_t)splits * a.B * a.T * a.H * 8;
 }
 
-// The parts in which rows beyond the window are shared out for a sequence's first keys: about two workgroups a compute unit in all.
+// The parts in which rows beyond the window are shared out for a sequence's first keys: about one workgroup a compute unit in all, 256 rows or
+// more to each.
 int pieces_of(const WindowParams& p, int dtype) {
     if (dtype != GDN_BF16 || p.sinks == 0) return 0;
-    const int64_t blocks = (int64_t)p.N * p.HK * ((p.sinks + WINDOW_KEYS - 1) / WINDOW_KEYS), rows = (int64_t)p.T * p.G;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * compute_units() / blocks, (rows + 511) / 512));
+    const int64_t blocks = (int64_t)p.N * p.HK * ((p.sinks + WINDOW_FIRST_KEYS - 1) / WINDOW_FIRST_KEYS), rows = (int64_t)p.T * p.G;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(compute_units() / blocks, (rows + 255) / 256));
 }
-int first_keys_of(const WindowParams& p) { return (p.sinks + WINDOW_KEYS - 1) / WINDOW_KEYS * WINDOW_KEYS; }
+int first_keys_of(const WindowParams& p) { return (p.sinks + WINDOW_FIRST_KEYS - 1) / WINDOW_FIRST_KEYS * WINDOW_FIRST_KEYS; }
 
 uint64_t delta_bytes(const gdn_window_attn_args& a) { return ((uint64_t)a.B * a.T * a.H * 4 + 255) / 256 * 256; }
 uint64_t backward_bytes(const gdn_window_attn_args& a, const WindowParams& p) {
-    return delta_bytes(a) + (uint64_t)p.N * p.HK * pieces_of(p, a.dtype) * first_keys_of(p) * 2 * p.D * 4;
+    const int pieces = pieces_of(p, a.dtype);
+    if (pieces == 0) return delta_bytes(a);
+    return delta_bytes(a) + (uint64_t)p.N * p.HK * (pieces + 1) * first_keys_of(p) * 2 * p.D * 4;
 }
 
 }  // namespace

@@ -38,7 +38,7 @@ struct WindowParams {
     float* part_m;    // [splits, B, HK, rows, 2]: reference exponent, sum
     // gradients of a sequence's first keys from rows that see them beyond the window, in `pieces` parts per sequence
     int pieces, first_keys;  // first_keys: sinks, in whole blocks
-    float* part_dk;   // [N, HK, pieces, first_keys, 2, D]
+    float* part_dk;   // [N, HK, pieces + 1, first_keys, 2, D]; the last part is from the rows that have them in their window
 };
 
 // n / G and the rest, for n < 2^16
@@ -72,6 +72,13 @@ __device__ __forceinline__ void sequence_at(const WindowParams& p, int b, int at
     if (at < st || at >= en) en = st;
 }
 
+// sequence n's first position and length
+__device__ __forceinline__ void sequence_of(const WindowParams& p, int n, int& st, int& len) {
+    if (p.cu == nullptr) st = 0, len = p.S;
+    else if (p.padded) len = min(max(p.cu[n + 1] - p.cu[n], 0), p.S), st = p.S - len;
+    else packed_bounds(p.cu, n, p.S, st, len);
+}
+
 // What a row sees: keys [lo, a] and [st, sk); a < lo: none.
 struct RowView {
     int a, lo, st, sk;
@@ -94,11 +101,15 @@ __device__ __forceinline__ int wave_min(int x) {
 }
 __device__ __forceinline__ int wave_max(int x) { return -wave_min(-x); }
 
-// Whether the row sees key j, of a tile of the keys near it, or of one of the first keys (which ends at `sink_end`, where the near ones begin).
+// The keys of a tile that a row sees: an interval of the keys near it, or of the first keys (which end at `sink_end`, where the near ones
+// begin); where first keys lie among near ones (`mixed`, the same for the workgroup) also those.
 struct TileView {
-    int a, lo, st, sk;
-    __device__ __forceinline__ TileView(const RowView& v, bool near, int sink_end) : a(v.a), lo(near ? v.lo : 1 << 30), st(v.st), sk(near ? v.sk : min(v.sk, sink_end)) {}
-    __device__ __forceinline__ bool sees(int j) const { return j <= a && (j >= lo || (j >= st && j < sk)); }
+    int from, st;
+    unsigned span, first;
+    __device__ __forceinline__ TileView(const RowView& v, bool near, int sink_end)
+        : from(near ? v.lo : v.st), st(v.st), span(near ? max(v.a + 1 - v.lo, 0) : max(min(v.sk, sink_end) - v.st, 0)), first(max(v.sk - v.st, 0)) {}
+    __device__ __forceinline__ bool sees(int j) const { return (unsigned)(j - from) < span; }
+    __device__ __forceinline__ bool sees_mixed(int j) const { return sees(j) || (unsigned)(j - st) < first; }
 };
 
 // What a wave's rows see: keys from [lo, end) and [sink, sink_end), all of them those of [full_lo, full_end).
@@ -146,16 +157,16 @@ __device__ __forceinline__ bool work_item(const WindowParams& p, int x, int& pai
     return true;
 }
 
-// A tile of 64 rows of DP columns on its way into LDS, without registers in between: a wave's instruction fills 1 KB, the lanes' 16 bytes
+// A tile of rows of DP columns (WROWS a wave) on its way into LDS, without registers in between: a wave's instruction fills 1 KB, the lanes' 16 bytes
 // one behind the other, so the granules are swapped (tile_key) where they are read.  What lies past the rows or columns that there are is
 // read past the buffer's end, which gives zeros.
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 constexpr uint32_t PAST = 0x80000000u;
-template <int DP>
+template <int DP, int WROWS = 16>
 struct TileLoads {
-    static constexpr int GRANULES = DP / 8, RPI = 64 / GRANULES, ITERS = 16 / RPI;
-    static_assert(GRANULES <= 64 && 16 % RPI == 0, "a wave loads 16 rows");
-    static __device__ __forceinline__ int row(int wave, int lane, int i) { return 16 * wave + RPI * i + lane / GRANULES; }
+    static constexpr int GRANULES = DP / 8, RPI = 64 / GRANULES, ITERS = WROWS / RPI;
+    static_assert(GRANULES <= 64 && WROWS % RPI == 0, "a wave loads WROWS rows");
+    static __device__ __forceinline__ int row(int wave, int lane, int i) { return WROWS * wave + RPI * i + lane / GRANULES; }
     static __device__ __forceinline__ int column(int wave, int lane, int i) { return 8 * (lane % GRANULES ^ tile_key<DP>(row(wave, lane, i))); }
     // `to`: LDS address of the tile; offset in bytes from `base`
     static __device__ __forceinline__ void load(const void* base, uint32_t offset, uint32_t to, int wave, int i) {
@@ -163,7 +174,7 @@ struct TileLoads {
         i32x4 r;
         r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)a), r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32) & 0xffff);
         r[2] = (int)PAST, r[3] = 0x00020000;
-        const int at = __builtin_amdgcn_readfirstlane((int)(to + (16 * wave + RPI * i) * DP * 2));
+        const int at = __builtin_amdgcn_readfirstlane((int)(to + (WROWS * wave + RPI * i) * DP * 2));
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(offset), "s"(r) : "memory");
     }
 };
@@ -181,6 +192,8 @@ struct TileReader {
         pair = r * DP + (((c >> 3) ^ tile_key<DP>(r)) << 3) + (c & 7);
     }
     static constexpr int PERIOD = TileLane<DP>::PERIOD;
+    // x where it is used, rather than what follows from x in registers over a whole walk
+    __device__ __forceinline__ void recompute() { asm volatile("" : "+v"(row), "+v"(pair)); }
     // columns 16 s + 8 half .. + 7 of row row0 + (lane & 31); row0 a multiple of 32
     __device__ __forceinline__ bf16x8 across(const bf16_t* tile, int row0, int s) const {
         return *reinterpret_cast<const bf16x8*>(tile + (row ^ (16 * s % PERIOD)) + row0 * DP + 16 * s / PERIOD * PERIOD);
@@ -272,7 +285,8 @@ int launch_window_fwd_f32(const WindowParams& p, hipStream_t stream);       // g
 int launch_window_bwd_f32(const WindowParams& p, hipStream_t stream);
 int launch_window_combine(const WindowParams& p, int dtype, hipStream_t stream);
 constexpr int WINDOW_ROWS = 128;      // of a workgroup, bf16
-constexpr int WINDOW_KEYS = 128;      // of a workgroup of the keys' gradients, bf16
+constexpr int window_keys(int D) { return D <= 128 ? 128 : 64; }  // of a workgroup of the keys' gradients, bf16
+constexpr int WINDOW_FIRST_KEYS = 32;  // of a workgroup of a sequence's first keys
 constexpr int WINDOW_ROWS_F32 = 64;
 constexpr int WINDOW_KEYS_F32 = 64;
 

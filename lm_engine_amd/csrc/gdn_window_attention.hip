@@ -7,6 +7,7 @@
 // to fp32 sums, and bf16 rounds relative to the weight), so that the outputs are seldom rescaled.
 #include <algorithm>
 
+#include "gdn_join.h"
 #include "gdn_launch.h"
 #include "gdn_window_attention.h"
 
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_fwd_kernel(cons
     const TileReader<DP> reader(lane);
     f32x16 o[DT] = {};
     float m = LOWEST, l = 0.f;
-    bool taken_out = false;
+    bool careful = false, taken_out = false;
     if (first_tile < last_tile) load_tile(first_tile);
     for (int i = first_tile; i < last_tile; i++) {
         loads_done();
@@ -96,9 +97,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_fwd_kernel(cons
         tile_at(i, j0, count);
         const bf16_t *const kt = tiles[i & 1][0], *const vt = tiles[i & 1][1];
         const bool near = i >= sink_tiles, full = near && j0 >= w.full_lo && j0 + 64 <= w.full_end;
-        // A tile that some row does not see all of: 0 times a value that is not finite must not reach that row.  Such values are taken
-        // out here, and go to the rows that see them in the end.
-        if (!near || j0 < all.full_lo || j0 + 64 > all.full_end) {
+        if (careful && !(near && j0 >= all.full_lo && j0 + 64 <= all.full_end)) {
             bf16x8* const v8 = reinterpret_cast<bf16x8*>(tiles[i & 1][1]);
             bool found = false;
 #pragma unroll
@@ -121,13 +120,17 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_fwd_kernel(cons
             if (!full) {
                 const TileView own(view, near, sink_end);
                 c = 1.f;
+                if (!(near && j0 < all.sink_end)) {
 #pragma unroll
-                for (int x = 0; x < 2; x++)
+                    for (int x = 0; x < 2; x++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int j = j0 + 32 * x + acc_row(e, half);
-                        s[x][e] = own.sees(j) ? s[x][e] * p.c : -__builtin_inff();
-                    }
+                        for (int e = 0; e < 16; e++) s[x][e] = own.sees(j0 + 32 * x + acc_row(e, half)) ? s[x][e] * p.c : -__builtin_inff();
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) s[x][e] = own.sees_mixed(j0 + 32 * x + acc_row(e, half)) ? s[x][e] * p.c : -__builtin_inff();
+                }
             }
             float top = s[0][0];
 #pragma unroll
@@ -158,6 +161,22 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_fwd_kernel(cons
                 for (int x = 0; x < DT; x++) o[x] = mma(reader.down(vt, y, x), weights, o[x]);
             }
         }
+        if (i + 1 == last_tile && !careful) {
+            // 0 times a value that is not finite must not reach the rows that do not see it.  Where a result is not finite, the walk is
+            // taken once more, without such values in tiles that some row does not see all of; they go to the rows that see them in the end.
+            float zero = 0.f;
+#pragma unroll
+            for (int x = 0; x < DT; x++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) zero = __builtin_fmaf(o[x][e], 0.f, zero);
+            if (__syncthreads_or(zero != 0.f)) {
+                careful = true, m = LOWEST, l = 0.f;
+#pragma unroll
+                for (int x = 0; x < DT; x++) o[x] = f32x16{};
+                load_tile(first_tile);
+                i = first_tile - 1;
+            }
+        }
     }
 
     l += other_half(l);
@@ -184,32 +203,22 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_fwd_kernel(cons
     add_taken_out<bf16_t>(p, b, hk, r0, WINDOW_ROWS, all, first_tile, last_tile, sink_tiles, tile_at, part);
 }
 
-// The parts of a row joined: a wave a row.
+// The parts of a row joined: a workgroup a row.
 template <typename T>
 __global__ __launch_bounds__(256) void window_combine_kernel(const WindowParams p) {
-    const int64_t all = (int64_t)p.B * p.HK * p.rows, at = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;
-    const int lane = threadIdx.x % WAVE;
-    if (at >= all) return;
-    float m = LOWEST;
-    for (int s = 0; s < p.splits; s++) m = fmaxf(m, p.part_m[2 * (s * all + at)]);
-    float l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.splits; s++) {
-        const int64_t part = s * all + at;
-        const float weight = __builtin_amdgcn_exp2f(p.part_m[2 * part] - m);
-        l += weight * p.part_m[2 * part + 1];
-        if (4 * lane < p.D) o += *reinterpret_cast<const f32x4*>(p.part_o + part * p.D + 4 * lane) * weight;
-    }
+    const int64_t at = blockIdx.x;
+    float m, l;
+    f32x4 o;
+    int col;
+    if (!join_row(p.part_o, p.part_m, (int64_t)p.B * p.HK * p.rows, at, p.splits, p.D, m, l, o, col)) return;
     const int64_t pair = at / p.rows;
     const int r = (int)(at - pair * p.rows), b = (int)(pair / p.HK), hk = (int)(pair - (int64_t)b * p.HK), t = r / p.G, g = r - t * p.G;
-    if (p.lse != nullptr && lane == 0) {
+    if (p.lse != nullptr && col == 0) {
         const int64_t head = ((int64_t)b * p.T + t) * p.H + hk * p.G + g;
         if constexpr (sizeof(T) == 2) p.lse[head] = l == 0.f ? __builtin_inff() : m + log2f(l);
         else p.lse[2 * head] = l == 0.f ? 0.f : m, p.lse[2 * head + 1] = l == 0.f ? 0.f : 1.f / l;
     }
-    if (4 * lane >= p.D) return;
-    T* const to = static_cast<T*>(const_cast<void*>(p.o.p)) + b * p.o.b + t * p.o.t + (hk * p.G + g) * p.o.h;
-    store4<T>(to + 4 * lane, o * (l == 0.f ? 0.f : 1.f / l));
+    store4<T>(static_cast<T*>(const_cast<void*>(p.o.p)) + b * p.o.b + t * p.o.t + (hk * p.G + g) * p.o.h + col, o * (l == 0.f ? 0.f : 1.f / l));
 }
 
 }  // namespace
@@ -225,7 +234,7 @@ int launch_window_fwd(const WindowParams& p, hipStream_t stream) {
 }
 
 int launch_window_combine(const WindowParams& p, int dtype, hipStream_t stream) {
-    const dim3 grid((unsigned)(((int64_t)p.B * p.HK * p.rows + 3) / 4));
+    const dim3 grid((unsigned)((int64_t)p.B * p.HK * p.rows));
     if (dtype == GDN_BF16) hipLaunchKernelGGL((window_combine_kernel<bf16_t>), grid, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((window_combine_kernel<float>), grid, dim3(256), 0, stream, p);
     return (int)hipGetLastError();

@@ -4,8 +4,8 @@
 // window_dq_kernel goes over the keys of 128 rows, as the forward does, window_dkv_kernel over the rows of 128 keys (of all heads that share
 // them).  Scores are formed the way round that makes them operands as they lie: with a lane a row (S^T = K Q^T) for dq^T += K^T ds^T,
 // with a lane a key (S = Q K^T) for dv^T += do^T w and dk^T += q^T ds.
-// A sequence's first keys are seen by all of its rows: those beyond the window are shared out over many workgroups (window_first_keys, the
-// same walk), whose parts the keys' own workgroup adds to its sums.
+// A sequence's first keys are seen by all of its rows: those beyond the window are shared out over many workgroups, in a launch of their own, and
+// the parts joined by another.
 #include <algorithm>
 
 #include "gdn_launch.h"
@@ -98,10 +98,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dq_kernel(const
 #pragma unroll
             for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -lse)) * (dw[e] - delta);
             if (!full) {
+                if (!(near && j0 < all.sink_end)) {
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int j = j0 + 32 * x + acc_row(e, half);
-                    if (!own.sees(j)) s[e] = 0.f;
+                    for (int e = 0; e < 16; e++) s[e] = own.sees(j0 + 32 * x + acc_row(e, half)) ? s[e] : 0.f;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s[e] = own.sees_mixed(j0 + 32 * x + acc_row(e, half)) ? s[e] : 0.f;
                 }
             }
 #pragma unroll
@@ -116,20 +118,28 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dq_kernel(const
     store_transposed<DP>(static_cast<bf16_t*>(const_cast<void*>(p.dq.p)) + b * p.dq.b + t * p.dq.t + head * p.dq.h, p.D, half, dq, p.scale);
 }
 
-// Gradients of 128 keys, 32 to a wave.  FIRST: of the keys of a sequence that all of its rows see, from one part of the rows that do
-// not have them in their window; blockIdx.x goes over (sequence, head of k and v, block of 128 such keys, part).
+// Gradients of KEYS keys.  The keys and values lie in LDS for the whole walk, so that a wave's registers are its sums': two waves on a SIMD, one
+// of which has products to do while the other waits (with keys and values in registers, and one wave, the walk took 560 us instead of XXX).
+// A wave has 32 keys and 32 rows of each tile; the waves that share keys add up at the end.  Above 128 columns, where the sums of both
+// gradients would not fit into its registers, a wave has one of them, and scores are formed twice (ROLES 2).
+// Not FIRST: all keys, and the rows that have them in their window; 128 keys (64) and tiles of 64 rows (32), the next one on its way.
+// FIRST: the keys of a sequence that all of its rows see, 32 of them, and of those rows that do not have them in their window one part, in tiles of
+// 256 rows (64): (sequence, head of k and v, block of such keys, part).  Both leave their sums for such keys to window_first_keys_kernel.
 template <int DP, bool FIRST>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void window_dkv_kernel(const WindowParams p) {
-    constexpr int KS = DP / 16, DT = DP / 32;
-    using Loads = TileLoads<DP>;
-    __shared__ __attribute__((aligned(1024))) bf16_t tiles[2][2][64 * DP];
-    __shared__ __attribute__((aligned(16))) float row_lse[2][64], row_delta[2][64];
-    __shared__ __attribute__((aligned(16))) int row_at[2][64];
+__global__ __launch_bounds__(DP <= 128 ? 512 : 256, DP <= 128 ? 2 : 1) void window_dkv_kernel(const WindowParams p) {
+    constexpr int KS = DP / 16, DT = DP / 32, KEYS = FIRST ? WINDOW_FIRST_KEYS : window_keys(DP), ROLES = DP <= 128 ? 1 : 2, WAVES = DP <= 128 ? 8 : 4;
+    constexpr int KEY_WAVES = KEYS / 32, ROW_WAVES = WAVES / ROLES / KEY_WAVES, ROWS = 32 * ROW_WAVES, BUFFERS = FIRST ? 1 : 2;
+    using Loads = TileLoads<DP, ROWS / WAVES>;
+    using KeyLoads = TileLoads<DP, 16>;
+    __shared__ __attribute__((aligned(1024))) bf16_t lds_tiles[2 * KEYS * DP + BUFFERS * 2 * ROWS * DP];  // keys, values; rows of q, of do
+    __shared__ __attribute__((aligned(16))) float row_lse[BUFFERS][ROWS], row_delta[BUFFERS][ROWS];
+    __shared__ __attribute__((aligned(16))) int row_at[BUFFERS][ROWS];
+    __shared__ int bounds[WAVES][6];
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), half = lane >> 5;
-    int b, hk, n = 0, piece = 0, key0, keys;  // key0: of the workgroup
-    int64_t slot = 0;
+    const int key_wave = wave % KEY_WAVES, row_wave = wave / KEY_WAVES % ROW_WAVES, role = wave / KEY_WAVES / ROW_WAVES;  // role 0: dk (and dv), 1: dv
+    int b, hk, n = 0, piece = p.pieces, key0, keys;  // key0: of the workgroup
     if constexpr (FIRST) {
-        const int key_blocks = p.first_keys / WINDOW_KEYS;
+        const int key_blocks = p.first_keys / KEYS;
         int x = blockIdx.x;
         piece = x % p.pieces, x /= p.pieces;
         const int kblock = x % key_blocks;
@@ -137,64 +147,65 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void window_dkv_kernel(const
         hk = x % p.HK, n = x / p.HK;
         b = p.cu != nullptr && !p.padded ? 0 : n;
         int st, len;
-        if (p.cu == nullptr) st = 0, len = p.S;
-        else if (p.padded) len = min(max(p.cu[n + 1] - p.cu[n], 0), p.S), st = p.S - len;
-        else packed_bounds(p.cu, n, p.S, st, len);
-        key0 = st + kblock * WINDOW_KEYS, keys = min(WINDOW_KEYS, min(p.sinks, len) - kblock * WINDOW_KEYS);
-        slot = (((int64_t)n * p.HK + hk) * p.pieces + piece) * p.first_keys + kblock * WINDOW_KEYS;
+        sequence_of(p, n, st, len);
+        key0 = st + kblock * KEYS, keys = min(KEYS, min(p.sinks, len) - kblock * KEYS);
     } else {
         int pair, block;
         if (!work_item(p, blockIdx.x, pair, block)) return;
         b = pair / p.HK, hk = pair - b * p.HK;
-        key0 = block * WINDOW_KEYS, keys = min(WINDOW_KEYS, p.S - key0);
+        key0 = block * KEYS, keys = min(KEYS, p.S - key0);
     }
     // this lane's key, and the positions that see it: [from, upto]
-    const int own = 32 * wave + (lane & 31), j = key0 + own;
-    int st = 0, en = 0, sequence = 0, from = 1 << 30, upto = -1;
+    const int own = 32 * key_wave + (lane & 31), j = key0 + own;
+    int st = 0, en = 0, from = 1 << 30, upto = -1;
     if (own < keys) {
+        int sequence;
         sequence_at(p, b, j, st, en, sequence);
+        if (!FIRST) n = sequence;
         if (en > st) {
-            const bool first = j - st < p.sinks;
-            if constexpr (FIRST) from = p.window < en - j ? j + p.window : 1 << 30, upto = from < en ? en - 1 : -1;
-            else from = j, upto = p.window == 0 || p.window >= en - j || (first && p.pieces == 0) ? en - 1 : j + p.window - 1;
+            if (FIRST) from = p.window < en - j ? j + p.window : 1 << 30, upto = from < en ? en - 1 : -1;
+            else from = j, upto = p.window == 0 || p.window >= en - j ? en - 1 : j + p.window - 1;
             from = max(from, p.S - p.T);  // (positions in front of the queries)
             if (upto < from) from = 1 << 30, upto = -1;
         }
     }
     WaveView w;
-    w.lo = wave_min(from), w.end = wave_max(upto) + 1, w.full_lo = wave_max(from), w.full_end = upto < 0 ? 0 : upto + 1;
-    w.full_end = wave_min(w.full_end), w.sink = w.sink_end = 0;
-    __shared__ int bounds[4][6];
-    const WaveView all = join_waves<4>(w, bounds, wave, lane);
+    w.lo = wave_min(from), w.end = wave_max(upto) + 1, w.full_lo = wave_max(from), w.full_end = wave_min(upto) + 1, w.sink = w.sink_end = 0;
+    const WaveView all = join_waves<WAVES>(w, bounds, wave, lane);
     const int offset = p.S - p.T;
     int a0 = all.lo, a1 = all.end;  // positions whose rows are walked over
     if (a1 <= a0) a0 = a1 = offset;
     if constexpr (FIRST) {
-        const int each = (int)(((int64_t)a1 - a0 + p.pieces - 1) / p.pieces);
-        const int64_t begin = a0 + (int64_t)piece * each;
-        a1 = (int)min((int64_t)a1, begin + each), a0 = (int)min((int64_t)a1, begin);
+        const int each = (a1 - a0 + p.pieces - 1) / p.pieces;
+        a0 = min(a1, a0 + piece * each), a1 = min(a1, a0 + each);
     }
     const int r0 = (a0 - offset) * p.G, r1 = (a1 - offset) * p.G;
-    const int tile_count = (r1 - r0 + 63) / 64;
-
-    bf16x8 k[KS], v[KS];
-    {
-        const bool there = own < keys;
-        const int at = there ? j : key0 < p.S ? key0 : 0;
-        load_row_fragments<DP>(static_cast<const bf16_t*>(p.k.p) + b * p.k.b + at * p.k.t + hk * p.k.h, p.D, half, there, k);
-        load_row_fragments<DP>(static_cast<const bf16_t*>(p.v.p) + b * p.v.b + at * p.v.t + hk * p.v.h, p.D, half, there, v);
-    }
+    const int tile_count = (r1 - r0 + ROWS - 1) / ROWS;
 
     const char* const qb = reinterpret_cast<const char*>(static_cast<const bf16_t*>(p.q.p) + b * p.q.b + hk * p.G * p.q.h);
     const char* const db = reinterpret_cast<const char*>(static_cast<const bf16_t*>(p.dout.p) + b * p.dout.b + hk * p.G * p.dout.h);
-    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&tiles[0][0][0];
+    bf16_t *const kt = lds_tiles, *const vt = kt + KEYS * DP, *const rows = vt + KEYS * DP;
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&lds_tiles[0];
+    {
+        const char* const k0 = reinterpret_cast<const char*>(static_cast<const bf16_t*>(p.k.p) + b * p.k.b + hk * p.k.h + (keys > 0 ? key0 : 0) * p.k.t);
+        const char* const v0 = reinterpret_cast<const char*>(static_cast<const bf16_t*>(p.v.p) + b * p.v.b + hk * p.v.h + (keys > 0 ? key0 : 0) * p.v.t);
+        if (wave < KEYS / 16) {
+#pragma unroll
+            for (int x = 0; x < KeyLoads::ITERS; x++) {
+                const int kr = KeyLoads::row(wave, lane, x), col = KeyLoads::column(wave, lane, x);
+                const bool there = kr < keys && col < p.D;
+                KeyLoads::load(k0, there ? (uint32_t)(kr * (int)p.k.t + col) * 2 : PAST, lds, wave, x);
+                KeyLoads::load(v0, there ? (uint32_t)(kr * (int)p.v.t + col) * 2 : PAST, lds + KEYS * DP * 2, wave, x);
+            }
+        }
+    }
     float lse_next = 0.f, delta_next = 0.f;
     int at_next = 0;
     auto load_tile = [&](int i) {
-        const int first = r0 + 64 * i, count = min(64, r1 - first);
+        const int first = r0 + ROWS * i, count = min(ROWS, r1 - first);
         const int t0 = p.G == 1 ? first : first / p.G, g0 = first - t0 * p.G;
         const char *const q0 = qb + (int64_t)t0 * p.q.t * 2, *const d0 = db + (int64_t)t0 * p.dout.t * 2;
-        const uint32_t to = lds + (i & 1) * 2 * 64 * DP * 2;
+        const uint32_t to = lds + (2 * KEYS + (i % BUFFERS) * 2 * ROWS) * DP * 2;
 #pragma unroll
         for (int x = 0; x < Loads::ITERS; x++) {
             const int rr = Loads::row(wave, lane, x), col = Loads::column(wave, lane, x);
@@ -202,116 +213,187 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void window_dkv_kernel(const
             split_rows(p, g0 + rr, tt, g);
             const bool there = rr < count && col < p.D;
             Loads::load(q0, there ? (uint32_t)(tt * (int)p.q.t + g * (int)p.q.h + col) * 2 : PAST, to, wave, x);
-            Loads::load(d0, there ? (uint32_t)(tt * (int)p.dout.t + g * (int)p.dout.h + col) * 2 : PAST, to + 64 * DP * 2, wave, x);
+            Loads::load(d0, there ? (uint32_t)(tt * (int)p.dout.t + g * (int)p.dout.h + col) * 2 : PAST, to + ROWS * DP * 2, wave, x);
         }
-        if (wave == 0) {
+        if (threadIdx.x < ROWS) {
             int tt, g;
-            split_rows(p, g0 + lane, tt, g);
-            const bool there = lane < count;
+            split_rows(p, g0 + (int)threadIdx.x, tt, g);
+            const bool there = (int)threadIdx.x < count;
             const int64_t scalar = ((int64_t)b * p.T + t0 + (there ? tt : 0)) * p.H + hk * p.G + (there ? g : 0);
             lse_next = there ? p.lse[scalar] : __builtin_inff(), delta_next = there ? p.delta[scalar] : 0.f;
             at_next = there ? t0 + tt + offset : -1;
         }
     };
-    auto stage_scalars = [&](int i) {
-        if (wave == 0) row_lse[i & 1][lane] = lse_next, row_delta[i & 1][lane] = delta_next, row_at[i & 1][lane] = at_next;
-    };
 
-    const TileReader<DP> reader(lane);
+    TileReader<DP> reader(lane);
     const float c = p.negative ? -p.c : p.c;
-    f32x16 dk[DT] = {}, dv[DT] = {};
-    if (tile_count > 0) load_tile(0);
-    for (int i = 0; i < tile_count; i++) {
-        loads_done();
-        stage_scalars(i);
-        __syncthreads();
-        if (i + 1 < tile_count) load_tile(i + 1);
-        const int first = r0 + 64 * i, count = min(64, r1 - first);
-        const int p0 = (p.G == 1 ? first : first / p.G) + offset, p1 = (p.G == 1 ? first + count - 1 : (first + count - 1) / p.G) + offset;  // positions
-        if (!(p0 < w.end && p1 >= w.lo)) continue;
-        const bool full = p0 >= w.full_lo && p1 < w.full_end && count == 64;
-        const bf16_t *const qt = tiles[i & 1][0], *const dt = tiles[i & 1][1];
+    f32x16 dk[DT] = {}, dv[ROLES == 1 ? DT : 1] = {};  // (two roles: dk is the one gradient that there is)
+    // `full`: every row of the tile sees every key of the wave
+    auto add_tile = [&](int i, bool full) {
+        reader.recompute();
+        const bf16_t *const qt = rows + (i % BUFFERS) * 2 * ROWS * DP, *const dt = qt + ROWS * DP;
+        const int at0 = 32 * row_wave + 4 * half;
+        const bf16_t *const qx = qt + 32 * row_wave * DP, *const dx = dt + 32 * row_wave * DP;
+        f32x16 s = {}, dw = {};
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-            f32x16 s = {}, dw = {};
+        for (int y = 0; y < KS; y++) s = mma(reader.across(qx, 0, y), reader.across(kt + 32 * key_wave * DP, 0, y), s);
+        if (ROLES == 1 || role == 0) {
 #pragma unroll
-            for (int y = 0; y < KS; y++) s = mma(reader.across(qt, 32 * x, y), k[y], s);
+            for (int y = 0; y < KS; y++) dw = mma(reader.across(dx, 0, y), reader.across(vt + 32 * key_wave * DP, 0, y), dw);
+        }
 #pragma unroll
-            for (int y = 0; y < KS; y++) dw = mma(reader.across(dt, 32 * x, y), v[y], dw);
+        for (int y = 0; y < 4; y++) {
+            const f32x4 lse = *reinterpret_cast<const f32x4*>(&row_lse[i % BUFFERS][at0 + 8 * y]);
+            const f32x4 delta = *reinterpret_cast<const f32x4*>(&row_delta[i % BUFFERS][at0 + 8 * y]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                s[4 * y + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * y + e], c, -lse[e]));
+                dw[4 * y + e] = s[4 * y + e] * (dw[4 * y + e] - delta[e]);
+            }
+        }
+        if (!full) {
 #pragma unroll
             for (int y = 0; y < 4; y++) {
-                const f32x4 lse = *reinterpret_cast<const f32x4*>(&row_lse[i & 1][32 * x + 8 * y + 4 * half]);
-                const f32x4 delta = *reinterpret_cast<const f32x4*>(&row_delta[i & 1][32 * x + 8 * y + 4 * half]);
+                const i32x4 at = *reinterpret_cast<const i32x4*>(&row_at[i % BUFFERS][at0 + 8 * y]);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float weight = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * y + e], c, -lse[e]));
-                    dw[4 * y + e] = weight * (dw[4 * y + e] - delta[e]);
-                    s[4 * y + e] = weight;
-                }
-                if (!full) {
-                    const i32x4 at = *reinterpret_cast<const i32x4*>(&row_at[i & 1][32 * x + 8 * y + 4 * half]);
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (at[e] < from || at[e] > upto) s[4 * y + e] = dw[4 * y + e] = 0.f;
-                }
+                for (int e = 0; e < 4; e++)
+                    if (at[e] < from || at[e] > upto) s[4 * y + e] = dw[4 * y + e] = 0.f;
             }
+        }
+        if constexpr (ROLES == 1) {
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 const bf16x8 weights = pack8(s, y), ds = pack8(dw, y);
 #pragma unroll
-                for (int z = 0; z < DT; z++) dv[z] = mma(reader.down(dt, 2 * x + y, z), weights, dv[z]);
+                for (int z = 0; z < DT; z++) dv[z] = mma(reader.down(dx, y, z), weights, dv[z]);
 #pragma unroll
-                for (int z = 0; z < DT; z++) dk[z] = mma(reader.down(qt, 2 * x + y, z), ds, dk[z]);
+                for (int z = 0; z < DT; z++) dk[z] = mma(reader.down(qx, y, z), ds, dk[z]);
+            }
+        } else {
+            const bf16_t* const from_rows = role == 0 ? qx : dx;
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                const bf16x8 by = role == 0 ? pack8(dw, y) : pack8(s, y);
+#pragma unroll
+                for (int z = 0; z < DT; z++) dk[z] = mma(reader.down(from_rows, y, z), by, dk[z]);
             }
         }
+    };
+    if (tile_count > 0) load_tile(0);
+    for (int i = 0; i < tile_count; i++) {
+        loads_done();
+        if (threadIdx.x < ROWS) row_lse[i % BUFFERS][threadIdx.x] = lse_next, row_delta[i % BUFFERS][threadIdx.x] = delta_next, row_at[i % BUFFERS][threadIdx.x] = at_next;
+        __syncthreads();
+        if (BUFFERS == 2 && i + 1 < tile_count) load_tile(i + 1);
+        const int first = r0 + ROWS * i, count = min(ROWS, r1 - first);
+        const int p0 = (p.G == 1 ? first : first / p.G) + offset, p1 = (p.G == 1 ? first + count - 1 : (first + count - 1) / p.G) + offset;  // positions
+        if (p0 < w.end && p1 >= w.lo) add_tile(i, p0 >= w.full_lo && p1 < w.full_end && count == ROWS);
+        if (BUFFERS == 1 && i + 1 < tile_count) {
+            __syncthreads();
+            load_tile(i + 1);
+        }
     }
-    if constexpr (FIRST) {
-        if (own >= keys) return;
-        float* const to = p.part_dk + (slot + own) * 2 * p.D;
+    // the waves that share keys, half of them to the other half
+    if constexpr (ROW_WAVES > 1) {
+        constexpr int TENSORS = ROLES == 1 ? 2 : 1, PIECES = TENSORS * DT * 4;  // f32x4 of a lane
+        static_assert(ROW_WAVES / 2 * KEY_WAVES * ROLES * PIECES * 64 * 16 <= sizeof(lds_tiles), "the sums fit");
+        loads_done();
+#pragma unroll
+        for (int h = ROW_WAVES / 2; h >= 1; h /= 2) {
+            f32x4* const shared = reinterpret_cast<f32x4*>(lds_tiles) + ((row_wave % h) * KEY_WAVES * ROLES + role * KEY_WAVES + key_wave) * PIECES * 64 + lane;
+            __syncthreads();
+            if (row_wave >= h && row_wave < 2 * h) {
+#pragma unroll
+                for (int z = 0; z < DT; z++)
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        shared[(4 * z + y) * 64] = f32x4{dk[z][4 * y], dk[z][4 * y + 1], dk[z][4 * y + 2], dk[z][4 * y + 3]};
+                        if constexpr (ROLES == 1) shared[(4 * (DT + z) + y) * 64] = f32x4{dv[z][4 * y], dv[z][4 * y + 1], dv[z][4 * y + 2], dv[z][4 * y + 3]};
+                    }
+            }
+            __syncthreads();
+            if (row_wave < h) {
+#pragma unroll
+                for (int z = 0; z < DT; z++)
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        const f32x4 a = shared[(4 * z + y) * 64];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) dk[z][4 * y + e] += a[e];
+                        if constexpr (ROLES == 1) {
+                            const f32x4 d = shared[(4 * (DT + z) + y) * 64];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) dv[z][4 * y + e] += d[e];
+                        }
+                    }
+            }
+        }
+        if (row_wave > 0) return;
+    }
+    if (own >= keys) return;
+    const bool to_parts = p.pieces > 0 && en > st && j - st < p.sinks;
+    float* const part = p.part_dk + (to_parts ? ((((int64_t)n * p.HK + hk) * (p.pieces + 1) + piece) * p.first_keys + (j - st)) * 2 * p.D : 0);
+    auto leave = [&](const f32x16 (&sums)[DT], bool value) {
+        const WindowRows& out = value ? p.dv : p.dk;
+        if (!to_parts && !FIRST) store_transposed<DP>(static_cast<bf16_t*>(const_cast<void*>(out.p)) + b * out.b + j * out.t + hk * out.h, p.D, half, sums, value ? 1.f : p.scale);
+        if (!to_parts) return;
 #pragma unroll
         for (int z = 0; z < DT; z++)
 #pragma unroll
             for (int y = 0; y < 4; y++) {
                 const int col = 32 * z + 8 * y + 4 * half;
-                if (col >= p.D) continue;
-                *reinterpret_cast<f32x4*>(to + col) = f32x4{dk[z][4 * y], dk[z][4 * y + 1], dk[z][4 * y + 2], dk[z][4 * y + 3]};
-                *reinterpret_cast<f32x4*>(to + p.D + col) = f32x4{dv[z][4 * y], dv[z][4 * y + 1], dv[z][4 * y + 2], dv[z][4 * y + 3]};
+                if (col < p.D) *reinterpret_cast<f32x4*>(part + (value ? p.D : 0) + col) = f32x4{sums[z][4 * y], sums[z][4 * y + 1], sums[z][4 * y + 2], sums[z][4 * y + 3]};
             }
+    };
+    if constexpr (ROLES == 1) {
+        leave(dk, false);
+        leave(dv, true);
     } else {
-        if (own >= keys) return;
-        if (p.pieces > 0 && en > st && j - st < p.sinks) {
-            const float* const parts = p.part_dk + ((((int64_t)sequence * p.HK + hk) * p.pieces) * p.first_keys + (j - st)) * 2 * p.D;
-            for (int x = 0; x < p.pieces; x++) {
-                const float* const part = parts + (int64_t)x * p.first_keys * 2 * p.D;
-#pragma unroll
-                for (int z = 0; z < DT; z++)
-#pragma unroll
-                    for (int y = 0; y < 4; y++) {
-                        const int col = 32 * z + 8 * y + 4 * half;
-                        if (col >= p.D) continue;
-                        const f32x4 a = *reinterpret_cast<const f32x4*>(part + col), d = *reinterpret_cast<const f32x4*>(part + p.D + col);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) dk[z][4 * y + e] += a[e], dv[z][4 * y + e] += d[e];
-                    }
-            }
-        }
-        store_transposed<DP>(static_cast<bf16_t*>(const_cast<void*>(p.dk.p)) + b * p.dk.b + j * p.dk.t + hk * p.dk.h, p.D, half, dk, p.scale);
-        store_transposed<DP>(static_cast<bf16_t*>(const_cast<void*>(p.dv.p)) + b * p.dv.b + j * p.dv.t + hk * p.dv.h, p.D, half, dv, 1.f);
+        leave(dk, role == 1);
     }
+}
+
+// The parts of a sequence's first keys joined, in their order: a workgroup a key, the parts shared out over its threads' groups.
+__global__ __launch_bounds__(256) void window_first_keys_kernel(const WindowParams p) {
+    __shared__ f32x4 shared[256];
+    int x = blockIdx.x;
+    const int i = x % p.sinks;
+    x /= p.sinks;
+    const int hk = x % p.HK, n = x / p.HK, b = p.cu != nullptr && !p.padded ? 0 : n;
+    int st, len;
+    sequence_of(p, n, st, len);
+    if (i >= len) return;
+    const int quads = 2 * p.D / 4, groups = max(1, 256 / quads), group = threadIdx.x / quads, at = threadIdx.x - group * quads;  // 2 D <= 512 numbers a part
+    const float* const from = p.part_dk + (((int64_t)n * p.HK + hk) * (p.pieces + 1) * p.first_keys + i) * 2 * p.D + 4 * at;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (group < groups) {
+#pragma unroll 8
+        for (int y = group; y <= p.pieces; y += groups) sum += *reinterpret_cast<const f32x4*>(from + (int64_t)y * p.first_keys * 2 * p.D);
+    }
+    shared[threadIdx.x] = sum;
+    __syncthreads();
+    if (group != 0) return;
+    for (int y = 1; y < groups; y++) sum += shared[y * quads + at];
+    const int col = 4 * at;
+    if (col < p.D) store4<bf16_t>(static_cast<bf16_t*>(const_cast<void*>(p.dk.p)) + b * p.dk.b + (st + i) * p.dk.t + hk * p.dk.h + col, sum * p.scale);
+    else store4<bf16_t>(static_cast<bf16_t*>(const_cast<void*>(p.dv.p)) + b * p.dv.b + (st + i) * p.dv.t + hk * p.dv.h + col - p.D, sum);
 }
 
 template <int DP>
 int launch_bwd(const WindowParams& p, hipStream_t stream) {
     WindowParams r = p, k = p;
-    r.blocks = (p.rows + WINDOW_ROWS - 1) / WINDOW_ROWS, k.blocks = (p.S + WINDOW_KEYS - 1) / WINDOW_KEYS;
+    r.blocks = (p.rows + WINDOW_ROWS - 1) / WINDOW_ROWS, k.blocks = (p.S + window_keys(DP) - 1) / window_keys(DP);
     const auto grid = [&](const WindowParams& x) { return dim3((unsigned)(((int64_t)p.B * p.HK * x.blocks + 7) / 8 * 8)); };
     hipLaunchKernelGGL((window_dq_kernel<DP>), grid(r), dim3(256), 0, stream, r);
     if (const int e = (int)hipGetLastError(); e != 0) return e;
+    const dim3 threads(DP <= 128 ? 512 : 256);
     if (p.pieces > 0) {
-        hipLaunchKernelGGL((window_dkv_kernel<DP, true>), dim3((unsigned)((int64_t)p.N * p.HK * (p.first_keys / WINDOW_KEYS) * p.pieces)), dim3(256), 0, stream, k);
+        hipLaunchKernelGGL((window_dkv_kernel<DP, true>), dim3((unsigned)((int64_t)p.N * p.HK * (p.first_keys / WINDOW_FIRST_KEYS) * p.pieces)), threads, 0, stream, k);
         if (const int e = (int)hipGetLastError(); e != 0) return e;
     }
-    hipLaunchKernelGGL((window_dkv_kernel<DP, false>), grid(k), dim3(256), 0, stream, k);
+    hipLaunchKernelGGL((window_dkv_kernel<DP, false>), grid(k), threads, 0, stream, k);
+    if (const int e = (int)hipGetLastError(); e != 0 || p.pieces == 0) return e;
+    hipLaunchKernelGGL(window_first_keys_kernel, dim3((unsigned)((int64_t)p.N * p.HK * p.sinks)), dim3(256), 0, stream, k);
     return (int)hipGetLastError();
 }
 

@@ -168,7 +168,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void window_fwd_f32_kernel(c
         stage<DP>(vt, vf);
         __syncthreads();
         if (i + 1 < last) fetch_tile(i + 1);
-        const TileView own(x.view, i >= x.sink_tiles, x.all.sink_end);
+        TileView own(x.view, i >= x.sink_tiles, x.all.sink_end);
+        if (i < x.sink_tiles) own.first = own.span, own.st = own.from;
         f32x4 s[2];
         float top = -__builtin_inff();
 #pragma unroll
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void window_fwd_f32_kernel(c
             s[y] = scores<DP>(kt, y, x.lane, q);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                if (!own.sees(j0 + 16 * y + 4 * x.g + e)) s[y][e] = -__builtin_inff();
+                if (!own.sees_mixed(j0 + 16 * y + 4 * x.g + e)) s[y][e] = -__builtin_inff();
                 else top = fmaxf(top, s[y][e] * p.c);
             }
         }
@@ -252,14 +253,15 @@ __global__ __launch_bounds__(256, 1) void window_dq_f32_kernel(const WindowParam
         stage<DP>(vt, vf);
         __syncthreads();
         if (i + 1 < x.tiles) fetch_tile(i + 1);
-        const TileView own(x.view, i >= x.sink_tiles, x.all.sink_end);
+        TileView own(x.view, i >= x.sink_tiles, x.all.sink_end);
+        if (i < x.sink_tiles) own.first = own.span, own.st = own.from;
 #pragma unroll
         for (int y = 0; y < 2; y++) {
             f32x4 s = scores<DP>(kt, y, x.lane, q);
             const f32x4 dw = scores<DP>(vt, y, x.lane, d);
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                s[e] = own.sees(j0 + 16 * y + 4 * x.g + e) ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -m)) * by * (dw[e] - delta) : 0.f;
+                s[e] = own.sees_mixed(j0 + 16 * y + 4 * x.g + e) ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -m)) * by * (dw[e] - delta) : 0.f;
             add_rows<DP>(kt, y, x.lane, s, dq);
         }
     }
