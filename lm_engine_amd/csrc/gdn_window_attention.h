@@ -168,14 +168,33 @@ struct TileLoads {
     static_assert(GRANULES <= 64 && WROWS % RPI == 0, "a wave loads WROWS rows");
     static __device__ __forceinline__ int row(int wave, int lane, int i) { return WROWS * wave + RPI * i + lane / GRANULES; }
     static __device__ __forceinline__ int column(int wave, int lane, int i) { return 8 * (lane % GRANULES ^ tile_key<DP>(row(wave, lane, i))); }
-    // `to`: LDS address of the tile; offset in bytes from `base`
-    static __device__ __forceinline__ void load(const void* base, uint32_t offset, uint32_t to, int wave, int i) {
+    // `to`: LDS address of the tile; offset (and `more`, the same in all lanes) in bytes from `base`
+    static __device__ __forceinline__ void load(const void* base, uint32_t offset, uint32_t to, int wave, int i, int more = 0) {
         const uint64_t a = reinterpret_cast<uint64_t>(base);
         i32x4 r;
         r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)a), r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32) & 0xffff);
         r[2] = (int)PAST, r[3] = 0x00020000;
         const int at = __builtin_amdgcn_readfirstlane((int)(to + (WROWS * wave + RPI * i) * DP * 2));
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(offset), "s"(r) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(at), "v"(offset), "s"(r), "s"(more) : "memory");
+    }
+};
+// A tile whose rows lie `stride` elements apart, asked for in ITERS pieces, to be spread over the work on another one: a load takes the wave's
+// time until the compute unit's address path has taken it, and eight waves ask at once (800 cycles a tile in one go).
+template <int DP, int WROWS = 16>
+struct TileRequest {
+    using Loads = TileLoads<DP, WROWS>;
+    const char* base;
+    int stride, count, columns;
+    uint32_t to, row_bytes, place;
+    int row0;
+    // row RPI i on, the granule's place is the first one's with some bits turned
+    __device__ __forceinline__ void piece(int wave, int i) const {
+        const uint32_t at = place ^ (16 * tile_key<DP>(Loads::RPI * i));
+        Loads::load(base, row0 + Loads::RPI * i < count && (int)at < 2 * columns ? at + row_bytes : PAST, to, wave, i, Loads::RPI * i * stride * 2);
+    }
+    __device__ __forceinline__ void all(int wave) const {
+#pragma unroll
+        for (int i = 0; i < Loads::ITERS; i++) piece(wave, i);
     }
 };
 // everything that this wave has asked for is in LDS
@@ -234,6 +253,9 @@ __device__ __forceinline__ void load_row_fragments(const bf16_t* row, int D, int
     }
 }
 
+// In a branch that few tiles take: without it the compiler turns the branch into selects that all of them pay for.
+__device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
+
 // row of accumulator register r: (r & 3) + 8 (r >> 2) + 4 half
 __device__ __forceinline__ constexpr int acc_row(int r, int half) { return (r & 3) + 8 * (r >> 2) + 4 * half; }
 
@@ -285,7 +307,7 @@ int launch_window_fwd_f32(const WindowParams& p, hipStream_t stream);       // g
 int launch_window_bwd_f32(const WindowParams& p, hipStream_t stream);
 int launch_window_combine(const WindowParams& p, int dtype, hipStream_t stream);
 constexpr int WINDOW_ROWS = 128;      // of a workgroup, bf16
-constexpr int window_keys(int D) { return D <= 128 ? 128 : 64; }  // of a workgroup of the keys' gradients, bf16
+constexpr int window_keys(int D) { return D > 64 && D <= 128 ? 128 : 64; }  // of a workgroup of the keys' gradients, bf16
 constexpr int WINDOW_FIRST_KEYS = 32;  // of a workgroup of a sequence's first keys
 constexpr int WINDOW_ROWS_F32 = 64;
 constexpr int WINDOW_KEYS_F32 = 64;

@@ -32,7 +32,7 @@ template <int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_fwd_kernel(const WindowParams p) {
     constexpr int KS = DP / 16, DT = DP / 32;
     using Loads = TileLoads<DP>;
-    __shared__ __attribute__((aligned(1024))) bf16_t tiles[2][2][64 * DP];
+    __shared__ __attribute__((aligned(1024))) bf16_t tiles[2][2][64 * DP];  // keys, values; tiles in turn
     int pair, block;
     if (!work_item(p, blockIdx.x, pair, block)) return;
     block = p.blocks - 1 - block;  // the rows that see most keys first
@@ -70,35 +70,40 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_fwd_kernel(cons
         j0 = s ? sink + 64 * i : lo + 64 * (i - sink_tiles);
         count = min((s ? sink_end : end) - j0, 64);
     };
-    auto load_tile = [&](int i) {
+    const int row0 = Loads::row(wave, lane, 0);
+    const uint32_t place = 2 * Loads::column(wave, lane, 0), key_bytes = (uint32_t)(row0 * (int)p.k.t) * 2, value_bytes = (uint32_t)(row0 * (int)p.v.t) * 2;
+    // keys and values of tile i, into the half of their buffer that i's parity names
+    using Request = TileRequest<DP>;
+    auto keys_of = [&](int i) {
         int j0, count;
         tile_at(i, j0, count);
-        const char *const k0 = kb + (int64_t)j0 * p.k.t * 2, *const v0 = vb + (int64_t)j0 * p.v.t * 2;
-        const uint32_t to = lds + (i & 1) * 2 * 64 * DP * 2;
-#pragma unroll
-        for (int x = 0; x < Loads::ITERS; x++) {
-            const int kr = Loads::row(wave, lane, x), c = Loads::column(wave, lane, x);
-            const bool there = kr < count && c < p.D;
-            Loads::load(k0, there ? (uint32_t)(kr * (int)p.k.t + c) * 2 : PAST, to, wave, x);
-            Loads::load(v0, there ? (uint32_t)(kr * (int)p.v.t + c) * 2 : PAST, to + 64 * DP * 2, wave, x);
-        }
+        if (i >= last_tile) j0 = 0, count = 0;
+        return Request{kb + (int64_t)j0 * p.k.t * 2, (int)p.k.t, count, p.D, lds + (i & 1) * 64 * DP * 2, key_bytes, place, row0};
+    };
+    auto values_of = [&](int i) {
+        int j0, count;
+        tile_at(i, j0, count);
+        return Request{vb + (int64_t)j0 * p.v.t * 2, (int)p.v.t, count, p.D, lds + (2 + (i & 1)) * 64 * DP * 2, value_bytes, place, row0};
     };
 
-    const TileReader<DP> reader(lane);
-    f32x16 o[DT] = {};
-    float m = LOWEST, l = 0.f;
+    TileReader<DP> reader(lane);
+    f32x16 o[DT], s_even[2], s_odd[2];
+    float m, l;
     bool careful = false, taken_out = false;
-    if (first_tile < last_tile) load_tile(first_tile);
-    for (int i = first_tile; i < last_tile; i++) {
-        loads_done();
-        __syncthreads();
-        if (i + 1 < last_tile) load_tile(i + 1);
+    auto scores = [&](int i, f32x16 (&to)[2]) {
+        const bf16_t* const kt = tiles[0][i & 1];
+#pragma unroll
+        for (int y = 0; y < KS; y++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) to[x] = mma(reader.across(kt, 32 * x, y), q[y], y == 0 ? f32x16{} : to[x]);
+    };
+    // Tile i, whose scores are in s; NEXT: the next one's scores are formed beside its weights, where the matrix unit would have nothing to do
+    auto step = [&](int i, f32x16 (&s)[2], f32x16 (&s_next)[2], auto next) {
         int j0, count;
         tile_at(i, j0, count);
-        const bf16_t *const kt = tiles[i & 1][0], *const vt = tiles[i & 1][1];
         const bool near = i >= sink_tiles, full = near && j0 >= w.full_lo && j0 + 64 <= w.full_end;
         if (careful && !(near && j0 >= all.full_lo && j0 + 64 <= all.full_end)) {
-            bf16x8* const v8 = reinterpret_cast<bf16x8*>(tiles[i & 1][1]);
+            bf16x8* const v8 = reinterpret_cast<bf16x8*>(tiles[1][i & 1]);
             bool found = false;
 #pragma unroll
             for (int x = 0; x < 64 * DP / 8 / 256; x++) {
@@ -107,76 +112,137 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_fwd_kernel(cons
             }
             taken_out |= __syncthreads_or(found) != 0;
         }
-        f32x16 s[2];
-        if (w.meets(j0, count)) {
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                f32x16 acc = {};
-#pragma unroll
-                for (int y = 0; y < KS; y++) acc = mma(reader.across(kt, 32 * x, y), q[y], acc);
-                s[x] = acc;
+        Request keys, values;
+        if constexpr (next()) keys = keys_of(i + 2), values = values_of(i + 1);
+        if (!w.meets(j0, count)) {
+            if constexpr (next()) {
+                keys.all(wave), values.all(wave);
+                scores(i + 1, s_next);
             }
-            float c = p.c;
-            if (!full) {
-                const TileView own(view, near, sink_end);
-                c = 1.f;
-                if (!(near && j0 < all.sink_end)) {
+            return;
+        }
+        float c = p.c;
+        if (!full) {
+            stay_a_branch();
+            const TileView own(view, near, sink_end);
+            c = 1.f;
+            if (!(near && j0 < all.sink_end)) {
 #pragma unroll
-                    for (int x = 0; x < 2; x++)
+                for (int x = 0; x < 2; x++)
 #pragma unroll
-                        for (int e = 0; e < 16; e++) s[x][e] = own.sees(j0 + 32 * x + acc_row(e, half)) ? s[x][e] * p.c : -__builtin_inff();
-                } else {
+                    for (int e = 0; e < 16; e++) s[x][e] = own.sees(j0 + 32 * x + acc_row(e, half)) ? s[x][e] * p.c : -__builtin_inff();
+            } else {
 #pragma unroll
-                    for (int x = 0; x < 2; x++)
+                for (int x = 0; x < 2; x++)
 #pragma unroll
-                        for (int e = 0; e < 16; e++) s[x][e] = own.sees_mixed(j0 + 32 * x + acc_row(e, half)) ? s[x][e] * p.c : -__builtin_inff();
-                }
-            }
-            float top = s[0][0];
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) top = fmaxf(top, s[x][e]);
-            top = fmaxf(top, other_half(top)) * c;
-            if (__builtin_amdgcn_ballot_w64(top > m + 8.f) != 0) {
-                const float next = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - next);
-                m = next;
-                l *= alpha;
-#pragma unroll
-                for (int x = 0; x < DT; x++) o[x] *= alpha;
-            }
-            float sum = 0.f;
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    s[x][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], c, -m));
-                    sum += s[x][e];
-                }
-            l += sum;
-#pragma unroll
-            for (int y = 0; y < 4; y++) {
-                const bf16x8 weights = pack8(s[y >> 1], y & 1);
-#pragma unroll
-                for (int x = 0; x < DT; x++) o[x] = mma(reader.down(vt, y, x), weights, o[x]);
+                    for (int e = 0; e < 16; e++) s[x][e] = own.sees_mixed(j0 + 32 * x + acc_row(e, half)) ? s[x][e] * p.c : -__builtin_inff();
             }
         }
-        if (i + 1 == last_tile && !careful) {
-            // 0 times a value that is not finite must not reach the rows that do not see it.  Where a result is not finite, the walk is
-            // taken once more, without such values in tiles that some row does not see all of; they go to the rows that see them in the end.
-            float zero = 0.f;
+        float top = s[0][0];
 #pragma unroll
-            for (int x = 0; x < DT; x++)
+        for (int x = 0; x < 2; x++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) zero = __builtin_fmaf(o[x][e], 0.f, zero);
-            if (__syncthreads_or(zero != 0.f)) {
-                careful = true, m = LOWEST, l = 0.f;
+            for (int e = 0; e < 16; e++) top = fmaxf(top, s[x][e]);
+        top = fmaxf(top, other_half(top)) * c;
+        if (__builtin_amdgcn_ballot_w64(top > m + 8.f) != 0) {
+            const float reference = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - reference);
+            m = reference;
+            l *= alpha;
 #pragma unroll
-                for (int x = 0; x < DT; x++) o[x] = f32x16{};
-                load_tile(first_tile);
-                i = first_tile - 1;
+            for (int x = 0; x < DT; x++) o[x] *= alpha;
+        }
+        // Products one after the other, each with the reading of the operand for the one four further on, its share of the weights' arithmetic
+        // and of the loads of the tiles to come, in this order (the compiler's own has every product wait for its operand).
+        constexpr int AHEAD = 2, QK = 2 * KS, PV = 4 * DT, EACH = 32 / QK;
+        const bf16_t *const kt = tiles[0][(i + 1) & 1], *const vt = tiles[1][i & 1];
+        __builtin_amdgcn_s_setprio(1);  // before the wave that is between its products
+        bf16x8 ahead[AHEAD], weights[4];
+        float sum = 0.f;
+        auto fetch = [&](int k) {  // product k's operand: of keys, then of values
+            return k < QK ? reader.across(kt, 32 * (k & 1), k >> 1) : reader.down(vt, (k - QK) / DT, (k - QK) % DT);
+        };
+        constexpr int BEGIN = next() ? 0 : QK;
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) ahead[k] = fetch(BEGIN + k);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < QK; k++) {
+            if constexpr (next()) {
+                s_next[k & 1] = mma(ahead[k % AHEAD], q[k >> 1], k < 2 ? f32x16{} : s_next[k & 1]);
+                ahead[k % AHEAD] = fetch(k + AHEAD);
+                if (k % 2 == 0) k < QK / 2 ? values.piece(wave, k / 2) : keys.piece(wave, (k - QK / 2) / 2);
+            }
+#pragma unroll
+            for (int e = EACH * k; e < EACH * (k + 1); e++) {
+                s[e >> 4][e & 15] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 4][e & 15], c, -m));
+                sum += s[e >> 4][e & 15];
+                if (e % 8 == 7) weights[e >> 3] = pack8(s[e >> 4], e >> 3 & 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        l += sum;
+        __builtin_amdgcn_s_setprio(2);
+#pragma unroll
+        for (int k = 0; k < PV; k++) {
+            o[k % DT] = mma(ahead[k % AHEAD], weights[k / DT], o[k % DT]);
+            if (k + AHEAD < PV) ahead[k % AHEAD] = fetch(QK + k + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+    };
+    for (;;) {
+        m = LOWEST, l = 0.f;
+#pragma unroll
+        for (int x = 0; x < DT; x++) o[x] = f32x16{};
+        if (first_tile >= last_tile) break;
+        keys_of(first_tile).all(wave);
+        if constexpr (DP <= 128) {
+            loads_done();
+            __syncthreads();
+            values_of(first_tile).all(wave);
+            keys_of(first_tile + 1).all(wave);
+            scores(first_tile, s_even);
+            // here: the scores of tile i are in s, its values and the keys of the next one have been asked for
+            int i = first_tile;
+            auto advance = [&]() {
+                loads_done();
+                __syncthreads();
+                reader.recompute();
+            };
+            for (; i + 2 < last_tile; i++) {
+                advance();
+                step(i, s_even, s_odd, std::true_type{});
+                i++;
+                advance();
+                step(i, s_odd, s_even, std::true_type{});
+            }
+            if (i + 1 < last_tile) {
+                advance();
+                step(i, s_even, s_odd, std::true_type{});
+                s_even[0] = s_odd[0], s_even[1] = s_odd[1];
+            }
+            advance();
+            step(last_tile - 1, s_even, s_odd, std::false_type{});
+        } else {  // (the next tile's scores find no registers)
+            values_of(first_tile).all(wave);
+            for (int i = first_tile; i < last_tile; i++) {
+                loads_done();
+                __syncthreads();
+                if (i + 1 < last_tile) keys_of(i + 1).all(wave), values_of(i + 1).all(wave);
+                scores(i, s_even);
+                step(i, s_even, s_odd, std::false_type{});
             }
         }
+        if (careful) break;
+        // 0 times a value that is not finite must not reach the rows that do not see it.  Where a result is not finite, the walk is
+        // taken once more, without such values in tiles that some row does not see all of; they go to the rows that see them in the end.
+        float zero = 0.f;
+#pragma unroll
+        for (int x = 0; x < DT; x++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) zero = __builtin_fmaf(o[x][e], 0.f, zero);
+        if (!__syncthreads_or(zero != 0.f)) break;
+        careful = true;
     }
 
     l += other_half(l);

@@ -98,6 +98,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dq_kernel(const
 #pragma unroll
             for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -lse)) * (dw[e] - delta);
             if (!full) {
+                stay_a_branch();
                 if (!(near && j0 < all.sink_end)) {
 #pragma unroll
                     for (int e = 0; e < 16; e++) s[e] = own.sees(j0 + 32 * x + acc_row(e, half)) ? s[e] : 0.f;
@@ -126,8 +127,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dq_kernel(const
 // FIRST: the keys of a sequence that all of its rows see, 32 of them, and of those rows that do not have them in their window one part, in tiles of
 // 256 rows (64): (sequence, head of k and v, block of such keys, part).  Both leave their sums for such keys to window_first_keys_kernel.
 template <int DP, bool FIRST>
-__global__ __launch_bounds__(DP <= 128 ? 512 : 256, DP <= 128 ? 2 : 1) void window_dkv_kernel(const WindowParams p) {
-    constexpr int KS = DP / 16, DT = DP / 32, KEYS = FIRST ? WINDOW_FIRST_KEYS : window_keys(DP), ROLES = DP <= 128 ? 1 : 2, WAVES = DP <= 128 ? 8 : 4;
+__global__ __launch_bounds__(DP == 128 ? 512 : 256, DP == 64 ? 3 : DP == 128 ? 2 : 1) void window_dkv_kernel(const WindowParams p) {
+    constexpr int KS = DP / 16, DT = DP / 32, KEYS = FIRST ? WINDOW_FIRST_KEYS : window_keys(DP), ROLES = DP <= 128 ? 1 : 2, WAVES = DP == 128 ? 8 : 4;
     constexpr int KEY_WAVES = KEYS / 32, ROW_WAVES = WAVES / ROLES / KEY_WAVES, ROWS = 32 * ROW_WAVES, BUFFERS = FIRST ? 1 : 2;
     using Loads = TileLoads<DP, ROWS / WAVES>;
     using KeyLoads = TileLoads<DP, 16>;
@@ -236,10 +237,9 @@ __global__ __launch_bounds__(DP <= 128 ? 512 : 256, DP <= 128 ? 2 : 1) void wind
         const bf16_t *const qx = qt + 32 * row_wave * DP, *const dx = dt + 32 * row_wave * DP;
         f32x16 s = {}, dw = {};
 #pragma unroll
-        for (int y = 0; y < KS; y++) s = mma(reader.across(qx, 0, y), reader.across(kt + 32 * key_wave * DP, 0, y), s);
-        if (ROLES == 1 || role == 0) {
-#pragma unroll
-            for (int y = 0; y < KS; y++) dw = mma(reader.across(dx, 0, y), reader.across(vt + 32 * key_wave * DP, 0, y), dw);
+        for (int y = 0; y < KS; y++) {
+            s = mma(reader.across(qx, 0, y), reader.across(kt + 32 * key_wave * DP, 0, y), s);
+            if (ROLES == 1 || role == 0) dw = mma(reader.across(dx, 0, y), reader.across(vt + 32 * key_wave * DP, 0, y), dw);
         }
 #pragma unroll
         for (int y = 0; y < 4; y++) {
@@ -252,6 +252,7 @@ __global__ __launch_bounds__(DP <= 128 ? 512 : 256, DP <= 128 ? 2 : 1) void wind
             }
         }
         if (!full) {
+            stay_a_branch();
 #pragma unroll
             for (int y = 0; y < 4; y++) {
                 const i32x4 at = *reinterpret_cast<const i32x4*>(&row_at[i % BUFFERS][at0 + 8 * y]);
@@ -386,7 +387,7 @@ int launch_bwd(const WindowParams& p, hipStream_t stream) {
     const auto grid = [&](const WindowParams& x) { return dim3((unsigned)(((int64_t)p.B * p.HK * x.blocks + 7) / 8 * 8)); };
     hipLaunchKernelGGL((window_dq_kernel<DP>), grid(r), dim3(256), 0, stream, r);
     if (const int e = (int)hipGetLastError(); e != 0) return e;
-    const dim3 threads(DP <= 128 ? 512 : 256);
+    const dim3 threads(DP == 128 ? 512 : 256);
     if (p.pieces > 0) {
         hipLaunchKernelGGL((window_dkv_kernel<DP, true>), dim3((unsigned)((int64_t)p.N * p.HK * (p.first_keys / WINDOW_FIRST_KEYS) * p.pieces)), threads, 0, stream, k);
         if (const int e = (int)hipGetLastError(); e != 0) return e;
