@@ -24,18 +24,23 @@ struct Block {
     float v[16][8];
 };
 
+// Eight columns of a row, as they are in memory; rows of new tokens are read once, past the caches.
 template <typename T>
-__device__ __forceinline__ void load_row(const T* p, float (&v)[8]) {
-    if constexpr (sizeof(T) == 2) {
-        const bf16x8 x = *reinterpret_cast<const bf16x8*>(p);
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = (float)x[e];
-    } else {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = x[e], v[4 + e] = y[e];
+struct RowPiece;
+template <>
+struct RowPiece<bf16_t> {
+    bf16x8 x = {};
+    __device__ __forceinline__ void load(const bf16_t* p) { x = __builtin_nontemporal_load(reinterpret_cast<const bf16x8*>(p)); }
+    __device__ __forceinline__ float operator[](int e) const { return (float)x[e]; }
+};
+template <>
+struct RowPiece<float> {
+    f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
+    __device__ __forceinline__ void load(const float* p) {
+        x = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p)), y = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p + 4));
     }
-}
+    __device__ __forceinline__ float operator[](int e) const { return e < 4 ? x[e & 3] : y[e & 3]; }
+};
 
 // pages that the tokens [start, start + len) of a sequence lie in; what lies in front of position 0 or past the table is cut off before
 __device__ __forceinline__ int pages_of(int start, int len, int P) { return len > 0 ? (start + len - 1) / P - start / P + 1 : 0; }
@@ -92,10 +97,10 @@ __device__ __forceinline__ bool find_page(const WriteParams& p, int slot, int& n
 
 template <typename T>
 __global__ __launch_bounds__(256) void cache_write_kernel(const WriteParams p) {
-    const int value = blockIdx.z, h = blockIdx.y, P = p.c.P, D = p.c.D;
+    const int slot = blockIdx.x / p.c.HK, h = blockIdx.x - slot * p.c.HK, value = blockIdx.y, P = p.c.P, D = p.c.D;
     int n, nth;
-    if (p.each > 0) n = blockIdx.x / p.each, nth = blockIdx.x - n * p.each;
-    else if (!find_page(p, blockIdx.x, n, nth)) return;
+    if (p.each > 0) n = slot / p.each, nth = slot - n * p.each;
+    else if (!find_page(p, slot, n, nth)) return;
     const NewTokens s = new_tokens(p, n);
     const int index = s.start / P + nth;
     if (nth >= pages_of(s.start, s.len, P)) return;
@@ -110,18 +115,16 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const WriteParams p) {
     const int64_t stride = value ? p.t[1] : p.t[0], row0 = (int64_t)s.first + (index * P - s.start);
 
     const int columns = D / 8, tasks = P / 16 * columns;
-    auto load = [&](int task, Block& x) {
+    auto load = [&](int task, RowPiece<T> (&x)[16]) {
         const int g = task / columns, c = task - g * columns;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             const int o = 16 * g + i;
-            if (o >= o0 && o < o1) load_row<T>(rows + (row0 + o) * stride + 8 * c, x.v[i]);
-            else
-#pragma unroll
-                for (int e = 0; e < 8; e++) x.v[i][e] = 0.f;
+            x[i] = RowPiece<T>();
+            if (o >= o0 && o < o1) x[i].load(rows + (row0 + o) * stride + 8 * c);
         }
     };
-    Block x;
+    RowPiece<T> x[16];
     float top = 0.f;
     const int threads = blockDim.x;
     for (int task = threadIdx.x; task < tasks; task += threads) {
@@ -130,7 +133,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const WriteParams p) {
         for (int i = 0; i < 16; i++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float a = fabsf(x.v[i][e]);
+                const float a = fabsf(x[i][e]);
                 top = fmaxf(top, a < __builtin_inff() ? a : 0.f);
             }
     }
@@ -168,7 +171,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const WriteParams p) {
                 if (!whole) out = to[d];
 #pragma unroll
                 for (int w = 0; w < 4; w++) {
-                    const unsigned fresh = cache_codes(one(x.v[4 * w][d]), one(x.v[4 * w + 1][d]), one(x.v[4 * w + 2][d]), one(x.v[4 * w + 3][d]));
+                    const unsigned fresh = cache_codes(one(x[4 * w][d]), one(x[4 * w + 1][d]), one(x[4 * w + 2][d]), one(x[4 * w + 3][d]));
                     if (whole) {
                         out[w] = fresh;
                         continue;
@@ -191,8 +194,8 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const WriteParams p) {
                 u32x2* const to = reinterpret_cast<u32x2*>(codes + (int64_t)o * D + 8 * c);
                 if (o >= o0 && o < o1) {
                     u32x2 out;
-                    out.x = cache_codes(one(x.v[i][0]), one(x.v[i][1]), one(x.v[i][2]), one(x.v[i][3]));
-                    out.y = cache_codes(one(x.v[i][4]), one(x.v[i][5]), one(x.v[i][6]), one(x.v[i][7]));
+                    out.x = cache_codes(one(x[i][0]), one(x[i][1]), one(x[i][2]), one(x[i][3]));
+                    out.y = cache_codes(one(x[i][4]), one(x[i][5]), one(x[i][6]), one(x[i][7]));
                     *to = out;
                 } else if (again && o < o0) {
                     u32x2 out = *to;
@@ -221,14 +224,15 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const WriteParams p) 
     const T* const rows = static_cast<const T*>(value ? p.x[1] : p.x[0]) + s.b * (value ? p.b[1] : p.b[0]) + h * (value ? p.h[1] : p.h[0]) + col;
     const int64_t stride = value ? p.t[1] : p.t[0], row0 = (int64_t)s.first + (index * P - s.start);
     const bool there = col < D;
-    float first[8], top = 0.f;
+    RowPiece<T> first;
+    float top = 0.f;
     for (int o = o1 - 1; o >= o0; o--) {
-        float x[8] = {};
-        if (there) load_row<T>(rows + (row0 + o) * stride, x);
+        first = RowPiece<T>();
+        if (there) first.load(rows + (row0 + o) * stride);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const float a = fabsf(x[e]);
-            top = fmaxf(top, a < __builtin_inff() ? a : 0.f), first[e] = x[e];
+            const float a = fabsf(first[e]);
+            top = fmaxf(top, a < __builtin_inff() ? a : 0.f);
         }
     }
 #pragma unroll
@@ -272,13 +276,8 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const WriteParams p) 
     const float by = power_of_two(-e);
     auto one = [&](float v) { return fabsf(v) < __builtin_inff() ? v * by : __builtin_nanf(""); };
     for (int o = o0; o < o1; o++) {
-        float x[8];
-        if (o == o0) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = first[i];
-        } else {
-            load_row<T>(rows + (row0 + o) * stride, x);
-        }
+        RowPiece<T> x = first;
+        if (o > o0) x.load(rows + (row0 + o) * stride);
         const unsigned lo = cache_codes(one(x[0]), one(x[1]), one(x[2]), one(x[3])), hi = cache_codes(one(x[4]), one(x[5]), one(x[6]), one(x[7]));
         if (value) {
             uint8_t* const to = codes + ((int64_t)(o / 16) * D + col) * 16 + o % 16;
@@ -414,7 +413,8 @@ extern "C" int gdn_cache_write(const gdn_cache_write_args* a, void* stream) {
         else lanes == 8 ? go(cache_append_kernel<float, 8>) : lanes == 16 ? go(cache_append_kernel<float, 16>) : go(cache_append_kernel<float, 32>);
         return (int)hipGetLastError();
     }
-    const dim3 grid((unsigned)slots, a->cache.HK, 2), block(threads_for(P, a->cache.D));
+    if (slots * a->cache.HK > INT32_MAX) return GDN_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)(slots * a->cache.HK), 2), block(threads_for(P, a->cache.D));
     if (a->dtype == GDN_BF16) hipLaunchKernelGGL((cache_write_kernel<bf16_t>), grid, block, 0, static_cast<hipStream_t>(stream), p);
     else hipLaunchKernelGGL((cache_write_kernel<float>), grid, block, 0, static_cast<hipStream_t>(stream), p);
     return (int)hipGetLastError();

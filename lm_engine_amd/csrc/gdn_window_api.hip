@@ -70,13 +70,13 @@ WindowParams params_of(const gdn_window_attn_args& a) {
     return p;
 }
 
-// Parts that the keys of a block of rows are cut into: until two workgroups a compute unit are there, none of them under 256 keys.
+// Parts that the keys of a block of rows are cut into: until two workgroups a compute unit are there, none of them under 128 keys.
 int splits_of(const gdn_window_attn_args& a) {
     const int64_t rows = (int64_t)a.T * (a.H / a.HK), edge = a.dtype == GDN_BF16 ? WINDOW_ROWS : WINDOW_ROWS_F32;
     const int64_t groups = (int64_t)a.B * a.HK * ((rows + edge - 1) / edge);
     const int64_t tokens = (edge + a.H / a.HK - 1) / (a.H / a.HK);
     const int64_t keys = a.window == 0 ? a.S : std::min<int64_t>(a.S, (int64_t)a.window + tokens + a.sinks);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({2 * compute_units() / groups, keys / 256, JOIN_MOST}));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({2 * compute_units() / groups, keys / 128, JOIN_MOST}));
 }
 
 uint64_t part_o_bytes(const gdn_window_attn_args& a, int splits) {
