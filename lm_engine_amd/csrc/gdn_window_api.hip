@@ -38,7 +38,7 @@ int check_shape(const gdn_window_attn_args& a) {
     // what the kernels hold in 32 bits: positions with a window's length on top, rows of a head of k and v, work items
     const int64_t rows = (int64_t)a.T * (a.H / a.HK);
     if (a.S >= 1 << 29 || rows >= 1 << 30 || a.N > 1 << 28) return GDN_ERR_UNSUPPORTED;
-    if ((int64_t)a.B * a.HK * ((std::max<int64_t>(rows, a.S) + 63) / 64) >= 1 << 30) return GDN_ERR_UNSUPPORTED;
+    if ((int64_t)a.B * a.HK * ((std::max<int64_t>(rows, a.S) + 15) / 16) >= 1 << 30) return GDN_ERR_UNSUPPORTED;
     return GDN_OK;
 }
 

@@ -309,7 +309,7 @@ int launch_window_combine(const WindowParams& p, int dtype, hipStream_t stream);
 constexpr int WINDOW_ROWS = 128;      // of a workgroup, bf16
 constexpr int window_keys(int D) { return D > 64 && D <= 128 ? 128 : 64; }  // of a workgroup of the keys' gradients, bf16
 constexpr int WINDOW_FIRST_KEYS = 32;  // of a workgroup of a sequence's first keys
-constexpr int WINDOW_ROWS_F32 = 64;
-constexpr int WINDOW_KEYS_F32 = 64;
+constexpr int WINDOW_ROWS_F32 = 16;
+constexpr int WINDOW_KEYS_F32 = 16;
 
 }  // namespace gdn
