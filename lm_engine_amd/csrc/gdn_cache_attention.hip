@@ -8,6 +8,10 @@
 //     of S^T row i, keys 16 g .. + 15   (4 x + r in register r of product x)
 //     of V   column 16 t + i, keys 16 g .. + 15: the 16 tokens of a column that the cache holds together
 // so that all 16 keys of a lane lie in one page.  Codes become bf16 with their page's scale in one instruction per pair, exactly.
+// Bound by memory where there is work: 256 sequences of 4096 keys on average, 32 query heads over 4 of 128, 227 us, the codes at 4.8 TB/s.
+// One token of a few sequences is bound by latency, 8 us and 2.5 to join the parts: a chain of table, scales and codes, each behind the last.
+// Rounding: weights become bf16 for the second product (2^-9 of each at most half a step, so 2^-9 / sqrt(3) of the output's norm, as in attention
+// over bf16 keys); everything else is fp32.
 #include <algorithm>
 #include <cmath>
 
@@ -286,10 +290,15 @@ int check_attend(const gdn_cache_attn_args& a) {
     return GDN_OK;
 }
 
-// Parts of a sequence's keys: until there are two workgroups to a compute unit, none of them under four chunks (one for each wave).
+// Parts of a sequence's keys: until there are two workgroups to a compute unit, none of them under four chunks (one for each wave), and whole
+// below twelve.  Measured with 16 heads of 128 over 2, in us, for one workgroup to a compute unit, two and four: 32 sequences of 4096 keys 21.0,
+// 19.8, 22.5; 64 of 2048 (over 8 heads) 42.3, 42.2, 49.6.  For parts of eight chunks, four and two: one sequence of 4096 keys 12.5, 10.7, 10.8; 8 of
+// 4096 12.7, 11.1, 12.9.  The joining launch is 2.5 of it: 4 sequences of 600 keys take 8.3 us whole and 10.6 in two parts, one of 1024 13.1
+// whole and 10.3 in four.
 int splits_of(const gdn_cache_attn_args& a) {
     const int64_t groups = (int64_t)a.cache.N * a.cache.HK * (((int64_t)a.T * (a.H / a.cache.HK) + ROWS - 1) / ROWS);
     const int64_t room = (int64_t)a.cache.table_pages * a.cache.P, keys = a.window == 0 ? room : std::min<int64_t>(room, (int64_t)a.window + a.T + a.sinks + CHUNK);
+    if (keys < 12 * CHUNK) return 1;
     return (int)std::max<int64_t>(1, std::min<int64_t>({2 * compute_units() / groups, keys / (4 * CHUNK), JOIN_MOST}));
 }
 uint64_t part_o_bytes(const gdn_cache_attn_args& a, int splits) { return ((uint64_t)splits * a.cache.N * a.T * a.H * a.cache.D * 4 + 255) / 256 * 256; }

@@ -70,12 +70,15 @@ WindowParams params_of(const gdn_window_attn_args& a) {
     return p;
 }
 
-// Parts that the keys of a block of rows are cut into: until two workgroups a compute unit are there, none of them under 128 keys.
+// Parts that the keys of a block of rows are cut into: until two workgroups a compute unit are there, none of them under 128 keys, and whole below
+// 384.  The joining launch costs 4.5 us, 64 keys one (bf16, 128 columns): 1 x 300 tokens of 4 heads over one take 14.4 us whole and 16.1 in two
+// parts, 1 x 777 of 2 over one with a window of 512 21.2 whole, 19.8 in two and 17.8 in four (256 columns: 39.7, 30.6, 25.7).
 int splits_of(const gdn_window_attn_args& a) {
     const int64_t rows = (int64_t)a.T * (a.H / a.HK), edge = a.dtype == GDN_BF16 ? WINDOW_ROWS : WINDOW_ROWS_F32;
     const int64_t groups = (int64_t)a.B * a.HK * ((rows + edge - 1) / edge);
     const int64_t tokens = (edge + a.H / a.HK - 1) / (a.H / a.HK);
     const int64_t keys = a.window == 0 ? a.S : std::min<int64_t>(a.S, (int64_t)a.window + tokens + a.sinks);
+    if (keys < 384) return 1;
     return (int)std::max<int64_t>(1, std::min<int64_t>({2 * compute_units() / groups, keys / 128, JOIN_MOST}));
 }
 
@@ -96,11 +99,25 @@ int pieces_of(const WindowParams& p, int dtype) {
 }
 int first_keys_of(const WindowParams& p) { return (p.sinks + WINDOW_FIRST_KEYS - 1) / WINDOW_FIRST_KEYS * WINDOW_FIRST_KEYS; }
 
+// The shares that the rows of a block of keys are cut into, where few heads of k and v leave fewer blocks than the chip has room for: with a window
+// one workgroup to a compute unit (up to 64 columns three), without one twice that (four), since then blocks have from all rows to none;
+// 4 tiles of rows or more to each.  Backward in us, whole and shared: 1 x 4096, 16 heads of 128 over 2, window 512 225 and 121 (4 shares; 8: 137);
+// the same with 64 columns 142 and 77 (6; 2: 97); 4 x 4096 of them without a window 1384 and 1092 (2; 4: 1129); 1 x 777, 4 heads of 128 over
+// one, window 512 129 and 64 (8 tiles or more to each: 70).  What it costs: the sums once more in fp32, and a launch of about 4 us.
+int shares_of(const WindowParams& p, int dtype) {
+    if (dtype != GDN_BF16) return 1;
+    const int64_t blocks = (int64_t)p.B * p.HK * ((p.S + window_keys(p.D) - 1) / window_keys(p.D));
+    const int64_t tokens = p.window == 0 ? p.T : std::min(p.T, p.window + window_keys(p.D)), least = p.D > 128 ? 128 : 256;
+    const int64_t wanted = (p.D <= 64 ? p.window == 0 ? 4 : 3 : p.window == 0 ? 2 : 1) * compute_units();
+    return (int)std::max<int64_t>(1, std::min<int64_t>({wanted / blocks, tokens * p.G / least, 16}));
+}
+uint64_t shares_bytes(const WindowParams& p, int shares) { return shares <= 1 ? 0 : (uint64_t)shares * p.B * p.HK * p.S * 2 * p.D * 4; }
+
 uint64_t delta_bytes(const gdn_window_attn_args& a) { return ((uint64_t)a.B * a.T * a.H * 4 + 255) / 256 * 256; }
 uint64_t backward_bytes(const gdn_window_attn_args& a, const WindowParams& p) {
-    const int pieces = pieces_of(p, a.dtype);
-    if (pieces == 0) return delta_bytes(a);
-    return delta_bytes(a) + (uint64_t)p.N * p.HK * (pieces + 1) * first_keys_of(p) * 2 * p.D * 4;
+    const int pieces = pieces_of(p, a.dtype), shares = shares_of(p, a.dtype);
+    const uint64_t first = pieces == 0 ? 0 : (uint64_t)p.N * p.HK * (pieces + shares) * first_keys_of(p) * 2 * p.D * 4;
+    return delta_bytes(a) + shares_bytes(p, shares) + first;
 }
 
 }  // namespace
@@ -155,7 +172,9 @@ extern "C" int gdn_window_attn_bwd(const gdn_window_attn_bwd_args* args, void* s
     p.dv = {b.dv, b.dv_stride_b, b.dv_stride_t, b.dv_stride_h};
     p.delta = static_cast<float*>(b.workspace);
     p.pieces = pieces_of(p, a.dtype), p.first_keys = first_keys_of(p);
-    p.part_dk = reinterpret_cast<float*>(static_cast<char*>(b.workspace) + delta_bytes(a));
+    p.shares = shares_of(p, a.dtype);
+    p.part_all = reinterpret_cast<float*>(static_cast<char*>(b.workspace) + delta_bytes(a));
+    p.part_dk = reinterpret_cast<float*>(static_cast<char*>(b.workspace) + delta_bytes(a) + shares_bytes(p, p.shares));
     const hipStream_t st = static_cast<hipStream_t>(stream);
     return a.dtype == GDN_BF16 ? launch_window_bwd(p, st) : launch_window_bwd_f32(p, st);
 }

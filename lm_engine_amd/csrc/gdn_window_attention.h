@@ -38,7 +38,10 @@ struct WindowParams {
     float* part_m;    // [splits, B, HK, rows, 2]: reference exponent, sum
     // gradients of a sequence's first keys from rows that see them beyond the window, in `pieces` parts per sequence
     int pieces, first_keys;  // first_keys: sinks, in whole blocks
-    float* part_dk;   // [N, HK, pieces + 1, first_keys, 2, D]; the last part is from the rows that have them in their window
+    float* part_dk;   // [N, HK, pieces + shares, first_keys, 2, D]; the last parts are from the rows that have them in their window
+    // the rows of a block of keys cut into `shares`
+    int shares;
+    float* part_all;  // [shares, B, HK, S, 2, D]
 };
 
 // n / G and the rest, for n < 2^16
@@ -94,10 +97,20 @@ __device__ __forceinline__ RowView row_view(const WindowParams& p, int b, int r)
     return v;
 }
 
+template <int CTRL>
+__device__ __forceinline__ int lane_moved(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xF, 0xF, false);
+}
+// (over neighbours by moves within rows of 16 lanes, then rows, then halves: five of these took 2000 cycles by way of LDS, at the head of every kernel)
 __device__ __forceinline__ int wave_min(int x) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) x = min(x, __shfl_xor(x, off, WAVE));
-    return __builtin_amdgcn_readfirstlane(x);
+    x = min(x, lane_moved<0xB1>(x));   // lane l ^ 1
+    x = min(x, lane_moved<0x4E>(x));   // l ^ 2
+    x = min(x, lane_moved<0x141>(x));  // the other four of eight
+    x = min(x, lane_moved<0x128>(x));  // eight lanes on in the row
+    const auto rows = __builtin_amdgcn_permlane16_swap((unsigned)x, (unsigned)x, false, false);
+    x = min((int)rows[0], (int)rows[1]);
+    const auto halves = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)x, false, false);
+    return __builtin_amdgcn_readfirstlane(min((int)halves[0], (int)halves[1]));
 }
 __device__ __forceinline__ int wave_max(int x) { return -wave_min(-x); }
 

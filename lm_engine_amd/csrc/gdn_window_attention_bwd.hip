@@ -126,7 +126,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dq_kernel(const
 // Not FIRST: all keys, and the rows that have them in their window; 128 keys (64) and tiles of 64 rows (32), the next one on its way.
 // FIRST: the keys of a sequence that all of its rows see, 32 of them, and of those rows that do not have them in their window one part, in tiles of
 // 256 rows (64): (sequence, head of k and v, block of such keys, part).  Both leave their sums for such keys to window_first_keys_kernel.
-template <int DP, bool FIRST>
+template <int DP, bool FIRST, bool SHARED>
 __global__ __launch_bounds__(DP == 128 ? 512 : 256, DP == 64 ? 3 : DP == 128 ? 2 : 1) void window_dkv_kernel(const WindowParams p) {
     constexpr int KS = DP / 16, DT = DP / 32, KEYS = FIRST ? WINDOW_FIRST_KEYS : window_keys(DP), ROLES = DP <= 128 ? 1 : 2, WAVES = DP == 128 ? 8 : 4;
     constexpr int KEY_WAVES = KEYS / 32, ROW_WAVES = WAVES / ROLES / KEY_WAVES, ROWS = 32 * ROW_WAVES, BUFFERS = FIRST ? 1 : 2;
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, DP == 64 ? 3 : DP == 128 ? 2
     __shared__ int bounds[WAVES][6];
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), half = lane >> 5;
     const int key_wave = wave % KEY_WAVES, row_wave = wave / KEY_WAVES % ROW_WAVES, role = wave / KEY_WAVES / ROW_WAVES;  // role 0: dk (and dv), 1: dv
-    int b, hk, n = 0, piece = p.pieces, key0, keys;  // key0: of the workgroup
+    int b, hk, n = 0, piece = p.pieces + (SHARED ? (int)blockIdx.y : 0), key0, keys;  // key0: of the workgroup
     if constexpr (FIRST) {
         const int key_blocks = p.first_keys / KEYS;
         int x = blockIdx.x;
@@ -180,7 +180,11 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, DP == 64 ? 3 : DP == 128 ? 2
         const int each = (a1 - a0 + p.pieces - 1) / p.pieces;
         a0 = min(a1, a0 + piece * each), a1 = min(a1, a0 + each);
     }
-    const int r0 = (a0 - offset) * p.G, r1 = (a1 - offset) * p.G;
+    int r0 = (a0 - offset) * p.G, r1 = (a1 - offset) * p.G;
+    if constexpr (SHARED) {
+        const int each = ((r1 - r0 + ROWS - 1) / ROWS + p.shares - 1) / p.shares * ROWS;
+        r0 = min(r1, r0 + (int)blockIdx.y * each), r1 = min(r1, r0 + each);
+    }
     const int tile_count = (r1 - r0 + ROWS - 1) / ROWS;
 
     const char* const qb = reinterpret_cast<const char*>(static_cast<const bf16_t*>(p.q.p) + b * p.q.b + hk * p.G * p.q.h);
@@ -333,17 +337,18 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, DP == 64 ? 3 : DP == 128 ? 2
     }
     if (own >= keys) return;
     const bool to_parts = p.pieces > 0 && en > st && j - st < p.sinks;
-    float* const part = p.part_dk + (to_parts ? ((((int64_t)n * p.HK + hk) * (p.pieces + 1) + piece) * p.first_keys + (j - st)) * 2 * p.D : 0);
+    float* const part = p.part_dk + (to_parts ? ((((int64_t)n * p.HK + hk) * (p.pieces + p.shares) + piece) * p.first_keys + (j - st)) * 2 * p.D : 0);
     auto leave = [&](const f32x16 (&sums)[DT], bool value) {
         const WindowRows& out = value ? p.dv : p.dk;
-        if (!to_parts && !FIRST) store_transposed<DP>(static_cast<bf16_t*>(const_cast<void*>(out.p)) + b * out.b + j * out.t + hk * out.h, p.D, half, sums, value ? 1.f : p.scale);
-        if (!to_parts) return;
+        if (!FIRST && !SHARED && !to_parts) store_transposed<DP>(static_cast<bf16_t*>(const_cast<void*>(out.p)) + b * out.b + j * out.t + hk * out.h, p.D, half, sums, value ? 1.f : p.scale);
+        if (!SHARED && !to_parts) return;
+        float* const to = (to_parts ? part : p.part_all + ((((int64_t)blockIdx.y * p.B + b) * p.HK + hk) * p.S + j) * 2 * p.D) + (value ? p.D : 0);
 #pragma unroll
         for (int z = 0; z < DT; z++)
 #pragma unroll
             for (int y = 0; y < 4; y++) {
                 const int col = 32 * z + 8 * y + 4 * half;
-                if (col < p.D) *reinterpret_cast<f32x4*>(part + (value ? p.D : 0) + col) = f32x4{sums[z][4 * y], sums[z][4 * y + 1], sums[z][4 * y + 2], sums[z][4 * y + 3]};
+                if (col < p.D) *reinterpret_cast<f32x4*>(to + col) = f32x4{sums[z][4 * y], sums[z][4 * y + 1], sums[z][4 * y + 2], sums[z][4 * y + 3]};
             }
     };
     if constexpr (ROLES == 1) {
@@ -365,11 +370,11 @@ __global__ __launch_bounds__(256) void window_first_keys_kernel(const WindowPara
     sequence_of(p, n, st, len);
     if (i >= len) return;
     const int quads = 2 * p.D / 4, groups = max(1, 256 / quads), group = threadIdx.x / quads, at = threadIdx.x - group * quads;  // 2 D <= 512 numbers a part
-    const float* const from = p.part_dk + (((int64_t)n * p.HK + hk) * (p.pieces + 1) * p.first_keys + i) * 2 * p.D + 4 * at;
+    const float* const from = p.part_dk + (((int64_t)n * p.HK + hk) * (p.pieces + p.shares) * p.first_keys + i) * 2 * p.D + 4 * at;
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
     if (group < groups) {
 #pragma unroll 8
-        for (int y = group; y <= p.pieces; y += groups) sum += *reinterpret_cast<const f32x4*>(from + (int64_t)y * p.first_keys * 2 * p.D);
+        for (int y = group; y < p.pieces + p.shares; y += groups) sum += *reinterpret_cast<const f32x4*>(from + (int64_t)y * p.first_keys * 2 * p.D);
     }
     shared[threadIdx.x] = sum;
     __syncthreads();
@@ -378,6 +383,26 @@ __global__ __launch_bounds__(256) void window_first_keys_kernel(const WindowPara
     const int col = 4 * at;
     if (col < p.D) store4<bf16_t>(static_cast<bf16_t*>(const_cast<void*>(p.dk.p)) + b * p.dk.b + (st + i) * p.dk.t + hk * p.dk.h + col, sum * p.scale);
     else store4<bf16_t>(static_cast<bf16_t*>(const_cast<void*>(p.dv.p)) + b * p.dv.b + (st + i) * p.dv.t + hk * p.dv.h + col - p.D, sum);
+}
+
+// The shares of the other keys joined, in their order: a thread four columns.
+__global__ __launch_bounds__(256) void window_shares_kernel(const WindowParams p) {
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, keys = (int64_t)p.B * p.HK * p.S;
+    const int quads = 2 * p.D / 4;
+    const int64_t key = at / quads;
+    if (key >= keys) return;
+    const int64_t pair = key / p.S;
+    const int col = 4 * (int)(at - key * quads), j = (int)(key - pair * p.S), b = (int)(pair / p.HK), hk = (int)(pair - (int64_t)b * p.HK);
+    if (p.pieces > 0) {
+        int st, en, n;
+        sequence_at(p, b, j, st, en, n);
+        if (en > st && j - st < p.sinks) return;
+    }
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int y = 0; y < p.shares; y++) sum += *reinterpret_cast<const f32x4*>(p.part_all + (y * keys + key) * 2 * p.D + col);
+    if (col < p.D) store4<bf16_t>(static_cast<bf16_t*>(const_cast<void*>(p.dk.p)) + b * p.dk.b + j * p.dk.t + hk * p.dk.h + col, sum * p.scale);
+    else store4<bf16_t>(static_cast<bf16_t*>(const_cast<void*>(p.dv.p)) + b * p.dv.b + j * p.dv.t + hk * p.dv.h + col - p.D, sum);
 }
 
 template <int DP>
@@ -389,11 +414,18 @@ int launch_bwd(const WindowParams& p, hipStream_t stream) {
     if (const int e = (int)hipGetLastError(); e != 0) return e;
     const dim3 threads(DP == 128 ? 512 : 256);
     if (p.pieces > 0) {
-        hipLaunchKernelGGL((window_dkv_kernel<DP, true>), dim3((unsigned)((int64_t)p.N * p.HK * (p.first_keys / WINDOW_FIRST_KEYS) * p.pieces)), threads, 0, stream, k);
+        hipLaunchKernelGGL((window_dkv_kernel<DP, true, false>), dim3((unsigned)((int64_t)p.N * p.HK * (p.first_keys / WINDOW_FIRST_KEYS) * p.pieces)), threads, 0, stream, k);
         if (const int e = (int)hipGetLastError(); e != 0) return e;
     }
-    hipLaunchKernelGGL((window_dkv_kernel<DP, false>), grid(k), threads, 0, stream, k);
-    if (const int e = (int)hipGetLastError(); e != 0 || p.pieces == 0) return e;
+    if (p.shares > 1) hipLaunchKernelGGL((window_dkv_kernel<DP, false, true>), dim3(grid(k).x, p.shares), threads, 0, stream, k);
+    else hipLaunchKernelGGL((window_dkv_kernel<DP, false, false>), grid(k), threads, 0, stream, k);
+    if (const int e = (int)hipGetLastError(); e != 0) return e;
+    if (p.shares > 1) {
+        const int64_t quads = (int64_t)p.B * p.HK * p.S * (2 * p.D / 4);
+        hipLaunchKernelGGL(window_shares_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, k);
+        if (const int e = (int)hipGetLastError(); e != 0) return e;
+    }
+    if (p.pieces == 0) return GDN_OK;
     hipLaunchKernelGGL(window_first_keys_kernel, dim3((unsigned)((int64_t)p.N * p.HK * p.sinks)), dim3(256), 0, stream, k);
     return (int)hipGetLastError();
 }
