@@ -10,8 +10,8 @@
 // so that all 16 keys of a lane lie in one page.  Codes become bf16 with their page's scale in one instruction per pair, exactly.
 // Bound by memory where there is work: 256 sequences of 4096 keys on average, 32 query heads over 4 of 128, 227 us, the codes at 4.8 TB/s.
 // One token of a few sequences is bound by latency, 8 us and 2.5 to join the parts: a chain of table, scales and codes, each behind the last.
-// Rounding: weights become bf16 for the second product (2^-9 of each at most half a step, so 2^-9 / sqrt(3) of the output's norm, as in attention
-// over bf16 keys); everything else is fp32.
+// Rounding: weights become bf16 for the second product (half a step, 2^-8 of each, at most; up to 1.7e-3 rms of the output's norm); everything else is
+// fp32 up to the output's own rounding.
 #include <algorithm>
 #include <cmath>
 

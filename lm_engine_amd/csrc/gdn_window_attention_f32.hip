@@ -146,9 +146,9 @@ struct KeyWalk {
     RowView view;
     WaveView all;
     int sink_tiles, tiles;
-    __device__ __forceinline__ bool begin(const WindowParams& p) {
+    __device__ __forceinline__ void begin(const WindowParams& p) {
         int pair, block;
-        if (!work_item(p, blockIdx.x, pair, block)) return false;
+        work_item(p, blockIdx.x, pair, block);
         block = p.blocks - 1 - block;
         b = pair / p.HK, hk = pair - b * p.HK;
         lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), n = lane & 15, g = lane >> 4;
@@ -159,7 +159,6 @@ struct KeyWalk {
         all.sink_end = min(all.sink_end, all.lo);
         sink_tiles = all.sink_end > all.sink ? (all.sink_end - all.sink + TILE - 1) / TILE : 0;
         tiles = sink_tiles + (all.end > all.lo ? (all.end - all.lo + TILE - 1) / TILE : 0);
-        return true;
     }
     __device__ __forceinline__ void tile_at(int i, int& j0, int& count) const {
         const bool s = i < sink_tiles;
@@ -195,7 +194,7 @@ struct KeyWalk {
 template <int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_fwd_f32_kernel(const WindowParams p) {
     KeyWalk x;
-    if (!x.begin(p)) return;
+    x.begin(p);
     Across<DP> q;
     q.load(x.place(p.q, x.r, p), p.D, x.g);
     if (p.negative)
@@ -284,7 +283,7 @@ template <int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dq_f32_kernel(const WindowParams p) {
     __shared__ __attribute__((aligned(16))) Rows<DP> rows;
     KeyWalk x;
-    if (!x.begin(p)) return;
+    x.begin(p);
     Across<DP> q, d, k, v;
     q.load(x.place(p.q, x.r, p), p.D, x.g);
     d.load(x.place(p.dout, x.r, p), p.D, x.g);
@@ -332,7 +331,7 @@ template <int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dkv_f32_kernel(const WindowParams p) {
     __shared__ __attribute__((aligned(16))) Rows<DP> q_rows, d_rows;
     int pair, block;
-    if (!work_item(p, blockIdx.x, pair, block)) return;
+    work_item(p, blockIdx.x, pair, block);
     const int b = pair / p.HK, hk = pair - b * p.HK;
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), n = lane & 15, g = lane >> 4;
     const int j0 = WINDOW_KEYS_F32 * block, j = j0 + n;
@@ -401,7 +400,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dkv_f32_kernel(
     store(d_rows, p.dv);
 }
 
-dim3 grid_of(const WindowParams& p) { return dim3((unsigned)(((int64_t)p.B * p.HK * p.blocks + 7) / 8 * 8), p.splits); }
+dim3 grid_of(const WindowParams& p) { return dim3((unsigned)((int64_t)p.B * p.HK * p.blocks), p.splits); }
 
 template <int DP>
 int launch_bwd(const WindowParams& p, hipStream_t stream) {
