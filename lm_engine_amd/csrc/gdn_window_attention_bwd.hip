@@ -6,9 +6,12 @@
 // with a lane a key (S = Q K^T) for dv^T += do^T w and dk^T += q^T ds.
 // A sequence's first keys are seen by all of its rows: those beyond the window are shared out over many workgroups, in a launch of their own, and
 // the parts joined by another.  Where there are few blocks of keys, the rows of each are cut into shares, joined in the same way.
-// Rounding: w and ds become bf16 for the second product of each pass (at most half a step, 2^-8 of the value; 1.6e-3 rms), and delta is that of the
-// output as the forward stored it, w rounded for its product and o rounded again.  For dq and dk that is, in rms of their norm, 1.8e-3 from ds,
-// 1.3e-3 from delta and 1.7e-3 from their own rounding: 2.8e-3 where a computation in fp32 that rounds once has 1.7e-3.
+// Rounding: w and ds become bf16 for the second product of each pass, at most half a step (2^-8) of the value; everything else is fp32.  delta from the
+// output as it is stored, rounded and made of rounded weights, would be off by 1e-3, which goes into dq and dk times the mean of the keys and
+// queries.  But sum_j ds_j = 0: what that sum is short of zero is delta's error.  window_dq_kernel forms it, and leaves the exact
+// delta for dk; where it matters for dq (few keys, or keys with a mean; see there) it walks over the keys once more.  In rms of dq and dk:
+// 1.8e-3 from ds and 1.7e-3 from their own rounding, 2.4e-3 together, where delta from the output gave 2.8e-3; with keys, queries and values whose mean is
+// as large as their spread 2.6e-3 instead of 1.0e-2 (1200 tokens, 64 columns), with twice that mean 4.3e-3 instead of 3.7e-2 (window 500, 128).
 // Bound by the matrix unit together with the exponentials and the products' operands from LDS: at 4 x 4096 tokens, 16 heads of 128 over 2, window
 // 1024 and 4 first keys dq takes 224 us (805 TFLOP/s), the keys' 330 (670), the first keys' 27 and 4.5 to join them.  With 64 columns, where a score
 // has half the products but the same exponential, 530 and 440 TFLOP/s (6 x 1500, 16 heads over 8, all keys).
@@ -20,6 +23,13 @@
 namespace gdn {
 
 namespace {
+
+// window_dq_kernel walks over a block's keys twice, the first time for the exact delta, where they are this many tiles (of 64) or fewer, as few keys
+// have large weights, with errors that do not average out: 4 x 4096 tokens, 16 heads over 2, window 64 159 us backward instead of 142.  With more, a
+// second walk follows where delta's error, times the mean of 64 of the keys, is over REST of a wave's dq: not for keys without a mean
+// (4 x 4096, 16 heads of 128 over 2, window 1024: 578 us backward, with the sum and the question; 560 without, 696 with two walks everywhere).
+constexpr int EXACT_TILES = 4;
+constexpr float REST = 0x1p-10f;
 
 template <int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dq_kernel(const WindowParams p) {
@@ -47,13 +57,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dq_kernel(const
 #pragma unroll
             for (int e = 0; e < 8; e++) delta += (float)o[s][e] * (float)d[s][e];
         delta += other_half(delta);
-        if (half == 0 && row < p.rows) p.delta[scalar] = delta;
     }
     const float lse = p.lse[scalar], c = p.negative ? -p.c : p.c;
 
     const RowView view = row_view(p, b, r);
     const WaveView w = wave_view(view);
     __shared__ int bounds[4][6];
+    __shared__ float columns[4][DP];
     const WaveView all = join_waves<4>(w, bounds, wave, lane);
     const int lo = all.lo, end = all.end, sink = all.sink, sink_end = min(all.sink_end, lo);
     const int sink_tiles = sink_end > sink ? (sink_end - sink + 63) / 64 : 0, near_tiles = end > lo ? (end - lo + 63) / 64 : 0;
@@ -67,11 +77,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dq_kernel(const
         j0 = s ? sink + 64 * i : lo + 64 * (i - sink_tiles);
         count = min((s ? sink_end : end) - j0, 64);
     };
-    auto load_tile = [&](int i) {
+    auto load_tile = [&](int i, int buffer) {
         int j0, count;
         tile_at(i, j0, count);
         const char *const k0 = kb + (int64_t)j0 * p.k.t * 2, *const v0 = vb + (int64_t)j0 * p.v.t * 2;
-        const uint32_t to = lds + (i & 1) * 2 * 64 * DP * 2;
+        const uint32_t to = lds + buffer * 2 * 64 * DP * 2;
 #pragma unroll
         for (int x = 0; x < Loads::ITERS; x++) {
             const int kr = Loads::row(wave, lane, x), col = Loads::column(wave, lane, x);
@@ -83,15 +93,52 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dq_kernel(const
 
     const TileReader<DP> reader(lane);
     f32x16 dq[DT] = {};
-    if (tile_count > 0) load_tile(0);
-    for (int i = 0; i < tile_count; i++) {
+    float sum = 0.f;  // of ds: what delta lacks, since the weights add up to 1
+    const int before = tile_count <= EXACT_TILES ? tile_count : 0;  // steps of the first walk
+    if (tile_count > 0) load_tile(0, 0);
+    bool exact = before > 0;
+    int buffer = 1;
+    for (int step = -before;; step++) {
+        if (step == tile_count) {
+            if (exact || tile_count == 0) break;
+            // what delta's error has done to this wave's rows, against the rows themselves
+            const float rest = sum + other_half(sum);
+            float own = 0.f, mean = 0.f;
+#pragma unroll
+            for (int z = 0; z < DT; z++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) own = __builtin_fmaf(dq[z][e], dq[z][e], own);
+            for (int x = lane; x < DP; x += WAVE) {
+                const float k = (columns[0][x] + columns[1][x] + columns[2][x] + columns[3][x]) * (1.f / 64);
+                mean = __builtin_fmaf(k, k, mean);
+            }
+            const float most = wave_sum(rest * rest * 0.5f) * wave_sum(mean);
+            if (__syncthreads_or(!(most <= REST * REST * wave_sum(own))) == 0) break;
+            exact = true, step = 0;
+            delta += rest, sum = 0.f;
+#pragma unroll
+            for (int z = 0; z < DT; z++) dq[z] = f32x16{};
+            buffer = 1;
+            load_tile(0, 0);
+        }
+        if (step == 0 && before > 0) delta += sum + other_half(sum), sum = 0.f;
+        const int i = step < 0 ? step + tile_count : step;
         loads_done();
         __syncthreads();
-        if (i + 1 < tile_count) load_tile(i + 1);
+        buffer ^= 1;
+        if (step + 1 < tile_count) load_tile(i + 1 == tile_count ? 0 : i + 1, buffer ^ 1);
         int j0, count;
         tile_at(i, j0, count);
-        const bf16_t *const kt = tiles[i & 1][0], *const vt = tiles[i & 1][1];
+        const bf16_t *const kt = tiles[buffer][0], *const vt = tiles[buffer][1];
         const bool near = i >= sink_tiles, full = near && j0 >= w.full_lo && j0 + 64 <= w.full_end;
+        if (step == tile_count - 2 && !exact) {  // 64 keys that are there: their sum, 16 of them a wave's
+            stay_a_branch();
+            for (int x = lane; x < DP; x += WAVE) {
+                float k = 0.f;
+                for (int y = 16 * wave; y < 16 * wave + 16; y++) k += (float)kt[y * DP + (((x >> 3) ^ tile_key<DP>(y)) << 3) + (x & 7)];
+                columns[wave][x] = k;
+            }
+        }
         if (!w.meets(j0, count)) continue;
         const TileView own(view, near, sink_end);
 #pragma unroll
@@ -114,6 +161,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dq_kernel(const
                 }
             }
 #pragma unroll
+            for (int e = 0; e < 16; e++) sum += s[e];
+            if (step < 0) continue;
+#pragma unroll
             for (int y = 0; y < 2; y++) {
                 const bf16x8 ds = pack8(s, y);
 #pragma unroll
@@ -121,8 +171,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dq_kernel(const
             }
         }
     }
-    if (row >= p.rows) return;
-    store_transposed<DP>(static_cast<bf16_t*>(const_cast<void*>(p.dq.p)) + b * p.dq.b + t * p.dq.t + head * p.dq.h, p.D, half, dq, p.scale);
+    delta += sum + other_half(sum);
+    int last = row;
+    asm volatile("" : "+v"(last));  // (what follows from it is formed anew, rather than kept in registers over the walk)
+    if (last >= p.rows) return;
+    const int last_t = p.G == 1 ? last : last / p.G, last_head = hk * p.G + (last - last_t * p.G);
+    if (half == 0) p.delta[((int64_t)b * p.T + last_t) * p.H + last_head] = delta;
+    store_transposed<DP>(static_cast<bf16_t*>(const_cast<void*>(p.dq.p)) + b * p.dq.b + last_t * p.dq.t + last_head * p.dq.h, p.D, half, dq, p.scale);
 }
 
 // Gradients of KEYS keys.  The keys and values lie in LDS for the whole walk, so that a wave's registers are its sums': two waves on a SIMD, one

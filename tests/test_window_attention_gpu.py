@@ -117,3 +117,35 @@ def test_other_keys_than_queries(T, S, window, sinks, dtype):
 def test_scales(scale):
     for dtype in (BF16, F32):
         check_call(*inputs(1, 150, 2, 1, 64, dtype=dtype), dtype, window=100, sinks=3, scale=scale)
+
+
+@pytest.mark.parametrize("T, H, HK, D, window", [(1200, 4, 2, 64, None), (900, 4, 2, 128, 500), (600, 2, 1, 256, 400), (300, 4, 2, 64, 8)])
+def test_gradients_where_keys_and_values_have_a_mean(T, H, HK, D, window):
+    """The sum of a row's ds is zero, and what is left of it comes back times the mean key: 1e-2 of dq's norm and more here, if delta were formed
+    from the rounded output.  Exact sums leave ds's rounding (rms 2^-8 / sqrt(3) at most of terms that are up to sqrt(2) of dq's size, since a key is
+    its mean and a difference of the same size: 3.2e-3) and the result's own (2.3e-3): 4e-3, and half as much again for the few rows whose
+    weights are nearly all on one key."""
+    gen = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(1, T, h, D, generator=gen) + torch.randn(D, generator=gen) for h in (H, HK, HK))
+    q, k, v = (x.to(BF16) for x in (q, k, v))
+    do = torch.randn(1, T, H, D, generator=gen).to(BF16)
+    leaves = [x.cuda().requires_grad_() for x in (q, k, v)]
+    got = torch.autograd.grad(sliding_window_attention(*leaves, window=window), leaves, do.cuda())
+    ref = [x.double().requires_grad_() for x in (q, k, v)]
+    want = torch.autograd.grad(window_attention_ref(*ref, window=window), ref, do.double())
+    for name, x, y in zip(("dq", "dk", "dv"), got, want):
+        check(name, x, y, 6e-3)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_window_of_one_has_no_gradients_of_scores(dtype):
+    """Each query sees itself alone: o = v, and dq, dk are zero but for fp32 sums of D terms (1e-6 each of |do . v|, times |k| scale).  In fp32 o is
+    v w (1 / w) with w = 2^(c s - m), where m is c s rounded and c s is not: w is next to 1 but not 1, and the two products and the quotient are
+    rounded, 3 times 2^-24 of the value."""
+    q, k, v = inputs(1, 300, 4, 2, 64, dtype=dtype)
+    leaves = [x.cuda().requires_grad_() for x in (q, k, v)]
+    o = sliding_window_attention(*leaves, window=1)
+    dq, dk, dv = torch.autograd.grad(o, leaves, torch.ones_like(o))
+    values = leaves[2].repeat_interleave(2, dim=2)
+    assert ((o - values).abs() <= (0 if dtype == BF16 else 4 * 2**-24) * values.abs()).all() and (dv - 2).abs().max() <= 2**-6
+    assert dq.abs().max() <= 1e-4 and dk.abs().max() <= 1e-4
