@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attn_kernel(cons
     x /= p.row_tiles;
     const int hk = x % p.c.HK, n = x / p.c.HK, split = blockIdx.y;
     const int P = p.c.P, D = p.c.D;
-    const int length = min(p.lengths[n], p.c.table_pages * P);
+    const int length = min(max(p.lengths[n], 0), p.c.table_pages * P);
     const int row = ROWS * tile + i16, r = min(row, p.rows - 1), t = p.G == 1 ? r : r / p.G, head = hk * p.G + (r - t * p.G);
 
     bf16x8 q[2 * U];

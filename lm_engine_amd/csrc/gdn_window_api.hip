@@ -161,6 +161,7 @@ extern "C" int gdn_window_attn_bwd(const gdn_window_attn_bwd_args* args, void* s
     if (const int e = check_rows(b.dk, b.dk_stride_b, b.dk_stride_t, b.dk_stride_h, a.HK, a.dtype); e != GDN_OK) return e;
     if (const int e = check_rows(b.dv, b.dv_stride_b, b.dv_stride_t, b.dv_stride_h, a.HK, a.dtype); e != GDN_OK) return e;
     WindowParams p = params_of(a);
+    if ((uint64_t)p.N * p.HK * first_keys_of(p) > INT32_MAX) return GDN_ERR_UNSUPPORTED;  // a workgroup each, in the join
     if (b.workspace == nullptr || b.workspace_bytes < backward_bytes(a, p)) return GDN_ERR_WORKSPACE;
     if (!on16(b.workspace)) return GDN_ERR_ALIGN;
     p.dout = {b.dout, b.dout_stride_b, b.dout_stride_t, b.dout_stride_h};

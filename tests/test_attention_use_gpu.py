@@ -443,3 +443,59 @@ def test_a_run_of_them_together():
         check("single tokens, on the codes' values", out, exact, 1e-2)
         drafts = paged_cache_attention(a[:, prompt:].contiguous(), cache, table, lengths, window=window, sinks=sinks)  # the same tokens at once
         check("drafts", drafts, exact, OUT[BF16])
+
+
+def test_lengths_out_of_range():
+    """Below zero: no key is seen.  Past the table: what the table has."""
+    cache, table, lengths, _ = filled([70, 70, 70, 70], 2, 64, 16)
+    q = torch.randn(4, 3, 4, 64).to(BF16).cuda()
+    odd = torch.tensor([-(2**31), -1, 2**31 - 1, 70], dtype=torch.int32).cuda()
+    for window, sinks in ((None, 0), (20, 4)):
+        o = paged_cache_attention(q, cache, table, odd, window=window, sinks=sinks)
+        assert (o[:2] == 0).all() and o.isfinite().all()
+        at_end = torch.tensor([0, 0, table.size(1) * 16, 70], dtype=torch.int32).cuda()
+        assert torch.equal(o, paged_cache_attention(q, cache, table, at_end, window=window, sinks=sinks))
+    k, _ = read_paged_cache(cache, table, odd, 70)
+    assert (k[:2] == 0).all() and torch.equal(k[2:], read_paged_cache(cache, table, lengths, 70)[0][2:])
+
+
+def test_a_cache_past_32_bits():
+    """Pages of 512 KB, the last ones beyond 4 GB of codes: as in a small cache."""
+    HK, P, D, pages = 8, 256, 256, 8300
+    gen = torch.Generator("cuda").manual_seed(4)
+    k, v = (torch.randn(1, 700, HK, D, device="cuda", generator=gen).to(BF16) for _ in range(2))
+    q = torch.randn(1, 2, 16, D, device="cuda", generator=gen).to(BF16)
+    results = []
+    for total, table in ((4, [[1, 3, 0]]), (pages, [[8298, 8299, 8200]])):
+        cache = new_paged_cache(total, HK, D, page_size=P)
+        table = torch.tensor(table, dtype=torch.int32).cuda()
+        start = torch.zeros(1, dtype=torch.int32, device="cuda")
+        write_paged_cache(cache, k[:, :699], v[:, :699], table, start)
+        write_paged_cache(cache, k[:, 699:], v[:, 699:], table, start + 699)
+        results.append((paged_cache_attention(q, cache, table, start + 700), *read_paged_cache(cache, table, start + 700, 700)))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_rows_past_32_bits():
+    """Tensors of more than 2^31 elements: the last tokens as in a call that has only them and what they see."""
+    T, H, HK, D, window = 140000, 64, 8, 256, 64
+    q, k, v, do = (torch.empty(1, T, h, D, dtype=BF16, device="cuda").normal_() for h in (H, HK, HK, H))
+    assert q.numel() > 2**31
+    few = 256
+    tail = [x[:, T - few :].clone().requires_grad_() for x in (q, k, v)]
+    want = sliding_window_attention(*tail, window=window)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    o = sliding_window_attention(*leaves, window=window)
+    assert rel_l2(o[:, T - few + window :].detach().cpu(), want[:, window:].detach().cpu()) <= 2 * OUT[BF16]
+    do[:, : T - few + window] = 0  # (so that both have the same gradients of the last keys and queries)
+    got = torch.autograd.grad(o, leaves, do)
+    expected = torch.autograd.grad(want, tail, do[:, T - few :].clone())
+    for name, a, b in zip(("dq", "dk", "dv"), got, expected):
+        check(name, a[:, T - few :].cpu(), b.cpu(), 2 * 1e-2)
+        assert (a[:, : T - few] == 0).all()
+    with torch.no_grad():
+        cos, sin = rotary_table(T, D)
+        a, b = qk_norm_rotary(q, k, None, None, cos, sin)
+        at = torch.arange(T - 100, T, dtype=torch.int32, device="cuda")
+        c, d = qk_norm_rotary(q[:, T - 100 :], k[:, T - 100 :], None, None, cos, sin, at)
+        assert torch.equal(a[:, T - 100 :], c) and torch.equal(b[:, T - 100 :], d)
