@@ -8,8 +8,8 @@
 // Rounding: the weights become bf16 for the second product, at most half a step (2^-8) of each, 1.7e-3 rms of the output's norm; their sum l is of the
 // weights before that.  Everything else is fp32 up to the output's own rounding.
 // Bound by the matrix unit and the exponentials beside it: 4 x 4096 tokens, 16 heads of 128 over 2, window 1024 and 4 first keys 157 us
-// (770 TFLOP/s; a large library product reaches 1165), all keys 287 (770).  128 rows and four waves, two workgroups to a compute unit: 256 rows and
-// eight waves took 178 instead of 158 us.  With 64 columns, where the exponentials alone take twice the products' time, 413 TFLOP/s.  Small calls
+// (770 TFLOP/s; a large library product reaches 1165), over 16 and all keys 302 (910).  128 rows and four waves, two workgroups to a compute unit: 256 rows and
+// eight waves took 178 instead of 158 us.  With 64 columns, where the exponentials alone take twice the products' time, 700 TFLOP/s.  Small calls
 // are bound by latency, 8 to 14 us: a launch's instructions come from L2 once, and one workgroup after the other finds the same.
 #include <algorithm>
 

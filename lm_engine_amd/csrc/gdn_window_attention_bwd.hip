@@ -13,8 +13,8 @@
 // 1.8e-3 from ds and 1.7e-3 from their own rounding, 2.4e-3 together, where delta from the output gave 2.8e-3; with keys, queries and values whose mean is
 // as large as their spread 2.6e-3 instead of 1.0e-2 (1200 tokens, 64 columns), with twice that mean 4.3e-3 instead of 3.7e-2 (window 500, 128).
 // Bound by the matrix unit together with the exponentials and the products' operands from LDS: at 4 x 4096 tokens, 16 heads of 128 over 2, window
-// 1024 and 4 first keys dq takes 224 us (805 TFLOP/s), the keys' 330 (670), the first keys' 27 and 4.5 to join them.  With 64 columns, where a score
-// has half the products but the same exponential, 530 and 440 TFLOP/s (6 x 1500, 16 heads over 8, all keys).
+// 1024 and 4 first keys dq takes 228 us (790 TFLOP/s), the keys' 302 (740), the first keys' 26 and 5 to join them.  With 64 columns, where a score
+// has half the products but the same exponential, 950 and 800 TFLOP/s (4 x 4096, 16 heads, all keys) beside 980 and 840 with 128.
 #include <algorithm>
 
 #include "gdn_launch.h"
