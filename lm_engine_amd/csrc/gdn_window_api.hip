@@ -90,7 +90,8 @@ uint64_t workspace_of(const gdn_window_attn_args& a) {
 // The parts in which rows beyond the window are shared out for a sequence's first keys: about one workgroup a compute unit in all, 256 rows or
 // more to each.  (Half or twice as many: backward 549 and 550 us instead of 543 at 4 x 4096, 16 heads of 128 over 2, window 1024, 4 first keys.)
 int pieces_of(const WindowParams& p, int dtype) {
-    if (dtype != GDN_BF16 || p.sinks == 0) return 0;
+    // (first keys of more places than there are tokens: sequences of which most are first keys, which the blocks' own walks take as they come)
+    if (dtype != GDN_BF16 || p.sinks == 0 || (int64_t)p.N * p.sinks > (int64_t)p.B * p.S) return 0;
     const int64_t blocks = (int64_t)p.N * p.HK * ((p.sinks + WINDOW_FIRST_KEYS - 1) / WINDOW_FIRST_KEYS), rows = (int64_t)p.T * p.G;
     return (int)std::max<int64_t>(1, std::min<int64_t>(compute_units() / blocks, (rows + 255) / 256));
 }
@@ -161,7 +162,7 @@ extern "C" int gdn_window_attn_bwd(const gdn_window_attn_bwd_args* args, void* s
     if (const int e = check_rows(b.dk, b.dk_stride_b, b.dk_stride_t, b.dk_stride_h, a.HK, a.dtype); e != GDN_OK) return e;
     if (const int e = check_rows(b.dv, b.dv_stride_b, b.dv_stride_t, b.dv_stride_h, a.HK, a.dtype); e != GDN_OK) return e;
     WindowParams p = params_of(a);
-    if ((uint64_t)p.N * p.HK * first_keys_of(p) > INT32_MAX) return GDN_ERR_UNSUPPORTED;  // a workgroup each, in the join
+    if (pieces_of(p, a.dtype) > 0 && (uint64_t)p.N * p.HK * first_keys_of(p) > INT32_MAX) return GDN_ERR_UNSUPPORTED;  // a workgroup each, in the join
     if (b.workspace == nullptr || b.workspace_bytes < backward_bytes(a, p)) return GDN_ERR_WORKSPACE;
     if (!on16(b.workspace)) return GDN_ERR_ALIGN;
     p.dout = {b.dout, b.dout_stride_b, b.dout_stride_t, b.dout_stride_h};

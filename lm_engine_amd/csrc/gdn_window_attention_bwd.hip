@@ -227,7 +227,7 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, DP == 64 ? 3 : DP == 128 ? 2
         if (!FIRST) n = sequence;
         if (en > st) {
             if (FIRST) from = p.window < en - j ? j + p.window : 1 << 30, upto = from < en ? en - 1 : -1;
-            else from = j, upto = p.window == 0 || p.window >= en - j ? en - 1 : j + p.window - 1;
+            else from = j, upto = p.window == 0 || p.window >= en - j || (p.pieces == 0 && j - st < p.sinks) ? en - 1 : j + p.window - 1;
             from = max(from, p.S - p.T);  // (positions in front of the queries)
             if (upto < from) from = 1 << 30, upto = -1;
         }

@@ -149,3 +149,14 @@ def test_a_window_of_one_has_no_gradients_of_scores(dtype):
     values = leaves[2].repeat_interleave(2, dim=2)
     assert ((o - values).abs() <= (0 if dtype == BF16 else 4 * 2**-24) * values.abs()).all() and (dv - 2).abs().max() <= 2**-6
     assert dq.abs().max() <= 1e-4 and dk.abs().max() <= 1e-4
+
+
+@pytest.mark.parametrize("sinks", [4, 11, 100, 1 << 20])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_many_sequences_that_are_first_keys_for_the_most_part(sinks, D):
+    """Their gradients need no more memory than there are tokens."""
+    lens = [1, 30, 2, 17, 64, 5, 5, 90, 12, 3, 40, 7, 0, 33, 1, 26]
+    torch.cuda.reset_peak_memory_stats()
+    q, k, v = inputs(1, sum(lens), 4, 2, D)
+    check_call(q, k, v, BF16, cu_of(lens), window=6, sinks=sinks)
+    assert torch.cuda.max_memory_allocated() < 1 << 30
