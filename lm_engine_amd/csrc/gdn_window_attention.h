@@ -276,10 +276,11 @@ __device__ __forceinline__ void store_transposed(bf16_t* row, int D, int half, c
 constexpr float LOWEST = -3.402823466e38f;
 
 // What a forward took out of tiles that not all of its rows see (values that are not finite), added to the results of the rows that see it: a
-// few threads a row, behind the stores of the whole workgroup.  An infinite value stays what it is under any weight, and NaN too.
+// few threads a row, behind the stores of the whole workgroup.  An infinite value stays what it is under any weight, and NaN too.  `width`: keys of
+// a whole tile, by which the walk tells which tiles all rows see all of; a last tile that ends with the keys is not one of them.
 template <typename T, typename TileAt>
 __device__ __forceinline__ void add_taken_out(const WindowParams& p, int b, int hk, int r0, int rows, const WaveView& all, int first_tile, int last_tile, int sink_tiles,
-                                           const TileAt& tile_at, int64_t part) {
+                                           int width, const TileAt& tile_at, int64_t part) {
     __syncthreads();
     const int each = (int)blockDim.x / rows, own = r0 + (int)threadIdx.x / each;
     if (own >= p.rows) return;
@@ -289,7 +290,7 @@ __device__ __forceinline__ void add_taken_out(const WindowParams& p, int b, int 
     for (int i = first_tile; i < last_tile; i++) {
         int j0, count;
         tile_at(i, j0, count);
-        if (i >= sink_tiles && j0 >= all.full_lo && j0 + count <= all.full_end) continue;
+        if (i >= sink_tiles && j0 >= all.full_lo && j0 + width <= all.full_end) continue;
         for (int j = max(j0, v.st); j < j0 + count && j <= v.a; j++) {
             if (j < v.lo && j >= v.sk) continue;
             const T* const value = static_cast<const T*>(p.v.p) + b * p.v.b + j * p.v.t + hk * p.v.h;

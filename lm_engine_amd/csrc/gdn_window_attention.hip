@@ -272,7 +272,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_fwd_kernel(cons
         }
     }
     if (!taken_out) return;
-    add_taken_out<bf16_t>(p, b, hk, r0, WINDOW_ROWS, all, first_tile, last_tile, sink_tiles, tile_at, part);
+    add_taken_out<bf16_t>(p, b, hk, r0, WINDOW_ROWS, all, first_tile, last_tile, sink_tiles, 64, tile_at, part);
 }
 
 // The parts of a row joined: a workgroup a row.

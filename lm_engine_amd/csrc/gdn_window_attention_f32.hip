@@ -276,7 +276,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_fwd_f32_kernel(
         else if (p.lse != nullptr) p.lse[2 * scalar] = l == 0.f ? 0.f : m, p.lse[2 * scalar + 1] = inverse(l);
     }
     if (__syncthreads_or(taken_out))
-        add_taken_out<float>(p, x.b, x.hk, x.r0, WINDOW_ROWS_F32, x.all, first, last, x.sink_tiles, [&](int y, int& j0, int& count) { x.tile_at(y, j0, count); }, part);
+        add_taken_out<float>(p, x.b, x.hk, x.r0, WINDOW_ROWS_F32, x.all, first, last, x.sink_tiles, TILE, [&](int y, int& j0, int& count) { x.tile_at(y, j0, count); }, part);
 }
 
 template <int DP>

@@ -499,3 +499,21 @@ def test_rows_past_32_bits():
         at = torch.arange(T - 100, T, dtype=torch.int32, device="cuda")
         c, d = qk_norm_rotary(q[:, T - 100 :], k[:, T - 100 :], None, None, cos, sin, at)
         assert torch.equal(a[:, T - 100 :], c) and torch.equal(b[:, T - 100 :], d)
+
+
+@pytest.mark.parametrize("dtype, T, S, H, HK, window", [
+    (BF16, 1, 50, 4, 2, None), (BF16, 1, 700, 2, 2, None), (BF16, 1, 700, 4, 2, 333), (BF16, 129, 129, 2, 2, None), (BF16, 257, 257, 1, 1, 70), (BF16, 33, 33, 128, 1, None),
+    (F32, 1, 50, 4, 2, None), (F32, 1, 700, 2, 2, None), (F32, 40, 40, 16, 1, None), (F32, 40, 40, 16, 1, 21), (F32, 17, 17, 2, 2, None),
+], ids=str)  # fmt: skip
+def test_values_that_are_not_finite_in_the_last_keys_of_rows_at_one_position(dtype, T, S, H, HK, window):
+    """Blocks whose rows all stand at the last key's position: their last tile of keys ends with what they see, and is not whole."""
+    q, k, v = inputs(1, T, H, HK, 64, S=S, dtype=dtype)
+    for at in {S - 1, S - 2, (S - 1) // 16 * 16, (S - 1) // 64 * 64, S // 2}:
+        for value, d in ((float("nan"), 3), (float("inf"), 63), (-float("inf"), 0)):
+            dirty = v.clone()
+            dirty[0, at, HK - 1, d] = value
+            want = window_attention_ref(q, k, dirty, window=window)
+            got = sliding_window_attention(*cuda(q, k, dirty), window=window).cpu()
+            assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf()), (at, value)
+            fine = want.isfinite()
+            assert rel_l2(got[fine], want[fine]) <= OUT[dtype], (at, value)
