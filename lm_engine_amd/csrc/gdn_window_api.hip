@@ -17,8 +17,8 @@ int check_rows(const void* p, int64_t b, int64_t t, int64_t h, int heads, int dt
     const int64_t vec = dtype == GDN_BF16 ? 8 : 4;
     if (p == nullptr) return GDN_ERR_NULL;
     if (!on16(p) || b % vec != 0 || t % vec != 0 || h % vec != 0) return GDN_ERR_ALIGN;
-    // the bytes of 64 tokens and of a token's heads are counted in 32 bits, without a sign
-    if (t < 0 || t > 1 << 23 || h < 0 || h > ((int64_t)1 << 28) / heads) return GDN_ERR_UNSUPPORTED;
+    // the bytes from a base to the rows that a wave loads, or to 128 keys, are counted in 31 bits (row_offsets_fit, at each kernel's tiles)
+    if (t < 0 || t > MOST_APART || h < 0 || h > MOST_HEADS / heads) return GDN_ERR_UNSUPPORTED;
     return GDN_OK;
 }
 

@@ -164,6 +164,10 @@ __device__ __forceinline__ void work_item(const WindowParams& p, int x, int& pai
 // read past the buffer's end, which gives zeros.
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 constexpr uint32_t PAST = 0x80000000u;
+// What rows may lie apart, in elements: one token and the next, and the heads of a token in all (gdn_window_api.hip refuses more).
+constexpr int64_t MOST_APART = 1 << 23, MOST_HEADS = 1 << 28;
+// whether the bytes from one base to every column of `rows` rows (tokens, or heads of as many tokens and one more begun) stay below PAST
+constexpr bool row_offsets_fit(int rows, bool heads) { return ((rows - (heads ? 0 : 1)) * MOST_APART + (heads ? MOST_HEADS : 0) + 256) * 2 < PAST; }
 template <int DP, int WROWS = 16>
 struct TileLoads {
     static constexpr int GRANULES = DP / 8, RPI = 64 / GRANULES, ITERS = WROWS / RPI;

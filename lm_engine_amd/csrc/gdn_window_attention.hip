@@ -38,6 +38,7 @@ template <int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_fwd_kernel(const WindowParams p) {
     constexpr int KS = DP / 16, DT = DP / 32;
     using Loads = TileLoads<DP>;
+    static_assert(row_offsets_fit(64, false));
     __shared__ __attribute__((aligned(1024))) bf16_t tiles[2][2][64 * DP];  // keys, values; tiles in turn
     int pair, block;
     work_item(p, blockIdx.x, pair, block);

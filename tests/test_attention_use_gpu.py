@@ -517,3 +517,23 @@ def test_values_that_are_not_finite_in_the_last_keys_of_rows_at_one_position(dty
             assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf()), (at, value)
             fine = want.isfinite()
             assert rel_l2(got[fine], want[fine]) <= OUT[dtype], (at, value)
+
+
+# (T, H, HK, D, elements between tokens, between heads): each within what is read as it lies
+@pytest.mark.parametrize("T, H, HK, D, apart, heads_apart", [
+    (384, 1, 1, 128, 1 << 23, 128), (511, 1, 1, 72, (1 << 22) + (1 << 17), 128), (384, 2, 1, 128, 1 << 23, (1 << 27) - 1024), (300, 1, 1, 64, 1 << 23, 64),
+    (384, 2, 1, 64, 1 << 23, (1 << 27) - 1024), (300, 2, 1, 256, 1 << 23, (1 << 27) - 1024), (300, 3, 1, 128, 1 << 23, 89478480),
+])  # fmt: skip
+def test_gradients_of_first_keys_from_tokens_that_lie_far_apart(T, H, HK, D, apart, heads_apart):
+    """Queries and their gradients 2^23 elements apart, of more rows than one tile has: the results of dense copies, to the bit."""
+    buffer = torch.empty(T * apart + H * heads_apart + 1024, dtype=BF16, device="cuda")
+    q, k, v = cuda(*inputs(1, T, H, HK, D))
+    do = torch.randn(1, T, H, D, device="cuda").to(BF16)
+    far_q, far_do = (buffer[first:].as_strided((1, T, H, D), (T * apart, apart, heads_apart, 1)) for first in (0, 512))
+    far_q.copy_(q), far_do.copy_(do)
+    grads = []
+    for x, d in ((far_q, far_do), (q, do)):
+        leaves = [y.detach().requires_grad_() for y in (x, k, v)]
+        grads.append(torch.autograd.grad(sliding_window_attention(*leaves, window=8, sinks=4), leaves, d))
+    for name, a, b in zip(("dq", "dk", "dv"), *grads):
+        assert torch.equal(a, b), name
