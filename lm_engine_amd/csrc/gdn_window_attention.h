@@ -26,7 +26,7 @@ struct WindowParams {
     int padded;
     int B, T, S, H, HK, G, D, N;
     int rows;         // T G
-    uint32_t by_g;    // ceil(2^32 / G): n / G = umulhi(n, by_g) for small n
+    uint32_t by_g;    // ceil(2^32 / G), for split_rows
     int window, sinks;  // window 0: every key
     float scale, c;   // c = |scale| log2(e)
     int negative;     // of scale
@@ -43,9 +43,12 @@ struct WindowParams {
     float* part_all;  // [shares, B, HK, S, 2, D]
 };
 
-// n / G and the rest, for n < 2^16
+// n / G and the rest, for n < G + 256.  by_g is less than 1 / G too large in units of 2^32 / G, so that n by_g / 2^32 is n / G rounded down as long as
+// n G < 2^32; there are two tokens at most for more heads to one than that holds for.
+constexpr int MOST_BY_PRODUCT = 65280;
+static_assert((uint64_t)MOST_BY_PRODUCT * (MOST_BY_PRODUCT + 256) < (uint64_t)1 << 32);
 __device__ __forceinline__ void split_rows(const WindowParams& p, int n, int& t, int& g) {
-    t = p.G == 1 ? n : (int)__umulhi((unsigned)n, p.by_g);
+    t = p.G == 1 ? n : p.G > MOST_BY_PRODUCT ? (n >= p.G ? 1 : 0) : (int)__umulhi((unsigned)n, p.by_g);
     g = n - t * p.G;
 }
 

@@ -18,7 +18,7 @@ from lm_engine_amd import (
 from oracle.attention_oracle import attend, norm_rotary_ref, visible_keys, window_attention_ref
 from tests.helpers import rel_l2
 from tests.test_paged_cache_gpu import filled
-from tests.test_window_attention_gpu import BF16, F32, OUT, check, cu_of, inputs
+from tests.test_window_attention_gpu import BF16, F32, GRAD, OUT, check, cu_of, inputs
 
 
 pytestmark = pytest.mark.gpu
@@ -537,3 +537,20 @@ def test_gradients_of_first_keys_from_tokens_that_lie_far_apart(T, H, HK, D, apa
         grads.append(torch.autograd.grad(sliding_window_attention(*leaves, window=8, sinks=4), leaves, d))
     for name, a, b in zip(("dq", "dk", "dv"), *grads):
         assert torch.equal(a, b), name
+
+
+def test_more_heads_to_one_than_a_division_by_multiplication_holds():
+    """Rows are taken apart into tokens and heads: 2^32 / H rounded up, times the last head of a token, is the next one here."""
+    T, H, D = 3, 65537, 8
+    assert ((H - 1) * -(-(2**32) // H)) >> 32 != 0
+    q, k, v = cuda(*inputs(1, T, H, 1, D))
+    do = torch.zeros(1, T, H, D, device="cuda", dtype=BF16)
+    do[:, :, -1] = 1
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    got = torch.autograd.grad(sliding_window_attention(*leaves), leaves, do)
+    ref = [x.detach().double().requires_grad_() for x in leaves]
+    scores = (ref[0][0].transpose(0, 1) @ ref[1][0, :, 0].T) * D**-0.5
+    weights = scores.masked_fill(torch.ones(T, T, device="cuda").triu(1) > 0, -torch.inf).softmax(-1)
+    want = torch.autograd.grad((weights @ ref[2][0, :, 0]).transpose(0, 1)[None], ref, do.double())
+    for name, a, b in zip(("dq", "dk", "dv"), got, want):
+        check(name, a.cpu(), b.cpu(), GRAD[BF16])
