@@ -54,8 +54,6 @@ def _check(q, k, q_weight, k_weight, cos, sin, positions) -> None:
     R = 2 * cos.size(1)
     if R == 0 or R % 8 != 0 or R > D or cos.size(0) == 0:
         raise ValueError(f"the tables rotate R={R} dims; a multiple of 8, at most D={D}, and at least one position are needed")
-    if cos.requires_grad or sin.requires_grad:
-        raise ValueError("cos and sin are constants: they get no gradient")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None:
             if tuple(w.shape) != (D,):
@@ -174,13 +172,15 @@ def qk_norm_rotary(
     None (token t stands at position t).  Returns the normed and rotated q and k, contiguous, computed in fp32 and rounded once.
 
     D and R are multiples of 8, D at most 512.  A position that the tables do not have makes its rows NaN.  Differentiable in q, k and the
-    weights, but neither twice nor in forward mode."""
+    weights, but neither twice nor in forward mode; the tables are constants, and refused where a gradient of theirs is wanted."""
     eps = float(eps)
+    if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):  # (before a Function, inside of which nothing wants one)
+        raise ValueError("cos and sin are constants: they get no gradient")
     if torch.compiler.is_compiling():  # a graph is being captured: the kernels go in as opaque operators
         from . import _opaque
 
         return _opaque.qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, eps)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight, cos, sin)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         return _QkNormRotary.apply(q, k, q_weight, k_weight, cos, sin, positions, eps)
     result = _on_host_path(q, k, q_weight, k_weight, cos, sin, positions, eps)
     return _forward(q, k, q_weight, k_weight, cos, sin, positions, eps) if result is None else result

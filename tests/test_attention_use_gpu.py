@@ -554,3 +554,19 @@ def test_more_heads_to_one_than_a_division_by_multiplication_holds():
     want = torch.autograd.grad((weights @ ref[2][0, :, 0]).transpose(0, 1)[None], ref, do.double())
     for name, a, b in zip(("dq", "dk", "dv"), got, want):
         check(name, a.cpu(), b.cpu(), GRAD[BF16])
+
+
+def test_tables_that_want_a_gradient_are_refused():
+    q, k = cuda(*inputs(1, 6, 2, 1, 64))[:2]
+    cos, sin = rotary_table(6, 64)
+    for tables in ((cos.clone().requires_grad_(), sin), (cos, sin.clone().requires_grad_())):
+        for leaf in (q, q.clone().requires_grad_()):
+            with pytest.raises(ValueError, match="constants"):
+                qk_norm_rotary(leaf, k, None, None, *tables)
+            with pytest.raises(Exception, match="constants"):
+                torch.compile(qk_norm_rotary, backend="aot_eager", fullgraph=True)(leaf, k, None, None, *tables)
+        with torch.no_grad():  # none is asked for
+            for a, b in zip(qk_norm_rotary(q, k, None, None, *tables), qk_norm_rotary(q, k, None, None, cos, sin)):
+                assert torch.equal(a, b)
+            odd = [t.T.contiguous().T for t in tables]  # (not as the kernel reads them)
+            assert torch.equal(qk_norm_rotary(q, k, None, None, *odd)[0], qk_norm_rotary(q, k, None, None, cos, sin)[0])
