@@ -19,6 +19,17 @@ def kernel_rows(grad: torch.Tensor, stride_elements: int = 8, address_bytes: int
     return grad.clone(memory_format=torch.contiguous_format)  # (contiguous() returns a dense tensor at an odd offset as it is)
 
 
+def as_int32(x: torch.Tensor | None) -> torch.Tensor | None:
+    """Integers as the kernels read them.  What 32 bits do not hold becomes the nearest that they do, which is as far out of every range; a plain
+    conversion would keep the lower bits, which may be those of a valid position, page or length."""
+    if x is None or x.dtype == torch.int32:
+        return x if x is None else x.contiguous()
+    wide = x.to(torch.int64)
+    if x.dtype == torch.uint64:
+        wide = torch.where(wide < 0, torch.iinfo(torch.int64).max, wide)
+    return wide.clamp(-(2**31), 2**31 - 1).to(torch.int32).contiguous()
+
+
 def mark_written(x: torch.Tensor) -> None:
     """What a torch operation in place tells autograd: a backward that saved ``x``, or a tensor that shares its memory, raises from here on.
     (Tensors made in inference mode are never saved, and have no version.)"""

@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import torch
 
-from ._autograd import kernel_rows, refuse_tangents
+from ._autograd import as_int32, kernel_rows, refuse_tangents
 from ._host import host, raw_stream
 from .kernels import Kernel, is_kernel_allowed
 from .layer_ops import _dtype_code
@@ -99,7 +99,7 @@ def _forward(q, k, v, window, sinks, scale, cu_seqlens, left_padded, wants_lse):
     if q.numel() == 0 or k.numel() == 0:
         return torch.zeros_like(q, memory_format=torch.contiguous_format), _empty_lse(q) if wants_lse else None
     with torch.cuda.device(q.device), torch.no_grad():
-        cu_seqlens = None if cu_seqlens is None else cu_seqlens.to(torch.int32).contiguous()
+        cu_seqlens = as_int32(cu_seqlens)
         result = host().window_attention(raw_stream(q.get_device()), _rows(q), _rows(k), _rows(v), window, sinks, scale, cu_seqlens, left_padded, wants_lse)
         if result is None:
             raise refused("sliding_window_attention", q)
@@ -113,7 +113,7 @@ def _backward(q, k, v, o, lse, window, sinks, scale, cu_seqlens, left_padded, do
     if q.numel() == 0 or k.numel() == 0:
         return tuple(torch.zeros_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
     with torch.cuda.device(q.device), torch.no_grad():
-        cu_seqlens = None if cu_seqlens is None else cu_seqlens.to(torch.int32).contiguous()
+        cu_seqlens = as_int32(cu_seqlens)
         result = host().window_attention_bwd(raw_stream(q.get_device()), _rows(q), _rows(k), _rows(v), _rows(o), lse, window, sinks, scale, cu_seqlens,
                                              left_padded, _rows(do.to(q.dtype)))  # fmt: skip
         if result is None:

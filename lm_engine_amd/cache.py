@@ -17,7 +17,7 @@ from typing import NamedTuple
 
 import torch
 
-from ._autograd import kernel_rows, refuse_tangents
+from ._autograd import as_int32, kernel_rows, refuse_tangents
 from ._host import host, raw_stream
 from .kernels import Kernel, is_kernel_allowed
 from .layer_ops import _dtype_code
@@ -87,10 +87,6 @@ def _check_cache(cache, block_table, **per_sequence):
     return HK, P, D, N
 
 
-def _int32(x):
-    return None if x is None else x.to(torch.int32).contiguous()
-
-
 def _check_rows(x, name, like, heads, D):
     if x.dim() != 4 or x.size(2) != heads or x.size(3) != D:
         raise ValueError(f"{name} must be [B, T, {heads}, {D}], got {tuple(x.shape)}")
@@ -119,7 +115,7 @@ def _write(cache, k, v, block_table, start, cu_seqlens, left_padded):
         return
     with torch.cuda.device(k.device), torch.no_grad():
         rows = (kernel_rows(x.detach(), 16 // x.element_size()) for x in (k, v))
-        done = host().cache_write(raw_stream(k.get_device()), *cache, _int32(block_table), *rows, _int32(start), _int32(cu_seqlens), left_padded)
+        done = host().cache_write(raw_stream(k.get_device()), *cache, as_int32(block_table), *rows, as_int32(start), as_int32(cu_seqlens), left_padded)
         if done is None:
             raise refused("write_paged_cache")
 
@@ -162,7 +158,7 @@ def _read(cache, block_table, lengths, max_tokens, dtype):
         empty = cache.k.new_empty((N, max_tokens, HK, D), dtype=dtype)
         return empty, empty.clone()
     with torch.cuda.device(cache.k.device):
-        result = host().cache_read(raw_stream(cache.k.get_device()), *cache, _int32(block_table), _int32(lengths), max_tokens, code == 0)
+        result = host().cache_read(raw_stream(cache.k.get_device()), *cache, as_int32(block_table), as_int32(lengths), max_tokens, code == 0)
         if result is None:
             raise refused("read_paged_cache", *[torch.empty(N, max_tokens, HK, D, dtype=dtype, device=cache.k.device)] * 2)
     return result
@@ -197,7 +193,7 @@ def _attend(q, cache, block_table, lengths, window, sinks, scale):
     if q.numel() == 0 or block_table.size(1) == 0:
         return torch.zeros_like(q, memory_format=torch.contiguous_format)
     with torch.cuda.device(q.device), torch.no_grad():
-        result = host().cache_attention(raw_stream(q.get_device()), kernel_rows(q.detach()), *cache, _int32(block_table), _int32(lengths), window, sinks, scale)
+        result = host().cache_attention(raw_stream(q.get_device()), kernel_rows(q.detach()), *cache, as_int32(block_table), as_int32(lengths), window, sinks, scale)
         if result is None:
             raise refused("paged_cache_attention", q)
     return result

@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._autograd import kernel_rows, refuse_tangents
+from ._autograd import as_int32, kernel_rows, refuse_tangents
 from ._host import host, raw_stream
 from .kernels import Kernel, is_kernel_allowed
 from .layer_ops import _dtype_code
@@ -84,8 +84,7 @@ def _dense(x, dtype=None):
 def _operands(q, k, q_weight, k_weight, cos, sin, positions):
     """In the form the kernels read: copies where rows or tables do not lie so."""
     rows = lambda x: kernel_rows(x.detach(), 16 // x.element_size())  # noqa: E731
-    positions = None if positions is None else positions.to(torch.int32).contiguous()
-    return rows(q), rows(k), _dense(q_weight), _dense(k_weight), _dense(cos, torch.float32), _dense(sin, torch.float32), positions
+    return rows(q), rows(k), _dense(q_weight), _dense(k_weight), _dense(cos, torch.float32), _dense(sin, torch.float32), as_int32(positions)
 
 
 def refused(what: str, *outputs: torch.Tensor) -> Exception:

@@ -310,6 +310,19 @@ def test_opaque_operators_have_shape_only_implementations():
     assert ops.paged_cache_write_(*cache, k, k, pages, lengths, None, False) is None
 
 
+def test_integers_that_32_bits_do_not_hold_stay_out_of_range():
+    from lm_engine_amd._autograd import as_int32
+
+    top, low = 2**31 - 1, -(2**31)
+    x = torch.tensor([0, 5, -5, 2**31, 2**32 + 5, -(2**32) + 5, 2**63 - 1, -(2**63)])
+    assert as_int32(x).tolist() == [0, 5, -5, top, top, low, top, low] and as_int32(x).dtype == torch.int32
+    for dtype, values, want in ((torch.uint8, [0, 255], [0, 255]), (torch.int16, [-(2**15), 7], [-(2**15), 7]), (torch.uint16, [65535], [65535]),
+                                (torch.uint32, [2**32 - 1, 3], [top, 3]), (torch.uint64, [2**64 - 1, 2**32, 3], [top, top, 3])):  # fmt: skip
+        assert as_int32(torch.tensor(values, dtype=dtype)).tolist() == want
+    every_other = torch.arange(10, dtype=torch.int32)[::2]
+    assert as_int32(every_other).is_contiguous() and as_int32(every_other).tolist() == [0, 2, 4, 6, 8] and as_int32(None) is None
+
+
 # ---- the oracle itself
 def test_oracle_of_the_window():
     mask = visible_keys(3, 6, window=2, sinks=1)  # positions 3, 4, 5

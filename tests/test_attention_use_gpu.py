@@ -570,3 +570,33 @@ def test_tables_that_want_a_gradient_are_refused():
                 assert torch.equal(a, b)
             odd = [t.T.contiguous().T for t in tables]  # (not as the kernel reads them)
             assert torch.equal(qk_norm_rotary(q, k, None, None, *odd)[0], qk_norm_rotary(q, k, None, None, cos, sin)[0])
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+def test_wide_integers_past_32_bits_are_no_small_ones(sign):
+    """Positions, pages, starts, lengths and prefix sums in 64 bits whose lower 32 are those of a valid one."""
+    far = sign * 2**32
+    q, k, v = cuda(*inputs(1, 4, 4, 2, 64))
+    cos, sin = rotary_table(10, 64)
+    positions = torch.tensor([[0, far + 1, 2, far]], device="cuda")
+    for y in qk_norm_rotary(q, k, None, None, cos, sin, positions):
+        assert y[:, [0, 2]].isfinite().all() and y[:, [1, 3]].isnan().all()
+    cache, table, lengths, _ = filled([30, 40], 2, 64, 16)
+    before = [x.clone() for x in cache]
+    bits = lambda x: x.view(torch.uint8)  # noqa: E731
+    new = torch.randn(2, 3, 2, 64, device="cuda").to(BF16)
+    write_paged_cache(cache, new, new, table, lengths.long() + far)
+    assert all(torch.equal(bits(a), bits(b)) for a, b in zip(cache, before))
+    write_paged_cache(cache, new, new, table.long() + far, lengths)
+    assert all(torch.equal(bits(a), bits(b)) for a, b in zip(cache, before))
+    wide = table.long()
+    wide[0, 1] += far
+    held, _ = read_paged_cache(cache, wide, lengths, 40)
+    assert held[0, 16:30].isnan().all() and held[0, :16].isfinite().all() and held[1].isfinite().all()
+    few = torch.randn(2, 1, 4, 64, device="cuda").to(BF16)
+    assert paged_cache_attention(few, cache, wide, lengths)[0].isnan().all()
+    ends = torch.full_like(lengths, table.size(1) * 16 if sign > 0 else 0)  # what such a length is clamped to
+    got, want = paged_cache_attention(few, cache, table, lengths.long() + far), paged_cache_attention(few, cache, table, ends)
+    assert torch.equal(bits(got), bits(want))  # (NaN where the table has no page)
+    o = sliding_window_attention(q, k, v, cu_seqlens=torch.tensor([0, far + 2], device="cuda"))
+    assert torch.equal(o, sliding_window_attention(q, k, v, cu_seqlens=torch.tensor([0, 4 if sign > 0 else 0], dtype=torch.int32, device="cuda")))
