@@ -102,7 +102,7 @@ def _write(cache, k, v, block_table, start, cu_seqlens, left_padded):
     _dtype_code(k.dtype, "k and v")
     B, T = k.shape[:2]
     if cu_seqlens is not None:
-        if cu_seqlens.is_floating_point() or cu_seqlens.dim() != 1 or cu_seqlens.numel() != N + 1 or cu_seqlens.device != k.device:
+        if cu_seqlens.is_floating_point() or cu_seqlens.dtype == torch.bool or cu_seqlens.dim() != 1 or cu_seqlens.numel() != N + 1 or cu_seqlens.device != k.device:
             raise ValueError(f"cu_seqlens must be integers [N + 1] = [{N + 1}] on {k.device}")
         if not left_padded and B != 1:
             raise ValueError(f"with cu_seqlens the batch dim must be 1 (tokens packed along T), got B={B}")

@@ -600,3 +600,12 @@ def test_wide_integers_past_32_bits_are_no_small_ones(sign):
     assert torch.equal(bits(got), bits(want))  # (NaN where the table has no page)
     o = sliding_window_attention(q, k, v, cu_seqlens=torch.tensor([0, far + 2], device="cuda"))
     assert torch.equal(o, sliding_window_attention(q, k, v, cu_seqlens=torch.tensor([0, 4 if sign > 0 else 0], dtype=torch.int32, device="cuda")))
+
+
+def test_prefix_sums_of_truth_values_are_refused():
+    cache, table, lengths, _ = filled([10, 20], 2, 64, 16)
+    new = torch.zeros(1, 2, 2, 64, device="cuda", dtype=BF16)
+    with pytest.raises(ValueError, match="cu_seqlens must be integers"):
+        write_paged_cache(cache, new, new, table, lengths, cu_seqlens=torch.ones(3, dtype=torch.bool, device="cuda"))
+    with pytest.raises(ValueError, match="cu_seqlens must hold integers"):
+        sliding_window_attention(new, new, new, cu_seqlens=torch.ones(3, dtype=torch.bool, device="cuda"))
