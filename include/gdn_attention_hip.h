@@ -120,7 +120,8 @@ uint64_t gdn_window_attn_workspace_bytes(const gdn_window_attn_args *args);
 
 /*
  * Gradients from the forward's inputs, its o and lse, and dout [B, T, H, D]: dq [B, T, H, D], dk and dv [B, S, HK, D] (the gradients of
- * query heads that share one of k and v are added up in fp32), all in the inputs' dtype, with element strides, written whole.
+ * query heads that share one of k and v are added up in fp32), all in the inputs' dtype, with element strides, written whole.  In bf16 at most
+ * 65280 query heads share one.
  */
 typedef struct gdn_window_attn_bwd_args {
     gdn_window_attn_args fwd;

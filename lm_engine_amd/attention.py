@@ -14,7 +14,7 @@ packed sequences), read as zeros in ``o`` and in the gradients.  A query's outpu
 whatever the others hold; a gradient may be spoiled by values of the same sequence or batch row that are not finite, seen or not.
 
 Differentiable in q, k and v; the backward works from the saved inputs, the output and one number per row.  Second derivatives and dual
-tensors (forward mode) are refused.  The kernels are those of ``csrc/gdn_window_attention*.hip``; there is no fallback.
+tensors (forward mode) are refused, and in bf16 gradients with more than 65280 query heads to one of k and v.  The kernels are those of ``csrc/gdn_window_attention*.hip``; there is no fallback.
 """
 
 from __future__ import annotations

@@ -42,6 +42,9 @@ int check_shape(const gdn_window_attn_args& a) {
     return GDN_OK;
 }
 
+// (rows of a tile are taken apart into tokens and heads)
+bool backward_fits(const gdn_window_attn_args& a) { return a.dtype != GDN_BF16 || a.H / a.HK <= MOST_GROUP; }
+
 int check_inputs(const gdn_window_attn_args& a) {
     int e;
     if ((e = check_rows(a.q, a.q_stride_b, a.q_stride_t, a.q_stride_h, a.H, a.dtype)) != GDN_OK) return e;
@@ -147,7 +150,7 @@ extern "C" int gdn_window_attn_fwd(const gdn_window_attn_args* args, void* strea
 }
 
 extern "C" uint64_t gdn_window_attn_bwd_workspace_bytes(const gdn_window_attn_bwd_args* b) {
-    return b == nullptr || check_shape(b->fwd) != GDN_OK ? 0 : backward_bytes(b->fwd, params_of(b->fwd));
+    return b == nullptr || check_shape(b->fwd) != GDN_OK || !backward_fits(b->fwd) ? 0 : backward_bytes(b->fwd, params_of(b->fwd));
 }
 
 extern "C" int gdn_window_attn_bwd(const gdn_window_attn_bwd_args* args, void* stream) {
@@ -155,6 +158,7 @@ extern "C" int gdn_window_attn_bwd(const gdn_window_attn_bwd_args* args, void* s
     const gdn_window_attn_bwd_args& b = *args;
     const gdn_window_attn_args& a = b.fwd;
     if (const int e = check_shape(a); e != GDN_OK) return e;
+    if (!backward_fits(a)) return GDN_ERR_UNSUPPORTED;
     if (const int e = check_inputs(a); e != GDN_OK) return e;
     if (a.lse == nullptr) return GDN_ERR_NULL;
     if (const int e = check_rows(b.dout, b.dout_stride_b, b.dout_stride_t, b.dout_stride_h, a.H, a.dtype); e != GDN_OK) return e;

@@ -44,11 +44,11 @@ struct WindowParams {
 };
 
 // n / G and the rest, for n < G + 256.  by_g is less than 1 / G too large in units of 2^32 / G, so that n by_g / 2^32 is n / G rounded down as long as
-// n G < 2^32; there are two tokens at most for more heads to one than that holds for.
-constexpr int MOST_BY_PRODUCT = 65280;
-static_assert((uint64_t)MOST_BY_PRODUCT * (MOST_BY_PRODUCT + 256) < (uint64_t)1 << 32);
+// n G < 2^32: the backward refuses more heads to one.
+constexpr int MOST_GROUP = 65280;
+static_assert((uint64_t)MOST_GROUP * (MOST_GROUP + 256) < (uint64_t)1 << 32);
 __device__ __forceinline__ void split_rows(const WindowParams& p, int n, int& t, int& g) {
-    t = p.G == 1 ? n : p.G > MOST_BY_PRODUCT ? (n >= p.G ? 1 : 0) : (int)__umulhi((unsigned)n, p.by_g);
+    t = p.G == 1 ? n : (int)__umulhi((unsigned)n, p.by_g);
     g = n - t * p.G;
 }
 

@@ -124,6 +124,15 @@ def test_window_attention_checks_workspaces_and_gradients():
         assert backward(**over) == status, over
 
 
+def test_window_attention_backward_refuses_more_heads_to_one_than_it_takes_apart():
+    lib = _lib.load_library()
+    b = _lib.GdnWindowAttnBwdArgs()
+    for heads, dtype, some in ((65280, _lib.GDN_BF16, True), (65281, _lib.GDN_BF16, False), (65281, _lib.GDN_F32, True)):
+        b.fwd = _window(H=heads, HK=1, dtype=dtype)
+        assert (lib.gdn_window_attn_bwd_workspace_bytes(ctypes.byref(b)) > 0) == some
+        assert lib.gdn_window_attn_bwd(ctypes.byref(b), None) == (-1 if some else -3)  # (no gradients to write to, or refused before)
+
+
 def test_qk_norm_rotary_rejects_bad_arguments_before_any_launch():
     lib = _lib.load_library()
 
