@@ -7,14 +7,14 @@
 // A sequence's first keys are seen by all of its rows: those beyond the window are shared out over many workgroups, in a launch of their own, and
 // the parts joined by another.  Where there are few blocks of keys, the rows of each are cut into shares, joined in the same way.
 // Rounding: w and ds become bf16 for the second product of each pass, at most half a step (2^-8) of the value; everything else is fp32.  delta from the
-// output as it is stored, rounded and made of rounded weights, would be off by 1e-3, which goes into dq and dk times the mean of the keys and
-// queries.  But sum_j ds_j = 0: what that sum is short of zero is delta's error.  window_dq_kernel forms it, and leaves the exact
-// delta for dk; where it matters for dq (few keys, or keys with a mean; see there) it walks over the keys once more.  In rms of dq and dk:
-// 1.8e-3 from ds and 1.7e-3 from their own rounding, 2.4e-3 together, where delta from the output gave 2.8e-3; with keys, queries and values whose mean is
-// as large as their spread 2.6e-3 instead of 1.0e-2 (1200 tokens, 64 columns), with twice that mean 4.3e-3 instead of 3.7e-2 (window 500, 128).
+// output as it is stored, rounded and made of rounded weights, is off by some 1e-3 of its terms, which goes into dq times the row's weighted mean of
+// the keys, and into dk times the queries.  But sum_j ds_j = 0: what that sum is short of zero is delta's error.  window_dq_kernel forms it, takes its
+// part out of dq (see there), and leaves the exact delta for dk.  In rms: dq 2.2e-3, dk 2.4e-3, of which 1.7e-3 are their own rounding (1200 tokens,
+// 64 columns); keys, queries and values with a mean as large as their spread: dq 2.3e-3 (1.0e-2 with delta from the output); 0.3 to 0.98 of a row's
+// weight on one key eight times as long as the others: 2.1e-3 down to 1.7e-3 (256 columns, with two walks: 2.3e-3 to 2.5e-3).
 // Bound by the matrix unit together with the exponentials and the products' operands from LDS: at 4 x 4096 tokens, 16 heads of 128 over 2, window
-// 1024 and 4 first keys dq takes 228 us (790 TFLOP/s), the keys' 302 (740), the first keys' 26 and 5 to join them.  With 64 columns, where a score
-// has half the products but the same exponential, 950 and 800 TFLOP/s (4 x 4096, 16 heads, all keys) beside 980 and 840 with 128.
+// 1024 and 4 first keys dq takes 266 us (its four products at 900 TFLOP/s), the keys' 302 to 309 (740), the first keys' 26 and 5 to join them.  With 64
+// columns, where a score has half the products but the same exponential, 930 and 810 TFLOP/s (4 x 4096, 16 heads, all keys) beside 1000 and 860 with 128.
 #include <algorithm>
 
 #include "gdn_launch.h"
@@ -24,19 +24,31 @@ namespace gdn {
 
 namespace {
 
-// window_dq_kernel walks over a block's keys twice, the first time for the exact delta, where they are this many tiles (of 64) or fewer, as few keys
-// have large weights, with errors that do not average out: 4 x 4096 tokens, 16 heads over 2, window 64 159 us backward instead of 142.  With more, a
-// second walk follows where delta's error, times the mean of 64 of the keys, is over REST of a wave's dq: not for keys without a mean
-// (4 x 4096, 16 heads of 128 over 2, window 1024: 578 us backward, with the sum and the question; 560 without, 696 with two walks everywhere).
-constexpr int EXACT_TILES = 4;
-constexpr float REST = 0x1p-10f;
+// sum + the eight values' sum
+__device__ __forceinline__ float sum8(const bf16x8& x, float sum) {
+    const bf16x2 one = {(bf16_t)1.f, (bf16_t)1.f};
+#pragma unroll
+    for (int e = 0; e < 4; e++) sum = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x[2 * e], x[2 * e + 1]}, one, sum, false);
+    return sum;
+}
 
+// Gradients of 128 rows, 32 to a wave.  delta is first formed from the output, and off by r; since the weights of a row add up to 1, r = sum_j ds_j.
+// Up to 128 columns sum_j w_j k_j is carried beside dq, and r times it taken off in the end.  Both products take operands in bf16; r is there
+// the quotient of their own sums, as they are rounded, so that the coefficients that the keys are left with add up to zero: where one key has nearly
+// all of a row's weight, its coefficient is as good as the others', however small they are.  That is a fourth product to each tile.  At 128 columns
+// there are registers for it with do's rows in LDS and tiles of 32 keys: backward, at 4 x 4096 tokens, 16 heads of 128 over 2, window 1024, 600 us (710
+// with two walks, 557 with neither); 64 columns, 16 heads, all keys 620 (780 and 577).
+// Above 128 columns the registers are short of it by far, and a walk of its own over the keys, without the third product, forms the exact delta
+// before: 8 x 4096 tokens, 2 heads of 256 over one, window 1024, 710 us (1087 with the product and what it spills, 640 with neither).
 template <int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dq_kernel(const WindowParams p) {
-    constexpr int KS = DP / 16, DT = DP / 32;
-    using Loads = TileLoads<DP>;
-    static_assert(row_offsets_fit(64, false));
-    __shared__ __attribute__((aligned(1024))) bf16_t tiles[2][2][64 * DP];
+    constexpr int KS = DP / 16, DT = DP / 32, KEYS = DP == 128 ? 32 : 64;
+    constexpr bool OWN = DP != 128, TWICE = DP > 128;  // rows of do in registers; two walks
+    using Loads = TileLoads<DP, KEYS / 4>;
+    using RowLoads = TileLoads<DP, 32>;
+    static_assert(row_offsets_fit(KEYS, false) && row_offsets_fit(32, true));
+    __shared__ __attribute__((aligned(1024))) bf16_t tiles[2][2][KEYS * DP];
+    __shared__ __attribute__((aligned(1024))) bf16_t do_rows[OWN ? 1 : WINDOW_ROWS * DP];
     int pair, block;
     work_item(p, blockIdx.x, pair, block);
     block = p.blocks - 1 - block;
@@ -64,10 +76,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dq_kernel(const
     const RowView view = row_view(p, b, r);
     const WaveView w = wave_view(view);
     __shared__ int bounds[4][6];
-    __shared__ float columns[4][DP];
     const WaveView all = join_waves<4>(w, bounds, wave, lane);
     const int lo = all.lo, end = all.end, sink = all.sink, sink_end = min(all.sink_end, lo);
-    const int sink_tiles = sink_end > sink ? (sink_end - sink + 63) / 64 : 0, near_tiles = end > lo ? (end - lo + 63) / 64 : 0;
+    const int sink_tiles = sink_end > sink ? (sink_end - sink + KEYS - 1) / KEYS : 0, near_tiles = end > lo ? (end - lo + KEYS - 1) / KEYS : 0;
     const int tile_count = sink_tiles + near_tiles;
 
     const char* const kb = reinterpret_cast<const char*>(static_cast<const bf16_t*>(p.k.p) + b * p.k.b + hk * p.k.h);
@@ -75,104 +86,105 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void window_dq_kernel(const
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&tiles[0][0][0];
     auto tile_at = [&](int i, int& j0, int& count) {
         const bool s = i < sink_tiles;
-        j0 = s ? sink + 64 * i : lo + 64 * (i - sink_tiles);
-        count = min((s ? sink_end : end) - j0, 64);
+        j0 = s ? sink + KEYS * i : lo + KEYS * (i - sink_tiles);
+        count = min((s ? sink_end : end) - j0, KEYS);
     };
     auto load_tile = [&](int i, int buffer) {
         int j0, count;
         tile_at(i, j0, count);
         const char *const k0 = kb + (int64_t)j0 * p.k.t * 2, *const v0 = vb + (int64_t)j0 * p.v.t * 2;
-        const uint32_t to = lds + buffer * 2 * 64 * DP * 2;
+        const uint32_t to = lds + buffer * 2 * KEYS * DP * 2;
 #pragma unroll
         for (int x = 0; x < Loads::ITERS; x++) {
             const int kr = Loads::row(wave, lane, x), col = Loads::column(wave, lane, x);
             const bool there = kr < count && col < p.D;
             Loads::load(k0, there ? (uint32_t)(kr * (int)p.k.t + col) * 2 : PAST, to, wave, x);
-            Loads::load(v0, there ? (uint32_t)(kr * (int)p.v.t + col) * 2 : PAST, to + 64 * DP * 2, wave, x);
+            Loads::load(v0, there ? (uint32_t)(kr * (int)p.v.t + col) * 2 : PAST, to + KEYS * DP * 2, wave, x);
         }
     };
 
-    const TileReader<DP> reader(lane);
-    f32x16 dq[DT] = {};
-    float sum = 0.f;  // of ds: what delta lacks, since the weights add up to 1
-    const int before = tile_count <= EXACT_TILES ? tile_count : 0;  // steps of the first walk
-    if (tile_count > 0) load_tile(0, 0);
-    bool exact = before > 0;
-    int buffer = 1;
-    for (int step = -before;; step++) {
-        if (step == tile_count) {
-            if (exact || tile_count == 0) break;
-            // what delta's error has done to this wave's rows, against the rows themselves
-            const float rest = sum + other_half(sum);
-            float own = 0.f, mean = 0.f;
+    TileReader<DP> reader(lane);
+    f32x16 dq[DT] = {}, wk[TWICE ? 1 : DT] = {};
+    float rest = 0.f, ds_sum = 0.f, w_sum = 0.f;  // the sum of ds; of ds and the weights as they are rounded
+    int step = TWICE ? -tile_count : 0;
+    if (!OWN && tile_count > 0) {  // a wave's own rows, which it reads behind the loads_done of its first tile
+        const int first = block * WINDOW_ROWS + 32 * wave, t0 = p.G == 1 ? first : first / p.G, g0 = first - t0 * p.G;
+        const char* const d0 = reinterpret_cast<const char*>(static_cast<const bf16_t*>(p.dout.p) + b * p.dout.b + hk * p.G * p.dout.h + t0 * p.dout.t);
+        const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&do_rows[0];
 #pragma unroll
-            for (int z = 0; z < DT; z++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) own = __builtin_fmaf(dq[z][e], dq[z][e], own);
-            for (int x = lane; x < DP; x += WAVE) {
-                const float k = (columns[0][x] + columns[1][x] + columns[2][x] + columns[3][x]) * (1.f / 64);
-                mean = __builtin_fmaf(k, k, mean);
-            }
-            const float most = wave_sum(rest * rest * 0.5f) * wave_sum(mean);
-            if (__syncthreads_or(!(most <= REST * REST * wave_sum(own))) == 0) break;
-            exact = true, step = 0;
-            delta += rest, sum = 0.f;
-#pragma unroll
-            for (int z = 0; z < DT; z++) dq[z] = f32x16{};
-            buffer = 1;
-            load_tile(0, 0);
+        for (int x = 0; x < RowLoads::ITERS; x++) {
+            const int rr = RowLoads::row(0, lane, x), col = RowLoads::column(0, lane, x);
+            int tt, g;
+            split_rows(p, g0 + rr, tt, g);
+            RowLoads::load(d0, first + rr < p.rows && col < p.D ? (uint32_t)(tt * (int)p.dout.t + g * (int)p.dout.h + col) * 2 : PAST, to, wave, x);
         }
-        if (step == 0 && before > 0) delta += sum + other_half(sum), sum = 0.f;
+    }
+    if (tile_count > 0) load_tile(0, step & 1);
+    for (; step < tile_count; step++) {
+        if (TWICE && step == 0) delta += rest + other_half(rest), rest = 0.f;
         const int i = step < 0 ? step + tile_count : step;
         loads_done();
         __syncthreads();
-        buffer ^= 1;
-        if (step + 1 < tile_count) load_tile(i + 1 == tile_count ? 0 : i + 1, buffer ^ 1);
+        reader.recompute();
+        if (step + 1 < tile_count) load_tile(i + 1 == tile_count ? 0 : i + 1, (step + 1) & 1);
         int j0, count;
         tile_at(i, j0, count);
-        const bf16_t *const kt = tiles[buffer][0], *const vt = tiles[buffer][1];
-        const bool near = i >= sink_tiles, full = near && j0 >= w.full_lo && j0 + 64 <= w.full_end;
-        if (step == tile_count - 2 && !exact) {  // 64 keys that are there: their sum, 16 of them a wave's
-            stay_a_branch();
-            for (int x = lane; x < DP; x += WAVE) {
-                float k = 0.f;
-                for (int y = 16 * wave; y < 16 * wave + 16; y++) k += (float)kt[y * DP + (((x >> 3) ^ tile_key<DP>(y)) << 3) + (x & 7)];
-                columns[wave][x] = k;
-            }
-        }
+        const bf16_t *const kt = tiles[step & 1][0], *const vt = tiles[step & 1][1];
+        const bool near = i >= sink_tiles, full = near && j0 >= w.full_lo && j0 + KEYS <= w.full_end;
         if (!w.meets(j0, count)) continue;
         const TileView own(view, near, sink_end);
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
+        for (int x = 0; x < KEYS / 32; x++) {
             f32x16 s = {}, dw = {};
 #pragma unroll
             for (int y = 0; y < KS; y++) s = mma(reader.across(kt, 32 * x, y), q[y], s);
+            if constexpr (!OWN) __builtin_amdgcn_sched_barrier(0);  // (registers: operands of one product at a time)
 #pragma unroll
-            for (int y = 0; y < KS; y++) dw = mma(reader.across(vt, 32 * x, y), d[y], dw);
+            for (int y = 0; y < KS; y++) dw = mma(reader.across(vt, 32 * x, y), OWN ? d[y] : reader.across(do_rows, 32 * wave, y), dw);
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -lse)) * (dw[e] - delta);
+            for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -lse)), dw[e] = s[e] * (dw[e] - delta);
             if (!full) {
                 stay_a_branch();
                 if (!(near && j0 < all.sink_end)) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) s[e] = own.sees(j0 + 32 * x + acc_row(e, half)) ? s[e] : 0.f;
+                    for (int e = 0; e < 16; e++)
+                        if (!own.sees(j0 + 32 * x + acc_row(e, half))) s[e] = dw[e] = 0.f;
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) s[e] = own.sees_mixed(j0 + 32 * x + acc_row(e, half)) ? s[e] : 0.f;
+                    for (int e = 0; e < 16; e++)
+                        if (!own.sees_mixed(j0 + 32 * x + acc_row(e, half))) s[e] = dw[e] = 0.f;
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 16; e++) sum += s[e];
-            if (step < 0) continue;
+            for (int e = 0; e < 16; e++) rest += dw[e];
+            if (TWICE && step < 0) continue;
 #pragma unroll
             for (int y = 0; y < 2; y++) {
-                const bf16x8 ds = pack8(s, y);
+                const bf16x8 ds = pack8(dw, y);
+                if constexpr (TWICE) {
 #pragma unroll
-                for (int z = 0; z < DT; z++) dq[z] = mma(reader.down(kt, 2 * x + y, z), ds, dq[z]);
+                    for (int z = 0; z < DT; z++) dq[z] = mma(reader.down(kt, 2 * x + y, z), ds, dq[z]);
+                } else {
+                    const bf16x8 weights = pack8(s, y);
+                    ds_sum = sum8(ds, ds_sum), w_sum = sum8(weights, w_sum);
+#pragma unroll
+                    for (int z = 0; z < DT; z++) {
+                        const bf16x8 k = reader.down(kt, 2 * x + y, z);
+                        dq[z] = mma(k, ds, dq[z]), wk[z] = mma(k, weights, wk[z]);
+                    }
+                }
             }
         }
     }
-    delta += sum + other_half(sum);
+    delta += rest + other_half(rest);
+    if constexpr (!TWICE) {
+        ds_sum += other_half(ds_sum), w_sum += other_half(w_sum);
+        const float by = w_sum == 0.f ? 0.f : ds_sum / w_sum;
+#pragma unroll
+        for (int z = 0; z < DT; z++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) dq[z][e] = __builtin_fmaf(wk[z][e], -by, dq[z][e]);
+    }
     int last = row;
     asm volatile("" : "+v"(last));  // (what follows from it is formed anew, rather than kept in registers over the walk)
     if (last >= p.rows) return;

@@ -13,7 +13,7 @@ import torch
 
 import lm_engine_amd
 from lm_engine_amd import sliding_window_attention
-from oracle.attention_oracle import window_attention_ref
+from oracle.attention_oracle import visible_keys, window_attention_ref
 from tests.helpers import rel_l2
 
 
@@ -160,3 +160,60 @@ def test_many_sequences_that_are_first_keys_for_the_most_part(sinks, D):
     q, k, v = inputs(1, sum(lens), 4, 2, D)
     check_call(q, k, v, BF16, cu_of(lens), window=6, sinks=sinks)
     assert torch.cuda.max_memory_allocated() < 1 << 30
+
+
+@pytest.mark.parametrize("weight", [0.3, 0.6, 0.9, 0.98, 0.9999])
+@pytest.mark.parametrize("T, H, HK, D, window, sinks", [(1200, 2, 1, 64, 400, 4), (1100, 2, 2, 64, None, 0), (1200, 2, 1, 128, 400, 4), (900, 2, 1, 128, None, 0), (700, 2, 1, 256, 300, 1), (200, 2, 1, 128, 90, 1)])
+def test_queries_gradients_where_a_first_key_draws_the_weight(T, H, HK, D, window, sinks, weight):
+    """A first key eight times as long as the others, which have no mean, with `weight` of every row's sum.  An error r of delta comes back as r times
+    the row's weighted mean of keys, here `weight` times the first one.
+
+    Whole: the coefficients of the keys add up to zero, rounded as they are, so that the first key's is off by what the others' are: 2^-8 / sqrt(3) rms
+    at most of the first one's, and that again from the result's own rounding: 3.2e-3, and 4e-3 is asked (below a weight of 1, where ds is no rest).
+
+    Row by row, in norm, with u = 2^-8 (bf16, half a step): delta from the output is off by rho, u sum |do| |o| from its rounding and u sum_j w_j
+    sum |do| |v_j| from its weights'.  A key's ds with that, and its weight, are rounded: u (|ds_j| + w_j rho) + u w_j rho; what is taken off again is
+    a sum over those, times w_j: w_j u (sum |ds| + 2 rho).  The result: u of itself.  fp32: scores and products of D terms, D 2^-24 of their
+    terms' sizes, sums of S terms, S 2^-24."""
+    gen = torch.Generator().manual_seed(T + D)
+    scale, u, eps = D**-0.5, 2.0**-8, 2.0**-24
+    towards = torch.randn(D, generator=gen)
+    towards = towards / towards.norm()
+    q, k, v = (torch.randn(1, T, h, D, generator=gen) for h in (H, HK, HK))
+    seen = visible_keys(T, T, window, sinks)
+    q -= (q @ towards)[..., None] * towards
+    k[:, 0] = 8 * D**0.5 * towards
+    for h in range(H):
+        scores = torch.where(seen, q[0, :, h] @ k[0, :, h * HK // H].T * scale, -torch.inf)
+        scores[:, 0] = -torch.inf
+        rest = scores.logsumexp(dim=1)
+        logit = torch.where(rest > -torch.inf, rest + torch.tensor(weight / (1 - weight)).log(), torch.zeros(()))
+        q[0, :, h] += (logit / (scale * 8 * D**0.5))[:, None] * towards
+    q, k, v, do = (x.to(BF16) for x in (q, k, v, torch.randn(1, T, H, D, generator=gen)))
+    leaves = [x.cuda().requires_grad_() for x in (q, k, v)]
+    dq, = torch.autograd.grad(sliding_window_attention(*leaves, window=window, sinks=sinks), leaves[:1], do.cuda())
+    dq = dq.double().cpu()[0]
+    errors, norms, worst = [], [], 0.0
+    for h in range(H):
+        Q, K, V, G = (x.double() for x in (q[0, :, h], k[0, :, h * HK // H], v[0, :, h * HK // H], do[0, :, h]))
+        scores = torch.where(seen, Q @ K.T * scale, -torch.inf)
+        w = scores.softmax(dim=1)
+        o = w @ V
+        dov, delta = G @ V.T, (G * o).sum(dim=1, keepdim=True)
+        ds = w * (dov - delta)
+        want = ds @ K * scale
+        longs, parts = K.norm(dim=1), G.abs() @ V.abs().T
+        rho = u * ((G.abs() * o.abs()).sum(1, keepdim=True) + (w * parts).sum(1, keepdim=True)) * (1 + u)
+        total = ds.abs().sum(1, keepdim=True)
+        bf16 = u * ds.abs() + 2 * u * w * rho + w * u * (total + 2 * rho)
+        exponent = eps * ((D + 2) * scale * (Q.abs() @ K.abs().T) + 8 * (scores.nan_to_num(neginf=0.0).abs() + scores.logsumexp(1, keepdim=True).abs() + 1))
+        products = (w * exponent * ((dov - delta).abs() + rho)) + w * eps * D * (parts + (G.abs() * o.abs()).sum(1, keepdim=True))
+        fp32 = products + w * products.sum(1, keepdim=True) + eps * T * (ds.abs() + w * (total + 3 * rho))
+        bound = (1 + u) * scale * ((bf16 + fp32) @ longs) + u * want.norm(dim=1)
+        error = (dq[:, h] - want).norm(dim=1)
+        worst = max(worst, (error / bound.clamp(min=1e-30)).max().item())
+        errors.append(error), norms.append(want.norm(dim=1))
+    whole = (torch.cat(errors).norm() / torch.cat(norms).norm()).item()
+    print(f"dq {whole:.2e}, rows at {worst:.2f} of their bound", flush=True)
+    assert worst <= 1, f"a row's error is {worst:.2f} of its bound"
+    assert whole <= 4e-3 or weight > 0.99, f"relative-L2 {whole:.2e}"
