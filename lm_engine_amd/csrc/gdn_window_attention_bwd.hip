@@ -270,7 +270,7 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, DP == 64 ? 3 : DP == 128 ? 2
     {
         const char* const k0 = reinterpret_cast<const char*>(static_cast<const bf16_t*>(p.k.p) + b * p.k.b + hk * p.k.h + (keys > 0 ? key0 : 0) * p.k.t);
         const char* const v0 = reinterpret_cast<const char*>(static_cast<const bf16_t*>(p.v.p) + b * p.v.b + hk * p.v.h + (keys > 0 ? key0 : 0) * p.v.t);
-        if (wave < KEYS / 16) {
+        if (tile_count > 0 && wave < KEYS / 16) {  // (the walk's first tile waits for them)
 #pragma unroll
             for (int x = 0; x < KeyLoads::ITERS; x++) {
                 const int kr = KeyLoads::row(wave, lane, x), col = KeyLoads::column(wave, lane, x);

@@ -217,3 +217,12 @@ def test_queries_gradients_where_a_first_key_draws_the_weight(T, H, HK, D, windo
     print(f"dq {whole:.2e}, rows at {worst:.2f} of their bound", flush=True)
     assert worst <= 1, f"a row's error is {worst:.2f} of its bound"
     assert whole <= 4e-3 or weight > 0.99, f"relative-L2 {whole:.2e}"
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_blocks_of_keys_that_no_query_sees(D):
+    """Behind a window, and in front of and behind the packed sequences: their gradients are zeros, next to blocks that have some."""
+    check_call(*inputs(2, 10, 4, 2, D, S=500), BF16, window=20)
+    check_call(*inputs(2, 10, 4, 2, D, S=500), BF16, window=20, sinks=3)
+    q, k, v = inputs(1, 600, 2, 1, D)
+    check_call(q, k, v, BF16, cu=[200, 210, 390], window=50, sinks=2)
