@@ -213,7 +213,8 @@ def paged_cache_attention(
     the last ``window`` (None: all) and the first ``sinks``.  Rows that see none are zeros.  A page number outside of the cache makes the rows
     that see it NaN.  The scores, weights and sums are fp32; the weights are rounded to bf16 as operands.
 
-    For single tokens and a few (drafts that are verified); the context is split over the GPU, so one long sequence is read as fast as many.
+    For single tokens and a few (drafts that are verified).  The contexts of few sequences are split over the GPU, so that one long sequence is read
+    as fast as many; parts go by the number of sequences, not by their lengths, so a long one among many short ones is read by few workgroups.
     For inference: q gets no gradient."""
     from .attention import check_window
 

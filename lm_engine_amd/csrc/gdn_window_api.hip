@@ -72,7 +72,8 @@ WindowParams params_of(const gdn_window_attn_args& a) {
 
 // Parts that the keys of a block of rows are cut into: until two workgroups a compute unit are there, none of them under 128 keys, and whole below
 // 384.  The joining launch costs 4.5 us, 64 keys one (bf16, 128 columns): 1 x 300 tokens of 4 heads over one take 14.4 us whole and 16.1 in two
-// parts, 1 x 777 of 2 over one with a window of 512 21.2 whole, 19.8 in two and 17.8 in four (256 columns: 39.7, 30.6, 25.7).
+// parts, 1 x 777 of 2 over one with a window of 512 21.2 whole, 19.8 in two and 17.8 in four (256 columns: 39.7, 30.6, 25.7, still falling at the last of
+// them; parts under 128 keys were not measured).
 int splits_of(const gdn_window_attn_args& a) {
     const int64_t rows = (int64_t)a.T * (a.H / a.HK), edge = a.dtype == GDN_BF16 ? WINDOW_ROWS : WINDOW_ROWS_F32;
     const int64_t groups = (int64_t)a.B * a.HK * ((rows + edge - 1) / edge);
@@ -91,7 +92,7 @@ uint64_t workspace_of(const gdn_window_attn_args& a) {
 }
 
 // The parts in which rows beyond the window are shared out for a sequence's first keys: about one workgroup a compute unit in all, 256 rows or
-// more to each.  (Half or twice as many: backward 549 and 550 us instead of 543 at 4 x 4096, 16 heads of 128 over 2, window 1024, 4 first keys.)
+// more to each.  (Half or twice as many: backward 617 us each instead of 611 at 4 x 4096, 16 heads of 128 over 2, window 1024, 4 first keys.)
 int pieces_of(const WindowParams& p, int dtype) {
     // (first keys of more places than there are tokens: sequences of which most are first keys, which the blocks' own walks take as they come)
     if (dtype != GDN_BF16 || p.sinks == 0 || (int64_t)p.N * p.sinks > (int64_t)p.B * p.S) return 0;
@@ -102,9 +103,9 @@ int first_keys_of(const WindowParams& p) { return (p.sinks + WINDOW_FIRST_KEYS -
 
 // The shares that the rows of a block of keys are cut into, where few heads of k and v leave fewer blocks than the chip has room for: with a window
 // one workgroup to a compute unit (up to 64 columns three), without one twice that (four), since then blocks have from all rows to none;
-// 4 tiles of rows or more to each.  Backward in us, whole and shared: 1 x 4096, 16 heads of 128 over 2, window 512 225 and 121 (4 shares; 8: 137);
-// the same with 64 columns 142 and 77 (6; 2: 97); 4 x 4096 of them without a window 1384 and 1092 (2; 4: 1129); 1 x 777, 4 heads of 128 over
-// one, window 512 129 and 64 (8 tiles or more to each: 70).  What it costs: the sums once more in fp32, and a launch of about 4 us.
+// 4 tiles of rows or more to each.  Backward in us, whole and shared: 1 x 4096, 16 heads of 128 over 2, window 512 215 and 117 (4 shares; 2: 146, 8:
+// 131); the same with 64 columns 136 and 72 (6; 2: 90, 8: 80); 4 x 4096 of them without a window 1536 and 1190 (2; 4: 1209); 1 x 777, 4 heads of 128
+// over one, window 512 114 and 51 (8 tiles or more to each: 57).  What it costs: the sums once more in fp32, and a launch of about 4 us.
 int shares_of(const WindowParams& p, int dtype) {
     if (dtype != GDN_BF16) return 1;
     const int64_t blocks = (int64_t)p.B * p.HK * ((p.S + window_keys(p.D) - 1) / window_keys(p.D));
